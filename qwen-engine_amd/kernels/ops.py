@@ -8,7 +8,7 @@ present, importing the kernels fails with the reason.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -148,6 +148,10 @@ def load_library():
         "qe_decode_chain_supported": [i32, i32, i32, i32, i32, i32, i32],
         "qe_decode_chain_preferred": [i32, i32, i32, i32, i32, i32, i32, i32],
         "qe_decode_chain_layers": [],
+        "qe_mxfp4_quantize": [vp, vp, vp, i32, i32, i32, vp],
+        "qe_mxfp4_values": [vp, vp, vp, i32, i32, i32, vp],
+        "qe_gemm_mxfp4": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp],
+        "qe_verify_drafts": [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, i64, vp],
         "qe_decode_chain": [vp, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, f32, f32, i32, i32, i32, i32, i32, i32, i32, i32, vp, i32, i32, vp, i64, vp],
     }
     for name, args in sigs.items():
@@ -170,6 +174,8 @@ def load_library():
     lib.qe_attention_prefill_workspace_bytes_for.restype = ctypes.c_long
     lib.qe_decode_chain_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32, i32]
     lib.qe_decode_chain_workspace_bytes.restype = ctypes.c_long
+    lib.qe_verify_drafts_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    lib.qe_verify_drafts_workspace_bytes.restype = ctypes.c_long
     _lib = lib
     return lib
 
@@ -2306,3 +2312,162 @@ def diff_heads(a: torch.Tensor, num_heads: int, num_kv_heads: int, v_dim: int, l
     _check(lib.qe_diff_heads(a.data_ptr(), out.data_ptr(), _ptr(gate), gs, T, H, G, Dv, Dc, float(lam), float(eps),
                              float(out_scale), _DT[a.dtype], _stream()), "diff_heads")
     return out
+
+
+# ---- drafting with 4-bit weights, and verifying the drafts -------------------------------------------
+def _on_current_device(t: torch.Tensor, what: str) -> None:
+    """The launch goes to the current device's stream, so that is where the operands have to be."""
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the operands are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+class MxFp4(NamedTuple):
+    """A matrix [T, K] in microscaled 4-bit floating point: blocks of 32 numbers along K, each with a scale 2^(s - 127) (a byte
+    s; 255: the block is NaN) and 32 codes of 4 bits (sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6),
+    two a byte, the first in its low half.  Numbers behind K in the last block do not count."""
+    codes: torch.Tensor      # uint8 [T, ceil(K / 32) * 16]
+    scales: torch.Tensor     # uint8 [T, ceil(K / 32)]
+    columns: int             # K
+
+
+def _need_mxfp4(m: MxFp4, name: str, device=None) -> Tuple[int, int]:
+    """Rows and columns of a 4-bit matrix whose parts are as the kernels assume."""
+    if not isinstance(m, MxFp4):
+        raise KernelError(f"{name} is no 4-bit matrix")
+    K = int(m.columns)
+    if K <= 0:
+        raise KernelError(f"{name} has {K} columns")
+    blocks = (K + 31) // 32
+    _need(m.codes, f"{name} (codes)", torch.uint8, (None, blocks * 16), device)
+    _need(m.scales, f"{name} (scales)", torch.uint8, (m.codes.shape[0], blocks), m.codes.device)
+    if m.codes.data_ptr() % 16:
+        raise KernelError(f"{name}: the codes do not begin at a whole 16-byte piece")
+    return m.codes.shape[0], K
+
+
+def mxfp4_quantize(x: torch.Tensor) -> MxFp4:
+    """x [T, K] (bfloat16 or float32, any K) in 4 bits.  A block's scale is the power of two of its largest magnitude, less the 2 of
+    the largest code (2^-127 at least); a number goes to the nearest code, ties to the even one, what is beyond 6 to 6.  A block with
+    an infinity or a NaN is all NaN."""
+    lib = load_library()
+    _need(x, "x", _ACT, (None, None))
+    T, K = x.shape
+    if K == 0:
+        raise KernelError("mxfp4_quantize: rows of no numbers")
+    _on_current_device(x, "mxfp4_quantize")
+    blocks = (K + 31) // 32
+    codes = torch.empty((T, blocks * 16), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((T, blocks), dtype=torch.uint8, device=x.device)
+    _check(lib.qe_mxfp4_quantize(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), T, K, _DT[x.dtype], _stream()), "mxfp4_quantize")
+    return MxFp4(codes, scales, K)
+
+
+def mxfp4_values(m: MxFp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The numbers that a 4-bit matrix stands for, [T, K] in bfloat16 or float32 (both hold them exactly)."""
+    lib = load_library()
+    T, K = _need_mxfp4(m, "the matrix")
+    if dtype not in _DT:
+        raise KernelError(f"mxfp4_values: element type {dtype}")
+    _on_current_device(m.codes, "mxfp4_values")
+    out = torch.empty((T, K), dtype=dtype, device=m.codes.device)
+    _check(lib.qe_mxfp4_values(m.codes.data_ptr(), m.scales.data_ptr(), out.data_ptr(), T, K, _DT[dtype], _stream()), "mxfp4_values")
+    return out
+
+
+def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+               epilogue: int = EPI_STORE) -> torch.Tensor:
+    """x [M, K] . w [N, K]^T (+ bias [N], 32-bit) -> [M, N] in out_dtype (default: x's; bfloat16 for a 4-bit x), w in 4 bits, x in
+    bfloat16, float32 or 4 bits.  Products are exact and summed in 32-bit.
+
+    epilogue EPI_RESIDUAL: the product is added into ``out``, the 32-bit stream [M, N].
+    epilogue EPI_SILU_MUL: w is [2 N, K] (gate rows, then up rows); the result is silu(x . gate^T) * (x . up^T), [M, N]; a bias
+    (in w's order of rows, [2 N]) joins before the activation."""
+    lib = load_library()
+    if isinstance(x, MxFp4):
+        M, K = _need_mxfp4(x, "x")
+        data, scales, kind, dev = x.codes, x.scales, 2, x.codes.device
+        out_dtype = out_dtype or torch.bfloat16
+    else:
+        _need(x, "x", _ACT, (None, None))
+        M, K = x.shape
+        data, scales, kind, dev = x, None, int(x.dtype is torch.float32), x.device
+        out_dtype = out_dtype or x.dtype
+    N, columns = _need_mxfp4(w, "w", dev)
+    if columns != K:
+        raise KernelError(f"gemm_mxfp4: x has {K} columns, w {columns}")
+    if N == 0:
+        raise KernelError("gemm_mxfp4: w has no rows")
+    if bias is not None:
+        _need(bias, "bias", torch.float32, (N,), dev)
+    wide, tail = N, 0
+    if epilogue == EPI_RESIDUAL:
+        if out is None:
+            raise KernelError("gemm_mxfp4: the residual epilogue needs the stream to add into")
+        out_dtype, tail = torch.float32, 1
+    elif epilogue == EPI_SILU_MUL:
+        if N % 2:
+            raise KernelError("gemm_mxfp4: gate|up weights have an odd number of rows")
+        wide, tail = N // 2, 2
+    elif epilogue != EPI_STORE:
+        raise KernelError(f"gemm_mxfp4: epilogue {epilogue} is not taken")
+    if out_dtype not in _DT:
+        raise KernelError(f"gemm_mxfp4: a result in {out_dtype}")
+    _on_current_device(data, "gemm_mxfp4")
+    if out is None:
+        out = torch.empty((M, wide), dtype=out_dtype, device=dev)
+    _need(out, "out", out_dtype, (M, wide), dev)
+    _check(lib.qe_gemm_mxfp4(data.data_ptr(), _ptr(scales), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), out.data_ptr(),
+                             M, N, K, kind, _DT[out_dtype], tail, _stream()), "gemm_mxfp4")
+    return out
+
+
+def verify_drafts(logits: torch.Tensor, first: torch.Tensor, drafts: torch.Tensor, draft_logits: Optional[torch.Tensor],
+                  temperature: torch.Tensor, accept_uniform: torch.Tensor, draw_uniform: torch.Tensor,
+                  tokens: Optional[torch.Tensor] = None, accepted: Optional[torch.Tensor] = None):
+    """Which of the drafted tokens stand, and the token behind them: (tokens int32 [rows], accepted int32 [R]).
+
+    Request r owns the rows first[r] .. first[r + 1] - 1 (first int32 [R + 1]) of logits (float32 [rows, V]): one more than it has
+    drafts, row j the model's logits behind j of them.  drafts (int32 [rows - R]), accept_uniform and draft_logits (float32
+    [rows - R, V], what the drafts were drawn from at the request's temperature; None: they were not drawn but looked up) are in
+    the same order, those of request r from first[r] - r on.  With p_j = softmax(logits / temperature[r]) and q_j that of
+    draft_logits (None: all on the draft), draft j is accepted if accept_uniform * q_j(draft) < p_j(draft).  At the first that is
+    not, the token is drawn from max(p_j - q_j, 0), behind the last from p_n: by inverse CDF with draw_uniform[r] in [0, 1), as
+    ``sample`` draws.  temperature <= 0: drafts are accepted as long as they are the largest logit (lowest index on ties), and
+    the token is that.  Weights and sums are 64-bit.
+
+    tokens holds, at the request's rows, the accepted drafts, the token, and -1 behind; rows of no request are not written.
+    Logits of -infinity and NaN weigh nothing; a row where nothing weighs gives the token -1.  A draft outside the vocabulary is
+    not accepted.  accepted[r] is -1 where first[] names rows that there are not."""
+    lib = load_library()
+    _need(logits, "logits", torch.float32, (None, None))
+    rows, V = logits.shape
+    dev = logits.device
+    _need(first, "first", torch.int32, (None,), dev)
+    R = first.shape[0] - 1
+    if R < 0 or rows < R:
+        raise KernelError(f"verify_drafts: {rows} rows of logits for {R} requests")
+    if V == 0:
+        raise KernelError("verify_drafts: a vocabulary of no tokens")
+    D = rows - R
+    _need(drafts, "drafts", torch.int32, (D,), dev)
+    if draft_logits is not None:
+        _need(draft_logits, "draft_logits", torch.float32, (D, V), dev)
+    _need(temperature, "temperature", torch.float32, (R,), dev)
+    _need(accept_uniform, "accept_uniform", torch.float32, (D,), dev)
+    _need(draw_uniform, "draw_uniform", torch.float32, (R,), dev)
+    _on_current_device(logits, "verify_drafts")
+    if tokens is None:
+        tokens = torch.empty((rows,), dtype=torch.int32, device=dev)
+    _need(tokens, "tokens", torch.int32, (rows,), dev)
+    if accepted is None:
+        accepted = torch.empty((R,), dtype=torch.int32, device=dev)
+    _need(accepted, "accepted", torch.int32, (R,), dev)
+    if R == 0:
+        return tokens, accepted
+    nbytes = lib.qe_verify_drafts_workspace_bytes(rows, V, R, int(draft_logits is not None))
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _check(lib.qe_verify_drafts(logits.data_ptr(), first.data_ptr(), drafts.data_ptr(), _ptr(draft_logits), temperature.data_ptr(),
+                                accept_uniform.data_ptr(), draw_uniform.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
+                                rows, V, R, ws.data_ptr(), nbytes, _stream()), "verify_drafts")
+    return tokens, accepted

@@ -1,0 +1,292 @@
+"""Microscaled 4-bit matrices: quantisation against its definition in 64 bits, and the products with them.
+
+Where a product's terms are small whole numbers every order of sums gives the same bits, so that the results are compared
+exactly; others with a bound on the sums: a sum of n terms in 32 bits, each addition cut or rounded, is off by at most
+(n + 8) 2^-23 of the terms' magnitudes (the 8 for the join of the waves' sums), the bias and the stream included among the terms."""
+import math
+
+import pytest
+import torch
+
+import qwen_engine_amd  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from qwen_engine_amd.kernels import ops
+    ops.load_library()
+    return ops
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def codes_of(x):
+    """Codes [T, blocks, 32] and scale bytes [T, blocks] of x by the definition: the nearest of the eight magnitudes, the even code
+    where two are as near."""
+    T, K = x.shape
+    b = torch.nn.functional.pad(x.double(), (0, -K % 32)).view(T, -1, 32)
+    top = b.abs().amax(-1)
+    # a float64's own exponent: exact, also next to powers of two
+    e = torch.frexp(top)[1] - 1 - 2
+    e = torch.where(top > 0, e.clamp(min=-127), torch.full_like(e, -127))
+    bad = ~torch.isfinite(top)
+    e = torch.where(bad, torch.zeros_like(e), e)
+    a = torch.where(bad.unsqueeze(-1), torch.zeros_like(b), b).abs() / torch.exp2(e.double()).unsqueeze(-1)
+    far = (a.clamp(max=6.0).unsqueeze(-1) - GRID).abs()
+    best = far.amin(-1, keepdim=True)
+    near = far == best
+    even = near & (torch.arange(8) % 2 == 0)
+    code = torch.where(even.any(-1), even.int().argmax(-1), near.int().argmax(-1))
+    code = code + 8 * torch.signbit(b)
+    return torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code), torch.where(bad, torch.full_like(e, 255), e + 127)
+
+
+def values_of(code, scale, K):
+    v = torch.cat([GRID, -GRID])[code.long()] * torch.exp2(scale.double() - 127).unsqueeze(-1)
+    v = torch.where((scale == 255).unsqueeze(-1), torch.full_like(v, math.nan), v)
+    return v.reshape(code.shape[0], -1)[:, :K]
+
+
+def unpack(codes):
+    return torch.stack([codes & 15, codes >> 4], -1).view(codes.shape[0], -1, 32)
+
+
+def packed(code):
+    p = code.reshape(code.shape[0], -1, 2)
+    return (p[..., 0] + 16 * p[..., 1]).to(torch.uint8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K", [(1, 1), (1, 32), (3, 31), (5, 33), (7, 64), (2, 100), (65, 96), (1, 4096), (130, 257), (1031, 1000)])
+def test_quantize(ops, dtype, T, K):
+    x = (torch.randn(T, K, generator=gen(1)) * torch.exp2(torch.randint(-20, 20, (T, 1), generator=gen(2)).float())).to(dtype)
+    m = ops.mxfp4_quantize(x.to(DEV))
+    code, scale = codes_of(x)
+    assert m.columns == K and m.codes.shape == (T, (K + 31) // 32 * 16) and m.scales.shape == (T, (K + 31) // 32)
+    assert torch.equal(m.scales.cpu().int(), scale.int())
+    assert torch.equal(unpack(m.codes.cpu()).int(), code.int())
+    for out in (torch.float32, torch.bfloat16):
+        assert torch.equal(ops.mxfp4_values(m, out).double().cpu(), values_of(code, scale, K))
+
+
+def test_quantize_borders(ops):
+    """Ties, the largest code's border, signs of zero, the smallest and largest numbers there are, blocks of zeros, NaN, infinities."""
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.999, 0.2500001, 0.7499999, 4.9999995, 5.0000005, 0.0, -0.0])
+    rows = []
+    for e in (-126, -100, -3, 0, 1, 90, 124):
+        for top in (4.0, 6.0, 7.999):
+            r = torch.cat([ties, -ties]).double() * 2.0 ** e
+            r[0] = top * 2.0 ** e
+            rows.append(r.float())
+    tiny = torch.zeros(32)
+    tiny[:6] = torch.tensor([2.0 ** -149, 2.0 ** -148, -(2.0 ** -128), 2.0 ** -129, 2.0 ** -127, 1.5 * 2.0 ** -127])
+    rows.append(tiny)
+    for top in (2.0 ** -125, 2.0 ** -126, 2.0 ** -127, 1.99 * 2.0 ** -126, 3.4e38):
+        r = torch.linspace(-1, 1, 32) * top
+        rows.append(r)
+    rows.append(torch.zeros(32))
+    rows.append(-torch.zeros(32))
+    for bad in (math.nan, math.inf, -math.inf):
+        r = torch.ones(32)
+        r[17] = bad
+        rows.append(r)
+    x = torch.stack(rows)
+    m = ops.mxfp4_quantize(x.to(DEV))
+    code, scale = codes_of(x)
+    assert torch.equal(m.scales.cpu().int(), scale.int())
+    assert torch.equal(unpack(m.codes.cpu()).int(), code.int())
+    for dtype in (torch.float32, torch.bfloat16):
+        got, want = ops.mxfp4_values(m, dtype).double().cpu(), values_of(code, scale, 32)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+def test_every_code_and_scale(ops):
+    """All 16 codes under all 256 scales stand for what they should, in both types."""
+    code = torch.arange(32).repeat(256, 1, 1) % 16
+    scale = torch.arange(256).view(256, 1)
+    m = ops.MxFp4(packed(code).to(DEV), scale.to(torch.uint8).to(DEV), 32)
+    want = values_of(code, scale, 32)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = ops.mxfp4_values(m, dtype).double().cpu()
+        w = torch.where(want.abs() > torch.finfo(dtype).max, want.sign() * math.inf, want)     # (6 * 2^127 and 4 * 2^127: beyond both types)
+        assert torch.equal(got.isnan(), w.isnan()) and torch.equal(got.nan_to_num(), w.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_at_odd_elements(ops, dtype):
+    """x and the values' place at no whole 16-byte piece; nothing beside the result is written."""
+    buf = torch.randn(1 + 6 * 64, generator=gen(5)).to(dtype).to(DEV)
+    x = buf[1:].view(6, 64)
+    m = ops.mxfp4_quantize(x)
+    code, scale = codes_of(x.cpu())
+    assert torch.equal(unpack(m.codes.cpu()).int(), code.int()) and torch.equal(m.scales.cpu().int(), scale.int())
+
+
+def whole_matrix(N, K, seed):
+    """A 4-bit matrix of whole numbers and halves, junk behind its columns."""
+    blocks = (K + 31) // 32
+    code = torch.randint(0, 16, (N, blocks, 32), generator=gen(seed))
+    scale = torch.randint(127, 129, (N, blocks), generator=gen(seed + 1))
+    return packed(code), scale.to(torch.uint8), values_of(code, scale, K)
+
+
+ROWS = [1, 2, 16, 17, 33, 64, 65, 130, 300]
+SHAPES = [(16, 32), (48, 128), (77, 100), (1, 1), (30, 257), (512, 1024), (300, 992), (20, 4160)]
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M", ROWS)
+def test_product_of_whole_numbers(ops, kind, M):
+    """Every order of sums is exact: the results are equal, whatever the split; in bfloat16 rounded once."""
+    for N, K in SHAPES:
+        codes, scales, v = whole_matrix(N, K, N + K)
+        w = ops.MxFp4(codes.to(DEV), scales.to(DEV), K)
+        if kind == "fp4":
+            xc, xs, xv = whole_matrix(M, K, 7)
+            x = ops.MxFp4(xc.to(DEV), xs.to(DEV), K)
+        else:
+            xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+            x = xv.to(torch.float32 if kind == "float32" else torch.bfloat16).to(DEV)
+        want = xv @ v.T                                        # halves (fp4: quarters) below 2^22: exact in 32 bits
+        got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32).cpu()
+        assert torch.equal(got.double(), want), (N, K)
+        got = ops.gemm_mxfp4(x, w, out_dtype=torch.bfloat16).cpu()
+        assert torch.equal(got, want.float().to(torch.bfloat16)), (N, K)
+        bias = torch.randint(-50, 50, (N,), generator=gen(3)).float()
+        stream = torch.randint(-50, 50, (M, N), generator=gen(4)).float()
+        out = stream.to(DEV)
+        assert ops.gemm_mxfp4(x, w, bias.to(DEV), out=out, epilogue=ops.EPI_RESIDUAL) is out
+        assert torch.equal(out.cpu().double(), want + bias + stream), (N, K)
+
+
+def sums_bound(n, magnitudes):
+    return (n + 8) * 2.0 ** -23 * magnitudes
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M,N,K", [(1, 96, 512), (5, 64, 330), (33, 100, 256), (130, 160, 320), (257, 384, 96)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_silu_and_bias(ops, kind, M, N, K, out_dtype):
+    w_raw = torch.randn(N, K, generator=gen(11)) * 0.2
+    x_raw = torch.randn(M, K, generator=gen(12))
+    w = ops.mxfp4_quantize(w_raw.to(DEV))
+    v = values_of(*codes_of(w_raw), K)
+    if kind == "fp4":
+        x, xv = ops.mxfp4_quantize(x_raw.to(DEV)), values_of(*codes_of(x_raw), K)
+    else:
+        x = x_raw.to(torch.float32 if kind == "float32" else torch.bfloat16)
+        x, xv = x.to(DEV), x.double()
+    bias = torch.randn(N, generator=gen(13))
+    y = xv @ v.T + bias.double()
+    off = sums_bound(3 * K + 1, xv.abs() @ v.abs().T + bias.double().abs())    # (32-bit x: three terms a number)
+    got = ops.gemm_mxfp4(x, w, bias.to(DEV), out_dtype=out_dtype).cpu()
+    half = torch.finfo(out_dtype).eps / 2
+    assert got.dtype == out_dtype
+    assert ((got.double() - y).abs() <= off + half * (y.abs() + off)).all()
+    got = ops.gemm_mxfp4(x, w, bias.to(DEV), out_dtype=out_dtype, epilogue=ops.EPI_SILU_MUL).cpu().double()
+    g, u, og, ou = y[:, :N // 2], y[:, N // 2:], off[:, :N // 2], off[:, N // 2:]
+    want = g * torch.sigmoid(g) * u
+    # silu's slope is at most 1.1; its own arithmetic (an exponential good to 2 units in the last place of its argument's
+    # rounding, a sum, a quotient, a product): at most (4 + |g|) units
+    off = 1.1 * og * (u.abs() + ou) + (g * torch.sigmoid(g)).abs() * ou + (4 + g.abs()) * 2.0 ** -23 * want.abs()
+    assert ((got - want).abs() <= off + half * (want.abs() + off)).all()
+
+
+def test_float32_rows_lose_nothing(ops):
+    """Three numbers a row, of all magnitudes: a product that leaves out any of the 24 bits is off by more than the bound."""
+    M, N, K = 20, 48, 640
+    x = torch.zeros(M, K)
+    for m in range(M):
+        at = torch.randperm(K, generator=gen(m))[:3]
+        x[m, at] = torch.randn(3, generator=gen(100 + m)) * 2.0 ** (m * 6 - 60)
+    w_raw = torch.randn(N, K, generator=gen(21))
+    w = ops.mxfp4_quantize(w_raw.to(DEV))
+    v = values_of(*codes_of(w_raw), K)
+    got = ops.gemm_mxfp4(x.to(DEV), w).cpu().double()
+    assert ((got - x.double() @ v.T).abs() <= sums_bound(9, x.double().abs() @ v.abs().T)).all()
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+def test_nan_and_infinities(ops, kind):
+    """A NaN block of the matrix spoils its own output column and no other; a row with a NaN or an infinity its own row."""
+    M, N, K = 70, 80, 160
+    w_raw = torch.randn(N, K, generator=gen(31)).abs() + 1.0             # (no zeros: infinity stays infinity)
+    w_raw[33, 100] = math.nan
+    x_raw = torch.randn(M, K, generator=gen(32)).abs() + 1.0
+    x_raw[3, 64] = math.nan
+    x_raw[66, 5] = math.inf
+    w = ops.mxfp4_quantize(w_raw.to(DEV))
+    x = ops.mxfp4_quantize(x_raw.to(DEV)) if kind == "fp4" else x_raw.to(getattr(torch, kind)).to(DEV)
+    got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32).cpu()
+    assert got[3].isnan().all() and got[:, 33].isnan().all()
+    if kind == "fp4":
+        assert got[66].isnan().all()
+    else:
+        assert (got[66, torch.arange(N) != 33] == math.inf).all()
+    keep_m, keep_n = [m for m in range(M) if m not in (3, 66)], [n for n in range(N) if n != 33]
+    assert got[keep_m][:, keep_n].isfinite().all()
+
+
+def test_rows_at_odd_elements(ops):
+    """x, bias and out at no whole 16-byte piece; the numbers before and behind out stay."""
+    M, N, K = 19, 40, 96
+    codes, scales, v = whole_matrix(N, K, 3)
+    w = ops.MxFp4(codes.to(DEV), scales.to(DEV), K)
+    for dtype in (torch.bfloat16, torch.float32):
+        xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+        x = torch.zeros(M * K + 1, dtype=dtype, device=DEV)[1:].view(M, K)
+        x.copy_(xv)
+        bias = torch.arange(N + 1, device=DEV, dtype=torch.float32)[1:]
+        hold = torch.full((M * N + 6,), 7.0, dtype=dtype, device=DEV)
+        out = hold[3:3 + M * N].view(M, N)
+        ops.gemm_mxfp4(x, w, bias, out=out)
+        assert torch.equal(out.cpu(), (xv @ v.T + torch.arange(1, N + 1)).float().to(dtype))
+        assert (hold[:3] == 7).all() and (hold[3 + M * N:] == 7).all()
+
+
+def test_no_rows(ops):
+    w = ops.mxfp4_quantize(torch.randn(8, 64, device=DEV))
+    assert ops.gemm_mxfp4(torch.empty(0, 64, device=DEV), w).shape == (0, 8)
+    assert ops.gemm_mxfp4(ops.mxfp4_quantize(torch.empty(0, 64, device=DEV)), w).shape == (0, 8)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M", [1, 20, 100, 260])
+def test_recorded_and_on_another_stream(ops, kind, M):
+    """A recorded quantisation and product replayed on new numbers, twice over, with eager work between; a stream of its own."""
+    N, K = 256, 1024
+    w_raw = torch.randn(N, K, generator=gen(41)).to(DEV)
+    first = torch.randn(M, K, generator=gen(42)).to(DEV)
+    dtype = torch.float32 if kind == "float32" else torch.bfloat16
+
+    def go(x):
+        w = ops.mxfp4_quantize(w_raw)
+        x = x.to(dtype)
+        return ops.gemm_mxfp4(ops.mxfp4_quantize(x) if kind == "fp4" else x, w, out_dtype=torch.float32)
+
+    inputs = [torch.randn(M, K, generator=gen(50 + i)).to(DEV) for i in range(4)]
+    want = [go(x) for x in inputs]
+    static = first.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alone = go(static)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(alone, go(first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = go(static)
+    for _ in range(2):
+        for x, w in zip(inputs, want):
+            static.copy_(x)
+            graph.replay()
+            go(first)
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)

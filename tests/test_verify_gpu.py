@@ -1,0 +1,360 @@
+"""Verification of drafted tokens against a plain implementation in 64 bits, request by request."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import qwen_engine_amd  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from qwen_engine_amd.kernels import ops
+    ops.load_library()
+    return ops
+
+
+def weights(z, t):
+    z = np.where(np.isnan(z), -np.inf, z.astype(np.float64))
+    top = z.max()
+    if top == -np.inf:
+        return np.zeros_like(z)
+    if top == np.inf:
+        e = (z == np.inf).astype(np.float64)
+    else:
+        e = np.where(z == -np.inf, 0.0, np.exp((z - top) / t))
+    return e / e.sum()
+
+
+def pick(w, u):
+    run = np.cumsum(w)
+    if not run[-1] > 0:
+        return -1
+    over = (run > u * run[-1]) & (w > 0)
+    return int(np.argmax(over)) if over.any() else int(np.nonzero(w)[0][-1])
+
+
+def plain(logits, counts, drafts, guess, temperature, accept, draw):
+    tokens, accepted = [], []
+    row = d = 0
+    for r, n in enumerate(counts):
+        t = float(temperature[r])
+        V = logits.shape[1]
+        out = None
+        for j in range(n + 1):
+            z = logits[row + j]
+            if not t > 0:
+                z = np.where(np.isnan(z), -np.inf, z)
+                best = int(np.argmax(z)) if z.max() > -np.inf else -1
+                if j == n or drafts[d + j] != best or best < 0:
+                    out = best
+                    break
+                continue
+            p = weights(z, t)
+            if j == n:
+                out = pick(p, float(draw[r]))
+                break
+            x = int(drafts[d + j])
+            q = np.zeros(V)
+            if guess is not None:
+                q = weights(guess[d + j], t)
+            elif 0 <= x < V:
+                q[x] = 1.0
+            px, qx = (p[x], q[x]) if 0 <= x < V else (0.0, 1.0)
+            if px > 0 and float(accept[d + j]) * qx < px:
+                continue
+            w = np.maximum(p - q, 0.0)
+            out = pick(w if w.sum() > 0 else p, float(draw[r]))
+            break
+        tokens += [int(v) for v in drafts[d:d + j]] + [out] + [-1] * (n - j)
+        accepted.append(j)
+        row += n + 1
+        d += n
+    return tokens, accepted
+
+
+def case(counts, V, seed, spread=2.0, lookup=False, greedy_every=4):
+    g = torch.Generator().manual_seed(seed)
+    rows, R = sum(counts) + len(counts), len(counts)
+    D = rows - R
+    logits = torch.randn(rows, V, generator=g) * spread
+    t = 0.4 + torch.rand(R, generator=g)
+    t[greedy_every - 1::greedy_every] = 0.0
+    drafted = torch.cat([torch.arange(n + 1) < n for n in counts])
+    guess = logits[drafted] + torch.randn(D, V, generator=g)
+    per = t.repeat_interleave(torch.tensor(counts)).unsqueeze(1)
+    noise = torch.rand(D, V, generator=g).clamp(1e-7, 1 - 1e-7)
+    drafts = torch.where(per > 0, guess / per.clamp(min=0.1) - (-noise.log()).log(), logits[drafted]).argmax(1) if D else torch.zeros(0)
+    return dict(logits=logits, counts=counts, drafts=drafts.int(), guess=None if lookup else guess, temperature=t,
+                accept=torch.rand(D, generator=g), draw=torch.rand(R, generator=g))
+
+
+def first_of(counts):
+    return torch.tensor([0] + list(np.cumsum([n + 1 for n in counts])), dtype=torch.int32)
+
+
+def go(ops, c, **more):
+    up = lambda v: None if v is None else v.to(DEV)
+    return ops.verify_drafts(up(c["logits"]), first_of(c["counts"]).to(DEV), up(c["drafts"]), up(c["guess"]), up(c["temperature"]),
+                             up(c["accept"]), up(c["draw"]), **more)
+
+
+def check(ops, c):
+    tokens, accepted = go(ops, c)
+    n = lambda v: None if v is None else v.numpy()
+    want = plain(n(c["logits"]), c["counts"], n(c["drafts"]), n(c["guess"]), n(c["temperature"]), n(c["accept"]), n(c["draw"]))
+    assert accepted.tolist() == want[1]
+    assert tokens.tolist() == want[0]
+    return want
+
+
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("V", [1, 2, 63, 257, 4095, 4096, 4097, 20000, 151936])
+def test_against_64_bits(ops, V, lookup):
+    counts = [3, 0, 1, 5, 2, 0, 4, 7, 1, 1, 0, 2] if V < 100000 else [4, 0, 2, 3]
+    want = check(ops, case(counts, V, V, lookup=lookup))
+    if 63 <= V < 100000:
+        assert len(set(want[1])) > 1
+
+
+def test_one_request(ops):
+    for n in (0, 1, 9):
+        check(ops, case([n], 5000, 70 + n))
+
+
+def test_many_requests(ops):
+    counts = [(i * 5 + i // 7) % 6 for i in range(700)]
+    check(ops, case(counts, 300, 3))
+
+
+def test_flat_distributions(ops):
+    """Nearly equal weights: as many borders of running sums as tokens."""
+    check(ops, case([2, 1, 0, 3, 2, 2, 2, 1], 151936, 8, spread=1e-3, greedy_every=100))
+
+
+def test_same_distribution_accepts_all(ops):
+    """Drafts from the model's own logits stand whatever the numbers are, up to the largest below 1."""
+    c = case([4, 2, 3], 9000, 5, greedy_every=100)
+    drafted = torch.cat([torch.arange(n + 1) < n for n in c["counts"]])
+    c["guess"] = c["logits"][drafted].clone()
+    c["accept"].fill_(1 - 2.0 ** -24)
+    assert check(ops, c)[1] == [4, 2, 3]
+
+
+def test_masks(ops):
+    """Masked tokens, NaN, infinite logits, rows where nothing or one token is left, in the model's and in the drafts' rows."""
+    c = case([2, 2, 2, 2, 2, 2, 2, 2, 1, 0], 5000, 6, greedy_every=100)
+    z, q = c["logits"], c["guess"]
+    z[0, 1000:] = -math.inf                  # the second half of the vocabulary masked
+    z[3] = -math.inf                         # a row where nothing weighs
+    z[6, 10:4990] = math.nan
+    z[9, [17, 4099]] = math.inf              # two infinite ones share everything
+    z[12] = -math.inf
+    z[12, 4500] = -3.0                       # one token left
+    q[8] = -math.inf                         # the draft's own distribution is empty
+    q[10] = math.nan
+    q[12, 5:] = -math.inf
+    z[24:26] = -3e38                         # finite lowest numbers: all alike
+    c["temperature"][9] = 1e-30
+    z[26] = math.nan
+    z[26, 3] = 2.0
+    check(ops, c)
+    for t in (0.0, -1.0):
+        c["temperature"][:] = t
+        check(ops, c)
+    c["temperature"][:] = math.inf
+    z[9] = 0.0                               # (infinite logits at an infinite temperature have no meaning)
+    check(ops, c)
+
+
+def test_greedy_ties_and_drafts_outside(ops):
+    c = case([2, 2, 2, 1], 4200, 9, greedy_every=1)
+    z = c["logits"]
+    z[0, [40, 4150]] = 50.0                  # equal largest ones, in two spans: the lower index
+    z[3, [4150, 4199]] = 50.0
+    c["drafts"][0], c["drafts"][2] = 40, 4199
+    assert check(ops, c)[1][:2] != [0, 2]
+    for bad in (-1, 4200, 2 ** 31 - 1, -2 ** 31):
+        for t in (0.0, 0.8):
+            for guess in (c["guess"], None):
+                d = dict(c, drafts=c["drafts"].clone(), temperature=torch.full((4,), t), guess=guess)
+                d["drafts"][1::2] = bad
+                check(ops, d)
+
+
+def test_numbers_at_the_ends(ops):
+    c = case([3, 1, 0, 2], 4500, 10, greedy_every=100)
+    c["logits"][:, 0] = -math.inf            # the first token weighs nothing, nor the last
+    c["logits"][:, -1] = -math.inf
+    for u in (0.0, 1 - 2.0 ** -24):
+        for a in (0.0, 1 - 2.0 ** -24):
+            c["draw"].fill_(u)
+            c["accept"].fill_(a)
+            check(ops, c)
+    # numbers outside [0, 1) still give a token that weighs something
+    c["accept"].fill_(math.nan)
+    for u in (1.0, 5.0, -1.0, math.nan, math.inf):
+        c["draw"].fill_(u)
+        tokens, accepted = go(ops, c)
+        assert accepted.tolist() == [0, 0, 0, 0]
+        first = first_of(c["counts"])[:-1].tolist()
+        assert all(0 < tokens[i] < 4499 for i in first)
+
+
+def test_rows_of_no_request_and_bad_rows(ops):
+    """What no request owns stays as it was; a request whose rows are not there is marked, and the others are served."""
+    c = case([2, 1, 3], 600, 11)
+    want = plain(*(v.numpy() if isinstance(v, torch.Tensor) else v for v in (c["logits"], c["counts"], c["drafts"], c["guess"],
+                                                                             c["temperature"], c["accept"], c["draw"])))
+    pad = dict(c, logits=torch.cat([c["logits"], torch.zeros(4, 600)]), drafts=torch.cat([c["drafts"], torch.full((4,), 77, dtype=torch.int32)]),
+               guess=torch.cat([c["guess"], torch.zeros(4, 600)]), accept=torch.cat([c["accept"], torch.zeros(4)]))
+    tokens = torch.full((13,), 99, dtype=torch.int32, device=DEV)
+    tokens, accepted = go(ops, pad, tokens=tokens)
+    assert tokens.tolist() == want[0] + [99] * 4 and accepted.tolist() == want[1]
+    for first, good in (([0, 3, 5, 40], [0, 1]), ([0, 3, 2, 9], [0]), ([-4, 3, 5, 9], [1, 2]), ([0, 3, 5, 5], [0, 1]),
+                        ([9, 9, 9, 9], []), ([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 0], [])):
+        up = lambda v: v.to(DEV)
+        tokens = torch.full((9,), 99, dtype=torch.int32, device=DEV)
+        tokens, accepted = ops.verify_drafts(up(c["logits"]), up(torch.tensor(first, dtype=torch.int32)), up(c["drafts"]), up(c["guess"]),
+                                             up(c["temperature"]), up(c["accept"]), up(c["draw"]), tokens=tokens)
+        got = accepted.tolist()
+        for r in good:
+            assert got[r] == want[1][r], (first, r)
+        if not good:
+            assert got == [-1, -1, -1] and (tokens == 99).all()
+
+
+def test_no_requests(ops):
+    e = lambda *s, dtype=torch.float32: torch.empty(*s, dtype=dtype, device=DEV)
+    tokens, accepted = ops.verify_drafts(e(0, 50), torch.zeros(1, dtype=torch.int32, device=DEV), e(0, dtype=torch.int32), None, e(0), e(0), e(0))
+    assert tokens.shape == (0,) and accepted.shape == (0,)
+
+
+@pytest.mark.parametrize("lookup", [False, True])
+def test_tokens_are_distributed_as_the_models(ops, lookup):
+    """20 000 requests with one draft each from another distribution: the first token's frequencies are the model's.  A count of n
+    trials with probability p is within 5 sqrt(n p (1 - p)) + 5 of n p but once in a million."""
+    R, V = 20000, 12
+    g = torch.Generator().manual_seed(1)
+    p_row, q_row = torch.randn(V, generator=g) * 1.5, torch.randn(V, generator=g)
+    q = torch.softmax(q_row.double(), 0)
+    drafts = torch.multinomial(q, R, replacement=True, generator=g).int() if not lookup else torch.randint(0, 3, (R,), generator=g).int()
+    rows = p_row.repeat(2 * R, 1)
+    first = torch.arange(0, 2 * R + 1, 2, dtype=torch.int32)
+    tokens, _ = ops.verify_drafts(rows.to(DEV), first.to(DEV), drafts.to(DEV), None if lookup else q_row.repeat(R, 1).to(DEV),
+                                  torch.ones(R, device=DEV), torch.rand(R, generator=g).to(DEV), torch.rand(R, generator=g).to(DEV))
+    counts = torch.bincount(tokens[::2].cpu().long(), minlength=V).double()
+    p = torch.softmax(p_row.double(), 0)
+    assert ((counts - R * p).abs() <= 5 * (R * p * (1 - p)).sqrt() + 5).all()
+
+
+def test_recorded_and_on_another_stream(ops):
+    cs = [case([2, 0, 4, 1], 9001, 20 + i) for i in range(4)]
+    up = lambda v: v.to(DEV)
+    names = ("logits", "drafts", "guess", "temperature", "accept", "draw")
+    static = {k: up(cs[0][k]).clone() for k in names}
+    first = first_of([2, 0, 4, 1]).to(DEV)
+
+    def run(s):
+        return ops.verify_drafts(s["logits"], first, s["drafts"], s["guess"], s["temperature"], s["accept"], s["draw"])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alone = run(static)
+    torch.cuda.current_stream().wait_stream(side)
+    want = [run({k: up(c[k]) for k in names}) for c in cs]
+    assert torch.equal(alone[0], want[0][0]) and torch.equal(alone[1], want[0][1])
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(static)
+        graphs.append((graph, out))
+    for _ in range(2):
+        for c, w in zip(cs, want):
+            for k in names:
+                static[k].copy_(up(c[k]))
+            for graph, out in graphs:
+                graph.replay()
+            run({k: up(cs[1][k]) for k in names})
+            torch.cuda.synchronize()
+            for graph, out in graphs:
+                assert torch.equal(out[0], w[0]) and torch.equal(out[1], w[1])
+
+
+def test_sampler_verify(ops):
+    from qwen_engine_amd.sampling.sampler import Sampler
+    c = case([2, 0, 3], 700, 30)
+    flat, acc = c["drafts"].tolist(), c["accept"].tolist()
+    drafts, accept = [flat[:2], [], flat[2:]], [acc[:2], [], acc[2:]]
+    got = Sampler().verify(c["logits"].to(DEV), drafts, c["guess"].to(DEV), c["temperature"].tolist(), accept, c["draw"].tolist())
+    tokens, accepted = go(ops, c)
+    tokens, accepted = tokens.tolist(), accepted.tolist()
+    want = [tokens[lo:lo + n + 1] for lo, n in zip((0, 3, 4), accepted)]
+    assert got == want
+    assert Sampler().verify(torch.empty(0, 700, device=DEV), [], None, [], [], []) == []
+    with pytest.raises(ValueError):
+        Sampler().verify(c["logits"].to(DEV), drafts, None, [1.0, 1.0], accept, [0.5, 0.5, 0.5])
+    with pytest.raises(ValueError):
+        Sampler().verify(c["logits"].to(DEV), [[1], [], [2]], None, [1.0] * 3, [[0.1], [], [0.1]], [0.5] * 3)
+
+
+def test_drafting_with_a_4_bit_copy(ops):
+    """The operators together: a small model's matrices in 4 bits draft tokens that its own matrices verify; at temperature 0
+    the tokens are those of the model alone, whatever the copy proposes, and some drafts stand."""
+    from qwen_engine_amd.sampling.sampler import Sampler, uniform_for
+    g = torch.Generator().manual_seed(4)
+    V, H, I, R, n = 500, 128, 256, 3, 4
+    table, up, down, head = (torch.randn(*s, generator=g).to(torch.bfloat16).to(DEV) * k
+                             for s, k in (((V, H), 1.0), ((2 * I, H), 0.15), ((H, I), 0.15), ((V, H), 0.3)))
+    held = {k: ops.mxfp4_quantize(w.contiguous()) for k, w in (("up", up), ("down", down), ("head", head))}
+
+    def model(ids, four):
+        h = ops.embedding(torch.tensor(ids, dtype=torch.int32, device=DEV), table)
+        x = h.to(torch.bfloat16)
+        if four:
+            y = ops.gemm_mxfp4(x, held["up"], epilogue=ops.EPI_SILU_MUL)
+            ops.gemm_mxfp4(y, held["down"], out=h, epilogue=ops.EPI_RESIDUAL)
+            return ops.gemm_mxfp4(h.to(torch.bfloat16), held["head"], out_dtype=torch.float32)
+        y = ops.silu_mul(ops.gemm(x, up))
+        ops.residual_add(h, ops.gemm(y, down))
+        return ops.gemm(h.to(torch.bfloat16), head, out_dtype=torch.float32)
+
+    sampler = Sampler()
+
+    def run(temperatures, steps):
+        out, stood = [[5 + r] for r in range(R)], 0
+        for _ in range(steps):
+            drafts, rows = [[] for _ in range(R)], []
+            last = [o[-1] for o in out]
+            for j in range(n):
+                z = model(last, True)
+                rows.append(z)
+                last = sampler.sample(z, temperatures, [uniform_for(1, r, len(out[r]) + j) for r in range(R)])
+                for r in range(R):
+                    drafts[r].append(last[r])
+            logits = model([t for r in range(R) for t in [out[r][-1]] + drafts[r]], False)
+            guess = torch.stack(rows, 1).reshape(R * n, V)
+            accept = [[uniform_for(1, r, len(out[r]) + j, "accept") for j in range(n)] for r in range(R)]
+            got = sampler.verify(logits, drafts, guess, temperatures, accept, [uniform_for(1, r, len(out[r]), "draw") for r in range(R)])
+            stood += sum(len(t) - 1 for t in got)
+            for r in range(R):
+                out[r] += got[r]
+        return out, stood
+
+    out, stood = run([0.0] * R, 6)
+    assert stood > 0
+    for o in out:
+        for a, b in zip(o, o[1:]):
+            z = model([a], False)
+            row = z[0].double().cpu()
+            # (the verifying step multiplies more rows at a time: a near tie may fall the other way)
+            assert float(row.max() - row[b]) <= 2e-2 * float(row.abs().max())
+    out, stood = run([0.8, 0.0, 1.2], 6)
+    assert stood > 0 and all(0 <= t < V for o in out for t in o)
