@@ -6,75 +6,7 @@
 // bfloat16 x the codes become bfloat16 in registers (an instruction for two of them, the scale included) and v_mfma_f32_16x16x32_bf16
 // sums in 32-bit.  Numbers of 32-bit x are cut into three bfloat16 (8 + 8 + 8 bits, exact) and multiplied by three instructions.  With
 // both sides in 4 bits the codes go to v_mfma_scale_f32_16x16x128_f8f6f4 as they are.
-#include "common.h"
-
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-typedef __attribute__((ext_vector_type(4))) float floatx4_t;
-typedef __attribute__((ext_vector_type(4))) unsigned int uintx4_t;
-typedef __attribute__((ext_vector_type(8))) int intx8_t;
-
-enum { X_BF16 = 0, X_F32 = 1, X_FP4 = 2 };
-enum { TAIL_STORE = 0, TAIL_ADD = 1, TAIL_SILU = 2 };
-
-// Eight codes with their block's scale as eight bfloat16.
-__device__ __forceinline__ bf16x8_t fp4_to_bf16(uint32_t c, float scale) {
-    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1);
-    const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3);
-    bf16x8_t r;
-    r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1]; r[4] = d[0]; r[5] = d[1]; r[6] = e[0]; r[7] = e[1];
-    return r;
-}
-
-// v = hi + mid + lo, each of at most 8 significant bits (cut, not rounded: nothing overflows); an infinity or a NaN stays in hi alone.
-__device__ __forceinline__ void cut_in_three(float v, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
-    const uint32_t b = __float_as_uint(v);
-    hi = (uint16_t)(b >> 16);
-    mid = lo = 0;
-    if ((b & 0x7f800000u) == 0x7f800000u) {
-        if (b & 0x007fffffu) hi = 0x7fc0;
-        return;
-    }
-    const float r = v - __uint_as_float(b & 0xffff0000u);
-    const uint32_t c = __float_as_uint(r);
-    mid = (uint16_t)(c >> 16);
-    lo = (uint16_t)(__float_as_uint(r - __uint_as_float(c & 0xffff0000u)) >> 16);
-}
-
-// The codes of a block of which only the first n numbers count (n < 32): the others 0.
-__device__ __forceinline__ uintx4_t first_codes(uintx4_t c, int n) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int here = n - 8 * j;
-        if (here < 8) c[j] &= here <= 0 ? 0u : (1u << (4 * here)) - 1u;
-    }
-    return c;
-}
-
-struct Fp4Args {
-    const void* x;                  // rows of x (X_FP4: their codes)
-    const unsigned char* xs;        // X_FP4: their scales
-    const unsigned char* codes;     // [N, blocks * 16]
-    const unsigned char* scales;    // [N, blocks]
-    const float* bias;              // [N] or null
-    void* out;
-    int M, N, K, blocks;            // blocks = ceil(K / 32)
-    int out_f32;
-};
-
-// What becomes of a sum: row m, column n (silu: gate and up of column n of N / 2).
-template <int TAIL>
-__device__ __forceinline__ void fp4_store(const Fp4Args& a, long m, int n, float v, float up) {
-    if (a.bias) {
-        v += a.bias[n];
-        if constexpr (TAIL == TAIL_SILU) up += a.bias[a.N / 2 + n];
-    }
-    const long at = m * (TAIL == TAIL_SILU ? a.N / 2 : a.N) + n;
-    if constexpr (TAIL == TAIL_SILU) v = v / (1.f + expf(-v)) * up;
-    if constexpr (TAIL == TAIL_ADD) ((float*)a.out)[at] += v;
-    else if (a.out_f32) ((float*)a.out)[at] = v;
-    else ((bf16_t*)a.out)[at] = float_to_bf16(v);
-}
+#include "mxfp4.h"
 
 // A block of NW waves: MT tiles of 16 rows of x against 16 columns (silu: 16 of gate and the same 16 of up).  Its waves take steps of
 // four blocks of K in turn and their sums are added in the order of the waves.
@@ -220,11 +152,22 @@ static void fp4_launch(const Fp4Args& a, hipStream_t stream) {
     else fp4_rows_launch<X, TAIL, 4, WHOLE>(a, stream);
 }
 
+static bool fp4_by_tiles(int M, int N, int K, int x_kind) {
+    return x_kind != X_FP4 && M > 64 && fp4_tiles_take(M, N, K, x_kind);
+}
+
+// Bytes of workspace that qe_gemm_mxfp4 needs for these operands.
+extern "C" long qe_gemm_mxfp4_workspace_bytes(const void* x, const void* scales, int M, int N, int K, int x_kind) {
+    if (M <= 0 || N <= 0 || K <= 0 || !fp4_by_tiles(M, N, K, x_kind)) return 0;
+    return fp4_tiles_workspace(M, N, K, x_kind, (((uintptr_t)x & 15) | ((uintptr_t)scales & 3)) == 0);
+}
+
 // x: [M, K] bfloat16 (x_kind 0) or float32 (1), or the codes of x in 4 bits with their scales x_scales (2); codes [N, ceil(K / 32) * 16],
 // scales [N, ceil(K / 32)]; out [M, N] (silu: [M, N / 2], gate rows of the matrix first, then up rows); tail: 0 store, 1 add into out
 // (float32), 2 silu(gate) * up.
 extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* codes, const void* scales, const float* bias, void* out,
-                             int M, int N, int K, int x_kind, int out_dtype, int tail, hipStream_t stream) {
+                             int M, int N, int K, int x_kind, int out_dtype, int tail, void* workspace, long workspace_bytes,
+                             hipStream_t stream) {
     QE_REQUIRE(M >= 0 && N > 0 && K > 0, "gemm_mxfp4: bad sizes M=%d N=%d K=%d", M, N, K);
     QE_REQUIRE(x_kind >= 0 && x_kind <= 2 && tail >= 0 && tail <= 2, "gemm_mxfp4: unknown form");
     QE_REQUIRE(out_dtype == QE_F32 || out_dtype == QE_BF16, "gemm_mxfp4: unknown element type %d", out_dtype);
@@ -236,6 +179,9 @@ extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* co
     if (M == 0) return 0;
     const Fp4Args a{x, (const unsigned char*)x_scales, (const unsigned char*)codes, (const unsigned char*)scales, bias, out, M, N, K,
                     qe_cdiv(K, 32), out_dtype == QE_F32};
+    const long need = qe_gemm_mxfp4_workspace_bytes(x, scales, M, N, K, x_kind);
+    QE_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need), "gemm_mxfp4: workspace too small");
+    if (fp4_by_tiles(M, N, K, x_kind)) return fp4_tiles(a, x_kind, tail, workspace, stream);
     // whole blocks of 16-byte pieces of x
     const bool whole = K % 32 == 0 && ((uintptr_t)x & 15) == 0;
 #define QE_TAILS(X_, W_)                                                          \

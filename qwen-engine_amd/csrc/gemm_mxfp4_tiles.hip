@@ -1,0 +1,342 @@
+// Products of many rows of 16-bit or 32-bit numbers with a 4-bit matrix (see mxfp4.h): out[M, N] = x[M, K] . V[N, K]^T.
+//
+// A block of WR x WC waves computes BM rows by BN columns.  K is walked in stages of 128 through a ring in shared memory: 256 bytes of a
+// row of x, 64 of codes and 4 of scales of a row of the matrix, brought by loads that write to shared memory directly.  A
+// wave multiplies its part in tiles of 32 x 32 with v_mfma_f32_32x32x16_bf16: lane (r, h) = (lane % 32, lane / 32) takes, of row r,
+// block 2 b + h of the stage's four, so that a 16-byte piece of codes with one scale gives four matrix instructions' operands, eight numbers
+// each, by four conversions each.  The conversions for the next k step stand between the matrix instructions of this one.
+//
+// Rows of 32-bit numbers come as three planes of bfloat16 (cut_in_three) that are walked one after the other, the smallest
+// first, against the same matrix; they are made by a launch of their own, which also fills K up to whole stages.
+#include "mxfp4.h"
+
+#define FP4_STAGE 128      // numbers of K
+
+// x [M, K] float32 -> planes [3][M][Kp] (low, middle, high) of bfloat16, zeros from K on; bfloat16 -> [M][Kp]
+template <typename T>
+__global__ __launch_bounds__(256) void fp4_planes_kernel(const T* __restrict__ x, uint16_t* __restrict__ planes, int M, int K, int Kp) {
+    const long plane = (long)M * Kp;
+    for (long row = blockIdx.y; row < M; row += gridDim.y) {
+        const int k = (blockIdx.x * 256 + threadIdx.x) * 4;
+        if (k >= Kp) return;
+        uint16_t hi[4], mid[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool have = k + e < K;
+            if constexpr (sizeof(T) == 4) cut_in_three(have ? x[row * K + k + e] : 0.f, hi[e], mid[e], lo[e]);
+            else hi[e] = have ? x[row * K + k + e].bits : 0;
+        }
+        uint16_t* to = planes + row * Kp + k;
+        if constexpr (sizeof(T) == 4) {
+            *(ushort4*)to = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+            *(ushort4*)(to + plane) = make_ushort4(mid[0], mid[1], mid[2], mid[3]);
+            *(ushort4*)(to + 2 * plane) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        } else {
+            *(ushort4*)to = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        }
+    }
+}
+
+// scales [N, blocks] -> [N, padded], zeros behind
+__global__ __launch_bounds__(256) void fp4_scales_kernel(const unsigned char* __restrict__ scales, uint32_t* __restrict__ out, int N,
+                                                         int blocks, int words) {
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (long)N * words) return;
+    const long row = at / words;
+    const int b = (int)(at - row * words) * 4;
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (b + e < blocks) v |= (uint32_t)scales[row * blocks + b + e] << (8 * e);
+    out[at] = v;
+}
+
+struct Fp4Tiles {
+    Fp4Args a;
+    const uint16_t* planes;     // rows of x, row_bytes apart, plane after plane
+    const uint32_t* words;      // the scales, `words` words a row
+    unsigned row_bytes, plane_bytes, x_bytes;      // (x_bytes: of all planes)
+    int num_planes, nk, num_words;
+    int tiles_m, tiles_n;
+};
+
+template <int TAIL, int BM, int BN, int WR, int WC, int RING>
+__global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) {
+    constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, MI = WM / 32, NJ = WN / 32;
+    constexpr int LDA = BM / (4 * NW), LDB = BN / (16 * NW), LD = LDA + LDB + 1, SROWS = BN / NW;
+    constexpr int B_AT = BM * 256, S_AT = B_AT + BN * 64, STAGE = S_AT + NW * 256;
+    static_assert(BM % (4 * NW) == 0 && BN % (16 * NW) == 0 && SROWS <= 64 && (RING - 1) * LD + 4 < 64 && MI * NJ >= 2, "whole loads of every wave");
+    static_assert(TAIL != TAIL_SILU || NJ % 2 == 0, "a wave has the gate and the up of its columns");
+    constexpr int PER_STEP = (LD + 7) / 8;                 // loads of a k step
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const Fp4Args& a = t.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+
+    // Every eighth block goes to the same XCD, which has an L2 of its own: it takes an eighth of a walk through the tiles in bands of 8
+    // tile rows, column by column, so that what it runs at a time shares rows of x and of the matrix.
+    int tile_m, tile_n;
+    {
+        const int all = t.tiles_m * t.tiles_n, each = all / 8, over = all % 8, xcd = blockIdx.x % 8;
+        int local = blockIdx.x / 8;
+        if (local >= each + (xcd < over)) return;
+        local += xcd * each + min(xcd, over);
+        const int band = local / (8 * t.tiles_n), within = local - band * 8 * t.tiles_n, rows = min(8, t.tiles_m - band * 8);
+        tile_m = band * 8 + within % rows;
+        tile_n = within / rows;
+    }
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
+    const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+
+    // the loads: per lane the bytes within x (from row m0), the codes and the scales; beyond the matrix: out of range, which arrives as zero
+    constexpr int OUT = 0x7fffffff;
+    int va[LDA], vb[LDB], vs;
+#pragma unroll
+    for (int i = 0; i < LDA; ++i) {
+        const int row = (i * NW + wave) * 4 + (lane >> 4);
+        va[i] = m0 + row < a.M ? row * (int)t.row_bytes + ((lane & 15) ^ (row & 15)) * 16 : OUT;
+    }
+    // row i of the tile's columns: silu: blocks of 32, gate and up in turn
+    auto matrix_row = [&](int i) {
+        if constexpr (TAIL == TAIL_SILU) {
+            const int n = n0 / 2 + (i >> 6) * 32 + (i & 31);
+            return n < wide ? ((i >> 5) & 1) * wide + n : -1;
+        } else {
+            return n0 + i < wide ? n0 + i : -1;
+        }
+    };
+    int piece[LDB];                                        // the block of the stage that this lane brings
+#pragma unroll
+    for (int i = 0; i < LDB; ++i) {
+        const int line = (i * NW + wave) * 8 + (lane >> 3), idx = (lane & 7) ^ (line & 7);
+        const int row = matrix_row(line * 2 + (idx >> 2));
+        piece[i] = row >= 0 ? idx & 3 : 1 << 28;
+        vb[i] = row * (a.blocks * 16) + (idx & 3) * 16;
+    }
+    {
+        const int row = lane < SROWS ? matrix_row(wave * SROWS + lane) : -1;
+        vs = row >= 0 ? row * (t.num_words * 4) : OUT;
+    }
+    uintx4_t rsrc_a, rsrc_b, rsrc_s;
+    const unsigned long x_at = (unsigned long)t.planes + (unsigned long)m0 * t.row_bytes, b_at = (unsigned long)a.codes, s_at = (unsigned long)t.words;
+    rsrc_a[0] = (unsigned)x_at; rsrc_a[1] = (unsigned)(x_at >> 32) & 0xffffu; rsrc_a[2] = t.x_bytes - (unsigned)m0 * t.row_bytes; rsrc_a[3] = 0x00020000u;
+    rsrc_b[0] = (unsigned)b_at; rsrc_b[1] = (unsigned)(b_at >> 32) & 0xffffu; rsrc_b[2] = (unsigned)((long)a.N * a.blocks * 16); rsrc_b[3] = 0x00020000u;
+    rsrc_s[0] = (unsigned)s_at; rsrc_s[1] = (unsigned)(s_at >> 32) & 0xffffu; rsrc_s[2] = (unsigned)((long)a.N * t.num_words * 4); rsrc_s[3] = 0x00020000u;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        rsrc_a[c] = __builtin_amdgcn_readfirstlane(rsrc_a[c]);
+        rsrc_b[c] = __builtin_amdgcn_readfirstlane(rsrc_b[c]);
+        rsrc_s[c] = __builtin_amdgcn_readfirstlane(rsrc_s[c]);
+    }
+    const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
+    // the stage that is being asked for: its place in the ring, its plane's bytes and its step along K (t.nk: none is left)
+    int ask_k = 0, ask_plane = 0;
+    unsigned ask_x = 0, ask_at = lds0;
+#define LOAD_PIECE(i_)                                                                                                    \
+    {                                                                                                                     \
+        const bool there = ask_plane < t.num_planes;                                                                      \
+        if ((i_) < LDA) {                                                                                                 \
+            const int v_ = there ? va[(i_) < LDA ? (i_) : 0] : OUT;                                                       \
+            QE_LOAD_TO_SHARED(ask_at + ((i_) * NW + wave_s) * 1024, v_, rsrc_a, there ? ask_x + ask_k * 256 : 0, "0", ""); \
+        } else if ((i_) < LDA + LDB) {                                                                                    \
+            constexpr int b_ = (i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0;                                        \
+            const int v_ = there && ask_k * 4 + piece[b_] < a.blocks ? vb[b_] : OUT;                                      \
+            QE_LOAD_TO_SHARED(ask_at + B_AT + (b_ * NW + wave_s) * 1024, v_, rsrc_b, ask_k * 64, "0", "");                \
+        } else {                                                                                                          \
+            const int v_ = there ? vs : OUT;                                                                              \
+            asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"                                              \
+                         : : "{m0}"(ask_at + S_AT + wave_s * 256), "v"(v_), "s"(rsrc_s), "s"(ask_k * 4) : "memory");      \
+        }                                                                                                                 \
+    }
+#define ASKED()                                                                                                           \
+    {                                                                                                                     \
+        ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE;                                           \
+        if (++ask_k == t.nk) { ask_k = 0; ++ask_plane; ask_x += t.plane_bytes; }                                          \
+    }
+    // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
+#define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
+
+    // where a lane reads: of x its piece of k step q, of the codes its block of pair b, of the scales its row's word
+    int fa_at[8], fb_at[2], fs_at;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) fa_at[q] = (wm + r) * 256 + ((((q >> 2) * 8 + (q & 3)) ^ (h * 4) ^ (r & 15)) * 16);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int row = wn + r, line = row >> 1;
+        fb_at[b] = B_AT + line * 128 + ((((row & 1) * 4 + 2 * b + h) ^ (line & 7)) * 16);
+    }
+    floatx16_t acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    bf16x8_t fa[4][MI], fb[2][NJ];
+    uintx4_t code[2][NJ];
+    uint32_t word[NJ], word_next[NJ];
+#define READ_A(q_, place_) _Pragma("unroll") for (int i = 0; i < MI; ++i) fa[(q_) & 3][i] = *(const bf16x8_t*)(smem + (place_) + fa_at[(q_) & 7] + i * 8192);
+#define READ_CODES(b_, place_) _Pragma("unroll") for (int j = 0; j < NJ; ++j) code[b_][j] = *(const uintx4_t*)(smem + (place_) + fb_at[b_] + j * 2048);
+#define READ_SCALES(place_)                                                                                               \
+    _Pragma("unroll") for (int j = 0; j < NJ; ++j) {                                                                      \
+        const int row = wn + j * 32 + r;                                                                                  \
+        word_next[j] = *(const uint32_t*)(smem + (place_) + S_AT + (row / SROWS) * 256 + (row % SROWS) * 4);              \
+    }
+#define EXPAND(q_, j_) fb[(q_) & 1][j_] = fp4_to_bf16(code[((q_) >> 2) & 1][j_][(q_) & 3], __uint_as_float((word[j_] >> (((((q_) >> 2) & 1) * 2 + h) * 8) & 255u) << 23));
+    // k step q_: between its matrix instructions the fragments of x of the step after the next are read, the next step's codes expanded, and the
+    // loads of the stage that is being asked for go out, from the step behind the barrier on
+#define K_STEP(q_, place_, next_)                                                                                         \
+    {                                                                                                                     \
+        if ((q_) < 6) { READ_A((q_) + 2, place_) } else { READ_A((q_) - 6, next_) }                                       \
+        if ((q_) == 1) { READ_CODES(1, place_) }                                                                          \
+        if ((q_) == 6) { READ_CODES(0, next_) READ_SCALES(next_) }                                                        \
+        if ((q_) == 7) { _Pragma("unroll") for (int j = 0; j < NJ; ++j) word[j] = word_next[j]; }                         \
+        _Pragma("unroll") for (int sl = 0; sl < MI * NJ; ++sl) {                                                          \
+            acc[sl % MI][sl / MI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[(q_) & 3][sl % MI], fb[(q_) & 1][sl / MI], acc[sl % MI][sl / MI], 0, 0, 0); \
+            if (sl % MI == 0) { EXPAND(((q_) + 1) & 7, sl / MI) }                                                         \
+            if (sl < PER_STEP) LOADS_OF((((q_) + 2) & 7) * PER_STEP + sl)                                                 \
+            __builtin_amdgcn_sched_barrier(0);                                                                            \
+        }                                                                                                                 \
+        if ((q_) == 5) { ASKED() MEET((RING - 2) * LD) }                                                                  \
+    }
+#define LOADS_OF(n_)                                                                                                      \
+    switch (n_) {                                                                                                         \
+        case 0: LOAD_CASE(0) case 1: LOAD_CASE(1) case 2: LOAD_CASE(2) case 3: LOAD_CASE(3) case 4: LOAD_CASE(4)          \
+        case 5: LOAD_CASE(5) case 6: LOAD_CASE(6) case 7: LOAD_CASE(7) case 8: LOAD_CASE(8) case 9: LOAD_CASE(9)          \
+        case 10: LOAD_CASE(10) case 11: LOAD_CASE(11) case 12: LOAD_CASE(12) case 13: LOAD_CASE(13) case 14: LOAD_CASE(14) \
+        case 15: LOAD_CASE(15) default: break;                                                                            \
+    }
+#define LOAD_CASE(i_) if constexpr ((i_) < LD) LOAD_PIECE(i_) break;
+    static_assert(LD <= 16 && PER_STEP <= MI * NJ, "a case for every load, a slot for every load of a step");
+
+    constexpr int HEAD = 2 * PER_STEP < LD ? 2 * PER_STEP : LD;          // of a stage's loads, those that go out in the two steps behind the barrier
+#pragma unroll
+    for (int s = 0; s < RING; ++s) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i)
+            if (s + 1 < RING || i < HEAD) { LOADS_OF(i) }
+        if (s + 1 < RING) ASKED()
+    }
+    MEET((RING - 2) * LD + HEAD)
+    READ_CODES(0, 0)
+    READ_SCALES(0)
+    READ_A(0, 0)
+    READ_A(1, 0)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) word[j] = word_next[j];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) { EXPAND(0, j) }
+    const int stages = t.nk * t.num_planes;
+    int at = 0;
+    for (int st = 0; st < stages; ++st) {
+        const int next = at + STAGE == RING * STAGE ? 0 : at + STAGE;
+        K_STEP(0, at, next)
+        K_STEP(1, at, next)
+        K_STEP(2, at, next)
+        K_STEP(3, at, next)
+        K_STEP(4, at, next)
+        K_STEP(5, at, next)
+        K_STEP(6, at, next)
+        K_STEP(7, at, next)
+        at = next;
+    }
+    MEET(0)                                                // (what was asked for beyond the end has arrived)
+#undef K_STEP
+#undef LOADS_OF
+#undef LOAD_CASE
+#undef LOAD_PIECE
+#undef ASKED
+#undef MEET
+#undef READ_A
+#undef READ_CODES
+#undef READ_SCALES
+#undef EXPAND
+
+    // lane (r, h) has column r of a tile, its rows 8 b + 4 h + e
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const long m = m0 + wm + i * 32 + 8 * (e / 4) + 4 * h + e % 4;
+            if (m >= a.M) continue;
+            if constexpr (TAIL == TAIL_SILU) {
+#pragma unroll
+                for (int j = 0; j < NJ; j += 2) {
+                    const int n = n0 / 2 + (wn + j * 32) / 2 + r;
+                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], acc[i][j + 1][e]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = n0 + wn + j * 32 + r;
+                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], 0.f);
+                }
+            }
+        }
+}
+
+template <int TAIL, int BM, int BN, int WR, int WC, int RING>
+static int fp4_tiles_launch(Fp4Tiles t, hipStream_t stream) {
+    constexpr int NW = WR * WC, SHARED = RING * (BM * 256 + BN * 64 + NW * 256);
+    t.tiles_m = qe_cdiv(t.a.M, BM);
+    t.tiles_n = qe_cdiv(t.a.N, BN);
+    const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
+    QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
+    QE_RAISE_SHARED((fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING>), SHARED);
+    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING><<<(unsigned)blocks, 64 * NW, SHARED, stream>>>(t);
+    return 0;
+}
+
+static int padded(int K) { return qe_cdiv(K, FP4_STAGE) * FP4_STAGE; }
+
+// The kernel's 32-bit places reach all of the operands.
+bool fp4_tiles_take(int M, int N, int K, int x_kind) {
+    return (long)N * padded(K) / 2 < (1L << 31) && (long)M * padded(K) * 2 * (x_kind == X_F32 ? 3 : 1) < (1L << 31);
+}
+
+long fp4_tiles_workspace(int M, int N, int K, int x_kind, bool aligned) {
+    long bytes = 0;
+    if (x_kind == X_F32) bytes += 6L * M * padded(K);
+    else if (K % FP4_STAGE || !aligned) bytes += 2L * M * padded(K);
+    if (K % FP4_STAGE || !aligned) bytes += (long)N * (padded(K) / 32);
+    return bytes;
+}
+
+int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
+    Fp4Tiles t{};
+    t.a = a;
+    const int Kp = padded(a.K);
+    t.nk = Kp / FP4_STAGE;
+    t.num_words = Kp / FP4_STAGE;
+    t.num_planes = x_kind == X_F32 ? 3 : 1;
+    t.row_bytes = (unsigned)Kp * 2;
+    t.plane_bytes = (unsigned)((long)a.M * Kp * 2);
+    t.x_bytes = t.plane_bytes * t.num_planes;
+    unsigned char* ws = (unsigned char*)workspace;
+    const dim3 grid(qe_cdiv(Kp, 1024), a.M < 65535 ? a.M : 65535);
+    if (x_kind == X_F32) {
+        fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
+        t.planes = (const uint16_t*)ws;
+        ws += t.x_bytes;
+    } else if (a.K % FP4_STAGE || ((uintptr_t)a.x & 15)) {
+        fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
+        t.planes = (const uint16_t*)ws;
+        ws += t.x_bytes;
+    } else {
+        t.planes = (const uint16_t*)a.x;
+    }
+    if (a.K % FP4_STAGE || ((uintptr_t)a.scales & 3)) {
+        fp4_scales_kernel<<<qe_cdiv((long)a.N * t.num_words, 256), 256, 0, stream>>>(a.scales, (uint32_t*)ws, a.N, a.blocks, t.num_words);
+        t.words = (const uint32_t*)ws;
+    } else {
+        t.words = (const uint32_t*)a.scales;
+    }
+    int rc;
+    if (tail == TAIL_STORE) rc = fp4_tiles_launch<TAIL_STORE, 128, 128, 2, 2, 3>(t, stream);
+    else if (tail == TAIL_ADD) rc = fp4_tiles_launch<TAIL_ADD, 128, 128, 2, 2, 3>(t, stream);
+    else rc = fp4_tiles_launch<TAIL_SILU, 128, 128, 2, 2, 3>(t, stream);
+    if (rc) return rc;
+    QE_LAUNCH_CHECK();
+    return 0;
+}

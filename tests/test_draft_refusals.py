@@ -20,6 +20,9 @@ class NoLaunch:
     def qe_verify_drafts_workspace_bytes(self, *a):
         return 16
 
+    def qe_gemm_mxfp4_workspace_bytes(self, *a):
+        return 0
+
     def __getattr__(self, name):
         def call(*a):
             raise Launched(name)
@@ -147,7 +150,7 @@ def test_the_librarys_own_checks():
     refused(lib.qe_mxfp4_quantize(p, vp(4098), p, i(4), i(32), i(0), None), "whole word")
 
     def gemm(M=2, N=4, K=32, kind=0, out=0, tail=0, x=p, codes=p):
-        return lib.qe_gemm_mxfp4(x, p, codes, p, None, p, i(M), i(N), i(K), i(kind), i(out), i(tail), None)
+        return lib.qe_gemm_mxfp4(x, p, codes, p, None, p, i(M), i(N), i(K), i(kind), i(out), i(tail), None, ctypes.c_long(0), None)
 
     refused(gemm(M=-1), "sizes")
     refused(gemm(N=0), "sizes")
@@ -160,6 +163,7 @@ def test_the_librarys_own_checks():
     refused(gemm(codes=vp(4104)), "16-byte")
     refused(gemm(kind=2, x=vp(4104)), "16-byte")
     refused(gemm(M=2 ** 31 - 1), "too many")
+    refused(gemm(M=100, kind=1), "workspace")
     lib.qe_verify_drafts_workspace_bytes.restype = ctypes.c_long
 
     def verify(rows=6, V=50, R=2, ws=p, nbytes=1 << 40):
