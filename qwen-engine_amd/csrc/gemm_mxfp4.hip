@@ -152,13 +152,17 @@ static void fp4_launch(const Fp4Args& a, hipStream_t stream) {
     else fp4_rows_launch<X, TAIL, 4, WHOLE>(a, stream);
 }
 
+// More rows than this go by tiles.
+#define FP4_ROWS 64
+
 static bool fp4_by_tiles(int M, int N, int K, int x_kind) {
-    return x_kind != X_FP4 && M > 64 && fp4_tiles_take(M, N, K, x_kind);
+    return M > FP4_ROWS && (x_kind == X_FP4 ? fp4_both_take(M, N, K) : fp4_tiles_take(M, N, K, x_kind));
 }
 
 // Bytes of workspace that qe_gemm_mxfp4 needs for these operands.
-extern "C" long qe_gemm_mxfp4_workspace_bytes(const void* x, const void* scales, int M, int N, int K, int x_kind) {
+extern "C" long qe_gemm_mxfp4_workspace_bytes(const void* x, const void* x_scales, const void* scales, int M, int N, int K, int x_kind) {
     if (M <= 0 || N <= 0 || K <= 0 || !fp4_by_tiles(M, N, K, x_kind)) return 0;
+    if (x_kind == X_FP4) return fp4_both_workspace(M, N, K, x_scales, scales);
     return fp4_tiles_workspace(M, N, K, x_kind, (((uintptr_t)x & 15) | ((uintptr_t)scales & 3)) == 0);
 }
 
@@ -179,9 +183,9 @@ extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* co
     if (M == 0) return 0;
     const Fp4Args a{x, (const unsigned char*)x_scales, (const unsigned char*)codes, (const unsigned char*)scales, bias, out, M, N, K,
                     qe_cdiv(K, 32), out_dtype == QE_F32};
-    const long need = qe_gemm_mxfp4_workspace_bytes(x, scales, M, N, K, x_kind);
+    const long need = qe_gemm_mxfp4_workspace_bytes(x, x_scales, scales, M, N, K, x_kind);
     QE_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need), "gemm_mxfp4: workspace too small");
-    if (fp4_by_tiles(M, N, K, x_kind)) return fp4_tiles(a, x_kind, tail, workspace, stream);
+    if (fp4_by_tiles(M, N, K, x_kind)) return x_kind == X_FP4 ? fp4_both(a, tail, workspace, stream) : fp4_tiles(a, x_kind, tail, workspace, stream);
     // whole blocks of 16-byte pieces of x
     const bool whole = K % 32 == 0 && ((uintptr_t)x & 15) == 0;
 #define QE_TAILS(X_, W_)                                                          \

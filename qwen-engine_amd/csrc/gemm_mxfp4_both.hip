@@ -1,0 +1,254 @@
+// Products of many rows in 4 bits with a 4-bit matrix (see mxfp4.h): out[M, N] = sum_k x[m, k] v[n, k], by
+// v_mfma_scale_f32_32x32x64_f8f6f4, which multiplies codes with their blocks' scales.
+//
+// A block of 2 x 2 waves computes BM rows by BN columns.  K is walked in stages of 128 through a ring of four in shared memory: 64 bytes of
+// codes and 4 of scales a row, of both sides alike, brought by loads that write to shared memory directly.  Two rows are a line of 128
+// bytes there, its eight pieces exchanged by the line's number (so that what the lanes read at a time lies in distinct banks).  Lane (r, h) =
+// (lane % 32, lane / 32) takes blocks 2 h and 2 h + 1 of row r, one in each of the stage's two k steps; the fragments of a step are
+// read while the step before is multiplied.
+#include "mxfp4.h"
+
+#define FP4_STAGE 128      // numbers of K
+#define FP4_RING 4
+
+// The codes of x with nothing behind K in a row's last block.
+__global__ __launch_bounds__(256) void fp4_clear_tail_kernel(const uintx4_t* __restrict__ codes, uintx4_t* __restrict__ out, long pieces, int K,
+                                                             unsigned blocks) {
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= pieces) return;
+    const int left = K - (int)((unsigned)at % blocks) * 32;
+    const uintx4_t c = codes[at];
+    out[at] = left < 32 ? first_codes(c, left) : c;
+}
+
+struct Fp4Both {
+    Fp4Args a;
+    const unsigned char* x;     // codes, nothing behind K
+    const uint32_t *xw, *words; // the scales of x and of the matrix, num_words words a row
+    int nk, num_words, tiles_m, tiles_n;
+};
+
+template <int TAIL, int BM, int BN>
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Both t) {
+    constexpr int RING = FP4_RING, WM = BM / 2, WN = BN / 2, MI = WM / 32, NJ = WN / 32;
+    constexpr int LDA = BM / 64, LDB = BN / 64, LDS = (BM + BN) / 256, LD = LDA + LDB + LDS;       // a wave's loads of a stage: codes of x, of the matrix, scales
+    constexpr int B_AT = BM * 64, S_AT = B_AT + BN * 64, STAGE = S_AT + (BM + BN) * 4;
+    static_assert(BM % 128 == 0 && BN % 128 == 0 && (RING - 1) * LD < 63, "whole loads of every wave");
+    static_assert(TAIL != TAIL_SILU || NJ % 2 == 0, "a wave has the gate and the up of its columns");
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const Fp4Args& a = t.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+    int tile_m, tile_n;
+    if (!fp4_tile_of(blockIdx.x, t.tiles_m, t.tiles_n, tile_m, tile_n)) return;
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
+    const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+    const int row_bytes = a.blocks * 16;
+
+    // the loads: per lane its bytes within the codes and the scales; beyond the matrices: out of range
+    int va[LDA], vb[LDB], vs[LDS];
+    const int idx = (lane & 7) ^ ((lane >> 3) & 7), piece = idx & 3;      // (a load is eight lines: the line's number modulo 8 is lane / 8)
+#pragma unroll
+    for (int i = 0; i < LDA; ++i) {
+        const int row = m0 + ((i * 4 + wave) * 8 + (lane >> 3)) * 2 + (idx >> 2);
+        va[i] = row < a.M ? row * row_bytes + piece * 16 : FP4_OUT;
+    }
+#pragma unroll
+    for (int i = 0; i < LDB; ++i) {
+        const int row = fp4_matrix_row<TAIL>(n0, ((i * 4 + wave) * 8 + (lane >> 3)) * 2 + (idx >> 2), wide);
+        vb[i] = row >= 0 ? row * row_bytes + piece * 16 : FP4_OUT;
+    }
+    // scales: loads of 64 rows, those of x first
+    bool s_of_x[LDS];
+#pragma unroll
+    for (int i = 0; i < LDS; ++i) {
+        const int part = i * 4 + wave_s;
+        s_of_x[i] = part < BM / 64;
+        const int row = s_of_x[i] ? (m0 + part * 64 + lane < a.M ? m0 + part * 64 + lane : -1)
+                                  : fp4_matrix_row<TAIL>(n0, (part - BM / 64) * 64 + lane, wide);
+        vs[i] = row >= 0 ? row * (t.num_words * 4) : FP4_OUT;
+    }
+    const uintx4_t rsrc_a = fp4_buffer(t.x, (unsigned)((long)a.M * row_bytes)), rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * row_bytes));
+    const uintx4_t rsrc_x = fp4_buffer(t.xw, (unsigned)((long)a.M * t.num_words * 4)), rsrc_w = fp4_buffer(t.words, (unsigned)((long)a.N * t.num_words * 4));
+    const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
+    int ask_k = 0;                                         // the stage that is being asked for, and its place in the ring
+    unsigned ask_at = lds0;
+    const int last_pieces = a.blocks - (t.nk - 1) * 4;     // blocks of the last stage
+#define LOAD_PIECE(i_)                                                                                                    \
+    {                                                                                                                     \
+        const bool there = ask_k < t.nk;                                                                                  \
+        if ((i_) < LDA + LDB) {                                                                                           \
+            const int v_ = (i_) < LDA ? va[(i_) < LDA ? (i_) : 0] : vb[(i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0]; \
+            const int o_ = there && (ask_k + 1 < t.nk || piece < last_pieces) ? v_ : FP4_OUT;                             \
+            const int s_ = there ? ask_k * 64 : 0;                                                                        \
+            const unsigned to_ = ask_at + ((i_) < LDA ? ((i_) * 4 + wave_s) * 1024 : B_AT + (((i_) - LDA) * 4 + wave_s) * 1024); \
+            if ((i_) < LDA) { QE_LOAD_TO_SHARED(to_, o_, rsrc_a, s_, "0", ""); } else { QE_LOAD_TO_SHARED(to_, o_, rsrc_b, s_, "0", ""); } \
+        } else {                                                                                                          \
+            constexpr int n_ = (i_) < LDA + LDB ? 0 : (i_) < LD ? (i_) - LDA - LDB : 0;                                   \
+            const int o_ = there ? vs[n_] : FP4_OUT, s_ = there ? ask_k * 4 : 0;                                          \
+            const unsigned to_ = ask_at + S_AT + (n_ * 4 + wave_s) * 256;                                                 \
+            if (s_of_x[n_]) { QE_LOAD_WORD_TO_SHARED(to_, o_, rsrc_x, s_); } else { QE_LOAD_WORD_TO_SHARED(to_, o_, rsrc_w, s_); } \
+        }                                                                                                                 \
+    }
+#define LOAD_CASE(i_) case i_: if constexpr ((i_) < LD) LOAD_PIECE(i_) break;
+#define LOADS_OF(n_)                                                                                                      \
+    switch (n_) {                                                                                                         \
+        LOAD_CASE(0) LOAD_CASE(1) LOAD_CASE(2) LOAD_CASE(3) LOAD_CASE(4) LOAD_CASE(5) LOAD_CASE(6) LOAD_CASE(7) LOAD_CASE(8) LOAD_CASE(9) \
+        default: break;                                                                                                   \
+    }
+    static_assert(LD <= 10, "a case for every load");
+#define ASKED() { ++ask_k; ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE; }
+    // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
+#define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
+
+    int fa_at[2], fb_at[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int ra = wm + r, rb = wn + r;
+        fa_at[q] = (ra >> 1) * 128 + ((((ra & 1) * 4 + 2 * h + q) ^ ((ra >> 1) & 7)) * 16);
+        fb_at[q] = B_AT + (rb >> 1) * 128 + ((((rb & 1) * 4 + 2 * h + q) ^ ((rb >> 1) & 7)) * 16);
+    }
+    const int sa_at = S_AT + (wm + r) * 4, sb_at = S_AT + (BM + wn + r) * 4;
+    floatx16_t acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    uintx4_t fa[2][MI], fb[2][NJ];
+    uint32_t sa[2][MI], sb[2][NJ];                         // (by the stage's parity: a stage's last step multiplies while the next one's arrive)
+    // fragment p_ of step q_ (those of x and of the matrix in turn as they are wanted), scale p_
+#define READ_FRAG(q_, place_, p_)                                                                                         \
+    {                                                                                                                     \
+        if ((p_) < MI) fa[q_][(p_) < MI ? (p_) : 0] = *(const uintx4_t*)(smem + (place_) + fa_at[q_] + (p_) * 2048);      \
+        else fb[q_][(p_) < MI ? 0 : (p_) - MI] = *(const uintx4_t*)(smem + (place_) + fb_at[q_] + ((p_) - MI) * 2048);    \
+    }
+#define READ_SCALE(par_, place_, p_)                                                                                      \
+    {                                                                                                                     \
+        if ((p_) < MI) sa[par_][(p_) < MI ? (p_) : 0] = *(const uint32_t*)(smem + (place_) + sa_at + (p_) * 128) >> (16 * h); \
+        else sb[par_][(p_) < MI ? 0 : (p_) - MI] = *(const uint32_t*)(smem + (place_) + sb_at + ((p_) - MI) * 128) >> (16 * h); \
+    }
+    constexpr int R = MI + NJ, PER = MI * NJ, LHALF = (LD + 1) / 2;
+    // step q_ of a stage of parity par_: between its matrix instructions the fragments of the next step are read from place from_ (for step 0 of
+    // the next stage with its scales), and half of the loads of the stage that is being asked for go out
+#define K_STEP(q_, par_, from_)                                                                                           \
+    _Pragma("unroll") for (int sl = 0; sl < PER; ++sl) {                                                                  \
+        _Pragma("unroll") for (int p = 0; p < R; ++p)                                                                     \
+            if (p * PER / (2 * R) == sl) {                                                                                \
+                READ_FRAG((q_) ^ 1, from_, p)                                                                             \
+                if ((q_) == 1) READ_SCALE((par_) ^ 1, from_, p)                                                           \
+            }                                                                                                             \
+        const int i = sl / NJ, j = sl % NJ;                                                                               \
+        const intx8_t xa = {(int)fa[q_][i][0], (int)fa[q_][i][1], (int)fa[q_][i][2], (int)fa[q_][i][3], 0, 0, 0, 0};      \
+        const intx8_t wb = {(int)fb[q_][j][0], (int)fb[q_][j][1], (int)fb[q_][j][2], (int)fb[q_][j][3], 0, 0, 0, 0};      \
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xa, wb, acc[i][j], 4, 4, q_, sa[par_][i], q_, sb[par_][j]); \
+        _Pragma("unroll") for (int l = 0; l < LHALF; ++l)                                                                 \
+            if (l * PER / LHALF == sl && ((q_) == 1 || l + LHALF < LD)) { LOADS_OF((q_) == 1 ? l : l + LHALF) }           \
+        __builtin_amdgcn_sched_barrier(0);                                                                                \
+    }
+#pragma unroll
+    for (int s = 0; s < RING; ++s) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i)
+            if (s + 1 < RING || i < LHALF) { LOADS_OF(i) }
+        if (s + 1 < RING) ASKED()
+    }
+    MEET((RING - 2) * LD + LHALF)
+#pragma unroll
+    for (int p = 0; p < R; ++p) {
+        READ_FRAG(0, 0, p)
+        READ_SCALE(0, 0, p)
+    }
+    // behind the barrier in the middle of a stage nothing of its place is read any more, and the next stage has arrived
+#define STAGE_OF(par_)                                                                                                    \
+    {                                                                                                                     \
+        const int next = at + STAGE == RING * STAGE ? 0 : at + STAGE;                                                     \
+        K_STEP(0, par_, at)                                                                                               \
+        ASKED()                                                                                                           \
+        MEET((RING - 2) * LD)                                                                                             \
+        K_STEP(1, par_, next)                                                                                             \
+        at = next;                                                                                                        \
+    }
+    int at = 0, st = 0;
+    for (; st + 1 < t.nk; st += 2) {
+        STAGE_OF(0)
+        STAGE_OF(1)
+    }
+    if (st < t.nk) STAGE_OF(0)
+    MEET(0)                                                // (what was asked for beyond the end has arrived)
+#undef STAGE_OF
+#undef K_STEP
+#undef READ_FRAG
+#undef READ_SCALE
+#undef LOADS_OF
+#undef LOAD_CASE
+#undef LOAD_PIECE
+#undef ASKED
+#undef MEET
+    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn);
+}
+
+template <int TAIL, int BM, int BN>
+static int fp4_both_launch(Fp4Both t, hipStream_t stream) {
+    constexpr int SHARED = FP4_RING * (BM + BN) * 68;
+    t.tiles_m = qe_cdiv(t.a.M, BM);
+    t.tiles_n = qe_cdiv(t.a.N, BN);
+    const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
+    QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
+    QE_RAISE_SHARED((fp4_both_kernel<TAIL, BM, BN>), SHARED);
+    fp4_both_kernel<TAIL, BM, BN><<<(unsigned)blocks, 256, SHARED, stream>>>(t);
+    return 0;
+}
+
+static int words_of(int K) { return qe_cdiv(K, FP4_STAGE); }
+
+// The kernel's 32-bit places reach all of the operands.
+bool fp4_both_take(int M, int N, int K) {
+    return (long)N * qe_cdiv(K, 32) * 16 < (1L << 31) - 64 && (long)M * qe_cdiv(K, 32) * 16 < (1L << 31) - 64;
+}
+
+static bool pads(int K, const void* scales) { return K % FP4_STAGE || ((uintptr_t)scales & 3); }
+
+long fp4_both_workspace(int M, int N, int K, const void* xs, const void* scales) {
+    long bytes = K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0;
+    if (pads(K, xs)) bytes += (long)M * words_of(K) * 4;
+    if (pads(K, scales)) bytes += (long)N * words_of(K) * 4;
+    return bytes;
+}
+
+int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
+    Fp4Both t{};
+    t.a = a;
+    t.nk = t.num_words = words_of(a.K);
+    unsigned char* ws = (unsigned char*)workspace;
+    t.x = (const unsigned char*)a.x;
+    if (a.K % 32) {
+        const long pieces = (long)a.M * a.blocks;
+        fp4_clear_tail_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>((const uintx4_t*)a.x, (uintx4_t*)ws, pieces, a.K, (unsigned)a.blocks);
+        t.x = ws;
+        ws += pieces * 16;
+    }
+    t.xw = (const uint32_t*)a.xs;
+    if (pads(a.K, a.xs)) {
+        fp4_pad_scales(a.xs, (uint32_t*)ws, a.M, a.blocks, t.num_words, stream);
+        t.xw = (const uint32_t*)ws;
+        ws += (long)a.M * t.num_words * 4;
+    }
+    t.words = (const uint32_t*)a.scales;
+    if (pads(a.K, a.scales)) {
+        fp4_pad_scales(a.scales, (uint32_t*)ws, a.N, a.blocks, t.num_words, stream);
+        t.words = (const uint32_t*)ws;
+    }
+    const bool large = (long)qe_cdiv(a.M, 256) * qe_cdiv(a.N, 256) >= 128;
+    int rc;
+#define QE_GO(T_) rc = large ? fp4_both_launch<T_, 256, 256>(t, stream) : fp4_both_launch<T_, 128, 128>(t, stream)
+    if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
+    else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);
+    else QE_GO(TAIL_SILU);
+#undef QE_GO
+    if (rc) return rc;
+    QE_LAUNCH_CHECK();
+    return 0;
+}

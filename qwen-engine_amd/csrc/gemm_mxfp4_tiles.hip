@@ -51,6 +51,10 @@ __global__ __launch_bounds__(256) void fp4_scales_kernel(const unsigned char* __
     out[at] = v;
 }
 
+void fp4_pad_scales(const unsigned char* scales, uint32_t* words, int rows, int blocks, int num_words, hipStream_t stream) {
+    fp4_scales_kernel<<<qe_cdiv((long)rows * num_words, 256), 256, 0, stream>>>(scales, words, rows, blocks, num_words);
+}
+
 struct Fp4Tiles {
     Fp4Args a;
     const uint16_t* planes;     // rows of x, row_bytes apart, plane after plane
@@ -73,62 +77,33 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
     const int wave_s = __builtin_amdgcn_readfirstlane(wave);
 
-    // Every eighth block goes to the same XCD, which has an L2 of its own: it takes an eighth of a walk through the tiles in bands of 8
-    // tile rows, column by column, so that what it runs at a time shares rows of x and of the matrix.
     int tile_m, tile_n;
-    {
-        const int all = t.tiles_m * t.tiles_n, each = all / 8, over = all % 8, xcd = blockIdx.x % 8;
-        int local = blockIdx.x / 8;
-        if (local >= each + (xcd < over)) return;
-        local += xcd * each + min(xcd, over);
-        const int band = local / (8 * t.tiles_n), within = local - band * 8 * t.tiles_n, rows = min(8, t.tiles_m - band * 8);
-        tile_m = band * 8 + within % rows;
-        tile_n = within / rows;
-    }
+    if (!fp4_tile_of(blockIdx.x, t.tiles_m, t.tiles_n, tile_m, tile_n)) return;
     const int m0 = tile_m * BM, n0 = tile_n * BN;
     const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
     const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
 
     // the loads: per lane the bytes within x (from row m0), the codes and the scales; beyond the matrix: out of range, which arrives as zero
-    constexpr int OUT = 0x7fffffff;
     int va[LDA], vb[LDB], vs;
 #pragma unroll
     for (int i = 0; i < LDA; ++i) {
         const int row = (i * NW + wave) * 4 + (lane >> 4);
-        va[i] = m0 + row < a.M ? row * (int)t.row_bytes + ((lane & 15) ^ (row & 15)) * 16 : OUT;
+        va[i] = m0 + row < a.M ? row * (int)t.row_bytes + ((lane & 15) ^ (row & 15)) * 16 : FP4_OUT;
     }
-    // row i of the tile's columns: silu: blocks of 32, gate and up in turn
-    auto matrix_row = [&](int i) {
-        if constexpr (TAIL == TAIL_SILU) {
-            const int n = n0 / 2 + (i >> 6) * 32 + (i & 31);
-            return n < wide ? ((i >> 5) & 1) * wide + n : -1;
-        } else {
-            return n0 + i < wide ? n0 + i : -1;
-        }
-    };
     int piece[LDB];                                        // the block of the stage that this lane brings
 #pragma unroll
     for (int i = 0; i < LDB; ++i) {
         const int line = (i * NW + wave) * 8 + (lane >> 3), idx = (lane & 7) ^ (line & 7);
-        const int row = matrix_row(line * 2 + (idx >> 2));
+        const int row = fp4_matrix_row<TAIL>(n0, line * 2 + (idx >> 2), wide);
         piece[i] = row >= 0 ? idx & 3 : 1 << 28;
         vb[i] = row * (a.blocks * 16) + (idx & 3) * 16;
     }
     {
-        const int row = lane < SROWS ? matrix_row(wave * SROWS + lane) : -1;
-        vs = row >= 0 ? row * (t.num_words * 4) : OUT;
+        const int row = lane < SROWS ? fp4_matrix_row<TAIL>(n0, wave * SROWS + lane, wide) : -1;
+        vs = row >= 0 ? row * (t.num_words * 4) : FP4_OUT;
     }
-    uintx4_t rsrc_a, rsrc_b, rsrc_s;
-    const unsigned long x_at = (unsigned long)t.planes + (unsigned long)m0 * t.row_bytes, b_at = (unsigned long)a.codes, s_at = (unsigned long)t.words;
-    rsrc_a[0] = (unsigned)x_at; rsrc_a[1] = (unsigned)(x_at >> 32) & 0xffffu; rsrc_a[2] = t.x_bytes - (unsigned)m0 * t.row_bytes; rsrc_a[3] = 0x00020000u;
-    rsrc_b[0] = (unsigned)b_at; rsrc_b[1] = (unsigned)(b_at >> 32) & 0xffffu; rsrc_b[2] = (unsigned)((long)a.N * a.blocks * 16); rsrc_b[3] = 0x00020000u;
-    rsrc_s[0] = (unsigned)s_at; rsrc_s[1] = (unsigned)(s_at >> 32) & 0xffffu; rsrc_s[2] = (unsigned)((long)a.N * t.num_words * 4); rsrc_s[3] = 0x00020000u;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        rsrc_a[c] = __builtin_amdgcn_readfirstlane(rsrc_a[c]);
-        rsrc_b[c] = __builtin_amdgcn_readfirstlane(rsrc_b[c]);
-        rsrc_s[c] = __builtin_amdgcn_readfirstlane(rsrc_s[c]);
-    }
+    const uintx4_t rsrc_a = fp4_buffer((const unsigned char*)t.planes + (unsigned long)m0 * t.row_bytes, t.x_bytes - (unsigned)m0 * t.row_bytes);
+    const uintx4_t rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * a.blocks * 16)), rsrc_s = fp4_buffer(t.words, (unsigned)((long)a.N * t.num_words * 4));
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
     // the stage that is being asked for: its place in the ring, its plane's bytes and its step along K (t.nk: none is left)
     int ask_k = 0, ask_plane = 0;
@@ -137,16 +112,15 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     {                                                                                                                     \
         const bool there = ask_plane < t.num_planes;                                                                      \
         if ((i_) < LDA) {                                                                                                 \
-            const int v_ = there ? va[(i_) < LDA ? (i_) : 0] : OUT;                                                       \
+            const int v_ = there ? va[(i_) < LDA ? (i_) : 0] : FP4_OUT;                                                       \
             QE_LOAD_TO_SHARED(ask_at + ((i_) * NW + wave_s) * 1024, v_, rsrc_a, there ? ask_x + ask_k * 256 : 0, "0", ""); \
         } else if ((i_) < LDA + LDB) {                                                                                    \
             constexpr int b_ = (i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0;                                        \
-            const int v_ = there && ask_k * 4 + piece[b_] < a.blocks ? vb[b_] : OUT;                                      \
+            const int v_ = there && ask_k * 4 + piece[b_] < a.blocks ? vb[b_] : FP4_OUT;                                      \
             QE_LOAD_TO_SHARED(ask_at + B_AT + (b_ * NW + wave_s) * 1024, v_, rsrc_b, ask_k * 64, "0", "");                \
         } else {                                                                                                          \
-            const int v_ = there ? vs : OUT;                                                                              \
-            asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"                                              \
-                         : : "{m0}"(ask_at + S_AT + wave_s * 256), "v"(v_), "s"(rsrc_s), "s"(ask_k * 4) : "memory");      \
+            const int v_ = there ? vs : FP4_OUT;                                                                              \
+            QE_LOAD_WORD_TO_SHARED(ask_at + S_AT + wave_s * 256, v_, rsrc_s, ask_k * 4);                                  \
         }                                                                                                                 \
     }
 #define ASKED()                                                                                                           \
@@ -253,27 +227,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #undef READ_SCALES
 #undef EXPAND
 
-    // lane (r, h) has column r of a tile, its rows 8 b + 4 h + e
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const long m = m0 + wm + i * 32 + 8 * (e / 4) + 4 * h + e % 4;
-            if (m >= a.M) continue;
-            if constexpr (TAIL == TAIL_SILU) {
-#pragma unroll
-                for (int j = 0; j < NJ; j += 2) {
-                    const int n = n0 / 2 + (wn + j * 32) / 2 + r;
-                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], acc[i][j + 1][e]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const int n = n0 + wn + j * 32 + r;
-                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], 0.f);
-                }
-            }
-        }
+    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn);
 }
 
 template <int TAIL, int BM, int BN, int WR, int WC, int RING>
@@ -327,7 +281,7 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
         t.planes = (const uint16_t*)a.x;
     }
     if (a.K % FP4_STAGE || ((uintptr_t)a.scales & 3)) {
-        fp4_scales_kernel<<<qe_cdiv((long)a.N * t.num_words, 256), 256, 0, stream>>>(a.scales, (uint32_t*)ws, a.N, a.blocks, t.num_words);
+        fp4_pad_scales(a.scales, (uint32_t*)ws, a.N, a.blocks, t.num_words, stream);
         t.words = (const uint32_t*)ws;
     } else {
         t.words = (const uint32_t*)a.scales;

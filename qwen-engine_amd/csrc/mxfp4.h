@@ -71,7 +71,82 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, long m, int n, float
     else ((bf16_t*)a.out)[at] = float_to_bf16(v);
 }
 
+// Every eighth block goes to the same XCD, which has an L2 of its own: it takes an eighth of a walk through the tiles in bands of 8 tile rows,
+// column by column, so that what it runs at a time shares rows of x and of the matrix.  false: a block beyond the tiles.
+__device__ __forceinline__ bool fp4_tile_of(int block, int tiles_m, int tiles_n, int& tile_m, int& tile_n) {
+    const int all = tiles_m * tiles_n, each = all / 8, over = all % 8, xcd = block % 8;
+    int local = block / 8;
+    if (local >= each + (xcd < over)) return false;
+    local += xcd * each + min(xcd, over);
+    const int band = local / (8 * tiles_n), within = local - band * 8 * tiles_n, rows = min(8, tiles_m - band * 8);
+    tile_m = band * 8 + within % rows;
+    tile_n = within / rows;
+    return true;
+}
+
+// The row of the matrix behind column i of the tile that begins at column n0 (-1: none); silu: blocks of 32 columns, gate and up in turn.
+template <int TAIL>
+__device__ __forceinline__ int fp4_matrix_row(int n0, int i, int wide) {
+    if constexpr (TAIL == TAIL_SILU) {
+        const int n = n0 / 2 + (i >> 6) * 32 + (i & 31);
+        return n < wide ? ((i >> 5) & 1) * wide + n : -1;
+    } else {
+        return n0 + i < wide ? n0 + i : -1;
+    }
+}
+
+// The sums of a wave's tiles of 32 x 32 from row m0, column n0 of the whole product on: lane (r, h) = (lane % 32, lane / 32) has column
+// r of a tile and its rows 8 b + 4 h + e.
+template <int TAIL, int MI, int NJ>
+__device__ __forceinline__ void fp4_store_tiles(const Fp4Args& a, const floatx16_t (&acc)[MI][NJ], int m0, int n0) {
+    const int r = threadIdx.x & 31, h = (threadIdx.x & 63) >> 5, wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const long m = m0 + i * 32 + 8 * (e / 4) + 4 * h + e % 4;
+            if (m >= a.M) continue;
+            if constexpr (TAIL == TAIL_SILU) {
+#pragma unroll
+                for (int j = 0; j < NJ; j += 2) {
+                    const int n = (n0 + j * 32) / 2 + r;
+                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], acc[i][j + 1][e]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = n0 + j * 32 + r;
+                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], 0.f);
+                }
+            }
+        }
+}
+
+// A lane's offset of a buffer load that is beyond every buffer: it arrives as zero.
+constexpr int FP4_OUT = 0x7fffffff;
+
+// One descriptor of a buffer of so many bytes, the same in every lane.
+__device__ __forceinline__ uintx4_t fp4_buffer(const void* p, unsigned bytes) {
+    uintx4_t d;
+    d[0] = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)p);
+    d[1] = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long)p >> 32) & 0xffffu);
+    d[2] = __builtin_amdgcn_readfirstlane(bytes);
+    d[3] = 0x00020000u;
+    return d;
+}
+
+// 64 words, one a lane, to shared memory (see QE_LOAD_TO_SHARED)
+#define QE_LOAD_WORD_TO_SHARED(to_, offset_, rsrc_, soffset_)                                                        \
+    asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"                                                 \
+                 : : "{m0}"(to_), "v"(offset_), "s"(rsrc_), "s"(soffset_) : "memory")
+
 // gemm_mxfp4_tiles.hip: the products of many rows of 16 or 32 bits; the bytes of workspace that these sizes take
 bool fp4_tiles_take(int M, int N, int K, int x_kind);
 long fp4_tiles_workspace(int M, int N, int K, int x_kind, bool aligned);
 int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream);
+// gemm_mxfp4_both.hip: many rows that are in 4 bits themselves
+bool fp4_both_take(int M, int N, int K);
+long fp4_both_workspace(int M, int N, int K, const void* xs, const void* scales);
+int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream);
+// scales [rows, blocks] -> words [rows, num_words], zeros behind
+void fp4_pad_scales(const unsigned char* scales, uint32_t* words, int rows, int blocks, int num_words, hipStream_t stream);
