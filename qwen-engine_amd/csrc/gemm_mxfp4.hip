@@ -8,108 +8,130 @@
 // both sides in 4 bits the codes go to v_mfma_scale_f32_16x16x128_f8f6f4 as they are.
 #include "mxfp4.h"
 
-// A block of NW waves: MT tiles of 16 rows of x against 16 columns (silu: 16 of gate and the same 16 of up).  Its waves take steps of
-// four blocks of K in turn and their sums are added in the order of the waves.
-template <int X, int TAIL, int MT, int NW, bool WHOLE>
-__global__ __launch_bounds__(64 * NW) void fp4_rows_kernel(Fp4Args a) {
-    constexpr int NT = TAIL == TAIL_SILU ? 2 : 1;
-    __shared__ float sums[NW][NT][MT * 16][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
-    const int n = blockIdx.x * 16 + r;
+// Few rows: a block of up to 16 waves multiplies MT tiles of 16 rows of x with NT tiles of 16 columns (silu: the second half of the tiles
+// are the up rows of the first half's gate rows).  Its waves take steps of four blocks of K in turn, and their sums are added in the order
+// of the waves.
+//
+// Bound by the matrix's bytes on their way from memory: a wave asks for everything that the next U steps multiply before it multiplies.
+template <int X, int MT, int NT, bool WHOLE>
+__global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void fp4_rows_kernel(Fp4Args a, int tail) {
+    constexpr int U = MT == 1 && NT <= 2 && X != X_F32 ? 4 : MT <= 2 && X != X_F32 ? 2 : 1;
+    constexpr int XP = X == X_FP4 ? 1 : X == X_BF16 ? 4 : 8;           // 16-byte pieces of a block of x
+    extern __shared__ float sums[];                                    // [waves][NT][MT * 16][16]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, waves = blockDim.x >> 6;
+    const bool silu = tail == TAIL_SILU;
+    const int wide = silu ? a.N / 2 : a.N, cols = silu ? NT * 8 : NT * 16;
+    const int n0 = blockIdx.x * cols;
     const long m0 = (long)blockIdx.y * MT * 16;
+    // (columns and rows beyond the matrices are read as the last ones and not stored; blocks beyond K become zeros below: a branch around a
+    // load would make the next one wait for it)
     const unsigned char *codes[NT], *scales[NT];
-    bool have_n = n < wide;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const long row = have_n ? n + (long)t * wide : 0;
+        const bool up = silu && t >= NT / 2;
+        const int n = min(n0 + (up ? t - NT / 2 : t) * 16 + r, wide - 1);
+        const long row = n + (up ? (long)wide : 0);
         codes[t] = a.codes + row * a.blocks * 16;
         scales[t] = a.scales + row * a.blocks;
+    }
+    long x_row[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const long m = m0 + i * 16 + r;
+        x_row[i] = m < a.M ? m : a.M - 1;
     }
     floatx4_t acc[NT][MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[t][i] = {0.f, 0.f, 0.f, 0.f};
-    for (int step = wave; step * 4 < a.blocks; step += NW) {
-        const int b = step * 4 + g;                     // this lane's block of K
-        const bool have = b < a.blocks;
-        uintx4_t c[NT];
-        float scale[NT];
-        int sbyte[NT];
+    for (int step0 = wave; step0 * 4 < a.blocks; step0 += waves * U) {
+        uintx4_t c[U][NT], xp[U][MT][XP];
+        int sc[U][NT], xs[U][MT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            c[t] = {0u, 0u, 0u, 0u};
-            sbyte[t] = 0;
-            if (have && have_n) {
-                c[t] = *(const uintx4_t*)(codes[t] + (long)b * 16);
-                sbyte[t] = scales[t][b];
+        for (int u = 0; u < U; ++u) {
+            const int b = min((step0 + u * waves) * 4 + g, a.blocks - 1);      // this lane's block of K
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                c[u][t] = *(const uintx4_t*)(codes[t] + (long)b * 16);
+                sc[u][t] = scales[t][b];
             }
-            scale[t] = __uint_as_float((uint32_t)sbyte[t] << 23);
-        }
-        if constexpr (X == X_FP4) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const long m = m0 + i * 16 + r;
-                uintx4_t xc = {0u, 0u, 0u, 0u};
-                int xs = 0;
-                if (have && m < a.M) {
-                    xc = *(const uintx4_t*)((const unsigned char*)a.x + (m * a.blocks + b) * 16);
-                    xs = a.xs[m * a.blocks + b];
-                    if constexpr (!WHOLE) if (a.K - b * 32 < 32) xc = first_codes(xc, a.K - b * 32);
-                }
-                const intx8_t xa = {(int)xc[0], (int)xc[1], (int)xc[2], (int)xc[3], 0, 0, 0, 0};
+                if constexpr (X == X_FP4) {
+                    xp[u][i][0] = *(const uintx4_t*)((const unsigned char*)a.x + (x_row[i] * a.blocks + b) * 16);
+                    xs[u][i] = a.xs[x_row[i] * a.blocks + b];
+                } else if constexpr (WHOLE) {
+                    const uintx4_t* p = (const uintx4_t*)((const unsigned char*)a.x + (x_row[i] * a.K + b * 32) * (X == X_BF16 ? 2 : 4));
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const intx8_t wb = {(int)c[t][0], (int)c[t][1], (int)c[t][2], (int)c[t][3], 0, 0, 0, 0};
-                    acc[t][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][i], 4, 4, 0, xs, 0, sbyte[t]);
+                    for (int e = 0; e < XP; ++e) xp[u][i][e] = p[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < XP; ++e) xp[u][i][e] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const bool there = b * 32 + e < a.K;
+                        const long at = x_row[i] * a.K + (there ? b * 32 + e : 0);
+                        if constexpr (X == X_BF16) xp[u][i][e / 8][e / 2 % 4] |= there ? (uint32_t)((const uint16_t*)a.x)[at] << (16 * (e & 1)) : 0u;
+                        else xp[u][i][e / 4][e % 4] = there ? ((const uint32_t*)a.x)[at] : 0u;
+                    }
                 }
             }
-        } else {
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                bf16x8_t w[NT];
+        for (int u = 0; u < U; ++u) {
+            const int b = (step0 + u * waves) * 4 + g;
+            if (b >= a.blocks) {                       // (codes 0 of scale 2^-127 on both sides: x beyond K may be anything that a row holds)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) w[t] = fp4_to_bf16(c[t][j], scale[t]);
-                const int k = b * 32 + j * 8;
+                for (int t = 0; t < NT; ++t) { c[u][t] = {0u, 0u, 0u, 0u}; sc[u][t] = 0; }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    const long m = m0 + i * 16 + r;
-                    if constexpr (X == X_BF16) {
-                        union { bf16x8_t v; uintx4_t q; uint16_t e[8]; } xv;
-                        xv.q = {0u, 0u, 0u, 0u};
-                        const uint16_t* p = (const uint16_t*)a.x + m * a.K + k;
-                        if (have && m < a.M) {
-                            if constexpr (WHOLE) xv.q = *(const uintx4_t*)p;
-                            else
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) if (k + e < a.K) xv.e[e] = p[e];
-                        }
+                    for (int e = 0; e < XP; ++e) xp[u][i][e] = {0u, 0u, 0u, 0u};
+                    if constexpr (X == X_FP4) xs[u][i] = 0;
+                }
+            } else if constexpr (X == X_FP4 && !WHOLE) {
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv.v, w[t], acc[t][i], 0, 0, 0);
-                    } else {
-                        union { bf16x8_t v; uint16_t e[8]; } hi, mid, lo;
-                        float f[8];
-                        const float* p = (const float*)a.x + m * a.K + k;
+                for (int i = 0; i < MT; ++i)
+                    if (a.K - b * 32 < 32) xp[u][i][0] = first_codes(xp[u][i][0], a.K - b * 32);
+            }
+        }
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = 0.f;
-                        if (have && m < a.M) {
-                            if constexpr (WHOLE) {
-                                const floatx4_t u = *(const floatx4_t*)p, v = *(const floatx4_t*)(p + 4);
+        for (int u = 0; u < U; ++u) {
+            if constexpr (X == X_FP4) {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) { f[e] = u[e]; f[4 + e] = v[e]; }
-                            } else {
+                for (int i = 0; i < MT; ++i) {
+                    const uintx4_t& x = xp[u][i][0];
+                    const intx8_t xa = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) if (k + e < a.K) f[e] = p[e];
+                    for (int t = 0; t < NT; ++t) {
+                        const intx8_t wb = {(int)c[u][t][0], (int)c[u][t][1], (int)c[u][t][2], (int)c[u][t][3], 0, 0, 0, 0};
+                        acc[t][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][i], 4, 4, 0, xs[u][i], 0, sc[u][t]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    bf16x8_t w[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) w[t] = fp4_to_bf16(c[u][t][j], __uint_as_float((uint32_t)sc[u][t] << 23));
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        if constexpr (X == X_BF16) {
+                            const bf16x8_t x = __builtin_bit_cast(bf16x8_t, xp[u][i][j]);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w[t], acc[t][i], 0, 0, 0);
+                        } else {
+                            union { bf16x8_t v; uint16_t e[8]; } hi, mid, lo;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                cut_in_three(__uint_as_float(xp[u][i][2 * j + e / 4][e % 4]), hi.e[e], mid.e[e], lo.e[e]);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo.v, w[t], acc[t][i], 0, 0, 0);
+                                acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mid.v, w[t], acc[t][i], 0, 0, 0);
+                                acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi.v, w[t], acc[t][i], 0, 0, 0);
                             }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) cut_in_three(f[e], hi.e[e], mid.e[e], lo.e[e]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo.v, w[t], acc[t][i], 0, 0, 0);
-                            acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mid.v, w[t], acc[t][i], 0, 0, 0);
-                            acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi.v, w[t], acc[t][i], 0, 0, 0);
                         }
                     }
                 }
@@ -121,42 +143,52 @@ __global__ __launch_bounds__(64 * NW) void fp4_rows_kernel(Fp4Args a) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[wave][t][i * 16 + g * 4 + e][r] = acc[t][i][e];
+            for (int e = 0; e < 4; ++e) sums[((wave * NT + t) * MT * 16 + i * 16 + g * 4 + e) * 16 + r] = acc[t][i][e];
     __syncthreads();
-    for (int at = threadIdx.x; at < MT * 256; at += 64 * NW) {
-        const int row = at >> 4, col = at & 15;
+    const int out_tiles = silu ? NT / 2 : NT;
+    for (int at = threadIdx.x; at < out_tiles * MT * 256; at += blockDim.x) {
+        const int t = at / (MT * 256), row = at / 16 % (MT * 16), col = at & 15;
         const long m = m0 + row;
-        const int nn = blockIdx.x * 16 + col;
-        if (m >= a.M || nn >= wide) continue;
+        const int n = n0 + t * 16 + col;
+        if (m >= a.M || n >= wide) continue;
         float v = 0.f, up = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            v += sums[w][0][row][col];
-            if constexpr (NT == 2) up += sums[w][1][row][col];
+        for (int w = 0; w < waves; ++w) {
+            v += sums[((w * NT + t) * MT * 16 + row) * 16 + col];
+            if (silu) up += sums[((w * NT + t + NT / 2) * MT * 16 + row) * 16 + col];
         }
-        fp4_store<TAIL>(a, m, nn, v, up);
+        if (tail == TAIL_STORE) fp4_store<TAIL_STORE>(a, m, n, v, up);
+        else if (tail == TAIL_ADD) fp4_store<TAIL_ADD>(a, m, n, v, up);
+        else fp4_store<TAIL_SILU>(a, m, n, v, up);
     }
 }
 
-template <int X, int TAIL, int MT, bool WHOLE>
-static void fp4_rows_launch(const Fp4Args& a, hipStream_t stream) {
-    const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
-    const dim3 grid(qe_cdiv(wide, 16), qe_cdiv(a.M, MT * 16));
-    fp4_rows_kernel<X, TAIL, MT, 4, WHOLE><<<grid, 256, 0, stream>>>(a);
+template <int X, int MT, int NT, bool WHOLE>
+static int fp4_rows_launch(const Fp4Args& a, int tail, hipStream_t stream) {
+    const int wide = tail == TAIL_SILU ? a.N / 2 : a.N, cols = tail == TAIL_SILU ? NT * 8 : NT * 16;
+    const int steps = qe_cdiv(a.blocks, 4), most = MT * NT == 1 ? 16 : MT * NT <= 8 ? 8 : 4;       // (4: 64 KB of sums at most)
+    // about four steps a wave: what it asks for at once
+    int waves = steps >= 48 ? 16 : steps >= 12 ? 8 : steps >= 4 ? 4 : 2;
+    if (waves > most) waves = most;
+    const size_t shared = (size_t)waves * NT * MT * 1024;
+    const dim3 grid(qe_cdiv(wide, cols), qe_cdiv(a.M, MT * 16));
+    fp4_rows_kernel<X, MT, NT, WHOLE><<<grid, 64 * waves, shared, stream>>>(a, tail);
+    return 0;
 }
 
-template <int X, int TAIL, bool WHOLE>
-static void fp4_launch(const Fp4Args& a, hipStream_t stream) {
-    if (a.M <= 16) fp4_rows_launch<X, TAIL, 1, WHOLE>(a, stream);
-    else if (a.M <= 32) fp4_rows_launch<X, TAIL, 2, WHOLE>(a, stream);
-    else fp4_rows_launch<X, TAIL, 4, WHOLE>(a, stream);
+template <int X, bool WHOLE>
+static int fp4_rows(const Fp4Args& a, int tail, hipStream_t stream) {
+    const int wide = tail == TAIL_SILU ? a.N / 2 : a.N;
+    // Four tiles of columns a block where that leaves two blocks a compute unit: every block reads all of x.
+    const bool many = wide >= 2 * 256 * (tail == TAIL_SILU ? 32 : 64);
+    if (a.M <= 16) return many ? fp4_rows_launch<X, 1, 4, WHOLE>(a, tail, stream)
+                          : tail == TAIL_SILU ? fp4_rows_launch<X, 1, 2, WHOLE>(a, tail, stream) : fp4_rows_launch<X, 1, 1, WHOLE>(a, tail, stream);
+    if (a.M <= 32) return many ? fp4_rows_launch<X, 2, 4, WHOLE>(a, tail, stream) : fp4_rows_launch<X, 2, 2, WHOLE>(a, tail, stream);
+    if (a.M <= 48) return many ? fp4_rows_launch<X, 3, 4, WHOLE>(a, tail, stream) : fp4_rows_launch<X, 3, 2, WHOLE>(a, tail, stream);
+    return many && X != X_F32 ? fp4_rows_launch<X, 4, X == X_F32 ? 2 : 4, WHOLE>(a, tail, stream) : fp4_rows_launch<X, 4, 2, WHOLE>(a, tail, stream);
 }
-
-// More rows than this go by tiles.
-#define FP4_ROWS 64
 
 static bool fp4_by_tiles(int M, int N, int K, int x_kind) {
-    return M > FP4_ROWS && (x_kind == X_FP4 ? fp4_both_take(M, N, K) : fp4_tiles_take(M, N, K, x_kind));
+    return M > (x_kind == X_FP4 ? 64 : 16) && (x_kind == X_FP4 ? fp4_both_take(M, N, K) : fp4_tiles_take(M, N, K, x_kind));
 }
 
 // Bytes of workspace that qe_gemm_mxfp4 needs for these operands.
@@ -188,16 +220,11 @@ extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* co
     if (fp4_by_tiles(M, N, K, x_kind)) return x_kind == X_FP4 ? fp4_both(a, tail, workspace, stream) : fp4_tiles(a, x_kind, tail, workspace, stream);
     // whole blocks of 16-byte pieces of x
     const bool whole = K % 32 == 0 && ((uintptr_t)x & 15) == 0;
-#define QE_TAILS(X_, W_)                                                          \
-    do {                                                                          \
-        if (tail == TAIL_STORE) fp4_launch<X_, TAIL_STORE, W_>(a, stream);        \
-        else if (tail == TAIL_ADD) fp4_launch<X_, TAIL_ADD, W_>(a, stream);       \
-        else fp4_launch<X_, TAIL_SILU, W_>(a, stream);                            \
-    } while (0)
-    if (x_kind == X_FP4) { if (whole) QE_TAILS(X_FP4, true); else QE_TAILS(X_FP4, false); }
-    else if (x_kind == X_BF16) { if (whole) QE_TAILS(X_BF16, true); else QE_TAILS(X_BF16, false); }
-    else { if (whole) QE_TAILS(X_F32, true); else QE_TAILS(X_F32, false); }
-#undef QE_TAILS
+    int rc;
+    if (x_kind == X_FP4) rc = whole ? fp4_rows<X_FP4, true>(a, tail, stream) : fp4_rows<X_FP4, false>(a, tail, stream);
+    else if (x_kind == X_BF16) rc = whole ? fp4_rows<X_BF16, true>(a, tail, stream) : fp4_rows<X_BF16, false>(a, tail, stream);
+    else rc = whole ? fp4_rows<X_F32, true>(a, tail, stream) : fp4_rows<X_F32, false>(a, tail, stream);
+    if (rc) return rc;
     QE_LAUNCH_CHECK();
     return 0;
 }

@@ -62,7 +62,52 @@ struct Fp4Tiles {
     unsigned row_bytes, plane_bytes, x_bytes;      // (x_bytes: of all planes)
     int num_planes, nk, num_words;
     int tiles_m, tiles_n;
+    int per_split;              // stages of a cut: block (., y) sums the stages from y * per_split on
 };
+
+// The sum of the cuts' products, and what becomes of it: a thread four columns.
+template <int TAIL>
+__global__ __launch_bounds__(256) void fp4_join_kernel(Fp4Args a, const float* __restrict__ parts, int splits) {
+    const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (n >= wide) return;
+    const long size = (long)a.M * a.N;
+    for (long m = blockIdx.y; m < a.M; m += gridDim.y) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
+        const float* p = parts + m * a.N + n;
+        for (int s = 0; s < splits; ++s, p += size) {
+            if (a.N % 4 == 0 && wide % 4 == 0) {
+                const floatx4_t q = *(const floatx4_t*)p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += q[e];
+                if constexpr (TAIL == TAIL_SILU) {
+                    const floatx4_t u = *(const floatx4_t*)(p + wide);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) up[e] += u[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < wide) {
+                        v[e] += p[e];
+                        if constexpr (TAIL == TAIL_SILU) up[e] += p[wide + e];
+                    }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < wide) fp4_store<TAIL>(a, m, n + e, v[e], up[e]);
+    }
+}
+
+int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStream_t stream) {
+    const int wide = tail == TAIL_SILU ? a.N / 2 : a.N;
+    const dim3 grid(qe_cdiv(wide, 1024), a.M < 65535 ? a.M : 65535);
+    if (tail == TAIL_STORE) fp4_join_kernel<TAIL_STORE><<<grid, 256, 0, stream>>>(a, parts, splits);
+    else if (tail == TAIL_ADD) fp4_join_kernel<TAIL_ADD><<<grid, 256, 0, stream>>>(a, parts, splits);
+    else fp4_join_kernel<TAIL_SILU><<<grid, 256, 0, stream>>>(a, parts, splits);
+    return 0;
+}
 
 template <int TAIL, int BM, int BN, int WR, int WC, int RING>
 __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) {
@@ -105,28 +150,31 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     const uintx4_t rsrc_a = fp4_buffer((const unsigned char*)t.planes + (unsigned long)m0 * t.row_bytes, t.x_bytes - (unsigned)m0 * t.row_bytes);
     const uintx4_t rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * a.blocks * 16)), rsrc_s = fp4_buffer(t.words, (unsigned)((long)a.N * t.num_words * 4));
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
-    // the stage that is being asked for: its place in the ring, its plane's bytes and its step along K (t.nk: none is left)
-    int ask_k = 0, ask_plane = 0;
-    unsigned ask_x = 0, ask_at = lds0;
+    // the stage that is being asked for: its place in the ring, its plane's bytes, its step along K, and the stages left
+    const int first_stage = blockIdx.y * t.per_split, stages = min(t.nk * t.num_planes - first_stage, t.per_split);
+    int ask_k = first_stage % t.nk, ask_left = stages;
+    unsigned ask_x = (unsigned)(first_stage / t.nk) * t.plane_bytes, ask_at = lds0;
+    if constexpr (TAIL == TAIL_PARTIAL) t.a.out = (float*)t.a.out + (long)blockIdx.y * a.M * a.N;
 #define LOAD_PIECE(i_)                                                                                                    \
     {                                                                                                                     \
-        const bool there = ask_plane < t.num_planes;                                                                      \
+        const bool there = ask_left > 0;                                                                                  \
         if ((i_) < LDA) {                                                                                                 \
             const int v_ = there ? va[(i_) < LDA ? (i_) : 0] : FP4_OUT;                                                       \
             QE_LOAD_TO_SHARED(ask_at + ((i_) * NW + wave_s) * 1024, v_, rsrc_a, there ? ask_x + ask_k * 256 : 0, "0", ""); \
         } else if ((i_) < LDA + LDB) {                                                                                    \
             constexpr int b_ = (i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0;                                        \
             const int v_ = there && ask_k * 4 + piece[b_] < a.blocks ? vb[b_] : FP4_OUT;                                      \
-            QE_LOAD_TO_SHARED(ask_at + B_AT + (b_ * NW + wave_s) * 1024, v_, rsrc_b, ask_k * 64, "0", "");                \
+            QE_LOAD_TO_SHARED(ask_at + B_AT + (b_ * NW + wave_s) * 1024, v_, rsrc_b, there ? ask_k * 64 : 0, "0", "");   \
         } else {                                                                                                          \
             const int v_ = there ? vs : FP4_OUT;                                                                              \
-            QE_LOAD_WORD_TO_SHARED(ask_at + S_AT + wave_s * 256, v_, rsrc_s, ask_k * 4);                                  \
+            QE_LOAD_WORD_TO_SHARED(ask_at + S_AT + wave_s * 256, v_, rsrc_s, there ? ask_k * 4 : 0);                      \
         }                                                                                                                 \
     }
 #define ASKED()                                                                                                           \
     {                                                                                                                     \
         ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE;                                           \
-        if (++ask_k == t.nk) { ask_k = 0; ++ask_plane; ask_x += t.plane_bytes; }                                          \
+        --ask_left;                                                                                                       \
+        if (++ask_k == t.nk) { ask_k = 0; ask_x += t.plane_bytes; }                                                       \
     }
     // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
 #define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
@@ -201,7 +249,6 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     for (int j = 0; j < NJ; ++j) word[j] = word_next[j];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) { EXPAND(0, j) }
-    const int stages = t.nk * t.num_planes;
     int at = 0;
     for (int st = 0; st < stages; ++st) {
         const int next = at + STAGE == RING * STAGE ? 0 : at + STAGE;
@@ -231,14 +278,14 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 }
 
 template <int TAIL, int BM, int BN, int WR, int WC, int RING>
-static int fp4_tiles_launch(Fp4Tiles t, hipStream_t stream) {
+static int fp4_tiles_launch(Fp4Tiles t, int splits, hipStream_t stream) {
     constexpr int NW = WR * WC, SHARED = RING * (BM * 256 + BN * 64 + NW * 256);
     t.tiles_m = qe_cdiv(t.a.M, BM);
     t.tiles_n = qe_cdiv(t.a.N, BN);
     const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
     QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
     QE_RAISE_SHARED((fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING>), SHARED);
-    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING><<<(unsigned)blocks, 64 * NW, SHARED, stream>>>(t);
+    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING><<<dim3((unsigned)blocks, (unsigned)splits), 64 * NW, SHARED, stream>>>(t);
     return 0;
 }
 
@@ -249,8 +296,25 @@ bool fp4_tiles_take(int M, int N, int K, int x_kind) {
     return (long)N * padded(K) / 2 < (1L << 31) && (long)M * padded(K) * 2 * (x_kind == X_F32 ? 3 : 1) < (1L << 31);
 }
 
+// The rows of a tile, and in how many cuts of K the tiles fill the chip.
+static int fp4_tiles_shape(int M, int N, int K, int x_kind, int* per_split) {
+    const int stages = padded(K) / FP4_STAGE * (x_kind == X_F32 ? 3 : 1);
+    const long rows64 = qe_cdiv(M, 64) * 64L, rows128 = qe_cdiv(M, 128) * 128L;
+    const int bm = M <= 64 || (M <= 512 && rows128 * 100 > rows64 * 115) ? 64 : 128;
+    const long tiles = (long)qe_cdiv(M, bm) * qe_cdiv(N, 128), slots = bm == 64 ? 512 : 256;
+    long splits = slots / tiles;
+    if (splits > stages / 4) splits = stages / 4;
+    if (splits < 1) splits = 1;
+    *per_split = qe_cdiv(stages, (int)splits);
+    return bm;
+}
+
 long fp4_tiles_workspace(int M, int N, int K, int x_kind, bool aligned) {
-    long bytes = 0;
+    int per_split;
+    fp4_tiles_shape(M, N, K, x_kind, &per_split);
+    const int splits = qe_cdiv(padded(K) / FP4_STAGE * (x_kind == X_F32 ? 3 : 1), per_split);
+    long bytes = splits > 1 ? 4L * splits * M * N : 0;
+    bytes = (bytes + 15) / 16 * 16;
     if (x_kind == X_F32) bytes += 6L * M * padded(K);
     else if (K % FP4_STAGE || !aligned) bytes += 2L * M * padded(K);
     if (K % FP4_STAGE || !aligned) bytes += (long)N * (padded(K) / 32);
@@ -267,7 +331,15 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     t.row_bytes = (unsigned)Kp * 2;
     t.plane_bytes = (unsigned)((long)a.M * Kp * 2);
     t.x_bytes = t.plane_bytes * t.num_planes;
+    // the workspace: the cuts' products, then what is made of x and of the scales
+    float* parts = (float*)workspace;
     unsigned char* ws = (unsigned char*)workspace;
+    {
+        int per_split;
+        fp4_tiles_shape(a.M, a.N, a.K, x_kind, &per_split);
+        const int cuts = qe_cdiv(t.nk * t.num_planes, per_split);
+        if (cuts > 1) ws += (4L * cuts * a.M * a.N + 15) / 16 * 16;
+    }
     const dim3 grid(qe_cdiv(Kp, 1024), a.M < 65535 ? a.M : 65535);
     if (x_kind == X_F32) {
         fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
@@ -286,11 +358,18 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     } else {
         t.words = (const uint32_t*)a.scales;
     }
+    const int bm = fp4_tiles_shape(a.M, a.N, a.K, x_kind, &t.per_split);
+    const int splits = qe_cdiv(t.nk * t.num_planes, t.per_split);
+    if (splits > 1) t.a.out = parts;
     int rc;
-    if (tail == TAIL_STORE) rc = fp4_tiles_launch<TAIL_STORE, 128, 128, 2, 2, 3>(t, stream);
-    else if (tail == TAIL_ADD) rc = fp4_tiles_launch<TAIL_ADD, 128, 128, 2, 2, 3>(t, stream);
-    else rc = fp4_tiles_launch<TAIL_SILU, 128, 128, 2, 2, 3>(t, stream);
+#define QE_GO(T_) rc = bm == 64 ? fp4_tiles_launch<T_, 64, 128, 2, 2, 3>(t, splits, stream) : fp4_tiles_launch<T_, 128, 128, 2, 2, 3>(t, splits, stream)
+    if (splits > 1) QE_GO(TAIL_PARTIAL);
+    else if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
+    else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);
+    else QE_GO(TAIL_SILU);
+#undef QE_GO
     if (rc) return rc;
+    if (splits > 1 && (rc = fp4_join(a, parts, splits, tail, stream))) return rc;
     QE_LAUNCH_CHECK();
     return 0;
 }

@@ -10,7 +10,7 @@ typedef __attribute__((ext_vector_type(4))) unsigned int uintx4_t;
 typedef __attribute__((ext_vector_type(8))) int intx8_t;
 
 enum { X_BF16 = 0, X_F32 = 1, X_FP4 = 2 };
-enum { TAIL_STORE = 0, TAIL_ADD = 1, TAIL_SILU = 2 };
+enum { TAIL_STORE = 0, TAIL_ADD = 1, TAIL_SILU = 2, TAIL_PARTIAL = 3 };      // (PARTIAL: a cut of K, summed by fp4_join)
 
 // Eight codes with their block's scale as eight bfloat16.
 __device__ __forceinline__ bf16x8_t fp4_to_bf16(uint32_t c, float scale) {
@@ -60,6 +60,10 @@ struct Fp4Args {
 // What becomes of a sum: row m, column n (silu: gate and up of column n of N / 2).
 template <int TAIL>
 __device__ __forceinline__ void fp4_store(const Fp4Args& a, long m, int n, float v, float up) {
+    if constexpr (TAIL == TAIL_PARTIAL) {
+        ((float*)a.out)[m * a.N + n] = v;
+        return;
+    }
     if (a.bias) {
         v += a.bias[n];
         if constexpr (TAIL == TAIL_SILU) up += a.bias[a.N / 2 + n];
@@ -139,6 +143,9 @@ __device__ __forceinline__ uintx4_t fp4_buffer(const void* p, unsigned bytes) {
 #define QE_LOAD_WORD_TO_SHARED(to_, offset_, rsrc_, soffset_)                                                        \
     asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"                                                 \
                  : : "{m0}"(to_), "v"(offset_), "s"(rsrc_), "s"(soffset_) : "memory")
+
+// partial products [splits][M][N] -> a.out, summed in their order, with the tail
+int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStream_t stream);
 
 // gemm_mxfp4_tiles.hip: the products of many rows of 16 or 32 bits; the bytes of workspace that these sizes take
 bool fp4_tiles_take(int M, int N, int K, int x_kind);
