@@ -3,7 +3,7 @@
 //
 // A block of 2 x 2 waves computes BM rows by BN columns.  K is walked in stages of 128 through a ring of four in shared memory: 64 bytes of
 // codes and 4 of scales a row, of both sides alike, brought by loads that write to shared memory directly.  Two rows are a line of 128
-// bytes there, its eight pieces exchanged by the line's number (so that what the lanes read at a time lies in distinct banks).  Lane (r, h) =
+// bytes there, its eight pieces exchanged by the line's number (so that what 16 lanes read at a time lies in distinct banks).  Lane (r, h) =
 // (lane % 32, lane / 32) takes blocks 2 h and 2 h + 1 of row r, one in each of the stage's two k steps; the fragments of a step are
 // read while the step before is multiplied.
 #include "mxfp4.h"
@@ -11,14 +11,42 @@
 #define FP4_STAGE 128      // numbers of K
 #define FP4_RING 4
 
-// The codes of x with nothing behind K in a row's last block.
-__global__ __launch_bounds__(256) void fp4_clear_tail_kernel(const uintx4_t* __restrict__ codes, uintx4_t* __restrict__ out, long pieces, int K,
-                                                             unsigned blocks) {
-    const long at = (long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= pieces) return;
-    const int left = K - (int)((unsigned)at % blocks) * 32;
-    const uintx4_t c = codes[at];
-    out[at] = left < 32 ? first_codes(c, left) : c;
+// What the loads cannot take as it is, in one launch: the codes of x with nothing behind K in a row's last block (where K is no whole
+// blocks), and the scales of x and of the matrix in rows of whole words, zeros behind.
+struct Fp4Prepare {
+    const uintx4_t* codes;
+    uintx4_t* codes_out;
+    const unsigned char *xs, *scales;
+    uint32_t *xs_out, *scales_out;
+    long pieces, x_words, words;        // numbers of 16-byte pieces and of words to write, 0: none
+    unsigned blocks, num_words;
+    int K;
+};
+
+__global__ __launch_bounds__(256) void fp4_prepare_kernel(Fp4Prepare p) {
+    long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at < p.pieces) {
+        const int left = p.K - (int)((unsigned)at % p.blocks) * 32;
+        const uintx4_t c = p.codes[at];
+        p.codes_out[at] = left < 32 ? first_codes(c, left) : c;
+        return;
+    }
+    at -= p.pieces;
+    const unsigned char* from = p.xs;
+    uint32_t* to = p.xs_out;
+    if (at >= p.x_words) {
+        at -= p.x_words;
+        if (at >= p.words) return;
+        from = p.scales;
+        to = p.scales_out;
+    }
+    const long row = (unsigned)at / p.num_words;
+    const int b = (int)((unsigned)at % p.num_words) * 4;
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (b + e < (int)p.blocks) v |= (uint32_t)from[row * p.blocks + b + e] << (8 * e);
+    to[at] = v;
 }
 
 struct Fp4Both {
@@ -34,7 +62,6 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
     constexpr int LDA = BM / 64, LDB = BN / 64, LDS = (BM + BN) / 256, LD = LDA + LDB + LDS;       // a wave's loads of a stage: codes of x, of the matrix, scales
     constexpr int B_AT = BM * 64, S_AT = B_AT + BN * 64, STAGE = S_AT + (BM + BN) * 4;
     static_assert(BM % 128 == 0 && BN % 128 == 0 && (RING - 1) * LD < 63, "whole loads of every wave");
-    static_assert(TAIL != TAIL_SILU || NJ % 2 == 0, "a wave has the gate and the up of its columns");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Fp4Args& a = t.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
@@ -48,7 +75,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 
     // the loads: per lane its bytes within the codes and the scales; beyond the matrices: out of range
     int va[LDA], vb[LDB], vs[LDS];
-    const int idx = (lane & 7) ^ ((lane >> 3) & 7), piece = idx & 3;      // (a load is eight lines: the line's number modulo 8 is lane / 8)
+    const int idx = (lane & 7) ^ ((lane >> 4) & 3), piece = idx & 3;      // (a load is eight lines: line / 2 % 4 is lane / 16)
 #pragma unroll
     for (int i = 0; i < LDA; ++i) {
         const int row = m0 + ((i * 4 + wave) * 8 + (lane >> 3)) * 2 + (idx >> 2);
@@ -106,8 +133,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int ra = wm + r, rb = wn + r;
-        fa_at[q] = (ra >> 1) * 128 + ((((ra & 1) * 4 + 2 * h + q) ^ ((ra >> 1) & 7)) * 16);
-        fb_at[q] = B_AT + (rb >> 1) * 128 + ((((rb & 1) * 4 + 2 * h + q) ^ ((rb >> 1) & 7)) * 16);
+        fa_at[q] = (ra >> 1) * 128 + ((((ra & 1) * 4 + 2 * h + q) ^ ((ra >> 2) & 3)) * 16);
+        fb_at[q] = B_AT + (rb >> 1) * 128 + ((((rb & 1) * 4 + 2 * h + q) ^ ((rb >> 2) & 3)) * 16);
     }
     const int sa_at = S_AT + (wm + r) * 4, sb_at = S_AT + (BM + wn + r) * 4;
     floatx16_t acc[MI][NJ];
@@ -224,23 +251,33 @@ int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
     t.nk = t.num_words = words_of(a.K);
     unsigned char* ws = (unsigned char*)workspace;
     t.x = (const unsigned char*)a.x;
-    if (a.K % 32) {
-        const long pieces = (long)a.M * a.blocks;
-        fp4_clear_tail_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>((const uintx4_t*)a.x, (uintx4_t*)ws, pieces, a.K, (unsigned)a.blocks);
-        t.x = ws;
-        ws += pieces * 16;
-    }
     t.xw = (const uint32_t*)a.xs;
-    if (pads(a.K, a.xs)) {
-        fp4_pad_scales(a.xs, (uint32_t*)ws, a.M, a.blocks, t.num_words, stream);
-        t.xw = (const uint32_t*)ws;
-        ws += (long)a.M * t.num_words * 4;
-    }
     t.words = (const uint32_t*)a.scales;
-    if (pads(a.K, a.scales)) {
-        fp4_pad_scales(a.scales, (uint32_t*)ws, a.N, a.blocks, t.num_words, stream);
-        t.words = (const uint32_t*)ws;
+    Fp4Prepare p{};
+    p.blocks = a.blocks;
+    p.num_words = t.num_words;
+    p.K = a.K;
+    if (a.K % 32) {
+        p.codes = (const uintx4_t*)a.x;
+        p.codes_out = (uintx4_t*)ws;
+        p.pieces = (long)a.M * a.blocks;
+        t.x = ws;
+        ws += p.pieces * 16;
     }
+    if (pads(a.K, a.xs)) {
+        p.xs = a.xs;
+        p.xs_out = (uint32_t*)ws;
+        p.x_words = (long)a.M * t.num_words;
+        t.xw = p.xs_out;
+        ws += p.x_words * 4;
+    }
+    if (pads(a.K, a.scales)) {
+        p.scales = a.scales;
+        p.scales_out = (uint32_t*)ws;
+        p.words = (long)a.N * t.num_words;
+        t.words = p.scales_out;
+    }
+    if (const long all = p.pieces + p.x_words + p.words) fp4_prepare_kernel<<<(unsigned)((all + 255) / 256), 256, 0, stream>>>(p);
     const bool large = (long)qe_cdiv(a.M, 256) * qe_cdiv(a.N, 256) >= 128;
     int rc;
 #define QE_GO(T_) rc = large ? fp4_both_launch<T_, 256, 256>(t, stream) : fp4_both_launch<T_, 128, 128>(t, stream)

@@ -1,9 +1,9 @@
 // Products of many rows of 16-bit or 32-bit numbers with a 4-bit matrix (see mxfp4.h): out[M, N] = x[M, K] . V[N, K]^T.
 //
-// A block of WR x WC waves computes BM rows by BN columns.  K is walked in stages of 128 through a ring in shared memory: 256 bytes of a
-// row of x, 64 of codes and 4 of scales of a row of the matrix, brought by loads that write to shared memory directly.  A
+// A block of four waves computes BM rows by BN columns.  K is walked in stages of 128 or 64 through a ring in shared memory: of 128, 256 bytes of a
+// row of x, 64 of codes and 4 of scales (a word each there) of a row of the matrix, brought by loads that write to shared memory directly.  A
 // wave multiplies its part in tiles of 32 x 32 with v_mfma_f32_32x32x16_bf16: lane (r, h) = (lane % 32, lane / 32) takes, of row r,
-// block 2 b + h of the stage's four, so that a 16-byte piece of codes with one scale gives four matrix instructions' operands, eight numbers
+// block 2 b + h of the stage, so that a 16-byte piece of codes with one scale gives four matrix instructions' operands, eight numbers
 // each, by four conversions each.  The conversions for the next k step stand between the matrix instructions of this one.
 //
 // Rows of 32-bit numbers come as three planes of bfloat16 (cut_in_three) that are walked one after the other, the smallest
@@ -37,30 +37,11 @@ __global__ __launch_bounds__(256) void fp4_planes_kernel(const T* __restrict__ x
     }
 }
 
-// scales [N, blocks] -> [N, padded], zeros behind
-__global__ __launch_bounds__(256) void fp4_scales_kernel(const unsigned char* __restrict__ scales, uint32_t* __restrict__ out, int N,
-                                                         int blocks, int words) {
-    const long at = (long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (long)N * words) return;
-    const long row = at / words;
-    const int b = (int)(at - row * words) * 4;
-    uint32_t v = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (b + e < blocks) v |= (uint32_t)scales[row * blocks + b + e] << (8 * e);
-    out[at] = v;
-}
-
-void fp4_pad_scales(const unsigned char* scales, uint32_t* words, int rows, int blocks, int num_words, hipStream_t stream) {
-    fp4_scales_kernel<<<qe_cdiv((long)rows * num_words, 256), 256, 0, stream>>>(scales, words, rows, blocks, num_words);
-}
-
 struct Fp4Tiles {
     Fp4Args a;
     const uint16_t* planes;     // rows of x, row_bytes apart, plane after plane
-    const uint32_t* words;      // the scales, `words` words a row
     unsigned row_bytes, plane_bytes, x_bytes;      // (x_bytes: of all planes)
-    int num_planes, nk, num_words;
+    int num_planes, nk, k_in_row;                  // (numbers of K that a row holds: K, or whole stages where it is a plane's)
     int tiles_m, tiles_n;
     int per_split;              // stages of a cut: block (., y) sums the stages from y * per_split on
 };
@@ -109,14 +90,15 @@ int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStre
     return 0;
 }
 
-template <int TAIL, int BM, int BN, int WR, int WC, int RING>
+// BM x BN: the tile; WR x WC: the waves; SK: numbers of K of a stage, 128 or 64 (whole lines of x either way); RING: stages in shared memory
+template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>
 __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) {
-    constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, MI = WM / 32, NJ = WN / 32;
-    constexpr int LDA = BM / (4 * NW), LDB = BN / (16 * NW), LD = LDA + LDB + 1, SROWS = BN / NW;
-    constexpr int B_AT = BM * 256, S_AT = B_AT + BN * 64, STAGE = S_AT + NW * 256;
-    static_assert(BM % (4 * NW) == 0 && BN % (16 * NW) == 0 && SROWS <= 64 && (RING - 1) * LD + 4 < 64 && MI * NJ >= 2, "whole loads of every wave");
-    static_assert(TAIL != TAIL_SILU || NJ % 2 == 0, "a wave has the gate and the up of its columns");
-    constexpr int PER_STEP = (LD + 7) / 8;                 // loads of a k step
+    constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, MI = WM / 32, NJ = WN / 32, QS = SK / 16, BL = SK / 32;
+    constexpr int LDA = BM * SK / (512 * NW), LDB = BN * SK / (2048 * NW), LDS = BN * BL / (64 * NW), LD = LDA + LDB + LDS;      // a wave's loads of a stage: x, codes, scales
+    constexpr int B_AT = BM * SK * 2, S_AT = B_AT + BN * SK / 2, STAGE = S_AT + BN * BL * 4;
+    static_assert(NW == 4 && (SK == 128 || SK == 64) && BM * SK % (512 * NW) == 0 && BN * BL % (64 * NW) == 0, "whole loads of every wave");
+    constexpr int PER = MI * NJ, PER_STEP = (LD + QS - 1) / QS, HEAD = 2 * PER_STEP < LD ? 2 * PER_STEP : LD;      // loads of a k step; of the two steps behind the barrier
+    static_assert((RING - 2) * LD + HEAD < 64 && LD <= 16 && MI <= PER, "the loads in flight can be counted");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Fp4Args& a = t.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
@@ -128,66 +110,77 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
     const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
 
-    // the loads: per lane the bytes within x (from row m0), the codes and the scales; beyond the matrix: out of range, which arrives as zero
-    int va[LDA], vb[LDB], vs;
+    // The loads: per lane the bytes within x (from row m0), the codes and the scales; beyond the matrix: out of range, which arrives as zero.
+    // The pieces of a row (of x), of two or four rows that are a line (of the codes), are exchanged by the row's or line's number, so that what
+    // 16 lanes read at a time lies in distinct banks.
+    int va[LDA], vb[LDB], vs[LDS];
+    constexpr int AP = SK / 8, AR = 64 / AP;               // pieces of a row of x, rows of a load
+    const int a_row = wave * AR + lane / AP;
+    const int a_piece = SK == 128 ? (lane & 15) ^ (a_row & 15) : (lane & 7) ^ ((a_row >> 1) & 7);
 #pragma unroll
     for (int i = 0; i < LDA; ++i) {
-        const int row = (i * NW + wave) * 4 + (lane >> 4);
-        va[i] = m0 + row < a.M ? row * (int)t.row_bytes + ((lane & 15) ^ (row & 15)) * 16 : FP4_OUT;
+        const int row = i * NW * AR + a_row;
+        va[i] = m0 + row < a.M ? row * (int)t.row_bytes + a_piece * 16 : FP4_OUT;
     }
-    int piece[LDB];                                        // the block of the stage that this lane brings
+    const int line = lane >> 3, idx = (lane & 7) ^ ((line >> 1) & (SK == 128 ? 3 : 1)), b_piece = idx & (BL - 1);      // (a load is eight lines)
 #pragma unroll
     for (int i = 0; i < LDB; ++i) {
-        const int line = (i * NW + wave) * 8 + (lane >> 3), idx = (lane & 7) ^ (line & 7);
-        const int row = fp4_matrix_row<TAIL>(n0, line * 2 + (idx >> 2), wide);
-        piece[i] = row >= 0 ? idx & 3 : 1 << 28;
-        vb[i] = row * (a.blocks * 16) + (idx & 3) * 16;
+        const int row = fp4_matrix_row<TAIL>(n0, ((i * NW + wave) * 8 + line) * (8 / BL) + idx / BL, wide);
+        vb[i] = row >= 0 ? row * (a.blocks * 16) + b_piece * 16 : FP4_OUT;
     }
-    {
-        const int row = lane < SROWS ? fp4_matrix_row<TAIL>(n0, wave * SROWS + lane, wide) : -1;
-        vs = row >= 0 ? row * (t.num_words * 4) : FP4_OUT;
+    const int s_block = lane & (BL - 1);
+#pragma unroll
+    for (int i = 0; i < LDS; ++i) {
+        const int row = fp4_matrix_row<TAIL>(n0, (i * NW + wave) * (64 / BL) + lane / BL, wide);
+        vs[i] = row >= 0 ? row * a.blocks + s_block : FP4_OUT;
     }
-    const uintx4_t rsrc_a = fp4_buffer((const unsigned char*)t.planes + (unsigned long)m0 * t.row_bytes, t.x_bytes - (unsigned)m0 * t.row_bytes);
-    const uintx4_t rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * a.blocks * 16)), rsrc_s = fp4_buffer(t.words, (unsigned)((long)a.N * t.num_words * 4));
+    uintx4_t rsrc_a = fp4_buffer((const unsigned char*)t.planes + (unsigned long)m0 * t.row_bytes, t.x_bytes - (unsigned)m0 * t.row_bytes);
+    uintx4_t rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * a.blocks * 16)), rsrc_s = fp4_buffer(a.scales, (unsigned)((long)a.N * a.blocks));
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
-    // the stage that is being asked for: its place in the ring, its plane's bytes, its step along K, and the stages left
+    // the stage that is being asked for: its place in the ring, its step along K, its bytes within x, and the stages left
     const int first_stage = blockIdx.y * t.per_split, stages = min(t.nk * t.num_planes - first_stage, t.per_split);
-    int ask_k = first_stage % t.nk, ask_left = stages;
-    unsigned ask_x = (unsigned)(first_stage / t.nk) * t.plane_bytes, ask_at = lds0;
+    int ask_k = __builtin_amdgcn_readfirstlane(first_stage % t.nk), ask_left = __builtin_amdgcn_readfirstlane(stages);
+    unsigned ask_plane = __builtin_amdgcn_readfirstlane(first_stage / t.nk) * t.plane_bytes, ask_at = lds0;
+    // (K is no whole stages: of the last one's pieces some lie beyond the row; a lane's offset is then made one that is out of range)
+    const int x_left = t.k_in_row - (t.nk - 1) * SK, blocks_left = a.blocks - (t.nk - 1) * BL;
+    const int a_off = a_piece * 8 < x_left ? 0 : FP4_OUT, b_off = b_piece < blocks_left ? 0 : FP4_OUT, s_off = s_block < blocks_left ? 0 : FP4_OUT;
+    int a_not = t.nk == ask_k + 1 ? a_off : 0, b_not = t.nk == ask_k + 1 ? b_off : 0, s_not = t.nk == ask_k + 1 ? s_off : 0;
     if constexpr (TAIL == TAIL_PARTIAL) t.a.out = (float*)t.a.out + (long)blockIdx.y * a.M * a.N;
 #define LOAD_PIECE(i_)                                                                                                    \
     {                                                                                                                     \
-        const bool there = ask_left > 0;                                                                                  \
         if ((i_) < LDA) {                                                                                                 \
-            const int v_ = there ? va[(i_) < LDA ? (i_) : 0] : FP4_OUT;                                                       \
-            QE_LOAD_TO_SHARED(ask_at + ((i_) * NW + wave_s) * 1024, v_, rsrc_a, there ? ask_x + ask_k * 256 : 0, "0", ""); \
+            constexpr int n_ = (i_) < LDA ? (i_) : 0;                                                                     \
+            QE_LOAD_TO_SHARED(ask_at + (n_ * NW + wave_s) * 1024, va[n_] | a_not, rsrc_a, ask_plane + ask_k * (SK * 2), "0", ""); \
         } else if ((i_) < LDA + LDB) {                                                                                    \
-            constexpr int b_ = (i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0;                                        \
-            const int v_ = there && ask_k * 4 + piece[b_] < a.blocks ? vb[b_] : FP4_OUT;                                      \
-            QE_LOAD_TO_SHARED(ask_at + B_AT + (b_ * NW + wave_s) * 1024, v_, rsrc_b, there ? ask_k * 64 : 0, "0", "");   \
+            constexpr int n_ = (i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0;                                        \
+            QE_LOAD_TO_SHARED(ask_at + B_AT + (n_ * NW + wave_s) * 1024, vb[n_] | b_not, rsrc_b, ask_k * (SK / 2), "0", ""); \
         } else {                                                                                                          \
-            const int v_ = there ? vs : FP4_OUT;                                                                              \
-            QE_LOAD_WORD_TO_SHARED(ask_at + S_AT + wave_s * 256, v_, rsrc_s, there ? ask_k * 4 : 0);                      \
+            constexpr int n_ = (i_) < LDA + LDB ? 0 : (i_) < LD ? (i_) - LDA - LDB : 0;                                   \
+            QE_LOAD_BYTE_TO_SHARED(ask_at + S_AT + (n_ * NW + wave_s) * 256, vs[n_] | s_not, rsrc_s, ask_k * BL);         \
         }                                                                                                                 \
     }
+    // (beyond the last stage every load is out of range: the buffers have no bytes)
 #define ASKED()                                                                                                           \
     {                                                                                                                     \
         ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE;                                           \
-        --ask_left;                                                                                                       \
-        if (++ask_k == t.nk) { ask_k = 0; ask_x += t.plane_bytes; }                                                       \
+        if (++ask_k == t.nk) { ask_k = 0; ask_plane += t.plane_bytes; }                                                   \
+        if (--ask_left <= 0) { rsrc_a[2] = 0; rsrc_b[2] = 0; rsrc_s[2] = 0; ask_k = 0; ask_plane = 0; }                   \
+        const int ends_ = ask_k + 1 == t.nk ? -1 : 0;                                                                     \
+        a_not = a_off & ends_; b_not = b_off & ends_; s_not = s_off & ends_;                                              \
     }
     // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
 #define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
 
-    // where a lane reads: of x its piece of k step q, of the codes its block of pair b, of the scales its row's word
-    int fa_at[8], fb_at[2], fs_at;
+    // where a lane reads: of x its piece of k step q, of the codes its block of pair b
+    int fa_at[QS], fb_at[BL / 2];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) fa_at[q] = (wm + r) * 256 + ((((q >> 2) * 8 + (q & 3)) ^ (h * 4) ^ (r & 15)) * 16);
+    for (int q = 0; q < QS; ++q)
+        fa_at[q] = SK == 128 ? (wm + r) * 256 + ((((q >> 2) * 8 + (q & 3)) ^ (h * 4) ^ (r & 15)) * 16) : (wm + r) * 128 + ((q ^ (h * 4) ^ ((r >> 1) & 7)) * 16);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int row = wn + r, line = row >> 1;
-        fb_at[b] = B_AT + line * 128 + ((((row & 1) * 4 + 2 * b + h) ^ (line & 7)) * 16);
-    }
+    for (int b = 0; b < BL / 2; ++b)
+        fb_at[b] = B_AT + (SK == 128 ? (wn + r) / 2 * 128 + ((((r & 1) * 4 + 2 * b + h) ^ ((r >> 2) & 3)) * 16)
+                                     : (wn + r) / 4 * 128 + ((((r & 3) * 2 + h) ^ ((r >> 3) & 1)) * 16));
+    const int fs_at = S_AT + ((wn + r) * BL + h) * 4;
     floatx16_t acc[MI][NJ];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -196,31 +189,40 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     bf16x8_t fa[4][MI], fb[2][NJ];
-    uintx4_t code[2][NJ];
-    uint32_t word[NJ], word_next[NJ];
-#define READ_A(q_, place_) _Pragma("unroll") for (int i = 0; i < MI; ++i) fa[(q_) & 3][i] = *(const bf16x8_t*)(smem + (place_) + fa_at[(q_) & 7] + i * 8192);
-#define READ_CODES(b_, place_) _Pragma("unroll") for (int j = 0; j < NJ; ++j) code[b_][j] = *(const uintx4_t*)(smem + (place_) + fb_at[b_] + j * 2048);
-#define READ_SCALES(place_)                                                                                               \
-    _Pragma("unroll") for (int j = 0; j < NJ; ++j) {                                                                      \
-        const int row = wn + j * 32 + r;                                                                                  \
-        word_next[j] = *(const uint32_t*)(smem + (place_) + S_AT + (row / SROWS) * 256 + (row % SROWS) * 4);              \
+    uintx4_t code[2][NJ];                                  // stages of 128: of pairs 0 and 1; of 64: of this stage and of the next
+    uint32_t word[2][NJ];
+#define READ_A(q_, place_, i_) fa[(q_) & 3][i_] = *(const bf16x8_t*)(smem + (place_) + fa_at[(q_) & (QS - 1)] + (i_) * (SK * 64));
+#define READ_CODES(to_, b_, place_, j_)                                                                                   \
+    {                                                                                                                     \
+        code[to_][j_] = *(const uintx4_t*)(smem + (place_) + fb_at[(b_) < BL / 2 ? (b_) : 0] + (j_) * (SK * 16));         \
+        word[to_][j_] = *(const uint32_t*)(smem + (place_) + fs_at + (j_) * (32 * BL * 4) + (b_) * 8);                    \
     }
-#define EXPAND(q_, j_) fb[(q_) & 1][j_] = fp4_to_bf16(code[((q_) >> 2) & 1][j_][(q_) & 3], __uint_as_float((word[j_] >> (((((q_) >> 2) & 1) * 2 + h) * 8) & 255u) << 23));
+    // the eight numbers of k step q_, of the codes that are in registers
+#define EXPAND(q_, j_)                                                                                                    \
+    {                                                                                                                     \
+        constexpr int of_ = SK == 128 ? ((q_) >> 2) & 1 : 0;                                                              \
+        fb[(q_) & 1][j_] = fp4_to_bf16(code[of_][j_][(q_) & 3], __uint_as_float(word[of_][j_] << 23));                    \
+    }
     // k step q_: between its matrix instructions the fragments of x of the step after the next are read, the next step's codes expanded, and the
     // loads of the stage that is being asked for go out, from the step behind the barrier on
 #define K_STEP(q_, place_, next_)                                                                                         \
     {                                                                                                                     \
-        if ((q_) < 6) { READ_A((q_) + 2, place_) } else { READ_A((q_) - 6, next_) }                                       \
-        if ((q_) == 1) { READ_CODES(1, place_) }                                                                          \
-        if ((q_) == 6) { READ_CODES(0, next_) READ_SCALES(next_) }                                                        \
-        if ((q_) == 7) { _Pragma("unroll") for (int j = 0; j < NJ; ++j) word[j] = word_next[j]; }                         \
-        _Pragma("unroll") for (int sl = 0; sl < MI * NJ; ++sl) {                                                          \
+        if (SK == 64 && (q_) == QS - 1) {                                                                                 \
+            _Pragma("unroll") for (int j = 0; j < NJ; ++j) { code[0][j] = code[1][j]; word[0][j] = word[1][j]; }          \
+        }                                                                                                                 \
+        _Pragma("unroll") for (int sl = 0; sl < PER; ++sl) {                                                              \
+            if (sl < MI) { if ((q_) < QS - 2) { READ_A((q_) + 2, place_, sl < MI ? sl : 0) } else { READ_A((q_) + 2 - QS, next_, sl < MI ? sl : 0) } } \
+            if (sl < NJ) {                                                                                                \
+                if (SK == 128 && (q_) == 1) READ_CODES(1, 1, place_, sl < NJ ? sl : 0)                                    \
+                if ((q_) == QS - 2) READ_CODES(SK == 128 ? 0 : 1, 0, next_, sl < NJ ? sl : 0)                             \
+            }                                                                                                             \
             acc[sl % MI][sl / MI] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[(q_) & 3][sl % MI], fb[(q_) & 1][sl / MI], acc[sl % MI][sl / MI], 0, 0, 0); \
-            if (sl % MI == 0) { EXPAND(((q_) + 1) & 7, sl / MI) }                                                         \
-            if (sl < PER_STEP) LOADS_OF((((q_) + 2) & 7) * PER_STEP + sl)                                                 \
+            if (sl % MI == 0) { EXPAND(((q_) + 1) & (QS - 1), sl / MI) }                                                  \
+            _Pragma("unroll") for (int l = 0; l < PER_STEP; ++l)                                                          \
+                if (l * PER / PER_STEP == sl) LOADS_OF((((q_) + 2) & (QS - 1)) * PER_STEP + l)                            \
             __builtin_amdgcn_sched_barrier(0);                                                                            \
         }                                                                                                                 \
-        if ((q_) == 5) { ASKED() MEET((RING - 2) * LD) }                                                                  \
+        if ((q_) == QS - 3) { ASKED() MEET((RING - 2) * LD) }                                                             \
     }
 #define LOADS_OF(n_)                                                                                                      \
     switch (n_) {                                                                                                         \
@@ -230,9 +232,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
         case 15: LOAD_CASE(15) default: break;                                                                            \
     }
 #define LOAD_CASE(i_) if constexpr ((i_) < LD) LOAD_PIECE(i_) break;
-    static_assert(LD <= 16 && PER_STEP <= MI * NJ, "a case for every load, a slot for every load of a step");
 
-    constexpr int HEAD = 2 * PER_STEP < LD ? 2 * PER_STEP : LD;          // of a stage's loads, those that go out in the two steps behind the barrier
 #pragma unroll
     for (int s = 0; s < RING; ++s) {
 #pragma unroll
@@ -241,14 +241,12 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
         if (s + 1 < RING) ASKED()
     }
     MEET((RING - 2) * LD + HEAD)
-    READ_CODES(0, 0)
-    READ_SCALES(0)
-    READ_A(0, 0)
-    READ_A(1, 0)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) word[j] = word_next[j];
+    for (int j = 0; j < NJ; ++j) READ_CODES(0, 0, 0, j)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) { EXPAND(0, j) }
+    for (int i = 0; i < MI; ++i) { READ_A(0, 0, i) READ_A(1, 0, i) }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) EXPAND(0, j)
     int at = 0;
     for (int st = 0; st < stages; ++st) {
         const int next = at + STAGE == RING * STAGE ? 0 : at + STAGE;
@@ -256,10 +254,12 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
         K_STEP(1, at, next)
         K_STEP(2, at, next)
         K_STEP(3, at, next)
-        K_STEP(4, at, next)
-        K_STEP(5, at, next)
-        K_STEP(6, at, next)
-        K_STEP(7, at, next)
+        if constexpr (SK == 128) {
+            K_STEP(4, at, next)
+            K_STEP(5, at, next)
+            K_STEP(6, at, next)
+            K_STEP(7, at, next)
+        }
         at = next;
     }
     MEET(0)                                                // (what was asked for beyond the end has arrived)
@@ -271,21 +271,20 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #undef MEET
 #undef READ_A
 #undef READ_CODES
-#undef READ_SCALES
 #undef EXPAND
-
     fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn);
 }
 
-template <int TAIL, int BM, int BN, int WR, int WC, int RING>
+template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>
 static int fp4_tiles_launch(Fp4Tiles t, int splits, hipStream_t stream) {
-    constexpr int NW = WR * WC, SHARED = RING * (BM * 256 + BN * 64 + NW * 256);
+    constexpr int SHARED = RING * (BM * SK * 2 + BN * SK / 2 + BN * SK / 8);
+    static_assert(SHARED <= 160 * 1024, "the ring must fit a compute unit");
     t.tiles_m = qe_cdiv(t.a.M, BM);
     t.tiles_n = qe_cdiv(t.a.N, BN);
     const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
     QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
-    QE_RAISE_SHARED((fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING>), SHARED);
-    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, RING><<<dim3((unsigned)blocks, (unsigned)splits), 64 * NW, SHARED, stream>>>(t);
+    QE_RAISE_SHARED((fp4_tiles_kernel<TAIL, BM, BN, WR, WC, SK, RING>), SHARED);
+    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, SK, RING><<<dim3((unsigned)blocks, (unsigned)splits), 256, SHARED, stream>>>(t);
     return 0;
 }
 
@@ -296,80 +295,73 @@ bool fp4_tiles_take(int M, int N, int K, int x_kind) {
     return (long)N * padded(K) / 2 < (1L << 31) && (long)M * padded(K) * 2 * (x_kind == X_F32 ? 3 : 1) < (1L << 31);
 }
 
-// The rows of a tile, and in how many cuts of K the tiles fill the chip.
-static int fp4_tiles_shape(int M, int N, int K, int x_kind, int* per_split) {
-    const int stages = padded(K) / FP4_STAGE * (x_kind == X_F32 ? 3 : 1);
+// The rows of a tile, the numbers of K of its stages, and in how many cuts of K the tiles fill the chip.
+struct Fp4Shape {
+    int bm, sk, per_split, splits;
+};
+
+static Fp4Shape fp4_tiles_shape(int M, int N, int K, int x_kind) {
+    const int planes = x_kind == X_F32 ? 3 : 1;
     const long rows64 = qe_cdiv(M, 64) * 64L, rows128 = qe_cdiv(M, 128) * 128L;
-    const int bm = M <= 64 || (M <= 512 && rows128 * 100 > rows64 * 115) ? 64 : 128;
-    const long tiles = (long)qe_cdiv(M, bm) * qe_cdiv(N, 128), slots = bm == 64 ? 512 : 256;
-    long splits = slots / tiles;
+    Fp4Shape s;
+    s.bm = M <= 64 || (M <= 512 && rows128 * 100 > rows64 * 115) ? 64 : 128;
+    if (s.bm == 128 && (long)qe_cdiv(M, 256) * qe_cdiv(N, 256) >= 192) s.bm = 256;
+    s.sk = s.bm == 256 ? 64 : 128;
+    const int stages = qe_cdiv(K, s.sk) * planes;
+    const long tiles = (long)qe_cdiv(M, s.bm) * qe_cdiv(N, 128);
+    long splits = s.bm == 256 ? 1 : (s.bm == 64 ? 512 : 256) / tiles;
     if (splits > stages / 4) splits = stages / 4;
     if (splits < 1) splits = 1;
-    *per_split = qe_cdiv(stages, (int)splits);
-    return bm;
+    s.per_split = qe_cdiv(stages, (int)splits);
+    s.splits = qe_cdiv(stages, s.per_split);
+    return s;
 }
 
 long fp4_tiles_workspace(int M, int N, int K, int x_kind, bool aligned) {
-    int per_split;
-    fp4_tiles_shape(M, N, K, x_kind, &per_split);
-    const int splits = qe_cdiv(padded(K) / FP4_STAGE * (x_kind == X_F32 ? 3 : 1), per_split);
-    long bytes = splits > 1 ? 4L * splits * M * N : 0;
-    bytes = (bytes + 15) / 16 * 16;
+    const Fp4Shape s = fp4_tiles_shape(M, N, K, x_kind);
+    long bytes = s.splits > 1 ? (4L * s.splits * M * N + 15) / 16 * 16 : 0;
     if (x_kind == X_F32) bytes += 6L * M * padded(K);
-    else if (K % FP4_STAGE || !aligned) bytes += 2L * M * padded(K);
-    if (K % FP4_STAGE || !aligned) bytes += (long)N * (padded(K) / 32);
+    else if (K % 8 || !aligned) bytes += 2L * M * padded(K);
     return bytes;
 }
 
 int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
+    const Fp4Shape s = fp4_tiles_shape(a.M, a.N, a.K, x_kind);
     Fp4Tiles t{};
     t.a = a;
     const int Kp = padded(a.K);
-    t.nk = Kp / FP4_STAGE;
-    t.num_words = Kp / FP4_STAGE;
+    t.nk = qe_cdiv(a.K, s.sk);
     t.num_planes = x_kind == X_F32 ? 3 : 1;
-    t.row_bytes = (unsigned)Kp * 2;
-    t.plane_bytes = (unsigned)((long)a.M * Kp * 2);
+    t.per_split = s.per_split;
+    const bool as_it_is = x_kind == X_BF16 && a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
+    t.k_in_row = as_it_is ? a.K : Kp;
+    t.row_bytes = (unsigned)t.k_in_row * 2;
+    t.plane_bytes = t.row_bytes * (unsigned)a.M;
     t.x_bytes = t.plane_bytes * t.num_planes;
-    // the workspace: the cuts' products, then what is made of x and of the scales
+    // the workspace: the cuts' products, then what is made of x
     float* parts = (float*)workspace;
-    unsigned char* ws = (unsigned char*)workspace;
-    {
-        int per_split;
-        fp4_tiles_shape(a.M, a.N, a.K, x_kind, &per_split);
-        const int cuts = qe_cdiv(t.nk * t.num_planes, per_split);
-        if (cuts > 1) ws += (4L * cuts * a.M * a.N + 15) / 16 * 16;
+    unsigned char* ws = (unsigned char*)workspace + (s.splits > 1 ? (4L * s.splits * a.M * a.N + 15) / 16 * 16 : 0);
+    t.planes = as_it_is ? (const uint16_t*)a.x : (const uint16_t*)ws;
+    if (!as_it_is) {
+        const dim3 grid(qe_cdiv(Kp, 1024), a.M < 65535 ? a.M : 65535);
+        if (x_kind == X_F32) fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
+        else fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
     }
-    const dim3 grid(qe_cdiv(Kp, 1024), a.M < 65535 ? a.M : 65535);
-    if (x_kind == X_F32) {
-        fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
-        t.planes = (const uint16_t*)ws;
-        ws += t.x_bytes;
-    } else if (a.K % FP4_STAGE || ((uintptr_t)a.x & 15)) {
-        fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
-        t.planes = (const uint16_t*)ws;
-        ws += t.x_bytes;
-    } else {
-        t.planes = (const uint16_t*)a.x;
-    }
-    if (a.K % FP4_STAGE || ((uintptr_t)a.scales & 3)) {
-        fp4_pad_scales(a.scales, (uint32_t*)ws, a.N, a.blocks, t.num_words, stream);
-        t.words = (const uint32_t*)ws;
-    } else {
-        t.words = (const uint32_t*)a.scales;
-    }
-    const int bm = fp4_tiles_shape(a.M, a.N, a.K, x_kind, &t.per_split);
-    const int splits = qe_cdiv(t.nk * t.num_planes, t.per_split);
-    if (splits > 1) t.a.out = parts;
+    if (s.splits > 1) t.a.out = parts;
     int rc;
-#define QE_GO(T_) rc = bm == 64 ? fp4_tiles_launch<T_, 64, 128, 2, 2, 3>(t, splits, stream) : fp4_tiles_launch<T_, 128, 128, 2, 2, 3>(t, splits, stream)
-    if (splits > 1) QE_GO(TAIL_PARTIAL);
+#define QE_GO(T_)                                                                            \
+    rc = s.bm == 256   ? fp4_tiles_launch<T_, 256, 256, 2, 2, 64, 3>(t, s.splits, stream)     \
+         : s.bm == 128 ? fp4_tiles_launch<T_, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)    \
+                       : fp4_tiles_launch<T_, 64, 128, 1, 4, 128, 3>(t, s.splits, stream)
+    if (s.splits > 1)
+        rc = s.bm == 128 ? fp4_tiles_launch<TAIL_PARTIAL, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)
+                         : fp4_tiles_launch<TAIL_PARTIAL, 64, 128, 1, 4, 128, 3>(t, s.splits, stream);
     else if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
     else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);
     else QE_GO(TAIL_SILU);
 #undef QE_GO
     if (rc) return rc;
-    if (splits > 1 && (rc = fp4_join(a, parts, splits, tail, stream))) return rc;
+    if (s.splits > 1 && (rc = fp4_join(a, parts, s.splits, tail, stream))) return rc;
     QE_LAUNCH_CHECK();
     return 0;
 }

@@ -88,35 +88,38 @@ __device__ __forceinline__ bool fp4_tile_of(int block, int tiles_m, int tiles_n,
     return true;
 }
 
-// The row of the matrix behind column i of the tile that begins at column n0 (-1: none); silu: blocks of 32 columns, gate and up in turn.
+// The row of the matrix behind column i of the tile that begins at column n0 (-1: none); silu: 16 of gate and their 16 of up in turn.
 template <int TAIL>
 __device__ __forceinline__ int fp4_matrix_row(int n0, int i, int wide) {
     if constexpr (TAIL == TAIL_SILU) {
-        const int n = n0 / 2 + (i >> 6) * 32 + (i & 31);
-        return n < wide ? ((i >> 5) & 1) * wide + n : -1;
+        const int n = n0 / 2 + (i >> 5) * 16 + (i & 15);
+        return n < wide ? ((i >> 4) & 1) * wide + n : -1;
     } else {
         return n0 + i < wide ? n0 + i : -1;
     }
 }
 
 // The sums of a wave's tiles of 32 x 32 from row m0, column n0 of the whole product on: lane (r, h) = (lane % 32, lane / 32) has column
-// r of a tile and its rows 8 b + 4 h + e.
+// r of a tile and its rows 8 b + 4 h + e.  Silu: lanes r < 16 have gates, the others their ups; of two rows the former finish the first, the
+// latter the second.
 template <int TAIL, int MI, int NJ>
 __device__ __forceinline__ void fp4_store_tiles(const Fp4Args& a, const floatx16_t (&acc)[MI][NJ], int m0, int n0) {
     const int r = threadIdx.x & 31, h = (threadIdx.x & 63) >> 5, wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 16; e += TAIL == TAIL_SILU ? 2 : 1) {
             const long m = m0 + i * 32 + 8 * (e / 4) + 4 * h + e % 4;
-            if (m >= a.M) continue;
             if constexpr (TAIL == TAIL_SILU) {
 #pragma unroll
-                for (int j = 0; j < NJ; j += 2) {
-                    const int n = (n0 + j * 32) / 2 + r;
-                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], acc[i][j + 1][e]);
+                for (int j = 0; j < NJ; ++j) {
+                    const bool up = r >= 16;
+                    const int n = (n0 + j * 32) / 2 + (r & 15);
+                    const float mine = up ? acc[i][j][e + 1] : acc[i][j][e], other = __shfl_xor(up ? acc[i][j][e] : acc[i][j][e + 1], 16, 64);
+                    if (m + up < a.M && n < wide) fp4_store<TAIL>(a, m + up, n, up ? other : mine, up ? mine : other);
                 }
             } else {
+                if (m >= a.M) continue;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const int n = n0 + j * 32 + r;
@@ -144,6 +147,11 @@ __device__ __forceinline__ uintx4_t fp4_buffer(const void* p, unsigned bytes) {
     asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"                                                 \
                  : : "{m0}"(to_), "v"(offset_), "s"(rsrc_), "s"(soffset_) : "memory")
 
+// 64 bytes, one a lane, to 64 words of shared memory
+#define QE_LOAD_BYTE_TO_SHARED(to_, offset_, rsrc_, soffset_)                                                        \
+    asm volatile("s_nop 0\n\tbuffer_load_ubyte %1, %2, %3 offen lds"                                                 \
+                 : : "{m0}"(to_), "v"(offset_), "s"(rsrc_), "s"(soffset_) : "memory")
+
 // partial products [splits][M][N] -> a.out, summed in their order, with the tail
 int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStream_t stream);
 
@@ -155,5 +163,3 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
 bool fp4_both_take(int M, int N, int K);
 long fp4_both_workspace(int M, int N, int K, const void* xs, const void* scales);
 int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream);
-// scales [rows, blocks] -> words [rows, num_words], zeros behind
-void fp4_pad_scales(const unsigned char* scales, uint32_t* words, int rows, int blocks, int num_words, hipStream_t stream);

@@ -234,6 +234,40 @@ def test_nan_and_infinities(ops, kind):
     assert got[keep_m][:, keep_n].isfinite().all()
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("K", [40, 64, 96, 160, 200])
+def test_large_tiles_and_what_lies_behind_a_row(ops, kind, K):
+    """Enough rows and columns for the largest tiles; K ends inside a stage, and the row behind is NaN: every other column is exact."""
+    M, N = 3100, 4200
+    codes, scales, v = whole_matrix(N, K, K)
+    scales[1::7] = 255
+    v = torch.where((scales == 255).any(1, keepdim=True), torch.full_like(v, math.nan), v).to(DEV)
+    w = ops.MxFp4(codes.to(DEV), scales.to(DEV), K)
+    if kind == "fp4":
+        xc, xs, xv = whole_matrix(M, K, 7)
+        xs[1::5] = 255
+        xv = torch.where((xs == 255).any(1, keepdim=True), torch.full_like(xv, math.nan), xv)
+        x = ops.MxFp4(xc.to(DEV), xs.to(DEV), K)
+    else:
+        xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+        xv[1::5] = math.nan
+        x = xv.to(torch.float32 if kind == "float32" else torch.bfloat16).to(DEV)
+    want = xv.to(DEV) @ v.T
+    for m in (M, 200):
+        part = ops.MxFp4(x.codes[:m], x.scales[:m], K) if kind == "fp4" else x[:m]
+        got = ops.gemm_mxfp4(part, w, out_dtype=torch.float32).double()
+        assert torch.equal(got.isnan(), want[:m].isnan()) and torch.equal(got.nan_to_num(), want[:m].nan_to_num())
+        # (gates and ups that are 0 or NaN: the places of the activation's operands)
+        up = want[:m, N // 2:]
+        gate = want[:m, :N // 2]
+        got = ops.gemm_mxfp4(part, w, out_dtype=torch.float32, epilogue=ops.EPI_SILU_MUL).double()
+        act = gate * torch.sigmoid(gate) * up
+        assert torch.equal(got.isnan(), act.isnan())
+        # (below a gate of -88.73 the exponential, beyond 2^128, is infinite in 32 bits and silu 0 instead of 88.73 * 2^-128 < 2^-121 at the most)
+        bound = (8 + gate.abs()).nan_to_num() * 2.0 ** -23 * act.nan_to_num().abs() + 2.0 ** -121 * up.nan_to_num().abs()
+        assert ((got - act).nan_to_num().abs() <= bound).all()
+
+
 def test_rows_at_odd_elements(ops):
     """x, bias and out at no whole 16-byte piece; the numbers before and behind out stay."""
     M, N, K = 19, 40, 96
