@@ -195,7 +195,7 @@ static bool fp4_by_tiles(int M, int N, int K, int x_kind) {
 extern "C" long qe_gemm_mxfp4_workspace_bytes(const void* x, const void* x_scales, const void* scales, int M, int N, int K, int x_kind) {
     if (M <= 0 || N <= 0 || K <= 0 || !fp4_by_tiles(M, N, K, x_kind)) return 0;
     if (x_kind == X_FP4) return fp4_both_workspace(M, N, K, x_scales, scales);
-    return fp4_tiles_workspace(M, N, K, x_kind, (((uintptr_t)x & 15) | ((uintptr_t)scales & 3)) == 0);
+    return fp4_tiles_workspace(M, N, K, x_kind, x, scales);
 }
 
 // x: [M, K] bfloat16 (x_kind 0) or float32 (1), or the codes of x in 4 bits with their scales x_scales (2); codes [N, ceil(K / 32) * 16],

@@ -2,7 +2,7 @@
 // v_mfma_scale_f32_32x32x64_f8f6f4, which multiplies codes with their blocks' scales.
 //
 // A block of 2 x 2 waves computes BM rows by BN columns.  K is walked in stages of 128 through a ring of four in shared memory: 64 bytes of
-// codes and 4 of scales a row, of both sides alike, brought by loads that write to shared memory directly.  Two rows are a line of 128
+// codes a row, of both sides alike, and for every four stages 16 of scales, brought by loads that write to shared memory directly.  Two rows are a line of 128
 // bytes there, its eight pieces exchanged by the line's number (so that what 16 lanes read at a time lies in distinct banks).  Lane (r, h) =
 // (lane % 32, lane / 32) takes blocks 2 h and 2 h + 1 of row r, one in each of the stage's two k steps; the fragments of a step are
 // read while the step before is multiplied.
@@ -12,21 +12,21 @@
 #define FP4_RING 4
 
 // What the loads cannot take as it is, in one launch: the codes of x with nothing behind K in a row's last block (where K is no whole
-// blocks), and the scales of x and of the matrix in rows of whole words, zeros behind.
+// blocks), and the scales of x and of the matrix in rows of whole spans, zeros behind.
 struct Fp4Prepare {
     const uintx4_t* codes;
     uintx4_t* codes_out;
     const unsigned char *xs, *scales;
     uint32_t *xs_out, *scales_out;
-    long pieces, x_words, words;        // numbers of 16-byte pieces and of words to write, 0: none
+    unsigned pieces, x_words, words;    // numbers of 16-byte pieces and of words to write, 0: none
     unsigned blocks, num_words;
     int K;
 };
 
 __global__ __launch_bounds__(256) void fp4_prepare_kernel(Fp4Prepare p) {
-    long at = (long)blockIdx.x * 256 + threadIdx.x;
+    unsigned at = blockIdx.x * 256 + threadIdx.x;
     if (at < p.pieces) {
-        const int left = p.K - (int)((unsigned)at % p.blocks) * 32;
+        const int left = p.K - (int)(at % p.blocks) * 32;
         const uintx4_t c = p.codes[at];
         p.codes_out[at] = left < 32 ? first_codes(c, left) : c;
         return;
@@ -40,8 +40,8 @@ __global__ __launch_bounds__(256) void fp4_prepare_kernel(Fp4Prepare p) {
         from = p.scales;
         to = p.scales_out;
     }
-    const long row = (unsigned)at / p.num_words;
-    const int b = (int)((unsigned)at % p.num_words) * 4;
+    const long row = at / p.num_words;
+    const int b = (int)(at % p.num_words) * 4;
     uint32_t v = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -52,15 +52,15 @@ __global__ __launch_bounds__(256) void fp4_prepare_kernel(Fp4Prepare p) {
 struct Fp4Both {
     Fp4Args a;
     const unsigned char* x;     // codes, nothing behind K
-    const uint32_t *xw, *words; // the scales of x and of the matrix, num_words words a row
-    int nk, num_words, tiles_m, tiles_n;
+    const unsigned char *xs, *scales;   // of x and of the matrix, scale_bytes a row
+    int nk, scale_bytes, tiles_m, tiles_n;
 };
 
 template <int TAIL, int BM, int BN>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Both t) {
     constexpr int RING = FP4_RING, WM = BM / 2, WN = BN / 2, MI = WM / 32, NJ = WN / 32;
-    constexpr int LDA = BM / 64, LDB = BN / 64, LDS = (BM + BN) / 256, LD = LDA + LDB + LDS;       // a wave's loads of a stage: codes of x, of the matrix, scales
-    constexpr int B_AT = BM * 64, S_AT = B_AT + BN * 64, STAGE = S_AT + (BM + BN) * 4;
+    constexpr int LDA = BM / 64, LDB = BN / 64, LD = LDA + LDB, LDS = (BM + BN) / 256;       // a wave's loads of a stage: codes of x, of the matrix; of a span: scales
+    constexpr int SPAN = FP4_SPAN / FP4_STAGE, SPANS = 3, B_AT = BM * 64, STAGE = B_AT + BN * 64, S_AT = RING * STAGE, S_BYTES = (BM + BN) * 16;
     static_assert(BM % 128 == 0 && BN % 128 == 0 && (RING - 1) * LD < 63, "whole loads of every wave");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Fp4Args& a = t.a;
@@ -86,46 +86,60 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         const int row = fp4_matrix_row<TAIL>(n0, ((i * 4 + wave) * 8 + (lane >> 3)) * 2 + (idx >> 2), wide);
         vb[i] = row >= 0 ? row * row_bytes + piece * 16 : FP4_OUT;
     }
+    uintx4_t rsrc_a = fp4_buffer(t.x, (unsigned)((long)a.M * row_bytes)), rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * row_bytes));
     // scales: loads of 64 rows, those of x first
-    bool s_of_x[LDS];
+    uintx4_t rsrc_s[LDS];
 #pragma unroll
     for (int i = 0; i < LDS; ++i) {
         const int part = i * 4 + wave_s;
-        s_of_x[i] = part < BM / 64;
-        const int row = s_of_x[i] ? (m0 + part * 64 + lane < a.M ? m0 + part * 64 + lane : -1)
-                                  : fp4_matrix_row<TAIL>(n0, (part - BM / 64) * 64 + lane, wide);
-        vs[i] = row >= 0 ? row * (t.num_words * 4) : FP4_OUT;
+        const bool of_x = part < BM / 64;
+        const int row = of_x ? (m0 + part * 64 + lane < a.M ? m0 + part * 64 + lane : -1)
+                             : fp4_matrix_row<TAIL>(n0, (part - BM / 64) * 64 + lane, wide);
+        vs[i] = row >= 0 ? row * t.scale_bytes : FP4_OUT;
+        rsrc_s[i] = fp4_buffer(of_x ? t.xs : t.scales, (unsigned)((long)(of_x ? a.M : a.N) * t.scale_bytes));
     }
-    const uintx4_t rsrc_a = fp4_buffer(t.x, (unsigned)((long)a.M * row_bytes)), rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * row_bytes));
-    const uintx4_t rsrc_x = fp4_buffer(t.xw, (unsigned)((long)a.M * t.num_words * 4)), rsrc_w = fp4_buffer(t.words, (unsigned)((long)a.N * t.num_words * 4));
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
     int ask_k = 0;                                         // the stage that is being asked for, and its place in the ring
-    unsigned ask_at = lds0;
-    const int last_pieces = a.blocks - (t.nk - 1) * 4;     // blocks of the last stage
+    unsigned ask_at = lds0, ask_span = lds0 + S_AT;
+    // (blocks of the last stage that lie beyond the row: a lane's offset is then made one that is out of range)
+    const int off = piece < a.blocks - (t.nk - 1) * 4 ? 0 : FP4_OUT;
+    int piece_not = t.nk == 1 ? off : 0;
 #define LOAD_PIECE(i_)                                                                                                    \
     {                                                                                                                     \
-        const bool there = ask_k < t.nk;                                                                                  \
-        if ((i_) < LDA + LDB) {                                                                                           \
-            const int v_ = (i_) < LDA ? va[(i_) < LDA ? (i_) : 0] : vb[(i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0]; \
-            const int o_ = there && (ask_k + 1 < t.nk || piece < last_pieces) ? v_ : FP4_OUT;                             \
-            const int s_ = there ? ask_k * 64 : 0;                                                                        \
-            const unsigned to_ = ask_at + ((i_) < LDA ? ((i_) * 4 + wave_s) * 1024 : B_AT + (((i_) - LDA) * 4 + wave_s) * 1024); \
-            if ((i_) < LDA) { QE_LOAD_TO_SHARED(to_, o_, rsrc_a, s_, "0", ""); } else { QE_LOAD_TO_SHARED(to_, o_, rsrc_b, s_, "0", ""); } \
+        if ((i_) < LDA) {                                                                                                 \
+            constexpr int n_ = (i_) < LDA ? (i_) : 0;                                                                     \
+            QE_LOAD_TO_SHARED(ask_at + (n_ * 4 + wave_s) * 1024, va[n_] | piece_not, rsrc_a, ask_k * 64, "0", "");        \
         } else {                                                                                                          \
-            constexpr int n_ = (i_) < LDA + LDB ? 0 : (i_) < LD ? (i_) - LDA - LDB : 0;                                   \
-            const int o_ = there ? vs[n_] : FP4_OUT, s_ = there ? ask_k * 4 : 0;                                          \
-            const unsigned to_ = ask_at + S_AT + (n_ * 4 + wave_s) * 256;                                                 \
-            if (s_of_x[n_]) { QE_LOAD_WORD_TO_SHARED(to_, o_, rsrc_x, s_); } else { QE_LOAD_WORD_TO_SHARED(to_, o_, rsrc_w, s_); } \
+            constexpr int n_ = (i_) < LDA ? 0 : (i_) < LD ? (i_) - LDA : 0;                                               \
+            QE_LOAD_TO_SHARED(ask_at + B_AT + (n_ * 4 + wave_s) * 1024, vb[n_] | piece_not, rsrc_b, ask_k * 64, "0", ""); \
         }                                                                                                                 \
+    }
+    // the scales of a span of stages come with its first stage into a ring of their own
+#define LOAD_SPAN()                                                                                                       \
+    {                                                                                                                     \
+        _Pragma("unroll") for (int i = 0; i < LDS; ++i)                                                                   \
+            QE_LOAD_TO_SHARED(ask_span + (i * 4 + wave_s) * 1024, vs[i], rsrc_s[i], ask_k / SPAN * 16, "0", "");          \
+        ask_span = ask_span + S_BYTES == lds0 + S_AT + SPANS * S_BYTES ? lds0 + S_AT : ask_span + S_BYTES;                \
     }
 #define LOAD_CASE(i_) case i_: if constexpr ((i_) < LD) LOAD_PIECE(i_) break;
 #define LOADS_OF(n_)                                                                                                      \
     switch (n_) {                                                                                                         \
-        LOAD_CASE(0) LOAD_CASE(1) LOAD_CASE(2) LOAD_CASE(3) LOAD_CASE(4) LOAD_CASE(5) LOAD_CASE(6) LOAD_CASE(7) LOAD_CASE(8) LOAD_CASE(9) \
+        LOAD_CASE(0) LOAD_CASE(1) LOAD_CASE(2) LOAD_CASE(3) LOAD_CASE(4) LOAD_CASE(5) LOAD_CASE(6) LOAD_CASE(7)                           \
         default: break;                                                                                                   \
     }
-    static_assert(LD <= 10, "a case for every load");
-#define ASKED() { ++ask_k; ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE; }
+    static_assert(LD <= 8, "a case for every load");
+    // (beyond the last stage every load is out of range: the buffers have no bytes)
+    int ask_left = t.nk;
+#define ASKED()                                                                                                           \
+    {                                                                                                                     \
+        ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE;                                           \
+        ++ask_k;                                                                                                          \
+        if (--ask_left <= 0) {                                                                                            \
+            rsrc_a[2] = 0; rsrc_b[2] = 0; ask_k = 0;                                                                      \
+            _Pragma("unroll") for (int i = 0; i < LDS; ++i) rsrc_s[i][2] = 0;                                             \
+        }                                                                                                                 \
+        piece_not = off & (ask_k + 1 == t.nk ? -1 : 0);                                                                   \
+    }
     // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
 #define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
 
@@ -136,7 +150,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         fa_at[q] = (ra >> 1) * 128 + ((((ra & 1) * 4 + 2 * h + q) ^ ((ra >> 2) & 3)) * 16);
         fb_at[q] = B_AT + (rb >> 1) * 128 + ((((rb & 1) * 4 + 2 * h + q) ^ ((rb >> 2) & 3)) * 16);
     }
-    const int sa_at = S_AT + (wm + r) * 4, sb_at = S_AT + (BM + wn + r) * 4;
+    const int sa_at = S_AT + (wm + r) * 16 + 2 * h, sb_at = S_AT + (BM + wn + r) * 16 + 2 * h;
+    int read_k = 0, read_span = 0;                         // the stage whose scales are read, and the place of its span
     floatx16_t acc[MI][NJ];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -152,10 +167,15 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         if ((p_) < MI) fa[q_][(p_) < MI ? (p_) : 0] = *(const uintx4_t*)(smem + (place_) + fa_at[q_] + (p_) * 2048);      \
         else fb[q_][(p_) < MI ? 0 : (p_) - MI] = *(const uintx4_t*)(smem + (place_) + fb_at[q_] + ((p_) - MI) * 2048);    \
     }
-#define READ_SCALE(par_, place_, p_)                                                                                      \
+#define READ_SCALE(par_, p_)                                                                                              \
     {                                                                                                                     \
-        if ((p_) < MI) sa[par_][(p_) < MI ? (p_) : 0] = *(const uint32_t*)(smem + (place_) + sa_at + (p_) * 128) >> (16 * h); \
-        else sb[par_][(p_) < MI ? 0 : (p_) - MI] = *(const uint32_t*)(smem + (place_) + sb_at + ((p_) - MI) * 128) >> (16 * h); \
+        const int at_ = read_span + read_k % SPAN * 4;                                                                    \
+        if ((p_) < MI) sa[par_][(p_) < MI ? (p_) : 0] = *(const uint16_t*)(smem + at_ + sa_at + (p_) * 512);              \
+        else sb[par_][(p_) < MI ? 0 : (p_) - MI] = *(const uint16_t*)(smem + at_ + sb_at + ((p_) - MI) * 512);            \
+    }
+#define READ_ON()                                                                                                         \
+    {                                                                                                                     \
+        if (++read_k % SPAN == 0) read_span = read_span + S_BYTES == SPANS * S_BYTES ? 0 : read_span + S_BYTES;           \
     }
     constexpr int R = MI + NJ, PER = MI * NJ, LHALF = (LD + 1) / 2;
     // step q_ of a stage of parity par_: between its matrix instructions the fragments of the next step are read from place from_ (for step 0 of
@@ -165,7 +185,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         _Pragma("unroll") for (int p = 0; p < R; ++p)                                                                     \
             if (p * PER / (2 * R) == sl) {                                                                                \
                 READ_FRAG((q_) ^ 1, from_, p)                                                                             \
-                if ((q_) == 1) READ_SCALE((par_) ^ 1, from_, p)                                                           \
+                if ((q_) == 1) READ_SCALE((par_) ^ 1, p)                                                                  \
             }                                                                                                             \
         const int i = sl / NJ, j = sl % NJ;                                                                               \
         const intx8_t xa = {(int)fa[q_][i][0], (int)fa[q_][i][1], (int)fa[q_][i][2], (int)fa[q_][i][3], 0, 0, 0, 0};      \
@@ -175,8 +195,11 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
             if (l * PER / LHALF == sl && ((q_) == 1 || l + LHALF < LD)) { LOADS_OF((q_) == 1 ? l : l + LHALF) }           \
         __builtin_amdgcn_sched_barrier(0);                                                                                \
     }
+    // (the scales come before their stages' codes, and a stage is waited for by the loads behind it: with more of those than are counted,
+    // where a span lies between, the wait is only longer)
 #pragma unroll
     for (int s = 0; s < RING; ++s) {
+        if (ask_left > 0 && s % SPAN == 0) LOAD_SPAN()
 #pragma unroll
         for (int i = 0; i < LD; ++i)
             if (s + 1 < RING || i < LHALF) { LOADS_OF(i) }
@@ -186,7 +209,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 #pragma unroll
     for (int p = 0; p < R; ++p) {
         READ_FRAG(0, 0, p)
-        READ_SCALE(0, 0, p)
+        READ_SCALE(0, p)
     }
     // behind the barrier in the middle of a stage nothing of its place is read any more, and the next stage has arrived
 #define STAGE_OF(par_)                                                                                                    \
@@ -195,6 +218,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         K_STEP(0, par_, at)                                                                                               \
         ASKED()                                                                                                           \
         MEET((RING - 2) * LD)                                                                                             \
+        if (ask_left > 0 && ask_k % SPAN == 0) LOAD_SPAN()                                                                \
+        READ_ON()                                                                                                         \
         K_STEP(1, par_, next)                                                                                             \
         at = next;                                                                                                        \
     }
@@ -212,6 +237,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 #undef LOADS_OF
 #undef LOAD_CASE
 #undef LOAD_PIECE
+#undef LOAD_SPAN
+#undef READ_ON
 #undef ASKED
 #undef MEET
     fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn);
@@ -219,7 +246,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 
 template <int TAIL, int BM, int BN>
 static int fp4_both_launch(Fp4Both t, hipStream_t stream) {
-    constexpr int SHARED = FP4_RING * (BM + BN) * 68;
+    constexpr int SHARED = (BM + BN) * (FP4_RING * 64 + 3 * 16);
+    static_assert(SHARED <= 160 * 1024, "the ring must fit a compute unit");
     t.tiles_m = qe_cdiv(t.a.M, BM);
     t.tiles_n = qe_cdiv(t.a.N, BN);
     const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
@@ -229,55 +257,50 @@ static int fp4_both_launch(Fp4Both t, hipStream_t stream) {
     return 0;
 }
 
-static int words_of(int K) { return qe_cdiv(K, FP4_STAGE); }
-
 // The kernel's 32-bit places reach all of the operands.
 bool fp4_both_take(int M, int N, int K) {
     return (long)N * qe_cdiv(K, 32) * 16 < (1L << 31) - 64 && (long)M * qe_cdiv(K, 32) * 16 < (1L << 31) - 64;
 }
 
-static bool pads(int K, const void* scales) { return K % FP4_STAGE || ((uintptr_t)scales & 3); }
-
 long fp4_both_workspace(int M, int N, int K, const void* xs, const void* scales) {
-    long bytes = K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0;
-    if (pads(K, xs)) bytes += (long)M * words_of(K) * 4;
-    if (pads(K, scales)) bytes += (long)N * words_of(K) * 4;
-    return bytes;
+    return (K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0) + (fp4_scales_whole(K, xs) ? 0 : fp4_scales_bytes(M, K)) +
+           (fp4_scales_whole(K, scales) ? 0 : fp4_scales_bytes(N, K));
 }
 
 int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
     Fp4Both t{};
     t.a = a;
-    t.nk = t.num_words = words_of(a.K);
+    t.nk = qe_cdiv(a.K, FP4_STAGE);
+    t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
     unsigned char* ws = (unsigned char*)workspace;
     t.x = (const unsigned char*)a.x;
-    t.xw = (const uint32_t*)a.xs;
-    t.words = (const uint32_t*)a.scales;
+    t.xs = a.xs;
+    t.scales = a.scales;
     Fp4Prepare p{};
     p.blocks = a.blocks;
-    p.num_words = t.num_words;
+    p.num_words = t.scale_bytes / 4;
     p.K = a.K;
     if (a.K % 32) {
         p.codes = (const uintx4_t*)a.x;
         p.codes_out = (uintx4_t*)ws;
-        p.pieces = (long)a.M * a.blocks;
+        p.pieces = (unsigned)a.M * a.blocks;
         t.x = ws;
-        ws += p.pieces * 16;
+        ws += (long)p.pieces * 16;
     }
-    if (pads(a.K, a.xs)) {
+    if (!fp4_scales_whole(a.K, a.xs)) {
         p.xs = a.xs;
         p.xs_out = (uint32_t*)ws;
-        p.x_words = (long)a.M * t.num_words;
-        t.xw = p.xs_out;
-        ws += p.x_words * 4;
+        p.x_words = (unsigned)(fp4_scales_bytes(a.M, a.K) / 4);
+        t.xs = ws;
+        ws += (long)p.x_words * 4;
     }
-    if (pads(a.K, a.scales)) {
+    if (!fp4_scales_whole(a.K, a.scales)) {
         p.scales = a.scales;
         p.scales_out = (uint32_t*)ws;
-        p.words = (long)a.N * t.num_words;
-        t.words = p.scales_out;
+        p.words = (unsigned)(fp4_scales_bytes(a.N, a.K) / 4);
+        t.scales = ws;
     }
-    if (const long all = p.pieces + p.x_words + p.words) fp4_prepare_kernel<<<(unsigned)((all + 255) / 256), 256, 0, stream>>>(p);
+    if (const long all = (long)p.pieces + p.x_words + p.words) fp4_prepare_kernel<<<qe_cdiv(all, 256), 256, 0, stream>>>(p);
     const bool large = (long)qe_cdiv(a.M, 256) * qe_cdiv(a.N, 256) >= 128;
     int rc;
 #define QE_GO(T_) rc = large ? fp4_both_launch<T_, 256, 256>(t, stream) : fp4_both_launch<T_, 128, 128>(t, stream)

@@ -37,10 +37,34 @@ __global__ __launch_bounds__(256) void fp4_planes_kernel(const T* __restrict__ x
     }
 }
 
+// scales [rows, blocks] -> [rows, words * 4], zeros behind
+__global__ __launch_bounds__(256) void fp4_scales_kernel(const unsigned char* __restrict__ scales, uint32_t* __restrict__ out, int rows,
+                                                         int blocks, unsigned words) {
+    const unsigned at = blockIdx.x * 256 + threadIdx.x, row = at / words;
+    if (row >= (unsigned)rows) return;
+    const int b = (int)(at - row * words) * 4;
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (b + e < blocks) v |= (uint32_t)scales[(long)row * blocks + b + e] << (8 * e);
+    out[at] = v;
+}
+
+bool fp4_scales_whole(int K, const void* scales) { return K % FP4_SPAN == 0 && ((uintptr_t)scales & 15) == 0; }
+
+long fp4_scales_bytes(int rows, int K) { return (long)rows * qe_cdiv(K, FP4_SPAN) * (FP4_SPAN / 32); }
+
+void fp4_pad_scales(const unsigned char* scales, unsigned char* out, int rows, int blocks, int K, hipStream_t stream) {
+    const long words = fp4_scales_bytes(rows, K) / 4;      // (below 2^31 / 16: fp4_tiles_take, fp4_both_take)
+    fp4_scales_kernel<<<qe_cdiv(words, 256), 256, 0, stream>>>(scales, (uint32_t*)out, rows, blocks, (unsigned)(words / rows));
+}
+
 struct Fp4Tiles {
     Fp4Args a;
     const uint16_t* planes;     // rows of x, row_bytes apart, plane after plane
     unsigned row_bytes, plane_bytes, x_bytes;      // (x_bytes: of all planes)
+    const unsigned char* scales;
+    int scale_bytes;            // of a row
     int num_planes, nk, k_in_row;                  // (numbers of K that a row holds: K, or whole stages where it is a plane's)
     int tiles_m, tiles_n;
     int per_split;              // stages of a cut: block (., y) sums the stages from y * per_split on
@@ -94,9 +118,10 @@ int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStre
 template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>
 __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) {
     constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, MI = WM / 32, NJ = WN / 32, QS = SK / 16, BL = SK / 32;
-    constexpr int LDA = BM * SK / (512 * NW), LDB = BN * SK / (2048 * NW), LDS = BN * BL / (64 * NW), LD = LDA + LDB + LDS;      // a wave's loads of a stage: x, codes, scales
-    constexpr int B_AT = BM * SK * 2, S_AT = B_AT + BN * SK / 2, STAGE = S_AT + BN * BL * 4;
-    static_assert(NW == 4 && (SK == 128 || SK == 64) && BM * SK % (512 * NW) == 0 && BN * BL % (64 * NW) == 0, "whole loads of every wave");
+    constexpr int LDA = BM * SK / (512 * NW), LDB = BN * SK / (2048 * NW), LD = LDA + LDB;      // a wave's loads of a stage: x, codes
+    constexpr int SPAN = FP4_SPAN / SK, SLOADS = BN / (64 * NW) > 0 ? BN / (64 * NW) : 1, SROWS = BN / (NW * SLOADS);      // stages of a span of scales; a wave's loads of it, of so many rows
+    constexpr int B_AT = BM * SK * 2, STAGE = B_AT + BN * SK / 2, S_AT = RING * STAGE, S_BYTES = BN * 16;
+    static_assert(NW == 4 && (SK == 128 || SK == 64) && BM * SK % (512 * NW) == 0 && SROWS * NW * SLOADS == BN, "whole loads of every wave");
     constexpr int PER = MI * NJ, PER_STEP = (LD + QS - 1) / QS, HEAD = 2 * PER_STEP < LD ? 2 * PER_STEP : LD;      // loads of a k step; of the two steps behind the barrier
     static_assert((RING - 2) * LD + HEAD < 64 && LD <= 16 && MI <= PER, "the loads in flight can be counted");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -113,7 +138,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     // The loads: per lane the bytes within x (from row m0), the codes and the scales; beyond the matrix: out of range, which arrives as zero.
     // The pieces of a row (of x), of two or four rows that are a line (of the codes), are exchanged by the row's or line's number, so that what
     // 16 lanes read at a time lies in distinct banks.
-    int va[LDA], vb[LDB], vs[LDS];
+    int va[LDA], vb[LDB], vs[SLOADS];
     constexpr int AP = SK / 8, AR = 64 / AP;               // pieces of a row of x, rows of a load
     const int a_row = wave * AR + lane / AP;
     const int a_piece = SK == 128 ? (lane & 15) ^ (a_row & 15) : (lane & 7) ^ ((a_row >> 1) & 7);
@@ -128,36 +153,41 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
         const int row = fp4_matrix_row<TAIL>(n0, ((i * NW + wave) * 8 + line) * (8 / BL) + idx / BL, wide);
         vb[i] = row >= 0 ? row * (a.blocks * 16) + b_piece * 16 : FP4_OUT;
     }
-    const int s_block = lane & (BL - 1);
 #pragma unroll
-    for (int i = 0; i < LDS; ++i) {
-        const int row = fp4_matrix_row<TAIL>(n0, (i * NW + wave) * (64 / BL) + lane / BL, wide);
-        vs[i] = row >= 0 ? row * a.blocks + s_block : FP4_OUT;
+    for (int i = 0; i < SLOADS; ++i) {
+        const int row = lane < SROWS ? fp4_matrix_row<TAIL>(n0, (i * NW + wave) * SROWS + lane, wide) : -1;
+        vs[i] = row >= 0 ? row * t.scale_bytes : FP4_OUT;
     }
     uintx4_t rsrc_a = fp4_buffer((const unsigned char*)t.planes + (unsigned long)m0 * t.row_bytes, t.x_bytes - (unsigned)m0 * t.row_bytes);
-    uintx4_t rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * a.blocks * 16)), rsrc_s = fp4_buffer(a.scales, (unsigned)((long)a.N * a.blocks));
+    uintx4_t rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * a.blocks * 16)), rsrc_s = fp4_buffer(t.scales, (unsigned)((long)a.N * t.scale_bytes));
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
-    // the stage that is being asked for: its place in the ring, its step along K, its bytes within x, and the stages left
+    // The stage that is being asked for: its place in the ring, its step along K, its bytes within x, and the stages left.  The scales of a span of
+    // stages come with its first one (or the first of all) into a ring of their own, of one span more than stages are on their way.
     const int first_stage = blockIdx.y * t.per_split, stages = min(t.nk * t.num_planes - first_stage, t.per_split);
     int ask_k = __builtin_amdgcn_readfirstlane(first_stage % t.nk), ask_left = __builtin_amdgcn_readfirstlane(stages);
-    unsigned ask_plane = __builtin_amdgcn_readfirstlane(first_stage / t.nk) * t.plane_bytes, ask_at = lds0;
+    unsigned ask_plane = __builtin_amdgcn_readfirstlane(first_stage / t.nk) * t.plane_bytes, ask_at = lds0, ask_span = lds0 + S_AT;
     // (K is no whole stages: of the last one's pieces some lie beyond the row; a lane's offset is then made one that is out of range)
     const int x_left = t.k_in_row - (t.nk - 1) * SK, blocks_left = a.blocks - (t.nk - 1) * BL;
-    const int a_off = a_piece * 8 < x_left ? 0 : FP4_OUT, b_off = b_piece < blocks_left ? 0 : FP4_OUT, s_off = s_block < blocks_left ? 0 : FP4_OUT;
-    int a_not = t.nk == ask_k + 1 ? a_off : 0, b_not = t.nk == ask_k + 1 ? b_off : 0, s_not = t.nk == ask_k + 1 ? s_off : 0;
+    const int a_off = a_piece * 8 < x_left ? 0 : FP4_OUT, b_off = b_piece < blocks_left ? 0 : FP4_OUT;
+    int a_not = t.nk == ask_k + 1 ? a_off : 0, b_not = t.nk == ask_k + 1 ? b_off : 0;
     if constexpr (TAIL == TAIL_PARTIAL) t.a.out = (float*)t.a.out + (long)blockIdx.y * a.M * a.N;
 #define LOAD_PIECE(i_)                                                                                                    \
     {                                                                                                                     \
         if ((i_) < LDA) {                                                                                                 \
             constexpr int n_ = (i_) < LDA ? (i_) : 0;                                                                     \
             QE_LOAD_TO_SHARED(ask_at + (n_ * NW + wave_s) * 1024, va[n_] | a_not, rsrc_a, ask_plane + ask_k * (SK * 2), "0", ""); \
-        } else if ((i_) < LDA + LDB) {                                                                                    \
-            constexpr int n_ = (i_) < LDA ? 0 : (i_) < LDA + LDB ? (i_) - LDA : 0;                                        \
-            QE_LOAD_TO_SHARED(ask_at + B_AT + (n_ * NW + wave_s) * 1024, vb[n_] | b_not, rsrc_b, ask_k * (SK / 2), "0", ""); \
         } else {                                                                                                          \
-            constexpr int n_ = (i_) < LDA + LDB ? 0 : (i_) < LD ? (i_) - LDA - LDB : 0;                                   \
-            QE_LOAD_BYTE_TO_SHARED(ask_at + S_AT + (n_ * NW + wave_s) * 256, vs[n_] | s_not, rsrc_s, ask_k * BL);         \
+            constexpr int n_ = (i_) < LDA ? 0 : (i_) < LD ? (i_) - LDA : 0;                                               \
+            QE_LOAD_TO_SHARED(ask_at + B_AT + (n_ * NW + wave_s) * 1024, vb[n_] | b_not, rsrc_b, ask_k * (SK / 2), "0", ""); \
         }                                                                                                                 \
+    }
+#define LOAD_SPAN()                                                                                                       \
+    {                                                                                                                     \
+        if (SROWS == 64 || lane < SROWS) {                                                                                \
+            _Pragma("unroll") for (int i = 0; i < SLOADS; ++i)                                                            \
+                QE_LOAD_TO_SHARED(ask_span + (i * NW + wave_s) * (SROWS * 16), vs[i], rsrc_s, ask_k / SPAN * 16, "0", ""); \
+        }                                                                                                                 \
+        ask_span = ask_span + S_BYTES == lds0 + S_AT + (RING + 1) * S_BYTES ? lds0 + S_AT : ask_span + S_BYTES;           \
     }
     // (beyond the last stage every load is out of range: the buffers have no bytes)
 #define ASKED()                                                                                                           \
@@ -166,7 +196,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
         if (++ask_k == t.nk) { ask_k = 0; ask_plane += t.plane_bytes; }                                                   \
         if (--ask_left <= 0) { rsrc_a[2] = 0; rsrc_b[2] = 0; rsrc_s[2] = 0; ask_k = 0; ask_plane = 0; }                   \
         const int ends_ = ask_k + 1 == t.nk ? -1 : 0;                                                                     \
-        a_not = a_off & ends_; b_not = b_off & ends_; s_not = s_off & ends_;                                              \
+        a_not = a_off & ends_; b_not = b_off & ends_;                                                                     \
     }
     // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
 #define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
@@ -180,7 +210,14 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     for (int b = 0; b < BL / 2; ++b)
         fb_at[b] = B_AT + (SK == 128 ? (wn + r) / 2 * 128 + ((((r & 1) * 4 + 2 * b + h) ^ ((r >> 2) & 3)) * 16)
                                      : (wn + r) / 4 * 128 + ((((r & 3) * 2 + h) ^ ((r >> 3) & 1)) * 16));
-    const int fs_at = S_AT + ((wn + r) * BL + h) * 4;
+    const int fs_at = S_AT + (wn + r) * 16 + h;
+    // of the stage that is read from: its step along K and the place of its span
+    int read_k = ask_k, read_span = 0;
+#define READ_ON()                                                                                                         \
+    {                                                                                                                     \
+        if (++read_k == t.nk) read_k = 0;                                                                                 \
+        if (read_k % SPAN == 0) read_span = read_span + S_BYTES == (RING + 1) * S_BYTES ? 0 : read_span + S_BYTES;        \
+    }
     floatx16_t acc[MI][NJ];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -195,7 +232,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #define READ_CODES(to_, b_, place_, j_)                                                                                   \
     {                                                                                                                     \
         code[to_][j_] = *(const uintx4_t*)(smem + (place_) + fb_at[(b_) < BL / 2 ? (b_) : 0] + (j_) * (SK * 16));         \
-        word[to_][j_] = *(const uint32_t*)(smem + (place_) + fs_at + (j_) * (32 * BL * 4) + (b_) * 8);                    \
+        word[to_][j_] = smem[read_span + read_k % SPAN * BL + fs_at + (b_) * 2 + (j_) * 512];                             \
     }
     // the eight numbers of k step q_, of the codes that are in registers
 #define EXPAND(q_, j_)                                                                                                    \
@@ -210,6 +247,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
         if (SK == 64 && (q_) == QS - 1) {                                                                                 \
             _Pragma("unroll") for (int j = 0; j < NJ; ++j) { code[0][j] = code[1][j]; word[0][j] = word[1][j]; }          \
         }                                                                                                                 \
+        if ((q_) == QS - 2) READ_ON()                                                                                     \
         _Pragma("unroll") for (int sl = 0; sl < PER; ++sl) {                                                              \
             if (sl < MI) { if ((q_) < QS - 2) { READ_A((q_) + 2, place_, sl < MI ? sl : 0) } else { READ_A((q_) + 2 - QS, next_, sl < MI ? sl : 0) } } \
             if (sl < NJ) {                                                                                                \
@@ -222,7 +260,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
                 if (l * PER / PER_STEP == sl) LOADS_OF((((q_) + 2) & (QS - 1)) * PER_STEP + l)                            \
             __builtin_amdgcn_sched_barrier(0);                                                                            \
         }                                                                                                                 \
-        if ((q_) == QS - 3) { ASKED() MEET((RING - 2) * LD) }                                                             \
+        if ((q_) == QS - 3) { ASKED() MEET((RING - 2) * LD) if (ask_left > 0 && ask_k % SPAN == 0) LOAD_SPAN() }          \
     }
 #define LOADS_OF(n_)                                                                                                      \
     switch (n_) {                                                                                                         \
@@ -233,8 +271,12 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     }
 #define LOAD_CASE(i_) if constexpr ((i_) < LD) LOAD_PIECE(i_) break;
 
+    // (the scales come before their stages' codes, and a stage is waited for by the loads behind it: with more of those than are counted,
+    // where a span lies between, the wait is only longer)
+    LOAD_SPAN()
 #pragma unroll
     for (int s = 0; s < RING; ++s) {
+        if (s > 0 && ask_left > 0 && ask_k % SPAN == 0) LOAD_SPAN()
 #pragma unroll
         for (int i = 0; i < LD; ++i)
             if (s + 1 < RING || i < HEAD) { LOADS_OF(i) }
@@ -267,6 +309,8 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #undef LOADS_OF
 #undef LOAD_CASE
 #undef LOAD_PIECE
+#undef LOAD_SPAN
+#undef READ_ON
 #undef ASKED
 #undef MEET
 #undef READ_A
@@ -277,7 +321,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 
 template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>
 static int fp4_tiles_launch(Fp4Tiles t, int splits, hipStream_t stream) {
-    constexpr int SHARED = RING * (BM * SK * 2 + BN * SK / 2 + BN * SK / 8);
+    constexpr int SHARED = RING * (BM * SK * 2 + BN * SK / 2) + (RING + 1) * BN * 16;
     static_assert(SHARED <= 160 * 1024, "the ring must fit a compute unit");
     t.tiles_m = qe_cdiv(t.a.M, BM);
     t.tiles_n = qe_cdiv(t.a.N, BN);
@@ -317,12 +361,13 @@ static Fp4Shape fp4_tiles_shape(int M, int N, int K, int x_kind) {
     return s;
 }
 
-long fp4_tiles_workspace(int M, int N, int K, int x_kind, bool aligned) {
+long fp4_tiles_workspace(int M, int N, int K, int x_kind, const void* x, const void* scales) {
+    const bool aligned = ((uintptr_t)x & 15) == 0;
     const Fp4Shape s = fp4_tiles_shape(M, N, K, x_kind);
     long bytes = s.splits > 1 ? (4L * s.splits * M * N + 15) / 16 * 16 : 0;
     if (x_kind == X_F32) bytes += 6L * M * padded(K);
     else if (K % 8 || !aligned) bytes += 2L * M * padded(K);
-    return bytes;
+    return bytes + (fp4_scales_whole(K, scales) ? 0 : fp4_scales_bytes(N, K));
 }
 
 int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
@@ -338,7 +383,7 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     t.row_bytes = (unsigned)t.k_in_row * 2;
     t.plane_bytes = t.row_bytes * (unsigned)a.M;
     t.x_bytes = t.plane_bytes * t.num_planes;
-    // the workspace: the cuts' products, then what is made of x
+    // the workspace: the cuts' products, then what is made of x, then of the scales
     float* parts = (float*)workspace;
     unsigned char* ws = (unsigned char*)workspace + (s.splits > 1 ? (4L * s.splits * a.M * a.N + 15) / 16 * 16 : 0);
     t.planes = as_it_is ? (const uint16_t*)a.x : (const uint16_t*)ws;
@@ -346,6 +391,13 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
         const dim3 grid(qe_cdiv(Kp, 1024), a.M < 65535 ? a.M : 65535);
         if (x_kind == X_F32) fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
         else fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
+        ws += t.x_bytes;
+    }
+    t.scales = a.scales;
+    t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
+    if (!fp4_scales_whole(a.K, a.scales)) {
+        fp4_pad_scales(a.scales, ws, a.N, a.blocks, a.K, stream);
+        t.scales = ws;
     }
     if (s.splits > 1) t.a.out = parts;
     int rc;

@@ -142,22 +142,19 @@ __device__ __forceinline__ uintx4_t fp4_buffer(const void* p, unsigned bytes) {
     return d;
 }
 
-// 64 words, one a lane, to shared memory (see QE_LOAD_TO_SHARED)
-#define QE_LOAD_WORD_TO_SHARED(to_, offset_, rsrc_, soffset_)                                                        \
-    asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"                                                 \
-                 : : "{m0}"(to_), "v"(offset_), "s"(rsrc_), "s"(soffset_) : "memory")
-
-// 64 bytes, one a lane, to 64 words of shared memory
-#define QE_LOAD_BYTE_TO_SHARED(to_, offset_, rsrc_, soffset_)                                                        \
-    asm volatile("s_nop 0\n\tbuffer_load_ubyte %1, %2, %3 offen lds"                                                 \
-                 : : "{m0}"(to_), "v"(offset_), "s"(rsrc_), "s"(soffset_) : "memory")
+// Scales travel 16 at a time, those of FP4_SPAN numbers of a row: the kernels of many rows want rows of whole such pieces.  Rows of other
+// lengths are copied, zeros behind.
+#define FP4_SPAN 512
+bool fp4_scales_whole(int K, const void* scales);
+long fp4_scales_bytes(int rows, int K);
+void fp4_pad_scales(const unsigned char* scales, unsigned char* out, int rows, int blocks, int K, hipStream_t stream);
 
 // partial products [splits][M][N] -> a.out, summed in their order, with the tail
 int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStream_t stream);
 
 // gemm_mxfp4_tiles.hip: the products of many rows of 16 or 32 bits; the bytes of workspace that these sizes take
 bool fp4_tiles_take(int M, int N, int K, int x_kind);
-long fp4_tiles_workspace(int M, int N, int K, int x_kind, bool aligned);
+long fp4_tiles_workspace(int M, int N, int K, int x_kind, const void* x, const void* scales);
 int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream);
 // gemm_mxfp4_both.hip: many rows that are in 4 bits themselves
 bool fp4_both_take(int M, int N, int K);
