@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
     {                                                                                                                     \
         if (++read_k % SPAN == 0) read_span = read_span + S_BYTES == SPANS * S_BYTES ? 0 : read_span + S_BYTES;           \
     }
-    constexpr int R = MI + NJ, PER = MI * NJ, LHALF = (LD + 1) / 2;
+    constexpr int R = MI + NJ, PER = MI * NJ, LHALF = LD;                // (all of a stage's loads go out in the step behind the barrier)
     // step q_ of a stage of parity par_: between its matrix instructions the fragments of the next step are read from place from_ (for step 0 of
     // the next stage with its scales), and half of the loads of the stage that is being asked for go out
 #define K_STEP(q_, par_, from_)                                                                                           \
@@ -241,7 +241,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 #undef READ_ON
 #undef ASKED
 #undef MEET
-    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn);
+    static_assert(4 * fp4_strip_bytes<NJ>() <= S_AT, "the waves' strips must fit the ring");
+    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn, smem + wave * fp4_strip_bytes<NJ>());
 }
 
 template <int TAIL, int BM, int BN>

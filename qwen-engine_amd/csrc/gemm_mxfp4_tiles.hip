@@ -122,8 +122,8 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     constexpr int SPAN = FP4_SPAN / SK, SLOADS = BN / (64 * NW) > 0 ? BN / (64 * NW) : 1, SROWS = BN / (NW * SLOADS);      // stages of a span of scales; a wave's loads of it, of so many rows
     constexpr int B_AT = BM * SK * 2, STAGE = B_AT + BN * SK / 2, S_AT = RING * STAGE, S_BYTES = BN * 16;
     static_assert(NW == 4 && (SK == 128 || SK == 64) && BM * SK % (512 * NW) == 0 && SROWS * NW * SLOADS == BN, "whole loads of every wave");
-    constexpr int PER = MI * NJ, PER_STEP = (LD + QS - 1) / QS, HEAD = 2 * PER_STEP < LD ? 2 * PER_STEP : LD;      // loads of a k step; of the two steps behind the barrier
-    static_assert((RING - 2) * LD + HEAD < 64 && LD <= 16 && MI <= PER, "the loads in flight can be counted");
+    constexpr int PER = MI * NJ, PER_STEP = (LD + QS / 2 - 1) / (QS / 2) < PER ? (LD + QS / 2 - 1) / (QS / 2) : PER, HEAD = 2 * PER_STEP < LD ? 2 * PER_STEP : LD;      // loads of a k step; of the two steps behind the barrier
+    static_assert((RING - 2) * LD + HEAD < 64 && LD <= 16 && MI <= PER && PER_STEP * QS >= LD, "the loads in flight can be counted");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Fp4Args& a = t.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
@@ -316,7 +316,8 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #undef READ_A
 #undef READ_CODES
 #undef EXPAND
-    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn);
+    static_assert(4 * fp4_strip_bytes<NJ>() <= S_AT, "the waves' strips must fit the ring");
+    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn, smem + wave * fp4_strip_bytes<NJ>());
 }
 
 template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>

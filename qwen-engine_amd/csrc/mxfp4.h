@@ -60,10 +60,6 @@ struct Fp4Args {
 // What becomes of a sum: row m, column n (silu: gate and up of column n of N / 2).
 template <int TAIL>
 __device__ __forceinline__ void fp4_store(const Fp4Args& a, long m, int n, float v, float up) {
-    if constexpr (TAIL == TAIL_PARTIAL) {
-        ((float*)a.out)[m * a.N + n] = v;
-        return;
-    }
     if (a.bias) {
         v += a.bias[n];
         if constexpr (TAIL == TAIL_SILU) up += a.bias[a.N / 2 + n];
@@ -99,34 +95,76 @@ __device__ __forceinline__ int fp4_matrix_row(int n0, int i, int wide) {
     }
 }
 
-// The sums of a wave's tiles of 32 x 32 from row m0, column n0 of the whole product on: lane (r, h) = (lane % 32, lane / 32) has column
-// r of a tile and its rows 8 b + 4 h + e.  Silu: lanes r < 16 have gates, the others their ups; of two rows the former finish the first, the
-// latter the second.
+// The sums of a wave's tiles of 32 x 32, from row m0 and column n0 of the whole product on: lane (r, h) = (lane % 32, lane / 32) has column
+// r of a tile and its rows 8 b + 4 h + e.  Stored from there, an instruction would write 2 rows of 64 or 128 bytes, two or four bytes a
+// lane (a tile of 256 x 256 took 20 us to store); so a strip of 32 rows at a time is turned round in the wave's own piece of shared
+// memory, and a lane stores four columns.  Silu: of 32 columns of a tile 16 are gates and 16 their ups.
+template <int NJ> constexpr int fp4_strip_bytes() { return 32 * (NJ * 32 + 8) * 4; }     // (8: the rows that two halves of a wave write lie in other banks)
+
 template <int TAIL, int MI, int NJ>
-__device__ __forceinline__ void fp4_store_tiles(const Fp4Args& a, const floatx16_t (&acc)[MI][NJ], int m0, int n0) {
-    const int r = threadIdx.x & 31, h = (threadIdx.x & 63) >> 5, wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+__device__ __forceinline__ void fp4_store_tiles(const Fp4Args& a, const floatx16_t (&acc)[MI][NJ], int m0, int n0, unsigned char* strip_at) {
+    constexpr int ROW = NJ * 32 + 8, COLS = TAIL == TAIL_SILU ? NJ * 16 : NJ * 32, LANES = COLS / 4, ROWS = 64 / LANES;      // lanes of a row, rows of an instruction
+    float* strip = (float*)strip_at;
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5, wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+    const int col = lane % LANES * 4, from = TAIL == TAIL_SILU ? col / 16 * 32 + col % 16 : col;
+    const int n = (TAIL == TAIL_SILU ? n0 / 2 : n0) + col;
+    const bool four = wide % 4 == 0 && ((unsigned long)a.out & 15) == 0 && n + 4 <= wide;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f}, bias_up[4] = {0.f, 0.f, 0.f, 0.f};
+    if (TAIL != TAIL_PARTIAL && a.bias) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int e = 0; e < 4; ++e)
+            if (n + e < wide) {
+                bias[e] = a.bias[n + e];
+                if constexpr (TAIL == TAIL_SILU) bias_up[e] = a.bias[wide + n + e];
+            }
+    }
 #pragma unroll
-        for (int e = 0; e < 16; e += TAIL == TAIL_SILU ? 2 : 1) {
-            const long m = m0 + i * 32 + 8 * (e / 4) + 4 * h + e % 4;
-            if constexpr (TAIL == TAIL_SILU) {
+    for (int i = 0; i < MI; ++i) {
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const bool up = r >= 16;
-                    const int n = (n0 + j * 32) / 2 + (r & 15);
-                    const float mine = up ? acc[i][j][e + 1] : acc[i][j][e], other = __shfl_xor(up ? acc[i][j][e] : acc[i][j][e + 1], 16, 64);
-                    if (m + up < a.M && n < wide) fp4_store<TAIL>(a, m + up, n, up ? other : mine, up ? mine : other);
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) strip[(8 * (e / 4) + 4 * h + e % 4) * ROW + j * 32 + r] = acc[i][j][e];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 4
+        for (int k = 0; k < 32 / ROWS; ++k) {
+            const int row = k * ROWS + lane / LANES;
+            const long m = m0 + i * 32 + row;
+            if (m >= a.M || n >= wide) continue;
+            const floatx4_t s = *(const floatx4_t*)(strip + row * ROW + from);
+            floatx4_t u = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (TAIL == TAIL_SILU) u = *(const floatx4_t*)(strip + row * ROW + from + 16);
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = s[e] + bias[e];
+                if constexpr (TAIL == TAIL_SILU) v[e] = v[e] / (1.f + expf(-v[e])) * (u[e] + bias_up[e]);
+            }
+            const long at = m * wide + n;
+            if (four) {
+                if (TAIL == TAIL_ADD) {
+                    float old[4];
+                    Vec4<float>::load((const float*)a.out + at, old);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += old[e];
                 }
+                if (TAIL == TAIL_ADD || TAIL == TAIL_PARTIAL || a.out_f32) Vec4<float>::store((float*)a.out + at, v);
+                else Vec4<bf16_t>::store((bf16_t*)a.out + at, v);
             } else {
-                if (m >= a.M) continue;
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const int n = n0 + j * 32 + r;
-                    if (n < wide) fp4_store<TAIL>(a, m, n, acc[i][j][e], 0.f);
+                for (int e = 0; e < 4; ++e) {
+                    if (n + e >= wide) break;
+                    if (TAIL == TAIL_ADD) ((float*)a.out)[at + e] += v[e];
+                    else if (TAIL == TAIL_PARTIAL || a.out_f32) ((float*)a.out)[at + e] = v[e];
+                    else ((bf16_t*)a.out)[at + e] = float_to_bf16(v[e]);
                 }
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // the reads before the next strip's writes
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
 }
 
 // A lane's offset of a buffer load that is beyond every buffer: it arrives as zero.
