@@ -221,7 +221,8 @@ extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* co
     // whole blocks of 16-byte pieces of x
     const bool whole = K % 32 == 0 && ((uintptr_t)x & 15) == 0;
     int rc;
-    if (x_kind == X_FP4) rc = whole ? fp4_rows<X_FP4, true>(a, tail, stream) : fp4_rows<X_FP4, false>(a, tail, stream);
+    if (fp4_few_takes(x, M, N, K, x_kind, tail)) rc = fp4_few(a, x_kind, tail, stream);
+    else if (x_kind == X_FP4) rc = whole ? fp4_rows<X_FP4, true>(a, tail, stream) : fp4_rows<X_FP4, false>(a, tail, stream);
     else if (x_kind == X_BF16) rc = whole ? fp4_rows<X_BF16, true>(a, tail, stream) : fp4_rows<X_BF16, false>(a, tail, stream);
     else rc = whole ? fp4_rows<X_F32, true>(a, tail, stream) : fp4_rows<X_F32, false>(a, tail, stream);
     if (rc) return rc;
