@@ -15,7 +15,6 @@
 #include "common.h"
 
 #define VERIFY_SPAN 4096
-#define VERIFY_EACH (VERIFY_SPAN / 256)        // logits of a thread
 
 struct VerifyArgs {
     const float* logits;        // [rows, V]
@@ -37,37 +36,57 @@ struct VerifyPart {             // of a span of a row: the largest logit, the lo
     int at;
 };
 
-struct VerifyChoice {           // of a request: the row that its token is drawn from
-    double p_sum, q_sum;
-    float p_top, q_top;
-    int row, guess_row;         // (row -1: none; guess_row -1: no draft's distribution to take away, -2: all on the draft)
-    int draft, accepted;
-};
-
 __device__ __forceinline__ bool verify_greedy(float t) { return !(t > 0.f); }
 
-// log2(e) / t, by which a difference of logits becomes a power of two's exponent
-__device__ __forceinline__ double verify_scale(float t) { return 1.4426950408889634074 / (double)t; }
+// A difference of logits times k is a power of two's exponent; below `least` that is -1080, which stands for nothing.
+struct VerifyScale {
+    double k, least;
+    VerifyScale() = default;
+    __device__ __forceinline__ explicit VerifyScale(float t) {
+        k = verify_greedy(t) ? 1.0 : __builtin_fmax(1.4426950408889634074 / (double)t, 1e-300);      // log2(e) / t (an infinite t: all alike, but nothing stays nothing)
+        least = -1080.0 / k;
+    }
+};
 
-// exp((z - top) / t) in 64-bit, k = verify_scale(t), top the row's largest logit: 2^y = 2^n 2^f with n = y rounded, f in [-1/2, 1/2], and 2^f by a
-// polynomial of degree 10 through the Chebyshev points of that interval (off by 3.2e-16 of it at the most).  What is NaN on the
-// way (a NaN logit; -infinity less itself) becomes 0 at the maximum, as what is below 2^-1080 does.
-__device__ __forceinline__ double verify_weight(float z, float top, double k) {
-    const double y = __builtin_fmax(((double)z - (double)top) * k, -1080.0);
-    const double n = __builtin_rint(y), f = y - n;
-    double v = 0x1.e6063f9b91935p-28;
-    v = __builtin_fma(v, f, 0x1.b675bd687d9b8p-24);
-    v = __builtin_fma(v, f, 0x1.62bfd477051e0p-20);
-    v = __builtin_fma(v, f, 0x1.ffcb540541227p-17);
-    v = __builtin_fma(v, f, 0x1.430913096fcb8p-13);
-    v = __builtin_fma(v, f, 0x1.5d87fe9d7ab80p-10);
-    v = __builtin_fma(v, f, 0x1.3b2ab6fba1de1p-7);
-    v = __builtin_fma(v, f, 0x1.c6b08d703ce45p-5);
-    v = __builtin_fma(v, f, 0x1.ebfbdff82c598p-3);
-    v = __builtin_fma(v, f, 0x1.62e42fefa3a19p-1);
+struct VerifyChoice {           // of a request: what its token is drawn from, the weights of row `row` less those of row guess_row or those of a column
+    VerifyScale t;
+    double p_each, q_each;      // 1 / the rows' sums; q_each 0: there is no guess_row
+    float p_top, q_top;
+    int row, guess_row;         // row -1: nothing is drawn
+    int point;                  // the column that a draft without logits was, -1: there is none
+    int pad;
+};
+
+// a b + c with c in scalar registers: the compiler's choice, b's product added into a copy of c, costs two more instructions a term
+__device__ __forceinline__ double verify_term(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+
+// exp((z - top) / t) in 64-bit, top the row's largest logit and not infinite: 2^y = 2^n 2^f with n = y rounded (1.5 2^52 added and taken away:
+// n stands in the sum's low bits), f in [-1/2, 1/2], and 2^f by a polynomial of degree 10 through the Chebyshev points of that
+// interval (off by 3.2e-16 of it at the most).  What is NaN on the way (a NaN logit; -infinity less itself) becomes 0 at the maximum, as what
+// is below 2^-1080 does.
+__device__ __forceinline__ double verify_finite_weight(float z, float top, const VerifyScale& t) {
+    const double d = __builtin_fmax((double)z - (double)top, t.least);
+    const double y = __builtin_fma(d, t.k, 0x1.8p52), f = __builtin_fma(d, t.k, -(y - 0x1.8p52));
+    double v = verify_term(f, 0x1.e6063f9b91935p-28, 0x1.b675bd687d9b8p-24);
+    v = verify_term(v, f, 0x1.62bfd477051e0p-20);
+    v = verify_term(v, f, 0x1.ffcb540541227p-17);
+    v = verify_term(v, f, 0x1.430913096fcb8p-13);
+    v = verify_term(v, f, 0x1.5d87fe9d7ab80p-10);
+    v = verify_term(v, f, 0x1.3b2ab6fba1de1p-7);
+    v = verify_term(v, f, 0x1.c6b08d703ce45p-5);
+    v = verify_term(v, f, 0x1.ebfbdff82c598p-3);
+    v = verify_term(v, f, 0x1.62e42fefa3a19p-1);
     v = __builtin_fma(v, f, 1.0);
-    v = __builtin_amdgcn_ldexp(v, (int)n);
-    return top == INFINITY ? (z == top ? 1.0 : 0.0) : v;        // (infinite logits share everything)
+    return __builtin_amdgcn_ldexp(v, (int)__builtin_bit_cast(unsigned long, y));
+}
+
+// The same for any row: infinite logits share everything.
+__device__ __forceinline__ double verify_weight(float z, float top, const VerifyScale& t) {
+    return top == INFINITY ? (z == top ? 1.0 : 0.0) : verify_finite_weight(z, top, t);
 }
 
 // The rows of request r, or false where first[] holds no rows and drafts that there are.
@@ -77,17 +96,24 @@ __device__ __forceinline__ bool verify_rows(const VerifyArgs& a, int r, int& lo,
     return lo >= r && hi > lo && hi <= a.rows && hi - 1 - r <= a.rows - a.R;
 }
 
-// Logits c0 + 4 tid .. + 3, c0 + 1024 + 4 tid .. and so on of a row, as 16-byte pieces or one by one; beyond the row -infinity.
-__device__ __forceinline__ void verify_load(const float* row, int c0, int V, int four, float (&v)[VERIFY_EACH]) {
+// The column of number e of a thread's share of a span, THREADS threads to a block: four neighbours, four a round further on, and so on.
+template <int THREADS> __device__ __forceinline__ int verify_column(int e) { return e / 4 * (4 * THREADS) + threadIdx.x * 4 + e % 4; }
+
+// A thread's share of the span from c0 on of a row, as 16-byte pieces or one by one; beyond the row -infinity.
+template <int THREADS>
+__device__ __forceinline__ void verify_load(const float* row, int c0, int V, int four, float (&v)[VERIFY_SPAN / THREADS]) {
+    if (four && c0 + VERIFY_SPAN <= V) {
 #pragma unroll
-    for (int e = 0; e < VERIFY_EACH; e += 4) {
-        const int c = c0 + e * 256 + threadIdx.x * 4;
-        if (four && c + 4 <= V) {
-            const float4 q = *(const float4*)(row + c);
+        for (int e = 0; e < VERIFY_SPAN / THREADS; e += 4) {
+            const float4 q = *(const float4*)(row + c0 + verify_column<THREADS>(e));
             v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[e + i] = c + i < V ? row[c + i] : -INFINITY;
+        for (int e = 0; e < VERIFY_SPAN / THREADS; ++e) {
+            const int c = c0 + verify_column<THREADS>(e);
+            v[e] = row[min(c, V - 1)];
+            if (c >= V) v[e] = -INFINITY;
         }
     }
 }
@@ -98,12 +124,16 @@ __device__ __forceinline__ double verify_wave_sum(double v) {
     return v;
 }
 
-__device__ __forceinline__ double verify_block_sum(double v, double* shared) {       // 256 threads
+template <int THREADS>
+__device__ __forceinline__ double verify_block_sum(double v, double* shared) {
     v = verify_wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
-    return shared[0] + shared[1] + shared[2] + shared[3];
+    v = 0.0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) v += shared[w];
+    return v;
 }
 
 // The largest of the wave and the lowest column that has it, in every lane.
@@ -123,8 +153,9 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
     __shared__ double sums[4];
     const bool is_guess = (int)blockIdx.y >= a.rows;
     const int i = is_guess ? blockIdx.y - a.rows : blockIdx.y;
-    float v[VERIFY_EACH];
-    verify_load((is_guess ? a.guess : a.logits) + (long)i * a.V, blockIdx.x * VERIFY_SPAN, a.V, a.four, v);      // (on its way while the request is looked up)
+    constexpr int EACH = VERIFY_SPAN / 256;
+    float v[EACH];
+    verify_load<256>((is_guess ? a.guess : a.logits) + (long)i * a.V, blockIdx.x * VERIFY_SPAN, a.V, a.four, v);      // (on its way while the request is looked up)
     // the request: the number of first[1 .. R] (less their index, for the drafts) that are not beyond i
     int low = 0, high = a.R;
     while (low < high) {
@@ -135,33 +166,40 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
     const float t = a.temperature[low];
     const bool greedy = verify_greedy(t);
     if (is_guess && greedy) return;
-    const double k = greedy ? 0.0 : verify_scale(t);
+    const VerifyScale k(t);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float top = -INFINITY;
     int at = 0x7fffffff;
+    if (greedy) {
 #pragma unroll
-    for (int e = 0; e < VERIFY_EACH; ++e)
-        if (v[e] > top) { top = v[e]; at = blockIdx.x * VERIFY_SPAN + (e / 4) * 1024 + threadIdx.x * 4 + e % 4; }      // (a NaN is larger than nothing)
-    verify_wave_top(top, at);
+        for (int e = 0; e < EACH; ++e)
+            if (v[e] > top) { top = v[e]; at = blockIdx.x * VERIFY_SPAN + verify_column<256>(e); }      // (no NaN is larger than anything)
+        verify_wave_top(top, at);
+    } else {                                       // (its column is not asked for)
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) top = fmaxf(top, v[e]);
+        top = wave_max(top);
+    }
     if (lane == 0) { tops[wave] = top; ats[wave] = at; }
     __syncthreads();
     for (int w = 0; w < 4; ++w)
         if (tops[w] > top || (tops[w] == top && ats[w] < at)) { top = tops[w]; at = ats[w]; }
     double sum = 0.0;
     if (!greedy) {
-        double more = 0.0;
+        if (top == INFINITY) {
 #pragma unroll
-        for (int e = 0; e < VERIFY_EACH; e += 2) {
-            sum += verify_weight(v[e], top, k);
-            more += verify_weight(v[e + 1], top, k);
+            for (int e = 0; e < EACH; ++e) sum += v[e] == top ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) sum += verify_finite_weight(v[e], top, k);
         }
-        sum = verify_block_sum(sum + more, sums);
+        sum = verify_block_sum<256>(sum, sums);
     }
     if (threadIdx.x == 0) parts[(long)blockIdx.y * a.spans + blockIdx.x] = {sum, top, at};
 }
 
 // The whole row's largest logit, its column and sum, from its spans: by one wave, the same in all lanes.
-__device__ __forceinline__ void verify_join(const VerifyPart* parts, int spans, double k, float& top, int& at, double& sum) {
+__device__ __forceinline__ void verify_join(const VerifyPart* parts, int spans, const VerifyScale& k, float& top, int& at, double& sum) {
     const int lane = threadIdx.x & 63;
     VerifyPart mine = {0.0, -INFINITY, 0x7fffffff};
     if (lane < spans) mine = parts[lane];
@@ -187,7 +225,7 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
     }
     const float t = a.temperature[r];
     const bool greedy = verify_greedy(t);
-    const double k = greedy ? 0.0 : verify_scale(t);
+    const VerifyScale k(t);
     const int n = hi - lo - 1;
     int j0 = 0, stop = -1;
     for (;; j0 += 16) {
@@ -197,23 +235,24 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
             const bool inside = x >= 0 && x < a.V;
             const float zp = inside ? a.logits[(long)(lo + j) * a.V + x] : -INFINITY;
             const float zq = inside && a.guess ? a.guess[(long)d * a.V + x] : -INFINITY;
+            const float u = j < n ? a.accept[d] : 0.f;
             VerifyChoice c{};
             int at, unused;
-            verify_join(parts + (long)(lo + j) * a.spans, a.spans, k, c.p_top, at, c.p_sum);
-            c.row = lo + j;
-            c.guess_row = j == n ? -1 : a.guess ? d : -2;
-            c.draft = x;
+            double p_sum, q_sum = 0.0;
+            verify_join(parts + (long)(lo + j) * a.spans, a.spans, k, c.p_top, at, p_sum);
+            if (!greedy && j < n && a.guess) verify_join(parts + (long)(a.rows + d) * a.spans, a.spans, k, c.q_top, unused, q_sum);
             const int token = c.p_top > -INFINITY ? at : -1;
+            c.t = k;
+            c.row = greedy || !(p_sum > 0.0) ? -1 : lo + j;      // (no draw: the token is there, or there is none)
+            c.p_each = p_sum > 0.0 ? 1.0 / p_sum : 0.0;
+            c.q_each = q_sum > 0.0 ? 1.0 / q_sum : 0.0;
+            c.guess_row = d;
+            c.point = j < n && !a.guess ? x : -1;
             bool take = false;
             if (j < n && greedy) take = token >= 0 && x == token;
             else if (j < n) {
-                double q = 1.0;
-                if (a.guess) {
-                    verify_join(parts + (long)(a.rows + d) * a.spans, a.spans, k, c.q_top, unused, c.q_sum);
-                    q = c.q_sum > 0.0 ? verify_weight(zq, c.q_top, k) / c.q_sum : 0.0;
-                }
-                const double p = inside && c.p_sum > 0.0 ? verify_weight(zp, c.p_top, k) / c.p_sum : 0.0;
-                take = p > 0.0 && (double)a.accept[d] * q < p;
+                const double p = verify_weight(zp, c.p_top, k) * c.p_each, q = a.guess ? verify_weight(zq, c.q_top, k) * c.q_each : 1.0;
+                take = p > 0.0 && (double)u * q < p;
             }
             if (lane == 0) { tries[wave] = c; tokens[wave] = token; stops[wave] = !take; }
         } else if (lane == 0) {
@@ -229,171 +268,126 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
     for (int i = threadIdx.x; i <= n; i += 1024) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? tokens[stop] : -1;
     if (threadIdx.x == 0) {
         a.accepted[r] = accepted;
-        VerifyChoice c = tries[stop];
-        c.accepted = accepted;
-        if (greedy || !(c.p_sum > 0.0)) c.row = -1;      // (no draw: the token is there, or there is none)
-        choices[r] = c;
+        choices[r] = tries[stop];
     }
 }
 
-// What the weights of choice c are made of, once for a thread.
-struct VerifyDraw {
-    double k, p_each, q_each;          // (1 / sums; q_each 0: nothing is taken away)
-    float p_top, q_top;
-    int point;                         // the column that a draft without logits was, or -1
-    __device__ __forceinline__ VerifyDraw(const VerifyChoice& c, float t, bool rest) {
-        k = verify_scale(t);
-        p_top = c.p_top;
-        q_top = c.q_top;
-        p_each = 1.0 / c.p_sum;
-        q_each = rest && c.guess_row >= 0 && c.q_sum > 0.0 ? 1.0 / c.q_sum : 0.0;
-        point = rest && c.guess_row == -2 ? c.draft : -1;
-    }
-    __device__ __forceinline__ double weight(float z, float zq, int i) const {
-        double w = verify_weight(z, p_top, k) * p_each;
-        if (q_each > 0.0) w = __builtin_fmax(w - verify_weight(zq, q_top, k) * q_each, 0.0);
-        return i == point ? 0.0 : w;
-    }
-};
+// The weight of column i in a draw, of its logits in the model's row and in the draft's (rest: with the draft's distribution taken away).
+__device__ __forceinline__ double verify_draw_weight(const VerifyChoice& c, float z, float zq, int i, bool rest) {
+    double w = verify_weight(z, c.p_top, c.t) * c.p_each;
+    if (rest && c.q_each > 0.0) w = __builtin_fmax(w - verify_weight(zq, c.q_top, c.t) * c.q_each, 0.0);
+    return rest && i == c.point ? 0.0 : w;
+}
+
+// A span's weights without the draft's: summed already.
+__device__ __forceinline__ double verify_plain_sum(const VerifyArgs& a, const VerifyPart* parts, const VerifyChoice& c, int span) {
+    const VerifyPart& p = parts[(long)c.row * a.spans + span];
+    return p.sum * verify_weight(p.top, c.p_top, c.t) * c.p_each;
+}
 
 // The sum of the weights of a span.
-__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, double* rests) {
-    __shared__ double shared[4];
-    const int r = blockIdx.y;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, double* rests) {
+    constexpr int EACH = VERIFY_SPAN / THREADS;
+    __shared__ double shared[THREADS / 64];
+    const int r = blockIdx.y, span = blockIdx.x;
     const VerifyChoice c = choices[r];
     if (c.row < 0) return;
-    const VerifyDraw w(c, a.temperature[r], true);
     double sum = 0.0;
-    if (w.q_each == 0.0 && (w.point < 0 || w.point / VERIFY_SPAN != (int)blockIdx.x)) {     // p alone: its span is summed already
+    if (c.q_each == 0.0 && (c.point < 0 || c.point / VERIFY_SPAN != span)) {
         if (threadIdx.x != 0) return;
-        const VerifyPart& p = parts[(long)c.row * a.spans + blockIdx.x];
-        sum = p.sum * verify_weight(p.top, c.p_top, w.k) * w.p_each;
+        sum = verify_plain_sum(a, parts, c, span);
     } else {
-        float v[VERIFY_EACH], q[VERIFY_EACH];
-        verify_load(a.logits + (long)c.row * a.V, blockIdx.x * VERIFY_SPAN, a.V, a.four, v);
+        float v[EACH], q[EACH];
+        verify_load<THREADS>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
 #pragma unroll
-        for (int e = 0; e < VERIFY_EACH; ++e) q[e] = 0.f;
-        if (w.q_each > 0.0) verify_load(a.guess + (long)c.guess_row * a.V, blockIdx.x * VERIFY_SPAN, a.V, a.four, q);
+        for (int e = 0; e < EACH; ++e) q[e] = 0.f;
+        if (c.q_each > 0.0) verify_load<THREADS>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
 #pragma unroll
-        for (int e = 0; e < VERIFY_EACH; ++e) sum += w.weight(v[e], q[e], blockIdx.x * VERIFY_SPAN + (e / 4) * 1024 + threadIdx.x * 4 + e % 4);
-        sum = verify_block_sum(sum, shared);
+        for (int e = 0; e < EACH; ++e) sum += verify_draw_weight(c, v[e], q[e], span * VERIFY_SPAN + verify_column<THREADS>(e), true);
+        sum = verify_block_sum<THREADS>(sum, shared);
     }
-    if (threadIdx.x == 0) rests[(long)r * a.spans + blockIdx.x] = sum;
+    if (threadIdx.x == 0) rests[(long)r * a.spans + span] = sum;
 }
 
-// The sum of the values of the threads before this one; total: of all 256.
-__device__ __forceinline__ double verify_sum_before(double v, double* shared, double& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double run = v;
+// The sums of the lanes up to this one's, each with its own.
+__device__ __forceinline__ double verify_wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const double other = __shfl_up(run, o, 64);
-        if (lane >= o) run += other;
+        const double other = __shfl_up(v, o, 64);
+        if (lane >= o) v += other;
     }
-    __syncthreads();
-    if (lane == 63) shared[wave] = run;
-    __syncthreads();
-    double before = 0.0;
-    total = 0.0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += shared[w];
-        total += shared[w];
-    }
-    const double mine = __shfl_up(run, 1, 64);
-    return before + (lane > 0 ? mine : 0.0);
+    return v;
 }
 
-// The draw: a block a request.  Its span is the first whose sum reaches beyond the random number's share of the whole, then
-// its token the first of the span: sums of 16 neighbours a thread, then a walk through those.  Where a rounding lets a span's own sum
-// fall short of the share, or the number is 1 or more, the token is the last one that weighs anything.
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
-    __shared__ double shared[4];
+// The draw: a block a request.  Its span is the first whose sum reaches beyond the random number's share of the whole (every wave finds
+// it for itself, 64 spans at a time), then its token the first of the span: sums of four neighbours a thread, then a walk through
+// those.  Where a rounding lets a span's own sum fall short of the share, or the number is 1 or more, the token is the last one that
+// weighs anything.
+__global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
+    constexpr int EACH = VERIFY_SPAN / 1024;
+    __shared__ double shared[16];
     __shared__ int found_s, last_s;
-    __shared__ double before_s;
-    const int r = blockIdx.x, tid = threadIdx.x;
-    const VerifyChoice c = choices[r];
-    if (c.row < 0) return;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) { found_s = 0x7fffffff; last_s = -1; }
     const double* rests = rests_all + (long)r * a.spans;
-    double total = 0.0, one;
-    for (int s0 = 0; s0 < a.spans; s0 += 256) {
-        verify_sum_before(s0 + tid < a.spans ? rests[s0 + tid] : 0.0, shared, one);
-        total += one;
-    }
+    double v0 = lane < a.spans ? rests[lane] : 0.0;        // (nothing of them is used where nothing is drawn)
+    const VerifyChoice c = choices[r];
+    const float u = a.draw[r];
+    if (c.row < 0) return;
+    double scan0 = verify_wave_scan(v0), total = __shfl(scan0, 63, 64);
+    for (int s0 = 64; s0 < a.spans; s0 += 64) total += __shfl(verify_wave_scan(s0 + lane < a.spans ? rests[s0 + lane] : 0.0), 63, 64);
     // (nothing left: the draft's distribution is the model's, and only a rounding or a number beyond 1 refused the draft: p alone)
     const bool rest = total > 0.0;
-    const VerifyDraw w(c, a.temperature[r], rest);
+    auto span_sum = [&](int s) { return s >= a.spans ? 0.0 : rest ? rests[s] : verify_plain_sum(a, parts, c, s); };
     if (!rest) {
-        for (int s0 = 0; s0 < a.spans; s0 += 256) {
-            double v = 0.0;
-            if (s0 + tid < a.spans) {
-                const VerifyPart& p = parts[(long)c.row * a.spans + s0 + tid];
-                v = p.sum * verify_weight(p.top, c.p_top, w.k) * w.p_each;
-            }
-            verify_sum_before(v, shared, one);
-            total += one;
-        }
+        v0 = span_sum(lane);
+        scan0 = verify_wave_scan(v0);
+        total = 0.0;
+        for (int s0 = 0; s0 < a.spans; s0 += 64) total += __shfl(verify_wave_scan(span_sum(s0 + lane)), 63, 64);
     }
-    const double target = a.draw[r] > 0.f ? (double)a.draw[r] * total : 0.0;     // (NaN: 0)
-    if (tid == 0) { found_s = 0x7fffffff; last_s = -1; }
-    double run = 0.0;
-    for (int s0 = 0; s0 < a.spans; s0 += 256) {
-        double v = 0.0;
-        if (s0 + tid < a.spans) {
-            if (rest) v = rests[s0 + tid];
-            else {
-                const VerifyPart& p = parts[(long)c.row * a.spans + s0 + tid];
-                v = p.sum * verify_weight(p.top, c.p_top, w.k) * w.p_each;
-            }
+    const double target = u > 0.f ? (double)u * total : 0.0;       // (NaN: 0)
+    int span = -1;
+    double before = 0.0, run = 0.0;
+    for (int s0 = 0; s0 < a.spans; s0 += 64) {
+        const double v = s0 == 0 ? v0 : span_sum(s0 + lane), scan = s0 == 0 ? scan0 : verify_wave_scan(v);
+        const unsigned long some = __ballot(v > 0.0), over = __ballot(v > 0.0 && run + scan > target);
+        if (some) {
+            const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+            span = s0 + at;
+            before = run + __shfl(scan, at, 64) - __shfl(v, at, 64);
         }
-        const double before = run + verify_sum_before(v, shared, one);           // (its barriers stand behind the values of found_s and last_s)
-        if (v > 0.0) {
-            if (before + v > target) atomicMin(&found_s, s0 + tid);
-            atomicMax(&last_s, s0 + tid);
-        }
-        __syncthreads();
-        const int span = found_s != 0x7fffffff ? found_s : last_s;
-        if (span == s0 + tid) before_s = before;
-        __syncthreads();
-        run += one;
-        if (found_s != 0x7fffffff) break;
+        if (over) break;
+        run += __shfl(scan, 63, 64);
     }
-    const int span = found_s != 0x7fffffff ? found_s : last_s;
-    const double before = before_s;
     if (span < 0) return;                      // (no weight anywhere)
-    __syncthreads();
-    if (tid == 0) { found_s = 0x7fffffff; last_s = -1; }
-    const int c0 = span * VERIFY_SPAN + tid * VERIFY_EACH;
-    const float* row = a.logits + (long)c.row * a.V + c0;
-    const float* guess = w.q_each > 0.0 ? a.guess + (long)c.guess_row * a.V + c0 : row;
-    double each[VERIFY_EACH], sum = 0.0;
-    float v[VERIFY_EACH], q[VERIFY_EACH];
+    const int c0 = span * VERIFY_SPAN + tid * EACH;
+    double each[EACH], sum = 0.0;
+    float v[EACH], q[EACH];
+    verify_load<1024>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
 #pragma unroll
-    for (int e = 0; e < VERIFY_EACH; e += 4) {
-        if (a.four && c0 + e + 4 <= a.V) {
-            const float4 x = *(const float4*)(row + e), y = *(const float4*)(guess + e);
-            v[e] = x.x; v[e + 1] = x.y; v[e + 2] = x.z; v[e + 3] = x.w;
-            q[e] = y.x; q[e + 1] = y.y; q[e + 2] = y.z; q[e + 3] = y.w;
-        } else {
-#pragma unroll
-            for (int i = e; i < e + 4; ++i) {
-                v[i] = q[i] = -INFINITY;
-                if (c0 + i < a.V) { v[i] = row[i]; q[i] = guess[i]; }
-            }
-        }
-    }
+    for (int e = 0; e < EACH; ++e) q[e] = 0.f;
+    if (rest && c.q_each > 0.0) verify_load<1024>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
     int last = -1;
 #pragma unroll
-    for (int e = 0; e < VERIFY_EACH; ++e) {
-        each[e] = w.weight(v[e], q[e], c0 + e);
+    for (int e = 0; e < EACH; ++e) {
+        each[e] = verify_draw_weight(c, v[e], q[e], c0 + e, rest);
         sum += each[e];
         if (each[e] > 0.0) last = c0 + e;
     }
-    run = before + verify_sum_before(sum, shared, one);
+    const double scan = verify_wave_scan(sum);
+    if (lane == 63) shared[wave] = scan;
+    __syncthreads();
+    run = before;
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+        if (w < wave) run += shared[w];
+    run += scan - sum;
     if (last >= 0) {
         int found = 0x7fffffff;
 #pragma unroll
-        for (int e = 0; e < VERIFY_EACH; ++e) {
+        for (int e = 0; e < EACH; ++e) {
             run += each[e];
             if (found == 0x7fffffff && each[e] > 0.0 && run > target) found = c0 + e;
         }
@@ -428,8 +422,10 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, four};
     verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts);
     verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
-    verify_rest_kernel<<<dim3(spans, R), 256, 0, stream>>>(a, parts, choices, rests);
-    verify_draw_kernel<<<R, 256, 0, stream>>>(a, parts, choices, rests);
+    // (few spans: a thread's 16 exponentials one after the other are what a block takes; 1 request 7.6 us, with four a thread 6.1; 64 requests 23 and 27)
+    if ((long)spans * R <= 512) verify_rest_kernel<1024><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
+    else verify_rest_kernel<256><<<dim3(spans, R), 256, 0, stream>>>(a, parts, choices, rests);
+    verify_draw_kernel<<<R, 1024, 0, stream>>>(a, parts, choices, rests);
     QE_LAUNCH_CHECK();
     return 0;
 }
