@@ -10,8 +10,8 @@
 // All weights and sums are 64-bit: a vocabulary of 150 000 has so many borders of running sums that 32-bit ones put the random number on
 // the other side of one in a few per cent of the draws.
 //
-// Four launches: spans of 4096 logits (all rows, bound by their bytes), acceptance (a block a request, a wave a draft), the spans' sums
-// of what the token is drawn from (one row a request, and its draft's), the draw.
+// Up to four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials), acceptance (a block a request, a wave a
+// draft), the spans' sums of what the token is drawn from (one row a request, and its draft's), the draw.
 #include "common.h"
 
 #define VERIFY_SPAN 4096
@@ -213,15 +213,18 @@ __device__ __forceinline__ void verify_join(const VerifyPart* parts, int spans, 
     sum = verify_wave_sum(sum);
 }
 
-// A block a request, a wave a draft, 16 at a time: which drafts are accepted, and what the token is drawn from.
-__global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices) {
+// Which drafts of request r are accepted, and what its token is drawn from: by a block of 16 waves, a wave a draft, 16 at a time.  One of the
+// blocks that ask writes it down.
+__device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const VerifyPart* parts, VerifyChoice* choices, int r, bool write) {
     __shared__ VerifyChoice tries[16];
     __shared__ int tokens[16], stops[16];
-    const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo, hi;
     if (!verify_rows(a, r, lo, hi)) {
-        if (threadIdx.x == 0) { a.accepted[r] = -1; choices[r].row = -1; }
-        return;
+        VerifyChoice none{};
+        none.row = -1;
+        if (write && threadIdx.x == 0) { a.accepted[r] = -1; choices[r] = none; }
+        return none;
     }
     const float t = a.temperature[r];
     const bool greedy = verify_greedy(t);
@@ -264,12 +267,19 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
         if (stop >= 0) break;                      // (row n is no draft: it stops)
         __syncthreads();
     }
-    const int accepted = j0 + stop;
-    for (int i = threadIdx.x; i <= n; i += 1024) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? tokens[stop] : -1;
-    if (threadIdx.x == 0) {
-        a.accepted[r] = accepted;
-        choices[r] = tries[stop];
+    if (write) {
+        const int accepted = j0 + stop;
+        for (int i = threadIdx.x; i <= n; i += 1024) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? tokens[stop] : -1;
+        if (threadIdx.x == 0) {
+            a.accepted[r] = accepted;
+            choices[r] = tries[stop];
+        }
     }
+    return tries[stop];
+}
+
+__global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices) {
+    verify_accept(a, parts, choices, blockIdx.x, true);
 }
 
 // The weight of column i in a draw, of its logits in the model's row and in the draft's (rest: with the draft's distribution taken away).
@@ -285,13 +295,15 @@ __device__ __forceinline__ double verify_plain_sum(const VerifyArgs& a, const Ve
     return p.sum * verify_weight(p.top, c.p_top, c.t) * c.p_each;
 }
 
-// The sum of the weights of a span.
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, double* rests) {
+// The sum of the weights of a span.  ACCEPT: the block finds the choice for itself.
+template <int THREADS, bool ACCEPT>
+__global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests) {
     constexpr int EACH = VERIFY_SPAN / THREADS;
     __shared__ double shared[THREADS / 64];
     const int r = blockIdx.y, span = blockIdx.x;
-    const VerifyChoice c = choices[r];
+    VerifyChoice c;
+    if constexpr (ACCEPT) c = verify_accept(a, parts, choices, r, span == 0);
+    else c = choices[r];
     if (c.row < 0) return;
     double sum = 0.0;
     if (c.q_each == 0.0 && (c.point < 0 || c.point / VERIFY_SPAN != span)) {
@@ -421,10 +433,14 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     const int four = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)guess) & 15) == 0;
     const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, four};
     verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts);
-    verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
-    // (few spans: a thread's 16 exponentials one after the other are what a block takes; 1 request 7.6 us, with four a thread 6.1; 64 requests 23 and 27)
-    if ((long)spans * R <= 512) verify_rest_kernel<1024><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
-    else verify_rest_kernel<256><<<dim3(spans, R), 256, 0, stream>>>(a, parts, choices, rests);
+    // Few spans: every block accepts for itself, which saves a launch, and takes four exponentials a thread instead of 16, one after the other
+    // (1 request of 38 spans 23 us, apart 28 with 16 and 25 with four a thread; 64 requests, apart, 129 with 16 and 134 with four).
+    if ((long)spans * R <= 512) {
+        verify_rest_kernel<1024, true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
+    } else {
+        verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
+        verify_rest_kernel<256, false><<<dim3(spans, R), 256, 0, stream>>>(a, parts, choices, rests);
+    }
     verify_draw_kernel<<<R, 1024, 0, stream>>>(a, parts, choices, rests);
     QE_LAUNCH_CHECK();
     return 0;
