@@ -1,18 +1,22 @@
 // Products of up to 16 rows with a 4-bit matrix (see mxfp4.h), for rows of whole blocks: bound by the matrix's bytes on their way from memory.
 //
-// A block takes NT tiles of 16 columns, its waves chunks of 256 of K in turn, each wave by itself: it asks for D chunks of its codes (128
-// bytes of a row, a line) and of x straight to its own piece of shared memory, and multiplies a chunk when it has come.  The scales of
+// A block takes NT tiles of 16 columns, its waves chunks of 256 of K in turn, each wave by itself: it asks for a chunk of the codes (128
+// bytes of a row, a line) and of x straight to its own piece of shared memory, and multiplies it when it has come.  The scales of
 // the block's columns lie side by side and come as they are, once.  The sums of the waves are added in the order of the waves.
+//
+// What is on its way at a time is the blocks' and waves' of a unit: a second chunk a wave, asked for ahead, takes the shared memory of another
+// block and is slower (16 rows against 24576 x 4096 with one chunk a wave 13.2 us, with two 14.2; 8 against gate and up of that size 12.2,
+// 12.9; 16 against 4096 x 4096 5.6, 6.0; only 4-bit rows against 4096 x 12288 are a little quicker with two, 7.7 us instead of 7.9).
 //
 // Loads to registers would do without shared memory, but a matrix instruction's lane wants 16 bytes of a row, neighbouring lanes of
 // other rows, and a load of 64 places of 64 lines takes four times the cycles of one of eight lines.
 #include "mxfp4.h"
 
-template <int X, int RX, int NT, int D>
-__global__ __launch_bounds__(1024) void fp4_few_kernel(Fp4Args a, int tail, int scale_bytes) {
+template <int X, int RX, int NT>
+__global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, int tail, int scale_bytes) {
     constexpr int LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8, LOADS = LX + 2 * NT;        // a chunk's loads: x, codes
     constexpr int SLOT = LOADS * 1024;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];                // scales (x's, the matrix's), then D slots a wave
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];                // scales (x's, the matrix's), then a slot a wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15, g = lane >> 4;
     const bool silu = tail == TAIL_SILU;
     const int wide = silu ? a.N / 2 : a.N, halves = silu ? 2 : 1, tiles = NT / halves;  // tiles of columns that are stored
@@ -53,40 +57,34 @@ __global__ __launch_bounds__(1024) void fp4_few_kernel(Fp4Args a, int tail, int 
 #pragma unroll
     for (int p = 0; p < 2; ++p) rsrc_w[p] = fp4_buffer(a.codes + ((long)(silu && p ? wide : 0) + n0) * row_bytes, (unsigned)(cols * row_bytes));
     const int left = a.blocks - (chunks - 1) * 8;          // blocks of the last chunk
-    const unsigned slots = lds0 + scale_bytes + wave * (D * SLOT);
-    int ask = wave, ask_slot = 0;                          // the chunk that is asked for next
-#define ASK()                                                                                                        \
+    const unsigned char* const slot = smem + scale_bytes + wave * SLOT;
+    const unsigned slot_to = lds0 + scale_bytes + wave * SLOT;
+#define ASK(c_)                                                                                                      \
     {                                                                                                                \
-        if (ask >= chunks) { rsrc_x[2] = 0; rsrc_w[0][2] = 0; rsrc_w[1][2] = 0; }      /* (nothing comes any more) */ \
-        const int ends_ = ask == chunks - 1 ? -1 : 0, c_ = ask < chunks ? ask : 0;                                   \
-        const unsigned to_ = slots + ask_slot * SLOT;                                                                \
+        const int ends_ = (c_) == chunks - 1 ? -1 : 0;                                                               \
         _Pragma("unroll") for (int i = 0; i < LX; ++i) {                                                             \
             const int not_ = ((X == X_BF16 ? px[i] >> 2 : px[i]) < left ? 0 : FP4_OUT) & ends_;                      \
-            QE_LOAD_TO_SHARED(to_ + i * 1024, vx[i] | not_, rsrc_x, c_ * (X == X_BF16 ? 512 : 128), "4", "");        \
+            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, (c_) * (X == X_BF16 ? 512 : 128), "4", "");  \
         }                                                                                                            \
         const int not_ = (pc < left ? 0 : FP4_OUT) & ends_;                                                          \
         _Pragma("unroll") for (int t = 0; t < NT; ++t)                                                               \
             _Pragma("unroll") for (int i = 0; i < 2; ++i) {                                                          \
                 const int in_ = silu ? t % (NT > 1 ? NT / 2 : 1) : t;        /* the tile within its half */          \
                 const int v_ = (vc[i] + in_ * 16 * row_bytes) | not_;                                                \
-                if (silu && t >= NT / 2) { QE_LOAD_TO_SHARED(to_ + (LX + t * 2 + i) * 1024, v_, rsrc_w[1], c_ * 128, "4", ""); } \
-                else QE_LOAD_TO_SHARED(to_ + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], c_ * 128, "4", "");             \
+                if (silu && t >= NT / 2) { QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[1], (c_) * 128, "4", ""); } \
+                else QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], (c_) * 128, "4", "");       \
             }                                                                                                        \
-        ask += waves;                                                                                                \
-        ask_slot = ask_slot + 1 == D ? 0 : ask_slot + 1;                                                             \
     }
     floatx4_t acc[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < D; ++d) ASK()
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((D - 1) * LOADS) : "memory");      // (the scales are there for all waves)
+    if (wave < chunks) ASK(wave)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");           // (the scales are there for all waves, too)
 
     const int xr = r & (RX - 1);                           // (a row of the tile that x does not have: another one's, and not stored)
-    int slot = 0;
     for (int c = wave; c < chunks; c += waves) {
-        asm volatile("s_waitcnt vmcnt(%0)" : : "n"((D - 1) * LOADS) : "memory");
-        const unsigned char* at = smem + scale_bytes + wave * (D * SLOT) + slot * SLOT;
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        const unsigned char* at = slot;
         uintx4_t xv[2][X == X_BF16 ? 4 : 1], cv[NT][2];
         int ws[NT][2], xs[2];
 #pragma unroll
@@ -107,6 +105,9 @@ __global__ __launch_bounds__(1024) void fp4_few_kernel(Fp4Args a, int tail, int 
                 ws[t][s] = smem[x_part + (silu && t >= NT / 2 ? part_bytes : 0) + row * a.blocks + block];
             }
         }
+        // (the slot is read: the next chunk may come)
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        if (c + waves < chunks) ASK(c + waves)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -122,15 +123,10 @@ __global__ __launch_bounds__(1024) void fp4_few_kernel(Fp4Args a, int tail, int 
                     acc[t][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][s], 4, 4, 0, xs[s], 0, ws[t][s]);
                 }
             }
-        // (the slot is read: its loads may go out)
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-        if (D > 1 || c + waves < chunks) ASK()
-        slot = slot + 1 == D ? 0 : slot + 1;
     }
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
 #undef ASK
-    float* sums = (float*)(smem + scale_bytes);            // of wave w from byte w D SLOT on: [NT][16][16]
-    constexpr int APART = D * SLOT / 4;
+    float* sums = (float*)(smem + scale_bytes);            // of wave w from byte w SLOT on: [NT][16][16]
+    constexpr int APART = SLOT / 4;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -150,51 +146,46 @@ __global__ __launch_bounds__(1024) void fp4_few_kernel(Fp4Args a, int tail, int 
     }
 }
 
-template <int X, int RX, int NT, int D>
+template <int X, int RX, int NT>
 static int fp4_few_launch(const Fp4Args& a, int tail, int waves, hipStream_t stream) {
     constexpr int LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8, SLOT = (LX + 2 * NT) * 1024;
     const int scale_bytes = ((X == X_FP4 ? (a.M * a.blocks + 15) / 16 * 16 : 0) + NT * 16 * a.blocks + 15) / 16 * 16;
     const int wide = tail == TAIL_SILU ? a.N / 2 : a.N, cols = tail == TAIL_SILU ? NT * 8 : NT * 16;
-    const int shared = scale_bytes + waves * D * SLOT;
-    QE_RAISE_SHARED((fp4_few_kernel<X, RX, NT, D>), 160 * 1024);
-    fp4_few_kernel<X, RX, NT, D><<<qe_cdiv(wide, cols), 64 * waves, shared, stream>>>(a, tail, scale_bytes);
+    QE_RAISE_SHARED((fp4_few_kernel<X, RX, NT>), 160 * 1024);
+    fp4_few_kernel<X, RX, NT><<<qe_cdiv(wide, cols), 64 * waves, scale_bytes + waves * SLOT, stream>>>(a, tail, scale_bytes);
     return 0;
 }
 
+// Tiles of columns and waves of a block; waves 0: not taken (the scales leave no room in shared memory).
 struct Fp4Few {
-    int nt, waves, depth;
+    int nt, waves;
 };
 
-// Columns a block, waves, chunks on their way: what the shared memory of a unit holds.  waves 0: not taken.
 static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
-    const int wide = tail == TAIL_SILU ? N / 2 : N, blocks = K / 32, chunks = qe_cdiv(blocks, 8);
-    const int rx = M <= 2 ? 2 : M <= 8 ? 8 : 16;
+    const int blocks = K / 32, chunks = qe_cdiv(blocks, 8), rx = M <= 2 ? 2 : M <= 8 ? 8 : 16;
     Fp4Few f{};
-    f.nt = wide >= 2 * 256 * (tail == TAIL_SILU ? 32 : 64) ? 4 : tail == TAIL_SILU ? 2 : 1;
-    const int slot = ((x_kind == X_BF16 ? rx / 2 : (rx + 7) / 8) + 2 * f.nt) * 1024;
-    const int scales = (x_kind == X_FP4 ? M * blocks : 0) + f.nt * 16 * blocks + 32;
-    const int grid = qe_cdiv(wide, f.nt * (tail == TAIL_SILU ? 8 : 16));
-    const int room = (grid > 256 ? 80 : 160) * 1024 - scales;
-    int waves = room / (2 * slot);
-    if (waves > 16) waves = 16;
-    const int want = qe_cdiv(chunks, 2);
-    if (waves > want) waves = want;
-    f.waves = waves < 1 ? 0 : waves;
-    f.depth = chunks <= f.waves ? 1 : 2;
+    // Two tiles where four blocks a unit are left then: every block reads all of x (16 rows against 24576 x 4096 13.2 us, with one tile 14.7; against
+    // 4096 x 4096, 128 blocks with two, 6.7 and 5.6; with four tiles 14.9 and more).
+    f.nt = tail == TAIL_SILU || N >= 1024 * 16 ? 2 : 1;
+    // Waves: up to a chunk each, eight with one tile, four with two, which leaves room for other blocks (1 row against 6144 x 4096 with eight 5.8 us,
+    // twelve 6.1; 8 rows against gate and up of 24576 x 4096 with four 12.2, eight 12.9; against 151936 x 1024, four chunks, with
+    // two 18.0, four 20.8).
+    const int room = 160 * 1024 - ((x_kind == X_FP4 ? M * blocks : 0) + f.nt * 16 * blocks + 32);
+    const int fit = room / (((x_kind == X_BF16 ? rx / 2 : (rx + 7) / 8) + 2 * f.nt) * 1024);
+    f.waves = f.nt == 1 ? (chunks < 8 ? chunks : 8) : chunks < 8 ? qe_cdiv(chunks, 2) : 4;
+    if (f.waves > fit) f.waves = fit;
     return f;
 }
 
 bool fp4_few_takes(const void* x, int M, int N, int K, int x_kind, int tail) {
-    return M <= 16 && x_kind != X_F32 && K % 32 == 0 && ((uintptr_t)x & 15) == 0 && (long)K * 16 * 64 < (1L << 31) && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
+    return M <= 16 && x_kind != X_F32 && K % 32 == 0 && K < (1 << 20) && ((uintptr_t)x & 15) == 0 && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
 }
 
 int fp4_few(const Fp4Args& a, int x_kind, int tail, hipStream_t stream) {
     const Fp4Few f = fp4_few_shape(a.M, a.N, a.K, x_kind, tail);
-#define QE_D(X_, RX_, NT_) (f.depth == 1 ? fp4_few_launch<X_, RX_, NT_, 1>(a, tail, f.waves, stream) : fp4_few_launch<X_, RX_, NT_, 2>(a, tail, f.waves, stream))
-#define QE_NT(X_, RX_) (f.nt == 1 ? QE_D(X_, RX_, 1) : f.nt == 2 ? QE_D(X_, RX_, 2) : QE_D(X_, RX_, 4))
+#define QE_NT(X_, RX_) (f.nt == 1 ? fp4_few_launch<X_, RX_, 1>(a, tail, f.waves, stream) : fp4_few_launch<X_, RX_, 2>(a, tail, f.waves, stream))
 #define QE_RX(X_) (a.M <= 2 ? QE_NT(X_, 2) : a.M <= 8 ? QE_NT(X_, 8) : QE_NT(X_, 16))
     return x_kind == X_BF16 ? QE_RX(X_BF16) : QE_RX(X_FP4);
 #undef QE_RX
 #undef QE_NT
-#undef QE_D
 }
