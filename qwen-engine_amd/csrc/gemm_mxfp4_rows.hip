@@ -1,4 +1,5 @@
-// Products of up to 16 rows with a 4-bit matrix (see mxfp4.h), for rows of whole blocks: bound by the matrix's bytes on their way from memory.
+// Products of few rows (up to 32, in 4 bits 64) with a 4-bit matrix (see mxfp4.h): bound by the matrix's bytes on their way from memory.
+// Rows of bfloat16 lie at whole 16-byte pieces; those of 32-bit numbers come as three planes, one behind the other, and K is walked three times.
 //
 // A block takes NT tiles of 16 columns, its waves chunks of 256 of K in turn, each wave by itself: it asks for a chunk of the codes (128
 // bytes of a row, a line) and of x straight to its own piece of shared memory, and multiplies it when it has come.  The scales of
@@ -13,15 +14,16 @@
 #include "mxfp4.h"
 
 template <int X, int RX, int NT>
-__global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, int tail, int scale_bytes) {
-    constexpr int LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8, LOADS = LX + 2 * NT;        // a chunk's loads: x, codes
-    constexpr int SLOT = LOADS * 1024;
+__global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int tail, int scale_bytes) {
+    constexpr int MT = (RX + 15) / 16, LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8;        // tiles of 16 rows; a chunk's loads of x (and 2 NT of codes)
+    constexpr int SLOT = (LX + 2 * NT) * 1024;
+    static_assert(NT * MT * 1024 <= SLOT, "a wave's sums go where its slot was");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];                // scales (x's, the matrix's), then a slot a wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15, g = lane >> 4;
     const bool silu = tail == TAIL_SILU;
     const int wide = silu ? a.N / 2 : a.N, halves = silu ? 2 : 1, tiles = NT / halves;  // tiles of columns that are stored
     const int n0 = blockIdx.x * tiles * 16, cols = min(tiles * 16, wide - n0);
-    const int row_bytes = a.blocks * 16, chunks = (a.blocks + 7) / 8;
+    const int row_bytes = a.blocks * 16, per = (a.blocks + 7) / 8, chunks = per * x.planes;       // chunks of a row, of all its planes
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
 
     // The scales: of x (in 4 bits), of the columns (silu: of the gates, of the ups).  Where a part is whole pieces of 16 bytes it is copied by
@@ -48,58 +50,65 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, int tail, int s
     for (int i = 0; i < LX; ++i) {
         const int row = (X == X_BF16 ? i * 2 : i * 8) + x_row;
         px[i] = X == X_BF16 ? (lane & 31) ^ (row & 7) : (lane & 7) ^ (row & 7);
-        vx[i] = row < RX && row < a.M ? row * (X == X_BF16 ? a.K * 2 : row_bytes) + px[i] * 16 : FP4_OUT;
+        vx[i] = row < RX && row < a.M ? row * x.row_bytes + px[i] * 16 : FP4_OUT;
     }
     const int pc = (lane & 7) ^ (lane >> 3);               // (a load is eight rows)
 #pragma unroll
     for (int i = 0; i < 2; ++i) vc[i] = (i * 8 + (lane >> 3)) * row_bytes + pc * 16;
-    uintx4_t rsrc_x = fp4_buffer(a.x, (unsigned)((long)a.M * (X == X_BF16 ? a.K * 2 : row_bytes))), rsrc_w[2];
+    const int plane_bytes = a.M * x.row_bytes;
+    const uintx4_t rsrc_x = fp4_buffer(x.data, (unsigned)(plane_bytes * x.planes));
+    uintx4_t rsrc_w[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) rsrc_w[p] = fp4_buffer(a.codes + ((long)(silu && p ? wide : 0) + n0) * row_bytes, (unsigned)(cols * row_bytes));
-    const int left = a.blocks - (chunks - 1) * 8;          // blocks of the last chunk
+    const int left = a.blocks - (per - 1) * 8, x_left = x.row_bytes - (per - 1) * (X == X_BF16 ? 512 : 128);      // blocks of the last chunk, bytes of its x
     const unsigned char* const slot = smem + scale_bytes + wave * SLOT;
     const unsigned slot_to = lds0 + scale_bytes + wave * SLOT;
 #define ASK(c_)                                                                                                      \
     {                                                                                                                \
-        const int ends_ = (c_) == chunks - 1 ? -1 : 0;                                                               \
+        const int plane_ = (c_) / per, k_ = (c_) - plane_ * per, ends_ = k_ == per - 1 ? -1 : 0;                     \
         _Pragma("unroll") for (int i = 0; i < LX; ++i) {                                                             \
-            const int not_ = ((X == X_BF16 ? px[i] >> 2 : px[i]) < left ? 0 : FP4_OUT) & ends_;                      \
-            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, (c_) * (X == X_BF16 ? 512 : 128), "4", "");  \
+            const int not_ = (px[i] * 16 < x_left ? 0 : FP4_OUT) & ends_;                                            \
+            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, plane_ * plane_bytes + k_ * (X == X_BF16 ? 512 : 128), "4", ""); \
         }                                                                                                            \
         const int not_ = (pc < left ? 0 : FP4_OUT) & ends_;                                                          \
         _Pragma("unroll") for (int t = 0; t < NT; ++t)                                                               \
             _Pragma("unroll") for (int i = 0; i < 2; ++i) {                                                          \
                 const int in_ = silu ? t % (NT > 1 ? NT / 2 : 1) : t;        /* the tile within its half */          \
                 const int v_ = (vc[i] + in_ * 16 * row_bytes) | not_;                                                \
-                if (silu && t >= NT / 2) { QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[1], (c_) * 128, "4", ""); } \
-                else QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], (c_) * 128, "4", "");       \
+                if (silu && t >= NT / 2) { QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[1], k_ * 128, "4", ""); } \
+                else QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], k_ * 128, "4", "");       \
             }                                                                                                        \
     }
-    floatx4_t acc[NT][2];
+    floatx4_t acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = {0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[t][i] = {0.f, 0.f, 0.f, 0.f};
     if (wave < chunks) ASK(wave)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");           // (the scales are there for all waves, too)
 
-    const int xr = r & (RX - 1);                           // (a row of the tile that x does not have: another one's, and not stored)
     for (int c = wave; c < chunks; c += waves) {
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-        const unsigned char* at = slot;
-        uintx4_t xv[2][X == X_BF16 ? 4 : 1], cv[NT][2];
-        int ws[NT][2], xs[2];
+        uintx4_t xv[2][MT][X == X_BF16 ? 4 : 1], cv[NT][2];
+        int ws[NT][2], xs[2][MT];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int b = s * 4 + g, block = min(c * 8 + b, a.blocks - 1);      // (beyond the last block codes and x are zero)
-            if constexpr (X == X_BF16) {
+            const int b = s * 4 + g, block = min(c % per * 8 + b, a.blocks - 1);      // (beyond the last block codes and x are zero)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) xv[s][j] = *(const uintx4_t*)(at + xr * 512 + (((b * 4 + j) ^ (xr & 7)) * 16));
-            } else {
-                xv[s][0] = *(const uintx4_t*)(at + xr * 128 + ((b ^ (xr & 7)) * 16));
-                xs[s] = smem[min(xr, a.M - 1) * a.blocks + block];
+            for (int i = 0; i < MT; ++i) {
+                const int xr = (i * 16 + r) & (RX - 1);    // (a row of the tile that x does not have: another one's, and not stored)
+                if constexpr (X == X_BF16) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) xv[s][i][j] = *(const uintx4_t*)(slot + xr * 512 + (((b * 4 + j) ^ (xr & 7)) * 16));
+                } else {
+                    xv[s][i][0] = *(const uintx4_t*)(slot + xr * 128 + ((b ^ (xr & 7)) * 16));
+                    xs[s][i] = smem[min(xr, a.M - 1) * a.blocks + block];
+                    if (a.K % 32 && c == chunks - 1 && a.K - block * 32 < 32) xv[s][i][0] = first_codes(xv[s][i][0], a.K - block * 32);
+                }
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                cv[t][s] = *(const uintx4_t*)(at + (LX + t * 2) * 1024 + r * 128 + ((b ^ (r & 7)) * 16));
+                cv[t][s] = *(const uintx4_t*)(slot + (LX + t * 2) * 1024 + r * 128 + ((b ^ (r & 7)) * 16));
                 const int in = silu ? t % (NT > 1 ? NT / 2 : 1) : t;
                 const int row = min(in * 16 + r, cols - 1);
                 ws[t][s] = smem[x_part + (silu && t >= NT / 2 ? part_bytes : 0) + row * a.blocks + block];
@@ -114,31 +123,40 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, int tail, int s
             for (int t = 0; t < NT; ++t) {
                 if constexpr (X == X_BF16) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, xv[s][j]),
-                                                                            fp4_to_bf16(cv[t][s][j], __uint_as_float((uint32_t)ws[t][s] << 23)), acc[t][s], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) {
+                        const bf16x8_t w = fp4_to_bf16(cv[t][s][j], __uint_as_float((uint32_t)ws[t][s] << 23));
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+                            acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, xv[s][i][j]), w, acc[t][i], 0, 0, 0);
+                    }
                 } else {
-                    const intx8_t xa = {(int)xv[s][0][0], (int)xv[s][0][1], (int)xv[s][0][2], (int)xv[s][0][3], 0, 0, 0, 0};
                     const intx8_t wb = {(int)cv[t][s][0], (int)cv[t][s][1], (int)cv[t][s][2], (int)cv[t][s][3], 0, 0, 0, 0};
-                    acc[t][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][s], 4, 4, 0, xs[s], 0, ws[t][s]);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const uintx4_t& q = xv[s][i][0];
+                        const intx8_t xa = {(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+                        acc[t][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][i], 4, 4, 0, xs[s][i], 0, ws[t][s]);
+                    }
                 }
             }
     }
 #undef ASK
-    float* sums = (float*)(smem + scale_bytes);            // of wave w from byte w SLOT on: [NT][16][16]
-    constexpr int APART = SLOT / 4;
+    float* sums = (float*)(smem + scale_bytes);            // of wave w from byte w SLOT on: [NT][MT * 16][16]
+    constexpr int APART = SLOT / 4, TILE = MT * 256;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sums[wave * APART + (t * 16 + g * 4 + e) * 16 + r] = acc[t][0][e] + acc[t][1][e];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[wave * APART + t * TILE + (i * 16 + g * 4 + e) * 16 + r] = acc[t][i][e];
     __syncthreads();
-    for (int at = threadIdx.x; at < tiles * 256; at += blockDim.x) {
-        const int t = at >> 8, m = at >> 4 & 15, n = n0 + t * 16 + (at & 15);
+    for (int at = threadIdx.x; at < tiles * TILE; at += blockDim.x) {
+        const int t = at / TILE, m = at % TILE >> 4, n = n0 + t * 16 + (at & 15);
         if (m >= a.M || n >= wide) continue;
         float v = 0.f, up = 0.f;
         for (int w = 0; w < waves; ++w) {
             v += sums[w * APART + at];
-            if (silu) up += sums[w * APART + at + tiles * 256];
+            if (silu) up += sums[w * APART + at + tiles * TILE];
         }
         if (tail == TAIL_STORE) fp4_store<TAIL_STORE>(a, m, n, v, up);
         else if (tail == TAIL_ADD) fp4_store<TAIL_ADD>(a, m, n, v, up);
@@ -147,12 +165,12 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, int tail, int s
 }
 
 template <int X, int RX, int NT>
-static int fp4_few_launch(const Fp4Args& a, int tail, int waves, hipStream_t stream) {
+static int fp4_few_launch(const Fp4Args& a, const Fp4Rows& x, int tail, int waves, hipStream_t stream) {
     constexpr int LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8, SLOT = (LX + 2 * NT) * 1024;
     const int scale_bytes = ((X == X_FP4 ? (a.M * a.blocks + 15) / 16 * 16 : 0) + NT * 16 * a.blocks + 15) / 16 * 16;
     const int wide = tail == TAIL_SILU ? a.N / 2 : a.N, cols = tail == TAIL_SILU ? NT * 8 : NT * 16;
     QE_RAISE_SHARED((fp4_few_kernel<X, RX, NT>), 160 * 1024);
-    fp4_few_kernel<X, RX, NT><<<qe_cdiv(wide, cols), 64 * waves, scale_bytes + waves * SLOT, stream>>>(a, tail, scale_bytes);
+    fp4_few_kernel<X, RX, NT><<<qe_cdiv(wide, cols), 64 * waves, scale_bytes + waves * SLOT, stream>>>(a, x, tail, scale_bytes);
     return 0;
 }
 
@@ -162,30 +180,41 @@ struct Fp4Few {
 };
 
 static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
-    const int blocks = K / 32, chunks = qe_cdiv(blocks, 8), rx = M <= 2 ? 2 : M <= 8 ? 8 : 16;
+    const int blocks = qe_cdiv(K, 32), chunks = qe_cdiv(blocks, 8) * (x_kind == X_F32 ? 3 : 1);
+    const int rx = M <= 2 ? 2 : M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
     Fp4Few f{};
     // Two tiles where four blocks a unit are left then: every block reads all of x (16 rows against 24576 x 4096 13.2 us, with one tile 14.7; against
     // 4096 x 4096, 128 blocks with two, 6.7 and 5.6; with four tiles 14.9 and more).
     f.nt = tail == TAIL_SILU || N >= 1024 * 16 ? 2 : 1;
-    // Waves: up to a chunk each, eight with one tile, four with two, which leaves room for other blocks (1 row against 6144 x 4096 with eight 5.8 us,
-    // twelve 6.1; 8 rows against gate and up of 24576 x 4096 with four 12.2, eight 12.9; against 151936 x 1024, four chunks, with
-    // two 18.0, four 20.8).
+    // Waves: up to a chunk each, eight where there are no more blocks than units or with one tile; with two tiles four, or two of more than 16
+    // rows, which leaves room for other blocks (1 row against 6144 x 4096 with eight 5.8 us, twelve 6.1; 8 rows against gate and up
+    // of 24576 x 4096 with four 12.2, eight 12.9; against 151936 x 1024, four chunks, with two 18.0, four 20.8; 17 rows against 24576 x 4096 with
+    // two 16.6, three 21.4; 32 against 4096 x 4096 with eight 8.2, four 9.2).
+    const int grid = qe_cdiv(tail == TAIL_SILU ? N / 2 : N, tail == TAIL_SILU ? 16 : f.nt * 16);
     const int room = 160 * 1024 - ((x_kind == X_FP4 ? M * blocks : 0) + f.nt * 16 * blocks + 32);
-    const int fit = room / (((x_kind == X_BF16 ? rx / 2 : (rx + 7) / 8) + 2 * f.nt) * 1024);
-    f.waves = f.nt == 1 ? (chunks < 8 ? chunks : 8) : chunks < 8 ? qe_cdiv(chunks, 2) : 4;
+    const int fit = room / (((x_kind == X_FP4 ? (rx + 7) / 8 : rx / 2) + 2 * f.nt) * 1024);
+    f.waves = f.nt == 1 || grid <= 256 ? (chunks < 8 ? chunks : 8) : chunks < 8 || rx > 16 ? 2 : 4;
     if (f.waves > fit) f.waves = fit;
     return f;
 }
 
-bool fp4_few_takes(const void* x, int M, int N, int K, int x_kind, int tail) {
-    return M <= 16 && x_kind != X_F32 && K % 32 == 0 && K < (1 << 20) && ((uintptr_t)x & 15) == 0 && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
+// Rows that the loads take as they are: of bfloat16, at whole 16-byte pieces.
+static bool as_it_is(const void* x, int K, int x_kind) { return x_kind == X_FP4 || (x_kind == X_BF16 && K % 8 == 0 && ((uintptr_t)x & 15) == 0); }
+
+bool fp4_few_takes(int M, int N, int K, int x_kind, int tail) {
+    return M <= (x_kind == X_FP4 ? 64 : 32) && K < (1 << 20) && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
 }
 
-int fp4_few(const Fp4Args& a, int x_kind, int tail, hipStream_t stream) {
+long fp4_few_workspace(const void* x, int M, int K, int x_kind) { return as_it_is(x, K, x_kind) ? 0 : fp4_planes_bytes(M, K, x_kind); }
+
+int fp4_few(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
     const Fp4Few f = fp4_few_shape(a.M, a.N, a.K, x_kind, tail);
-#define QE_NT(X_, RX_) (f.nt == 1 ? fp4_few_launch<X_, RX_, 1>(a, tail, f.waves, stream) : fp4_few_launch<X_, RX_, 2>(a, tail, f.waves, stream))
-#define QE_RX(X_) (a.M <= 2 ? QE_NT(X_, 2) : a.M <= 8 ? QE_NT(X_, 8) : QE_NT(X_, 16))
-    return x_kind == X_BF16 ? QE_RX(X_BF16) : QE_RX(X_FP4);
+    Fp4Rows x{a.x, x_kind == X_FP4 ? a.blocks * 16 : a.K * 2, 1};
+    if (!as_it_is(a.x, a.K, x_kind)) x = fp4_planes(a.x, a.M, a.K, x_kind, workspace, stream);
+#define QE_NT(X_, RX_) (f.nt == 1 ? fp4_few_launch<X_, RX_, 1>(a, x, tail, f.waves, stream) : fp4_few_launch<X_, RX_, 2>(a, x, tail, f.waves, stream))
+#define QE_RX(X_) (a.M <= 2 ? QE_NT(X_, 2) : a.M <= 8 ? QE_NT(X_, 8) : a.M <= 16 ? QE_NT(X_, 16) : QE_NT(X_, 32))
+    if (x_kind != X_FP4) return QE_RX(X_BF16);
+    return a.M > 32 ? QE_NT(X_FP4, 64) : QE_RX(X_FP4);
 #undef QE_RX
 #undef QE_NT
 }

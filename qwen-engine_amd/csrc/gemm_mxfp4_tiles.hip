@@ -335,6 +335,16 @@ static int fp4_tiles_launch(Fp4Tiles t, int splits, hipStream_t stream) {
 
 static int padded(int K) { return qe_cdiv(K, FP4_STAGE) * FP4_STAGE; }
 
+long fp4_planes_bytes(int M, int K, int x_kind) { return (x_kind == X_F32 ? 6L : 2L) * M * padded(K); }
+
+Fp4Rows fp4_planes(const void* x, int M, int K, int x_kind, void* out, hipStream_t stream) {
+    const int Kp = padded(K);
+    const dim3 grid(qe_cdiv(Kp, 1024), M < 65535 ? M : 65535);
+    if (x_kind == X_F32) fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)x, (uint16_t*)out, M, K, Kp);
+    else fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)x, (uint16_t*)out, M, K, Kp);
+    return {out, Kp * 2, x_kind == X_F32 ? 3 : 1};
+}
+
 // The kernel's 32-bit places reach all of the operands.
 bool fp4_tiles_take(int M, int N, int K, int x_kind) {
     return (long)N * padded(K) / 2 < (1L << 31) && (long)M * padded(K) * 2 * (x_kind == X_F32 ? 3 : 1) < (1L << 31);
@@ -366,8 +376,7 @@ long fp4_tiles_workspace(int M, int N, int K, int x_kind, const void* x, const v
     const bool aligned = ((uintptr_t)x & 15) == 0;
     const Fp4Shape s = fp4_tiles_shape(M, N, K, x_kind);
     long bytes = s.splits > 1 ? (4L * s.splits * M * N + 15) / 16 * 16 : 0;
-    if (x_kind == X_F32) bytes += 6L * M * padded(K);
-    else if (K % 8 || !aligned) bytes += 2L * M * padded(K);
+    if (x_kind == X_F32 || K % 8 || !aligned) bytes += fp4_planes_bytes(M, K, x_kind);
     return bytes + (fp4_scales_whole(K, scales) ? 0 : fp4_scales_bytes(N, K));
 }
 
@@ -375,25 +384,22 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     const Fp4Shape s = fp4_tiles_shape(a.M, a.N, a.K, x_kind);
     Fp4Tiles t{};
     t.a = a;
-    const int Kp = padded(a.K);
     t.nk = qe_cdiv(a.K, s.sk);
-    t.num_planes = x_kind == X_F32 ? 3 : 1;
     t.per_split = s.per_split;
-    const bool as_it_is = x_kind == X_BF16 && a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
-    t.k_in_row = as_it_is ? a.K : Kp;
-    t.row_bytes = (unsigned)t.k_in_row * 2;
-    t.plane_bytes = t.row_bytes * (unsigned)a.M;
-    t.x_bytes = t.plane_bytes * t.num_planes;
     // the workspace: the cuts' products, then what is made of x, then of the scales
     float* parts = (float*)workspace;
     unsigned char* ws = (unsigned char*)workspace + (s.splits > 1 ? (4L * s.splits * a.M * a.N + 15) / 16 * 16 : 0);
-    t.planes = as_it_is ? (const uint16_t*)a.x : (const uint16_t*)ws;
-    if (!as_it_is) {
-        const dim3 grid(qe_cdiv(Kp, 1024), a.M < 65535 ? a.M : 65535);
-        if (x_kind == X_F32) fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
-        else fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)a.x, (uint16_t*)ws, a.M, a.K, Kp);
-        ws += t.x_bytes;
+    Fp4Rows x{a.x, a.K * 2, 1};
+    if (x_kind == X_F32 || a.K % 8 || ((uintptr_t)a.x & 15)) {
+        x = fp4_planes(a.x, a.M, a.K, x_kind, ws, stream);
+        ws += fp4_planes_bytes(a.M, a.K, x_kind);
     }
+    t.planes = (const uint16_t*)x.data;
+    t.num_planes = x.planes;
+    t.row_bytes = (unsigned)x.row_bytes;
+    t.k_in_row = x.row_bytes / 2;
+    t.plane_bytes = t.row_bytes * (unsigned)a.M;
+    t.x_bytes = t.plane_bytes * t.num_planes;
     t.scales = a.scales;
     t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
     if (!fp4_scales_whole(a.K, a.scales)) {

@@ -190,9 +190,19 @@ void fp4_pad_scales(const unsigned char* scales, unsigned char* out, int rows, i
 // partial products [splits][M][N] -> a.out, summed in their order, with the tail
 int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStream_t stream);
 
-// gemm_mxfp4_rows.hip: up to 16 rows of whole blocks
-bool fp4_few_takes(const void* x, int M, int N, int K, int x_kind, int tail);
-int fp4_few(const Fp4Args& a, int x_kind, int tail, hipStream_t stream);
+// Rows of bfloat16 as the loads take them: at whole 16-byte pieces, plane after plane (or rows of codes).
+struct Fp4Rows {
+    const void* data;
+    int row_bytes, planes;
+};
+// gemm_mxfp4_tiles.hip: rows copied so, 32-bit ones in three planes of bfloat16 (low, middle, high), zeros from K to whole stages
+long fp4_planes_bytes(int M, int K, int x_kind);
+Fp4Rows fp4_planes(const void* x, int M, int K, int x_kind, void* out, hipStream_t stream);
+
+// gemm_mxfp4_rows.hip: few rows
+bool fp4_few_takes(int M, int N, int K, int x_kind, int tail);
+long fp4_few_workspace(const void* x, int M, int K, int x_kind);
+int fp4_few(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream);
 // gemm_mxfp4_tiles.hip: the products of many rows of 16 or 32 bits; the bytes of workspace that these sizes take
 bool fp4_tiles_take(int M, int N, int K, int x_kind);
 long fp4_tiles_workspace(int M, int N, int K, int x_kind, const void* x, const void* scales);

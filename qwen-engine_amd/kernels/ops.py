@@ -174,7 +174,7 @@ def load_library():
     lib.qe_attention_prefill_workspace_bytes_for.restype = ctypes.c_long
     lib.qe_decode_chain_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32, i32]
     lib.qe_decode_chain_workspace_bytes.restype = ctypes.c_long
-    lib.qe_gemm_mxfp4_workspace_bytes.argtypes = [vp, vp, vp, i32, i32, i32, i32]
+    lib.qe_gemm_mxfp4_workspace_bytes.argtypes = [vp, vp, vp, i32, i32, i32, i32, i32]
     lib.qe_gemm_mxfp4_workspace_bytes.restype = ctypes.c_long
     lib.qe_verify_drafts_workspace_bytes.argtypes = [i32, i32, i32, i32]
     lib.qe_verify_drafts_workspace_bytes.restype = ctypes.c_long
@@ -2423,8 +2423,7 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
         out = torch.empty((M, wide), dtype=out_dtype, device=dev)
     else:
         _need(out, "out", out_dtype, (M, wide), dev)
-    # (up to 16 rows need no workspace)
-    nbytes = lib.qe_gemm_mxfp4_workspace_bytes(data.data_ptr(), _ptr(scales), w.scales.data_ptr(), M, N, K, kind) if M > 16 else 0
+    nbytes = lib.qe_gemm_mxfp4_workspace_bytes(data.data_ptr(), _ptr(scales), w.scales.data_ptr(), M, N, K, kind, tail)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
     _check(lib.qe_gemm_mxfp4(data.data_ptr(), _ptr(scales), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), out.data_ptr(),
                              M, N, K, kind, _DT[out_dtype], tail, _ptr(ws), nbytes, _stream()), "gemm_mxfp4")

@@ -285,6 +285,34 @@ def test_rows_at_odd_elements(ops):
         assert (hold[:3] == 7).all() and (hold[3 + M * N:] == 7).all()
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("K", [330016, 400001])
+def test_very_wide_rows(ops, kind, K):
+    """Rows whose scales leave no room in shared memory.  One number in a thousand is not zero: the sums stay below 2^22."""
+    M, N = 3, 20
+    codes, scales, v = whole_matrix(N, K, 5)
+    w = ops.MxFp4(codes.to(DEV), scales.to(DEV), K)
+    some = torch.rand(M, K, generator=gen(6)) < 1e-3
+    some[:, -3:] = True
+    if kind == "fp4":
+        code = torch.zeros(M, (K + 31) // 32 * 32, dtype=torch.int64)
+        code[:, :K] = torch.where(some, 5, 0)                     # (threes)
+        code[:, K:] = 7
+        scale = torch.full((M, (K + 31) // 32), 127)
+        code = code.view(M, -1, 32)
+        x, xv = ops.MxFp4(packed(code).to(DEV), scale.to(torch.uint8).to(DEV), K), values_of(code, scale, K)
+    else:
+        xv = torch.where(some, torch.randint(-4, 5, (M, K), generator=gen(9)), 0).double()
+        x = xv.to(torch.float32 if kind == "float32" else torch.bfloat16).to(DEV)
+    want = xv @ v.T
+    assert torch.equal(ops.gemm_mxfp4(x, w, out_dtype=torch.float32).cpu().double(), want)
+    half = N // 2
+    act = want[:, :half] * torch.sigmoid(want[:, :half]) * want[:, half:]
+    got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32, epilogue=ops.EPI_SILU_MUL).cpu().double()
+    # (the activation's own arithmetic, and gates below -88.73, as above)
+    assert ((got - act).abs() <= (8 + want[:, :half].abs()) * 2.0 ** -23 * act.abs() + 2.0 ** -121 * want[:, half:].abs()).all()
+
+
 def test_no_rows(ops):
     w = ops.mxfp4_quantize(torch.randn(8, 64, device=DEV))
     assert ops.gemm_mxfp4(torch.empty(0, 64, device=DEV), w).shape == (0, 8)
