@@ -54,6 +54,7 @@ struct Fp4Both {
     const unsigned char* x;     // codes, nothing behind K
     const unsigned char *xs, *scales;   // of x and of the matrix, scale_bytes a row
     int nk, scale_bytes, tiles_m, tiles_n;
+    int per_split;                      // stages of a cut of K, whole spans: block (., y) sums those from y * per_split on
 };
 
 template <int TAIL, int BM, int BN>
@@ -99,11 +100,13 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         rsrc_s[i] = fp4_buffer(of_x ? t.xs : t.scales, (unsigned)((long)(of_x ? a.M : a.N) * t.scale_bytes));
     }
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
-    int ask_k = 0;                                         // the stage that is being asked for, and its place in the ring
+    const int first_stage = blockIdx.y * t.per_split, stages = min(t.nk - first_stage, t.per_split);
+    int ask_k = first_stage;                               // the stage that is being asked for, and its place in the ring
+    if constexpr (TAIL == TAIL_PARTIAL) t.a.out = (float*)t.a.out + (long)blockIdx.y * a.M * a.N;
     unsigned ask_at = lds0, ask_span = lds0 + S_AT;
     // (blocks of the last stage that lie beyond the row: a lane's offset is then made one that is out of range)
     const int off = piece < a.blocks - (t.nk - 1) * 4 ? 0 : FP4_OUT;
-    int piece_not = t.nk == 1 ? off : 0;
+    int piece_not = ask_k + 1 == t.nk ? off : 0;
 #define LOAD_PIECE(i_)                                                                                                    \
     {                                                                                                                     \
         if ((i_) < LDA) {                                                                                                 \
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
     }
     static_assert(LD <= 8, "a case for every load");
     // (beyond the last stage every load is out of range: the buffers have no bytes)
-    int ask_left = t.nk;
+    int ask_left = stages;
 #define ASKED()                                                                                                           \
     {                                                                                                                     \
         ask_at = ask_at + STAGE == lds0 + RING * STAGE ? lds0 : ask_at + STAGE;                                           \
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         fb_at[q] = B_AT + (rb >> 1) * 128 + ((((rb & 1) * 4 + 2 * h + q) ^ ((rb >> 2) & 3)) * 16);
     }
     const int sa_at = S_AT + (wm + r) * 16 + 2 * h, sb_at = S_AT + (BM + wn + r) * 16 + 2 * h;
-    int read_k = 0, read_span = 0;                         // the stage whose scales are read, and the place of its span
+    int read_k = ask_k, read_span = 0;                        // the stage whose scales are read, and the place of its span
     floatx16_t acc[MI][NJ];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
     // where a span lies between, the wait is only longer)
 #pragma unroll
     for (int s = 0; s < RING; ++s) {
-        if (ask_left > 0 && s % SPAN == 0) LOAD_SPAN()
+        if (ask_left > 0 && ask_k % SPAN == 0) LOAD_SPAN()
 #pragma unroll
         for (int i = 0; i < LD; ++i)
             if (s + 1 < RING || i < LHALF) { LOADS_OF(i) }
@@ -224,11 +227,11 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         at = next;                                                                                                        \
     }
     int at = 0, st = 0;
-    for (; st + 1 < t.nk; st += 2) {
+    for (; st + 1 < stages; st += 2) {
         STAGE_OF(0)
         STAGE_OF(1)
     }
-    if (st < t.nk) STAGE_OF(0)
+    if (st < stages) STAGE_OF(0)
     MEET(0)                                                // (what was asked for beyond the end has arrived)
 #undef STAGE_OF
 #undef K_STEP
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
 }
 
 template <int TAIL, int BM, int BN>
-static int fp4_both_launch(Fp4Both t, hipStream_t stream) {
+static int fp4_both_launch(Fp4Both t, int splits, hipStream_t stream) {
     constexpr int SHARED = (BM + BN) * (FP4_RING * 64 + 3 * 16);
     static_assert(SHARED <= 160 * 1024, "the ring must fit a compute unit");
     t.tiles_m = qe_cdiv(t.a.M, BM);
@@ -254,7 +257,7 @@ static int fp4_both_launch(Fp4Both t, hipStream_t stream) {
     const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
     QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
     QE_RAISE_SHARED((fp4_both_kernel<TAIL, BM, BN>), SHARED);
-    fp4_both_kernel<TAIL, BM, BN><<<(unsigned)blocks, 256, SHARED, stream>>>(t);
+    fp4_both_kernel<TAIL, BM, BN><<<dim3((unsigned)blocks, (unsigned)splits), 256, SHARED, stream>>>(t);
     return 0;
 }
 
@@ -263,8 +266,31 @@ bool fp4_both_take(int M, int N, int K) {
     return (long)N * qe_cdiv(K, 32) * 16 < (1L << 31) - 64 && (long)M * qe_cdiv(K, 32) * 16 < (1L << 31) - 64;
 }
 
+// 256 x 256 where its tiles keep half of the units busy, else 128 x 128 (both sides in 4 bits, quantisation included: 1024 rows against 4096 x 4096, 64
+// tiles, 22 us by 128 x 128; 2048 rows, 128 tiles, 46 by 256 x 256).
+static bool fp4_both_large(int M, int N) { return (long)qe_cdiv(M, 256) * qe_cdiv(N, 256) >= 128; }
+
+// K in cuts where that leaves a block a unit at the most and a cut two spans, and what the stages left out take (half a microsecond each) is
+// more than the cuts' products and their join do (130 rows against 4096 x 12288 in four cuts 22 us, uncut 36; 65 against 4096 x 4096 in four 14.9,
+// 15.9; 512 against that in two 25.7, 19.4).
+static int fp4_both_per_split(int M, int N, int K, int* splits) {
+    const int spans = qe_cdiv(K, FP4_SPAN), stages = qe_cdiv(K, FP4_STAGE);
+    long s = fp4_both_large(M, N) ? 1 : 256 / ((long)qe_cdiv(M, 128) * qe_cdiv(N, 128));
+    if (s > spans / 2) s = spans / 2;
+    if (s < 1 || 0.5 * stages * (double)(s - 1) / (double)s < 4.0 + 2e-6 * (double)s * M * N) s = 1;
+    const int per = qe_cdiv(spans, (int)s);
+    *splits = qe_cdiv(spans, per);
+    return per * (FP4_SPAN / FP4_STAGE);
+}
+
+static long fp4_both_parts(int M, int N, int K) {
+    int splits;
+    fp4_both_per_split(M, N, K, &splits);
+    return splits > 1 ? (4L * splits * M * N + 15) / 16 * 16 : 0;
+}
+
 long fp4_both_workspace(int M, int N, int K, const void* xs, const void* scales) {
-    return (K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0) + (fp4_scales_whole(K, xs) ? 0 : fp4_scales_bytes(M, K)) +
+    return fp4_both_parts(M, N, K) + (K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0) + (fp4_scales_whole(K, xs) ? 0 : fp4_scales_bytes(M, K)) +
            (fp4_scales_whole(K, scales) ? 0 : fp4_scales_bytes(N, K));
 }
 
@@ -273,7 +299,10 @@ int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
     t.a = a;
     t.nk = qe_cdiv(a.K, FP4_STAGE);
     t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
-    unsigned char* ws = (unsigned char*)workspace;
+    float* parts = (float*)workspace;          // the workspace: the cuts' products, then what the loads do not take as it is
+    unsigned char* ws = (unsigned char*)workspace + fp4_both_parts(a.M, a.N, a.K);
+    int splits;
+    t.per_split = fp4_both_per_split(a.M, a.N, a.K, &splits);
     t.x = (const unsigned char*)a.x;
     t.xs = a.xs;
     t.scales = a.scales;
@@ -302,14 +331,17 @@ int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
         t.scales = ws;
     }
     if (const long all = (long)p.pieces + p.x_words + p.words) fp4_prepare_kernel<<<qe_cdiv(all, 256), 256, 0, stream>>>(p);
-    const bool large = (long)qe_cdiv(a.M, 256) * qe_cdiv(a.N, 256) >= 128;
+    const bool large = fp4_both_large(a.M, a.N);
+    if (splits > 1) t.a.out = parts;
     int rc;
-#define QE_GO(T_) rc = large ? fp4_both_launch<T_, 256, 256>(t, stream) : fp4_both_launch<T_, 128, 128>(t, stream)
-    if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
+#define QE_GO(T_) rc = large ? fp4_both_launch<T_, 256, 256>(t, 1, stream) : fp4_both_launch<T_, 128, 128>(t, 1, stream)
+    if (splits > 1) rc = fp4_both_launch<TAIL_PARTIAL, 128, 128>(t, splits, stream);
+    else if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
     else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);
     else QE_GO(TAIL_SILU);
 #undef QE_GO
     if (rc) return rc;
+    if (splits > 1 && (rc = fp4_join(a, parts, splits, tail, stream))) return rc;
     QE_LAUNCH_CHECK();
     return 0;
 }

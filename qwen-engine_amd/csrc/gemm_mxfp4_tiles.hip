@@ -356,16 +356,18 @@ struct Fp4Shape {
 };
 
 static Fp4Shape fp4_tiles_shape(int M, int N, int K, int x_kind) {
-    const int planes = x_kind == X_F32 ? 3 : 1;
-    const long rows64 = qe_cdiv(M, 64) * 64L, rows128 = qe_cdiv(M, 128) * 128L;
     Fp4Shape s;
-    s.bm = M <= 64 || (M <= 512 && rows128 * 100 > rows64 * 115) ? 64 : 128;
-    if (s.bm == 128 && (long)qe_cdiv(M, 256) * qe_cdiv(N, 256) >= 192) s.bm = 256;
+    // 256 x 256 where a fifth of its rows is idle at the most and its tiles keep three quarters of the units busy (512 rows against 24576 x 4096, 192 tiles, 98 us, 128 x 128 103, 64 x 128 105;
+    // 2048 against 4096 x 4096, 128 tiles, 89, 69, 72); else 64 x 128 up to 512 rows, 128 x 128 beyond (256 against 24576 x 4096 58 and 63 us,
+    // 512 against 4096 x 4096 24 and 29, 1024 against that 36.7 and 35.3).  64 x 256 is as fast as 128 x 128 and no faster.
+    s.bm = qe_cdiv(M, 256) * 1024L <= 5L * M && (long)qe_cdiv(M, 256) * qe_cdiv(N, 256) >= 192 ? 256 : M <= 512 ? 64 : 128;
     s.sk = s.bm == 256 ? 64 : 128;
-    const int stages = qe_cdiv(K, s.sk) * planes;
+    // K in cuts where that leaves a block a unit at the most and a cut eight stages (64 rows against 4096 x 4096 in four cuts 13.9 us, eight
+    // 16.0; against 4096 x 12288 in eight 18.1, four 21.0; against 24576 x 4096, 192 tiles, uncut 24.1, two 26.2).
+    const int stages = qe_cdiv(K, s.sk) * (x_kind == X_F32 ? 3 : 1);
     const long tiles = (long)qe_cdiv(M, s.bm) * qe_cdiv(N, 128);
-    long splits = s.bm == 256 ? 1 : (s.bm == 64 ? 512 : 256) / tiles;
-    if (splits > stages / 4) splits = stages / 4;
+    long splits = s.bm == 256 ? 1 : 256 / tiles;
+    if (splits > stages / 8) splits = stages / 8;
     if (splits < 1) splits = 1;
     s.per_split = qe_cdiv(stages, (int)splits);
     s.splits = qe_cdiv(stages, s.per_split);
