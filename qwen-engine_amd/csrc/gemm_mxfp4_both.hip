@@ -248,6 +248,190 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
     fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn, smem + wave * fp4_strip_bytes<NJ>());
 }
 
+// The same in tiles of 256 x 256, a wave's part 128 x 128 with its sums in the 256 accumulation registers, and in stages of 256: whole lines of
+// 128 bytes a row (a load's 64 bytes of a line cost what 128 do: from an XCD's L2 loads of whole lines bring 33 TB/s to the chip's
+// shared memories, of half lines 17).  Two stages fit, so a stage is released by quarters: the halves of a wave's rows of x and of the matrix
+// are four regions, each read once into registers and kept there; a quarter is a half of x with a half of the matrix (16 instructions), in
+// an order in which a quarter's last operands are none of the next one's, so that each reads the region that is wanted in the next
+// quarter or the one after it.  Behind the barrier at its end that region's memory takes the same rows two stages later: seven quarters
+// for a load to arrive.  Even stages go x0 w0, x0 w1, x1 w1, x1 w0, odd ones x0 w1, x0 w0, x1 w0, x1 w1.  Lane (r, h) takes blocks 4 h .. 4 h + 3 of
+// row r, one a k step: its four scales are a word.  (4096 rows against 4096 x 12288: 101 us, in stages of 128 by the kernel above in such tiles 114.)
+template <int TAIL>
+__global__ __launch_bounds__(256, 1) void fp4_both_large_kernel(Fp4Both t) {
+    constexpr int SPANS = 3, S_AT = 2 * 65536, S_BYTES = 512 * 16;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const Fp4Args& a = t.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+    int tile_m, tile_n;
+    if (!fp4_tile_of(blockIdx.x, t.tiles_m, t.tiles_n, tile_m, tile_n)) return;
+    const int m0 = tile_m * 256, n0 = tile_n * 256;
+    const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
+    const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
+    const int row_bytes = a.blocks * 16, nk = t.nk;
+
+    // Region g (0, 1: the halves of x; 2, 3: of the matrix) of a stage holds, for each of the two waves that read it, 64 rows: 128 rows of 128
+    // bytes, the eight pieces of a row exchanged by its number.  A load is eight rows; a wave's i-th of a region: rows 32 i + 8 wave.
+    const int piece = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));      // (row / 2 % 8 of row 8 wave + lane / 8)
+    int va[2][4], vb[2][4], vs[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = (i / 2) * 128 + g * 64 + (i % 2) * 32 + wave * 8 + (lane >> 3);
+            const int n = fp4_matrix_row<TAIL>(n0, row, wide);
+            va[g][i] = m0 + row < a.M ? (m0 + row) * row_bytes + piece * 16 : FP4_OUT;
+            vb[g][i] = n >= 0 ? n * row_bytes + piece * 16 : FP4_OUT;
+        }
+    // scales of a span of two stages: 256 rows of x with its even stage, 256 of the matrix with its odd one, 64 a wave
+    vs[0] = m0 + wave * 64 + lane < a.M ? (m0 + wave * 64 + lane) * t.scale_bytes : FP4_OUT;
+    vs[1] = fp4_matrix_row<TAIL>(n0, wave * 64 + lane, wide);
+    vs[1] = vs[1] >= 0 ? vs[1] * t.scale_bytes : FP4_OUT;
+    const uintx4_t rsrc_a = fp4_buffer(t.x, (unsigned)((long)a.M * row_bytes)), rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * row_bytes));
+    const uintx4_t rsrc_x = fp4_buffer(t.xs, (unsigned)((long)a.M * t.scale_bytes)), rsrc_w = fp4_buffer(t.scales, (unsigned)((long)a.N * t.scale_bytes));
+    const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem + wave_s * 1024;
+    const int off = piece < a.blocks - (nk - 1) * 8 ? 0 : FP4_OUT;      // (blocks of the last stage that lie beyond the row: out of range)
+#define REGION_AT(g_, par_) (((par_) * 4 + (g_)) * 16384)
+#define LOAD_REGION(g_, st_, par_, i_)                                                                                    \
+    {                                                                                                                     \
+        const int not_ = (st_) < nk - 1 ? 0 : (st_) == nk - 1 ? off : FP4_OUT, s_ = (st_) < nk ? (st_) * 128 : 0;          \
+        if ((g_) < 2) { QE_LOAD_TO_SHARED(lds0 + REGION_AT(g_, par_) + (i_) * 4096, va[(g_) & 1][i_] | not_, rsrc_a, s_, "0", ""); } \
+        else { QE_LOAD_TO_SHARED(lds0 + REGION_AT(g_, par_) + (i_) * 4096, vb[(g_) & 1][i_] | not_, rsrc_b, s_, "0", ""); } \
+    }
+    // half_ 0: of x, 1: of the matrix; span_: its number, spans come in turn into a ring of three
+#define LOAD_SPAN(half_, span_)                                                                                           \
+    {                                                                                                                     \
+        const bool there_ = (span_) * 2 < nk;                                                                             \
+        const unsigned to_ = lds0 + S_AT + (span_) % SPANS * S_BYTES + (half_) * 4096;                                    \
+        const int v_ = there_ ? vs[half_] : FP4_OUT, s_ = there_ ? (span_) * 16 : 0;                                      \
+        if (half_) { QE_LOAD_TO_SHARED(to_, v_, rsrc_w, s_, "0", ""); } else { QE_LOAD_TO_SHARED(to_, v_, rsrc_x, s_, "0", ""); } \
+    }
+    // waits until at most younger_ loads of the wave are in flight and its reads of shared memory are done, then for the other waves
+#define MEET(younger_) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(younger_) : "memory");
+
+    floatx16_t acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    uintx4_t fa[2][2][4], fb[2][2][4];
+    uint32_t sa[2][2], sb[2][2];
+    const int f0 = r * 128 + (((h * 4) ^ ((r >> 1) & 7)) * 16);
+    const unsigned char* const fa0 = smem + (wave >> 1) * 8192;
+    const unsigned char* const fb0 = smem + (wave & 1) * 8192;
+    const unsigned char* const sa0 = smem + S_AT + (wm + r) * 16 + h * 4;
+    const unsigned char* const sb0 = smem + S_AT + 4096 + (wn + r) * 16 + h * 4;
+    // piece p_ of region g_ of stage st_ (parity par_): fragment p_ / 2 of its tile p_ % 2, and at first the tile's word of scales
+#define READ_REGION(g_, par_, st_, p_)                                                                                    \
+    {                                                                                                                     \
+        if ((g_) < 2) fa[(g_) & 1][(p_) & 1][(p_) >> 1] = *(const uintx4_t*)(fa0 + REGION_AT(g_, par_) + ((p_) & 1) * 4096 + (f0 ^ (((p_) >> 1) * 16))); \
+        else fb[(g_) & 1][(p_) & 1][(p_) >> 1] = *(const uintx4_t*)(fb0 + REGION_AT(g_, par_) + ((p_) & 1) * 4096 + (f0 ^ (((p_) >> 1) * 16))); \
+        if ((p_) < 2) {                                                                                                   \
+            const int at_ = (st_) / 2 % SPANS * S_BYTES + (par_) * 8 + (g_) % 2 * 1024 + ((p_) & 1) * 512;                \
+            if ((g_) < 2) sa[(g_) & 1][(p_) & 1] = *(const uint32_t*)(sa0 + at_);                                         \
+            else sb[(g_) & 1][(p_) & 1] = *(const uint32_t*)(sb0 + at_);                                                  \
+        }                                                                                                                 \
+    }
+#define MULTIPLY(ha_, hb_, i_, j_, ks_)                                                                                   \
+    {                                                                                                                     \
+        const uintx4_t &x_ = fa[ha_][i_][ks_], &w_ = fb[hb_][j_][ks_];                                                    \
+        const intx8_t xa_ = {(int)x_[0], (int)x_[1], (int)x_[2], (int)x_[3], 0, 0, 0, 0};                                 \
+        const intx8_t wb_ = {(int)w_[0], (int)w_[1], (int)w_[2], (int)w_[3], 0, 0, 0, 0};                                 \
+        floatx16_t& c_ = acc[(ha_) * 2 + (i_)][(hb_) * 2 + (j_)];                                                         \
+        c_ = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xa_, wb_, c_, 4, 4, ks_, sa[ha_][i_], ks_, sb[hb_][j_]);     \
+    }
+    // half ha_ of x with half hb_ of the matrix; meanwhile region rg_ of stage rst_ (parity rpar_) is read and region lg_ of stage lst_ (lpar_) asked for
+#define QUAD(ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_)                                                                \
+    {                                                                                                                     \
+        QUAD_STEP(0, ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_) QUAD_STEP(1, ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_) \
+        QUAD_STEP(2, ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_) QUAD_STEP(3, ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_) \
+        MEET(24)                                                                                                          \
+    }
+    // (a k step: four instructions, two pieces read in each of the first four... of the quarter's 16 places the first eight read, every fourth asks)
+#define QUAD_STEP(ks_, ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_)                                                      \
+    {                                                                                                                     \
+        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4)                                                           \
+        MULTIPLY(ha_, hb_, 0, 0, ks_)                                                                                     \
+        __builtin_amdgcn_sched_barrier(0);                                                                                \
+        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 1)                                                       \
+        MULTIPLY(ha_, hb_, 0, 1, ks_)                                                                                     \
+        LOAD_REGION(lg_, lst_, lpar_, ks_)                                                                                \
+        __builtin_amdgcn_sched_barrier(0);                                                                                \
+        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 2)                                                       \
+        MULTIPLY(ha_, hb_, 1, 0, ks_)                                                                                     \
+        __builtin_amdgcn_sched_barrier(0);                                                                                \
+        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 3)                                                       \
+        MULTIPLY(ha_, hb_, 1, 1, ks_)                                                                                     \
+        __builtin_amdgcn_sched_barrier(0);                                                                                \
+    }
+    // (the scales of the span four stages on: they are older than the loads of that stage, which are waited for)
+#define EVEN(st_)                                                                                                         \
+    LOAD_SPAN(0, (st_) / 2 + 2)                                                                                           \
+    QUAD(0, 0, 3, st_, 0, 2, (st_) + 2, 0)                                                                                \
+    QUAD(0, 1, 1, st_, 0, 3, (st_) + 2, 0)                                                                                \
+    QUAD(1, 1, 0, (st_) + 1, 1, 1, (st_) + 2, 0)                                                                          \
+    QUAD(1, 0, 3, (st_) + 1, 1, 0, (st_) + 3, 1)
+#define ODD(st_)                                                                                                          \
+    LOAD_SPAN(1, (st_) / 2 + 2)                                                                                           \
+    QUAD(0, 1, 2, st_, 1, 3, (st_) + 2, 1)                                                                                \
+    QUAD(0, 0, 1, st_, 1, 2, (st_) + 2, 1)                                                                                \
+    QUAD(1, 0, 0, (st_) + 1, 0, 1, (st_) + 2, 1)                                                                          \
+    QUAD(1, 1, 2, (st_) + 1, 0, 0, (st_) + 3, 0)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        LOAD_SPAN(half, 0)
+        LOAD_SPAN(half, 1)
+    }
+    constexpr int first[8] = {0, 2, 3, 1, 0 + 4, 3 + 4, 2 + 4, 1 + 4};      // regions in the order in which they are read (4: of the second stage)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) LOAD_REGION(first[k] & 3, first[k] >> 2, first[k] >> 2, i)
+    MEET(24)
+#pragma unroll
+    for (int p = 0; p < 8; ++p) READ_REGION(0, 0, 0, p)
+#pragma unroll
+    for (int p = 0; p < 8; ++p) READ_REGION(2, 0, 0, p)
+    MEET(24)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) LOAD_REGION(0, 2, 0, i)
+    MEET(24)
+    int st = 0;
+    for (; st + 1 < nk; st += 2) {
+        EVEN(st)
+        ODD(st + 1)
+    }
+    if (st < nk) { EVEN(st) }
+    MEET(0)                                                // (what was asked for beyond the end has arrived)
+#undef EVEN
+#undef ODD
+#undef QUAD_STEP
+#undef QUAD
+#undef MULTIPLY
+#undef READ_REGION
+#undef MEET
+#undef LOAD_SPAN
+#undef LOAD_REGION
+#undef REGION_AT
+    static_assert(4 * fp4_strip_bytes<4>() <= S_AT, "the waves' strips must fit the stages");
+    fp4_store_tiles<TAIL, 4, 4>(a, acc, m0 + wm, n0 + wn, smem + wave * fp4_strip_bytes<4>());
+}
+
+template <int TAIL>
+static int fp4_both_large_launch(Fp4Both t, hipStream_t stream) {
+    constexpr int SHARED = 2 * 65536 + 3 * 8192;
+    t.nk = qe_cdiv(t.a.K, 256);
+    t.tiles_m = qe_cdiv(t.a.M, 256);
+    t.tiles_n = qe_cdiv(t.a.N, 256);
+    const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
+    QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
+    QE_RAISE_SHARED(fp4_both_large_kernel<TAIL>, SHARED);
+    fp4_both_large_kernel<TAIL><<<(unsigned)blocks, 256, SHARED, stream>>>(t);
+    return 0;
+}
+
 template <int TAIL, int BM, int BN>
 static int fp4_both_launch(Fp4Both t, int splits, hipStream_t stream) {
     constexpr int SHARED = (BM + BN) * (FP4_RING * 64 + 3 * 16);
@@ -334,7 +518,7 @@ int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
     const bool large = fp4_both_large(a.M, a.N);
     if (splits > 1) t.a.out = parts;
     int rc;
-#define QE_GO(T_) rc = large ? fp4_both_launch<T_, 256, 256>(t, 1, stream) : fp4_both_launch<T_, 128, 128>(t, 1, stream)
+#define QE_GO(T_) rc = large ? fp4_both_large_launch<T_>(t, stream) : fp4_both_launch<T_, 128, 128>(t, 1, stream)
     if (splits > 1) rc = fp4_both_launch<TAIL_PARTIAL, 128, 128>(t, splits, stream);
     else if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
     else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);

@@ -235,7 +235,7 @@ def test_nan_and_infinities(ops, kind):
 
 
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
-@pytest.mark.parametrize("K", [40, 64, 96, 160, 200])
+@pytest.mark.parametrize("K", [40, 64, 96, 160, 200, 700, 1312])
 def test_large_tiles_and_what_lies_behind_a_row(ops, kind, K):
     """Enough rows and columns for the largest tiles; K ends inside a stage, and the row behind is NaN: every other column is exact."""
     M, N = 3100, 4200
