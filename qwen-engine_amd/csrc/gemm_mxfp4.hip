@@ -168,7 +168,7 @@ extern "C" long qe_gemm_mxfp4_workspace_bytes(const void* x, const void* x_scale
 extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* codes, const void* scales, const float* bias, void* out,
                              int M, int N, int K, int x_kind, int out_dtype, int tail, void* workspace, long workspace_bytes,
                              hipStream_t stream) {
-    QE_REQUIRE(M >= 0 && N > 0 && K > 0, "gemm_mxfp4: bad sizes M=%d N=%d K=%d", M, N, K);
+    QE_REQUIRE(M >= 0 && N > 0 && K > 0 && K < (1 << 30), "gemm_mxfp4: bad sizes M=%d N=%d K=%d", M, N, K);
     QE_REQUIRE(x_kind >= 0 && x_kind <= 2 && tail >= 0 && tail <= 2, "gemm_mxfp4: unknown form");
     QE_REQUIRE(out_dtype == QE_F32 || out_dtype == QE_BF16, "gemm_mxfp4: unknown element type %d", out_dtype);
     QE_REQUIRE(tail != TAIL_ADD || out_dtype == QE_F32, "gemm_mxfp4: the stream to add into is float32");

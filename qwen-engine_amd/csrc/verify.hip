@@ -421,7 +421,7 @@ extern "C" long qe_verify_drafts_workspace_bytes(int rows, int V, int R, int has
 extern "C" int qe_verify_drafts(const float* logits, const int* first, const int* drafts, const float* guess, const float* temperature,
                                 const float* accept, const float* draw, int* tokens, int* accepted, int rows, int V, int R,
                                 void* workspace, long workspace_bytes, hipStream_t stream) {
-    QE_REQUIRE(R >= 0 && V > 0 && rows >= R, "verify_drafts: bad sizes rows=%d V=%d R=%d", rows, V, R);
+    QE_REQUIRE(R >= 0 && V > 0 && V < (1 << 30) && rows >= R, "verify_drafts: bad sizes rows=%d V=%d R=%d", rows, V, R);
     if (R == 0) return 0;
     const int spans = qe_cdiv(V, VERIFY_SPAN), all = rows + (guess ? rows - R : 0);
     QE_REQUIRE(all <= 65535, "verify_drafts: %d rows of logits are too many", all);

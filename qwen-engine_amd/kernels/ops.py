@@ -2324,6 +2324,15 @@ def _on_current_device(t: torch.Tensor, what: str) -> None:
         raise KernelError(f"{what}: the operands are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _apart(written: torch.Tensor, read, what: str) -> None:
+    """What is written lies beside what is read: other blocks still read it then."""
+    a = written.data_ptr()
+    b = a + written.numel() * written.element_size()
+    for t in read:
+        if t is not None and t.data_ptr() < b and a < t.data_ptr() + t.numel() * t.element_size():
+            raise KernelError(f"{what}: the result lies over an operand")
+
+
 class MxFp4(NamedTuple):
     """A matrix [T, K] in microscaled 4-bit floating point: blocks of 32 numbers along K, each with a scale 2^(s - 127) (a byte
     s; 255: the block is NaN) and 32 codes of 4 bits (sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6),
@@ -2423,6 +2432,7 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
         out = torch.empty((M, wide), dtype=out_dtype, device=dev)
     else:
         _need(out, "out", out_dtype, (M, wide), dev)
+        _apart(out, (data, scales, w.codes, w.scales, bias), "gemm_mxfp4")
     nbytes = lib.qe_gemm_mxfp4_workspace_bytes(data.data_ptr(), _ptr(scales), w.scales.data_ptr(), M, N, K, kind, tail)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
     _check(lib.qe_gemm_mxfp4(data.data_ptr(), _ptr(scales), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), out.data_ptr(),
@@ -2469,10 +2479,12 @@ def verify_drafts(logits: torch.Tensor, first: torch.Tensor, drafts: torch.Tenso
         tokens = torch.empty((rows,), dtype=torch.int32, device=dev)
     else:
         _need(tokens, "tokens", torch.int32, (rows,), dev)
+        _apart(tokens, (logits, first, drafts, draft_logits, temperature, accept_uniform, draw_uniform, accepted), "verify_drafts")
     if accepted is None:
         accepted = torch.empty((R,), dtype=torch.int32, device=dev)
     else:
         _need(accepted, "accepted", torch.int32, (R,), dev)
+        _apart(accepted, (logits, first, drafts, draft_logits, temperature, accept_uniform, draw_uniform), "verify_drafts")
     if R == 0:
         return tokens, accepted
     nbytes = lib.qe_verify_drafts_workspace_bytes(rows, V, R, int(draft_logits is not None))

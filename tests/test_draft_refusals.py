@@ -44,6 +44,12 @@ def mat(t, N, K, device="cuda:0"):
     return ops.MxFp4(t(N, (K + 31) // 32 * 16, dtype=U8, device=device), t(N, (K + 31) // 32, dtype=U8, device=device), K)
 
 
+def place(monkeypatch, **at):
+    """Tensors with the given numbers of elements lie at the given places, all others far from them."""
+    at = {int(k[1:]): v for k, v in at.items()}
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: at.get(t.numel(), (1 << 40) + (id(t) << 16)))
+
+
 def refused(call, *words):
     with pytest.raises(ops.KernelError) as e:
         call()
@@ -113,6 +119,27 @@ def test_gemm(fake):
         refused(lambda: ops.gemm_mxfp4(t(2, 40), w, epilogue=e), "epilogue")
 
 
+def test_results_over_operands(fake, monkeypatch):
+    t = fake
+    x, w = t(2, 64), mat(t, 64, 64)
+    place(monkeypatch, n128=4096)                              # x and out: the same 128 numbers
+    refused(lambda: ops.gemm_mxfp4(x, w, out=t(2, 64)), "over an operand")
+    x, w, out = t(3, 64), mat(t, 64, 64), t(3, 64, dtype=B)
+    place(monkeypatch, n192=4096)
+    refused(lambda: ops.gemm_mxfp4(x, w, out_dtype=B, out=out), "over an operand")
+    place(monkeypatch, n192=4096, n2048=4096 + 368)            # (out is 384 bytes; the codes begin 16 before its end)
+    refused(lambda: ops.gemm_mxfp4(mat(t, 3, 64), mat(t, 64, 64), out=out), "over an operand")
+    place(monkeypatch, n192=4096, n2048=4096 + 384)            # behind it
+    with pytest.raises(Launched):
+        ops.gemm_mxfp4(mat(t, 3, 64), mat(t, 64, 64), out=out)
+    good = dict(logits=t(7, 50), first=t(4, dtype=I32), drafts=t(4, dtype=I32), draft_logits=None, temperature=t(3), accept_uniform=t(4),
+                draw_uniform=t(3))
+    place(monkeypatch, n7=4096, n4=4096 + 24)                  # tokens, and the drafts at its last element
+    refused(lambda: ops.verify_drafts(**good, tokens=t(7, dtype=I32)), "over an operand")
+    place(monkeypatch, n3=4096)                                # accepted, and the temperatures
+    refused(lambda: ops.verify_drafts(**good, accepted=t(3, dtype=I32)), "over an operand")
+
+
 def test_verify(fake):
     t = fake
     good = dict(logits=t(7, 50), first=t(4, dtype=I32), drafts=t(4, dtype=I32), draft_logits=t(4, 50), temperature=t(3),
@@ -156,6 +183,7 @@ def test_the_librarys_own_checks():
     refused(gemm(M=-1), "sizes")
     refused(gemm(N=0), "sizes")
     refused(gemm(K=0), "sizes")
+    refused(gemm(K=1 << 30), "sizes")
     refused(gemm(kind=3), "form")
     refused(gemm(tail=3), "form")
     refused(gemm(out=5), "element type")
@@ -172,6 +200,7 @@ def test_the_librarys_own_checks():
 
     refused(verify(rows=1), "sizes")
     refused(verify(V=0), "sizes")
+    refused(verify(V=1 << 30), "sizes")
     refused(verify(R=-1, rows=0), "sizes")
     refused(verify(rows=70000), "too many")
     refused(verify(ws=None), "workspace")

@@ -313,6 +313,53 @@ def test_very_wide_rows(ops, kind, K):
     assert ((got - act).abs() <= (8 + want[:, :half].abs()) * 2.0 ** -23 * act.abs() + 2.0 ** -121 * want[:, half:].abs()).all()
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M", [1, 9, 30, 50, 90])
+def test_rows_of_a_larger_matrix(ops, kind, M):
+    """Matrices that begin inside others, their scales at no whole word: x and w from their second row on."""
+    for N, K in ((40, 96), (333, 544), (256, 1024)):
+        codes, scales, v = whole_matrix(N + 1, K, 13)
+        codes, scales = codes.to(DEV), scales.to(DEV)
+        w = ops.MxFp4(codes[1:], scales[1:], K)
+        if kind == "fp4":
+            xc, xs, xv = whole_matrix(M + 1, K, 7)
+            x = ops.MxFp4(xc.to(DEV)[1:], xs.to(DEV)[1:], K)
+        else:
+            xv = torch.randint(-4, 5, (M + 1, K), generator=gen(9)).double()
+            x = xv.to(torch.float32 if kind == "float32" else torch.bfloat16).to(DEV)[1:]
+        want = xv[1:] @ v[1:].T
+        assert torch.equal(ops.gemm_mxfp4(x, w, out_dtype=torch.float32).cpu().double(), want), (N, K)
+        assert torch.equal(ops.mxfp4_values(w, torch.float32).cpu().double(), v[1:])
+
+
+def test_matrices_beyond_32_bits(ops):
+    """A matrix of more than 2^31 bytes of codes: its last columns, by every number of rows."""
+    N, K = 540001, 8192
+    some = torch.tensor([0, 1, 262143, 262144, 524287, 524289, N - 2, N - 1])
+    g = torch.Generator(device=DEV).manual_seed(1)
+    codes = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=DEV, generator=g)
+    scales = torch.randint(127, 129, (N, K // 32), device=DEV, generator=g).to(torch.uint8)
+    w = ops.MxFp4(codes, scales, K)
+    v = values_of(unpack(codes[some.to(DEV)].cpu()), scales[some.to(DEV)].cpu().int(), K)
+    for M in (1, 20, 40):
+        xv = torch.randint(-4, 5, (M, K), generator=gen(M)).double()
+        for x in (xv.to(torch.bfloat16).to(DEV), xv.float().to(DEV), ops.mxfp4_quantize(xv.float().to(DEV))):
+            want = (ops.mxfp4_values(x, torch.float32).cpu().double() if isinstance(x, ops.MxFp4) else xv) @ v.T
+            got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32)[:, some.to(DEV)].cpu().double()
+            assert torch.equal(got, want), M
+    last = ops.mxfp4_values(ops.MxFp4(codes[-3:], scales[-3:], K), torch.bfloat16)
+    assert torch.equal(ops.mxfp4_values(w, torch.bfloat16)[-3:], last)
+
+
+def test_quantize_beyond_32_bits(ops):
+    T, K = 66000, 32768                                        # more than 2^31 numbers
+    rows = torch.randn(7, K, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    x = rows.repeat(T // 7 + 1, 1)[:T]
+    m, few = ops.mxfp4_quantize(x), ops.mxfp4_quantize(rows)
+    at = torch.tensor([0, 1, 32767, 65535, 65536, T - 1], device=DEV)
+    assert torch.equal(m.codes[at], few.codes[at % 7]) and torch.equal(m.scales[at], few.scales[at % 7])
+
+
 def test_no_rows(ops):
     w = ops.mxfp4_quantize(torch.randn(8, 64, device=DEV))
     assert ops.gemm_mxfp4(torch.empty(0, 64, device=DEV), w).shape == (0, 8)

@@ -235,6 +235,39 @@ def test_no_requests(ops):
     assert tokens.shape == (0,) and accepted.shape == (0,)
 
 
+def test_logits_beyond_32_bits(ops):
+    """More than 2^31 logits: the last requests' tokens are those that they get alone."""
+    R, V = 14200, 151936
+    g = torch.Generator(device=DEV).manual_seed(2)
+    z = torch.randn(R, V, device=DEV, generator=g)
+    t = torch.tensor([0.0, 0.9], device=DEV).repeat(R // 2)
+    u = torch.rand(R, device=DEV, generator=g)
+    none = torch.empty(0, device=DEV)
+    first = torch.arange(R + 1, dtype=torch.int32, device=DEV)
+    tokens, accepted = ops.verify_drafts(z, first, none.int(), None, t, none, u)
+    assert (accepted == 0).all()
+    assert torch.equal(tokens[::2].long(), z[::2].argmax(1))
+    few, _ = ops.verify_drafts(z[-6:], first[:7], none.int(), None, t[-6:], none, u[-6:])
+    assert torch.equal(tokens[-6:], few)
+
+
+def test_two_streams_at_once(ops):
+    """Calls on two streams that overlap do not share anything."""
+    cs = [case([3, 1, 2, 4], 30000, 40 + i) for i in range(2)]
+    want = [tuple(v.tolist() for v in go(ops, c)) for c in cs]
+    up = lambda c: [c[k].to(DEV) for k in ("logits", "drafts", "guess", "temperature", "accept", "draw")] + [first_of(c["counts"]).to(DEV)]
+    held = [up(c) for c in cs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cs], [[], []]
+    for _ in range(20):
+        for i, (s, (z, d, q, t, a, u, f)) in enumerate(zip(streams, held)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.verify_drafts(z, f, d, q, t, a, u))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all((tokens.tolist(), accepted.tolist()) == w for tokens, accepted in g)
+
+
 @pytest.mark.parametrize("lookup", [False, True])
 def test_tokens_are_distributed_as_the_models(ops, lookup):
     """20 000 requests with one draft each from another distribution: the first token's frequencies are the model's.  A count of n
