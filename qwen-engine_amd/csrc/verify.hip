@@ -54,7 +54,6 @@ struct VerifyChoice {           // of a request: what its token is drawn from, t
     float p_top, q_top;
     int row, guess_row;         // row -1: nothing is drawn
     int point;                  // the column that a draft without logits was, -1: there is none
-    int pad;
 };
 
 // a b + c with c in scalar registers: the compiler's choice, b's product added into a copy of c, costs two more instructions a term
@@ -118,11 +117,36 @@ __device__ __forceinline__ void verify_load(const float* row, int c0, int V, int
     }
 }
 
-__device__ __forceinline__ double verify_wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Lane i's sum of the lanes up to i, each with its own: within rows of 16 lanes by shifts of a row, then the last lane of rows 0 and 2 to
+// rows 1 and 3, then lane 31 to rows 2 and 3.  These moves are operands of instructions, where a shuffle is a trip through the LDS
+// unit (six of them, of 64 bits, one after the other: 0.4 us).
+template <int CTRL, int ROWS> __device__ __forceinline__ double verify_moved(double v) {      // 0 where no lane sends
+    const unsigned long b = __builtin_bit_cast(unsigned long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned long)hi << 32 | lo);
+}
+#define ROW_SHR(n_) (0x110 + (n_))
+#define ROW_BCAST15 0x142
+#define ROW_BCAST31 0x143
+__device__ __forceinline__ double verify_wave_scan(double v) {
+    v += verify_moved<ROW_SHR(1), 0xf>(v);
+    v += verify_moved<ROW_SHR(2), 0xf>(v);
+    v += verify_moved<ROW_SHR(4), 0xf>(v);
+    v += verify_moved<ROW_SHR(8), 0xf>(v);
+    v += verify_moved<ROW_BCAST15, 0xa>(v);
+    v += verify_moved<ROW_BCAST31, 0xc>(v);
     return v;
 }
+
+// Lane `lane` of v, the same number in every lane (lane the same in every lane, too).
+__device__ __forceinline__ double verify_lane(double v, int lane) {
+    const unsigned long b = __builtin_bit_cast(unsigned long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), lane);
+    return __builtin_bit_cast(double, (unsigned long)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double verify_wave_sum(double v) { return verify_lane(verify_wave_scan(v), 63); }
 
 template <int THREADS>
 __device__ __forceinline__ double verify_block_sum(double v, double* shared) {
@@ -138,12 +162,13 @@ __device__ __forceinline__ double verify_block_sum(double v, double* shared) {
 
 // The largest of the wave and the lowest column that has it, in every lane.
 __device__ __forceinline__ void verify_wave_top(float& top, int& at) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float other = __shfl_xor(top, o, 64);
-        const int there = __shfl_xor(at, o, 64);
-        if (other > top || (other == top && there < at)) { top = other; at = there; }
-    }
+    const float mine = top;
+    top = wave_max(top);
+    at = mine == top ? at : 0x7fffffff;
+#define LOWER(ctrl_, rows_) at = min(at, __builtin_amdgcn_update_dpp(at, at, ctrl_, rows_, 0xf, false));
+    LOWER(ROW_SHR(1), 0xf) LOWER(ROW_SHR(2), 0xf) LOWER(ROW_SHR(4), 0xf) LOWER(ROW_SHR(8), 0xf) LOWER(ROW_BCAST15, 0xa) LOWER(ROW_BCAST31, 0xc)
+#undef LOWER
+    at = __builtin_amdgcn_readlane(at, 63);
 }
 
 // One block a span of a row: blockIdx.y counts the rows of the logits, then those of the drafts' logits.
@@ -322,17 +347,6 @@ __global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, cons
     if (threadIdx.x == 0) rests[(long)r * a.spans + span] = sum;
 }
 
-// The sums of the lanes up to this one's, each with its own.
-__device__ __forceinline__ double verify_wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double other = __shfl_up(v, o, 64);
-        if (lane >= o) v += other;
-    }
-    return v;
-}
-
 // The draw: a block a request.  Its span is the first whose sum reaches beyond the random number's share of the whole (every wave finds
 // it for itself, 64 spans at a time), then its token the first of the span: sums of four neighbours a thread, then a walk through
 // those.  Where a rounding lets a span's own sum fall short of the share, or the number is 1 or more, the token is the last one that
@@ -348,8 +362,8 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
     const VerifyChoice c = choices[r];
     const float u = a.draw[r];
     if (c.row < 0) return;
-    double scan0 = verify_wave_scan(v0), total = __shfl(scan0, 63, 64);
-    for (int s0 = 64; s0 < a.spans; s0 += 64) total += __shfl(verify_wave_scan(s0 + lane < a.spans ? rests[s0 + lane] : 0.0), 63, 64);
+    double scan0 = verify_wave_scan(v0), total = verify_lane(scan0, 63);
+    for (int s0 = 64; s0 < a.spans; s0 += 64) total += verify_wave_sum(s0 + lane < a.spans ? rests[s0 + lane] : 0.0);
     // (nothing left: the draft's distribution is the model's, and only a rounding or a number beyond 1 refused the draft: p alone)
     const bool rest = total > 0.0;
     auto span_sum = [&](int s) { return s >= a.spans ? 0.0 : rest ? rests[s] : verify_plain_sum(a, parts, c, s); };
@@ -357,7 +371,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
         v0 = span_sum(lane);
         scan0 = verify_wave_scan(v0);
         total = 0.0;
-        for (int s0 = 0; s0 < a.spans; s0 += 64) total += __shfl(verify_wave_scan(span_sum(s0 + lane)), 63, 64);
+        for (int s0 = 0; s0 < a.spans; s0 += 64) total += verify_wave_sum(span_sum(s0 + lane));
     }
     const double target = u > 0.f ? (double)u * total : 0.0;       // (NaN: 0)
     int span = -1;
@@ -368,10 +382,10 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
         if (some) {
             const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
             span = s0 + at;
-            before = run + __shfl(scan, at, 64) - __shfl(v, at, 64);
+            before = run + verify_lane(scan, at) - verify_lane(v, at);
         }
         if (over) break;
-        run += __shfl(scan, 63, 64);
+        run += verify_lane(scan, 63);
     }
     if (span < 0) return;                      // (no weight anywhere)
     const int c0 = span * VERIFY_SPAN + tid * EACH;
