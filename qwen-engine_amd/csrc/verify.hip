@@ -307,11 +307,29 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
     verify_accept(a, parts, choices, blockIdx.x, true);
 }
 
-// The weight of column i in a draw, of its logits in the model's row and in the draft's (rest: with the draft's distribution taken away).
-__device__ __forceinline__ double verify_draw_weight(const VerifyChoice& c, float z, float zq, int i, bool rest) {
-    double w = verify_weight(z, c.p_top, c.t) * c.p_each;
-    if (rest && c.q_each > 0.0) w = __builtin_fmax(w - verify_weight(zq, c.q_top, c.t) * c.q_each, 0.0);
-    return rest && i == c.point ? 0.0 : w;
+// The weights in a draw of a thread's share of the span from c0 on, of the logits in the model's row and in the draft's (rest: with the draft's
+// distribution taken away).  The forms are told apart once, not at every number, so that the polynomials go side by side (1 request 0.9 us less).
+__device__ __forceinline__ void verify_draw_weights(const VerifyChoice& c, const float (&z)[VERIFY_SPAN / 1024], const float (&zq)[VERIFY_SPAN / 1024], int c0,
+                                                    bool rest, double (&w)[VERIFY_SPAN / 1024]) {
+    constexpr int EACH = VERIFY_SPAN / 1024;
+    const bool with_q = rest && c.q_each > 0.0;
+    if (c.p_top == INFINITY || (with_q && c.q_top == INFINITY)) {
+#pragma unroll 1
+        for (int e = 0; e < EACH; ++e) {
+            w[e] = verify_weight(z[e], c.p_top, c.t) * c.p_each;
+            if (with_q) w[e] = __builtin_fmax(w[e] - verify_weight(zq[e], c.q_top, c.t) * c.q_each, 0.0);
+        }
+    } else if (with_q) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+            w[e] = __builtin_fmax(verify_finite_weight(z[e], c.p_top, c.t) * c.p_each - verify_finite_weight(zq[e], c.q_top, c.t) * c.q_each, 0.0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) w[e] = verify_finite_weight(z[e], c.p_top, c.t) * c.p_each;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+        if (rest && c0 + verify_column<1024>(e) == c.point) w[e] = 0.0;
 }
 
 // A span's weights without the draft's: summed already.
@@ -321,10 +339,10 @@ __device__ __forceinline__ double verify_plain_sum(const VerifyArgs& a, const Ve
 }
 
 // The sum of the weights of a span.  ACCEPT: the block finds the choice for itself.
-template <int THREADS, bool ACCEPT>
-__global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests) {
-    constexpr int EACH = VERIFY_SPAN / THREADS;
-    __shared__ double shared[THREADS / 64];
+template <bool ACCEPT>
+__global__ __launch_bounds__(1024) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests) {
+    constexpr int EACH = VERIFY_SPAN / 1024;
+    __shared__ double shared[16];
     const int r = blockIdx.y, span = blockIdx.x;
     VerifyChoice c;
     if constexpr (ACCEPT) c = verify_accept(a, parts, choices, r, span == 0);
@@ -336,13 +354,15 @@ __global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, cons
         sum = verify_plain_sum(a, parts, c, span);
     } else {
         float v[EACH], q[EACH];
-        verify_load<THREADS>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
+        verify_load<1024>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
 #pragma unroll
         for (int e = 0; e < EACH; ++e) q[e] = 0.f;
-        if (c.q_each > 0.0) verify_load<THREADS>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
+        if (c.q_each > 0.0) verify_load<1024>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
+        double each[EACH];
+        verify_draw_weights(c, v, q, span * VERIFY_SPAN, true, each);
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) sum += verify_draw_weight(c, v[e], q[e], span * VERIFY_SPAN + verify_column<THREADS>(e), true);
-        sum = verify_block_sum<THREADS>(sum, shared);
+        for (int e = 0; e < EACH; ++e) sum += each[e];
+        sum = verify_block_sum<1024>(sum, shared);
     }
     if (threadIdx.x == 0) rests[(long)r * a.spans + span] = sum;
 }
@@ -354,13 +374,14 @@ __global__ __launch_bounds__(THREADS) void verify_rest_kernel(VerifyArgs a, cons
 __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
     constexpr int EACH = VERIFY_SPAN / 1024;
     __shared__ double shared[16];
-    __shared__ int found_s, last_s;
+    __shared__ int founds[16], lasts[16];
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) { found_s = 0x7fffffff; last_s = -1; }
     const double* rests = rests_all + (long)r * a.spans;
     double v0 = lane < a.spans ? rests[lane] : 0.0;        // (nothing of them is used where nothing is drawn)
     const VerifyChoice c = choices[r];
     const float u = a.draw[r];
+    // (all of the choice at once, with the sums, not part by part as it is wanted)
+    asm volatile("" : : "s"(c.row), "s"(c.guess_row), "s"(c.point), "s"(c.p_top), "s"(c.q_top), "s"(c.p_each), "s"(c.q_each), "s"(c.t.k), "s"(c.t.least), "s"(u), "v"(v0));
     if (c.row < 0) return;
     double scan0 = verify_wave_scan(v0), total = verify_lane(scan0, 63);
     for (int s0 = 64; s0 < a.spans; s0 += 64) total += verify_wave_sum(s0 + lane < a.spans ? rests[s0 + lane] : 0.0);
@@ -388,7 +409,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
         run += verify_lane(scan, 63);
     }
     if (span < 0) return;                      // (no weight anywhere)
-    const int c0 = span * VERIFY_SPAN + tid * EACH;
+    const int c0 = span * VERIFY_SPAN + tid * EACH;        // (a thread's share is four neighbours)
     double each[EACH], sum = 0.0;
     float v[EACH], q[EACH];
     verify_load<1024>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
@@ -396,9 +417,9 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
     for (int e = 0; e < EACH; ++e) q[e] = 0.f;
     if (rest && c.q_each > 0.0) verify_load<1024>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
     int last = -1;
+    verify_draw_weights(c, v, q, span * VERIFY_SPAN, rest, each);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-        each[e] = verify_draw_weight(c, v[e], q[e], c0 + e, rest);
         sum += each[e];
         if (each[e] > 0.0) last = c0 + e;
     }
@@ -410,18 +431,25 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
     for (int w = 0; w < 16; ++w)
         if (w < wave) run += shared[w];
     run += scan - sum;
-    if (last >= 0) {
-        int found = 0x7fffffff;
+    int found = -1;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            run += each[e];
-            if (found == 0x7fffffff && each[e] > 0.0 && run > target) found = c0 + e;
-        }
-        if (found != 0x7fffffff) atomicMin(&found_s, found);
-        atomicMax(&last_s, last);
+    for (int e = 0; e < EACH; ++e) {
+        run += each[e];
+        if (found < 0 && each[e] > 0.0 && run > target) found = c0 + e;
     }
+    // the wave's first that reaches beyond, and its last that weighs anything, then the block's (columns rise with the threads)
+    const unsigned long over = __ballot(found >= 0), some = __ballot(last >= 0);
+    if (over) found = __builtin_amdgcn_readlane(found, __ffsll((unsigned long long)over) - 1);
+    if (some) last = __builtin_amdgcn_readlane(last, 63 - __clzll((long long)some));
+    if (lane == 0) { founds[wave] = over ? found : -1; lasts[wave] = some ? last : -1; }
     __syncthreads();
-    if (tid == 0) a.tokens[c.row] = found_s != 0x7fffffff ? found_s : last_s;
+    if (tid != 0) return;
+    int token = -1;
+    for (int w = 0; w < 16; ++w) {
+        if (founds[w] >= 0) { token = founds[w]; break; }
+        if (lasts[w] >= 0) token = lasts[w];
+    }
+    a.tokens[c.row] = token;
 }
 
 extern "C" long qe_verify_drafts_workspace_bytes(int rows, int V, int R, int has_guess) {
@@ -447,13 +475,13 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     const int four = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)guess) & 15) == 0;
     const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, four};
     verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts);
-    // Few spans: every block accepts for itself, which saves a launch, and takes four exponentials a thread instead of 16, one after the other
-    // (1 request of 38 spans 23 us, apart 28 with 16 and 25 with four a thread; 64 requests, apart, 129 with 16 and 134 with four).
-    if ((long)spans * R <= 512) {
-        verify_rest_kernel<1024, true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
+    // Few spans: every block accepts for itself, which saves a launch (spans of 1 request of 151936 15.1 us, in two launches 16.4; of 8, 304
+    // spans, 27.2 and 28.1; of 16 40.4 and 36.3).
+    if ((long)spans * R <= 320) {
+        verify_rest_kernel<true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
     } else {
         verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
-        verify_rest_kernel<256, false><<<dim3(spans, R), 256, 0, stream>>>(a, parts, choices, rests);
+        verify_rest_kernel<false><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
     }
     verify_draw_kernel<<<R, 1024, 0, stream>>>(a, parts, choices, rests);
     QE_LAUNCH_CHECK();
