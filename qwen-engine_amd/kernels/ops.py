@@ -2347,6 +2347,13 @@ def _need_mxfp4(m: MxFp4, name: str, device=None) -> Tuple[int, int]:
     if not isinstance(m, MxFp4):
         raise KernelError(f"{name} is no 4-bit matrix")
     codes, scales, K = m
+    # (as in _need, what passes is found out first)
+    if isinstance(K, int) and K > 0 and isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and \
+            codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous():
+        at, T, blocks = codes.get_device(), scales.shape[0] if scales.dim() == 2 else -1, (K + 31) // 32
+        if at >= 0 and scales.get_device() == at and (device is None or device.index == at) and scales.shape == (T, blocks) and \
+                codes.shape == (T, blocks * 16) and codes.data_ptr() % 16 == 0:
+            return T, K
     K = int(K)
     if K <= 0:
         raise KernelError(f"{name} has {K} columns")
@@ -2370,8 +2377,8 @@ def mxfp4_quantize(x: torch.Tensor) -> MxFp4:
         raise KernelError("mxfp4_quantize: rows of no numbers")
     _on_current_device(x, "mxfp4_quantize")
     blocks = (K + 31) // 32
-    codes = torch.empty((T, blocks * 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((T, blocks), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((T, blocks * 16), dtype=torch.uint8)
+    scales = x.new_empty((T, blocks), dtype=torch.uint8)
     _check(lib.qe_mxfp4_quantize(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), T, K, _DT[x.dtype], _stream()), "mxfp4_quantize")
     return MxFp4(codes, scales, K)
 
@@ -2383,7 +2390,7 @@ def mxfp4_values(m: MxFp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     if dtype not in _DT:
         raise KernelError(f"mxfp4_values: element type {dtype}")
     _on_current_device(m.codes, "mxfp4_values")
-    out = torch.empty((T, K), dtype=dtype, device=m.codes.device)
+    out = m.codes.new_empty((T, K), dtype=dtype)
     _check(lib.qe_mxfp4_values(m.codes.data_ptr(), m.scales.data_ptr(), out.data_ptr(), T, K, _DT[dtype], _stream()), "mxfp4_values")
     return out
 
@@ -2429,12 +2436,12 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
         raise KernelError(f"gemm_mxfp4: a result in {out_dtype}")
     _on_current_device(data, "gemm_mxfp4")
     if out is None:
-        out = torch.empty((M, wide), dtype=out_dtype, device=dev)
+        out = data.new_empty((M, wide), dtype=out_dtype)
     else:
         _need(out, "out", out_dtype, (M, wide), dev)
         _apart(out, (data, scales, w.codes, w.scales, bias), "gemm_mxfp4")
     nbytes = lib.qe_gemm_mxfp4_workspace_bytes(data.data_ptr(), _ptr(scales), w.scales.data_ptr(), M, N, K, kind, tail)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+    ws = data.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     _check(lib.qe_gemm_mxfp4(data.data_ptr(), _ptr(scales), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), out.data_ptr(),
                              M, N, K, kind, _DT[out_dtype], tail, _ptr(ws), nbytes, _stream()), "gemm_mxfp4")
     return out
