@@ -355,23 +355,45 @@ struct Fp4Shape {
     int bm, sk, per_split, splits;
 };
 
+// A round of tiles of so many rows (one a unit) takes `round` us and `stage` us for 128 of K, as measured (with rounds of them: 4096 x 24576, 12288, 6144;
+// 1024 x 40000, 3000; 12288 x 4096; 65 to 2048 rows).  Of 64 rows two share a unit, 1.04 us a stage; alone there, 0.62.
+struct Fp4TileCost {
+    int bm;
+    double round, stage;
+};
+static const Fp4TileCost fp4_tile_costs[] = {{64, 3.4, 1.04}, {96, 4.1, 0.68}, {128, 4.6, 0.80}, {160, 6.0, 0.93}, {256, 12.8, 2.27}};
+
+// The tiles that are done first by these times: what counts is how many rounds the units make and how many of a tile's rows are idle (65 rows
+// against 24576 x 4096 by 96 rows 27.5 us, by 64 36.4; 160 rows by 160 37.4, by 64 51.8; 256 rows by 64 58.8, by 160 71; 700 against
+// 6144 x 4096 by 160 39, by 128 60; 512 against 24576 x 4096 by 256 92, by 128 103).  Over 53 sizes the choice is 0.6 % slower than the best one on the
+// average, 9 % at the most.
+// K in cuts where that leaves a block a unit at the most and a cut eight stages, at the price of the join (64 rows against 4096 x 4096 in four cuts
+// 13.9 us, eight 16.0; against 4096 x 12288 in eight 18.1, four 21.0; against 24576 x 4096, 192 tiles, uncut 24.1, two 26.2).
 static Fp4Shape fp4_tiles_shape(int M, int N, int K, int x_kind) {
-    Fp4Shape s;
-    // 256 x 256 where a fifth of its rows is idle at the most and its tiles keep three quarters of the units busy (512 rows against 24576 x 4096, 192 tiles, 98 us, 128 x 128 103, 64 x 128 105;
-    // 2048 against 4096 x 4096, 128 tiles, 89, 69, 72); else 64 x 128 up to 512 rows, 128 x 128 beyond (256 against 24576 x 4096 58 and 63 us,
-    // 512 against 4096 x 4096 24 and 29, 1024 against that 36.7 and 35.3).  64 x 256 is as fast as 128 x 128 and no faster.
-    s.bm = qe_cdiv(M, 256) * 1024L <= 5L * M && (long)qe_cdiv(M, 256) * qe_cdiv(N, 256) >= 192 ? 256 : M <= 512 ? 64 : 128;
-    s.sk = s.bm == 256 ? 64 : 128;
-    // K in cuts where that leaves a block a unit at the most and a cut eight stages (64 rows against 4096 x 4096 in four cuts 13.9 us, eight
-    // 16.0; against 4096 x 12288 in eight 18.1, four 21.0; against 24576 x 4096, 192 tiles, uncut 24.1, two 26.2).
-    const int stages = qe_cdiv(K, s.sk) * (x_kind == X_F32 ? 3 : 1);
-    const long tiles = (long)qe_cdiv(M, s.bm) * qe_cdiv(N, 128);
-    long splits = s.bm == 256 ? 1 : 256 / tiles;
-    if (splits > stages / 8) splits = stages / 8;
-    if (splits < 1) splits = 1;
-    s.per_split = qe_cdiv(stages, (int)splits);
-    s.splits = qe_cdiv(stages, s.per_split);
-    return s;
+    Fp4Shape best{};
+    double least = 0.0;
+    for (const Fp4TileCost& c : fp4_tile_costs) {
+        Fp4Shape s;
+        s.bm = c.bm;
+        s.sk = c.bm == 256 ? 64 : 128;
+        const int planes = x_kind == X_F32 ? 3 : 1, stages = qe_cdiv(K, s.sk) * planes;
+        const long tiles = (long)qe_cdiv(M, s.bm) * qe_cdiv(N, s.bm == 256 ? 256 : 128);
+        long splits = s.bm == 256 ? 1 : 256 / tiles;
+        if (splits > stages / 8) splits = stages / 8;
+        if (splits < 1) splits = 1;
+        s.per_split = qe_cdiv(stages, (int)splits);
+        s.splits = qe_cdiv(stages, s.per_split);
+        const double walk = (double)s.per_split * s.sk / 128;      // in stages of 128
+        const long blocks = tiles * s.splits;
+        double time = (double)qe_cdiv(blocks, 256) * (c.round + c.stage * walk);
+        if (s.bm == 64) {
+            const long rest = blocks % 512;
+            time = (double)(blocks / 512 + (rest > 256)) * (c.round + c.stage * walk) + (rest > 0 && rest <= 256 ? 3.0 + 0.62 * walk : 0.0);
+        }
+        if (s.splits > 1) time += 3.0 + 2e-6 * s.splits * (double)M * N;
+        if (best.bm == 0 || time < least) { best = s; least = time; }
+    }
+    return best;
 }
 
 long fp4_tiles_workspace(int M, int N, int K, int x_kind, const void* x, const void* scales) {
@@ -412,11 +434,15 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     int rc;
 #define QE_GO(T_)                                                                            \
     rc = s.bm == 256   ? fp4_tiles_launch<T_, 256, 256, 2, 2, 64, 3>(t, s.splits, stream)     \
+         : s.bm == 160 ? fp4_tiles_launch<T_, 160, 128, 1, 4, 128, 3>(t, s.splits, stream)    \
          : s.bm == 128 ? fp4_tiles_launch<T_, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)    \
+         : s.bm == 96  ? fp4_tiles_launch<T_, 96, 128, 1, 4, 128, 3>(t, s.splits, stream)     \
                        : fp4_tiles_launch<T_, 64, 128, 1, 4, 128, 3>(t, s.splits, stream)
     if (s.splits > 1)
-        rc = s.bm == 128 ? fp4_tiles_launch<TAIL_PARTIAL, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)
-                         : fp4_tiles_launch<TAIL_PARTIAL, 64, 128, 1, 4, 128, 3>(t, s.splits, stream);
+        rc = s.bm == 160   ? fp4_tiles_launch<TAIL_PARTIAL, 160, 128, 1, 4, 128, 3>(t, s.splits, stream)
+             : s.bm == 128 ? fp4_tiles_launch<TAIL_PARTIAL, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)
+             : s.bm == 96  ? fp4_tiles_launch<TAIL_PARTIAL, 96, 128, 1, 4, 128, 3>(t, s.splits, stream)
+                           : fp4_tiles_launch<TAIL_PARTIAL, 64, 128, 1, 4, 128, 3>(t, s.splits, stream);
     else if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
     else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);
     else QE_GO(TAIL_SILU);

@@ -34,6 +34,7 @@ def fake(monkeypatch):
     monkeypatch.setattr(ops, "load_library", lambda: NoLaunch())
     monkeypatch.setattr(ops, "_stream", lambda: 0)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)      # (else a tensor without memory on cuda:1 asks for that device)
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
     monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 4096)
     with FakeTensorMode():

@@ -268,6 +268,35 @@ def test_large_tiles_and_what_lies_behind_a_row(ops, kind, K):
         assert ((got - act).nan_to_num().abs() <= bound).all()
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+@pytest.mark.parametrize("M,N,K", [(200, 8230, 712), (300, 8230, 712), (470, 8230, 712), (500, 4200, 1312), (1000, 4200, 330), (70, 20100, 200),
+                                   (330, 1000, 12000), (600, 1000, 12000), (600, 1000, 4160), (3100, 302, 12000), (270, 1002, 4168)])
+def test_tiles_of_every_height(ops, kind, M, N, K):
+    """Rows and columns that tiles of 64, 96, 128, 160 and 256 rows are taken for, with K in one piece and in cuts; every seventh column
+    and every fifth row is NaN, every other sum exact (halves of at most 48 K < 2^21), the activation within its own arithmetic."""
+    codes, scales, v = whole_matrix(N, K, K)
+    scales[1::7] = 255
+    v = torch.where((scales == 255).any(1, keepdim=True), torch.full_like(v, math.nan), v).to(DEV)
+    w = ops.MxFp4(codes.to(DEV), scales.to(DEV), K)
+    xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+    xv[1::5] = math.nan
+    x = xv.to(getattr(torch, kind)).to(DEV)
+    want = xv.to(DEV) @ v.T
+    same = lambda got, to: torch.equal(got.isnan(), to.isnan()) and torch.equal(got.nan_to_num(), to.nan_to_num())
+    assert same(ops.gemm_mxfp4(x, w, out_dtype=torch.float32).double(), want)
+    bias = torch.randint(-50, 50, (N,), generator=gen(3)).float().to(DEV)
+    stream = torch.randint(-50, 50, (M, N), generator=gen(4)).float().to(DEV)
+    to = want + bias + stream
+    assert same(ops.gemm_mxfp4(x, w, bias, out=stream, epilogue=ops.EPI_RESIDUAL).double(), to)
+    up, gate = want[:, N // 2:], want[:, :N // 2]
+    got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32, epilogue=ops.EPI_SILU_MUL).double()
+    act = gate * torch.sigmoid(gate) * up
+    assert torch.equal(got.isnan(), act.isnan())
+    # (the bound of the large tiles' test)
+    bound = (8 + gate.abs()).nan_to_num() * 2.0 ** -23 * act.nan_to_num().abs() + 2.0 ** -121 * up.nan_to_num().abs()
+    assert ((got - act).nan_to_num().abs() <= bound).all()
+
+
 def test_rows_at_odd_elements(ops):
     """x, bias and out at no whole 16-byte piece; the numbers before and behind out stay."""
     M, N, K = 19, 40, 96
