@@ -210,7 +210,7 @@ long fp4_few_workspace(const void* x, int M, int K, int x_kind) { return as_it_i
 int fp4_few(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
     const Fp4Few f = fp4_few_shape(a.M, a.N, a.K, x_kind, tail);
     Fp4Rows x{a.x, x_kind == X_FP4 ? a.blocks * 16 : a.K * 2, 1};
-    if (!as_it_is(a.x, a.K, x_kind)) x = fp4_planes(a.x, a.M, a.K, x_kind, workspace, stream);
+    if (!as_it_is(a.x, a.K, x_kind)) x = fp4_copies(a.x, a.M, a.K, x_kind, workspace, nullptr, 0, nullptr, stream);
 #define QE_NT(X_, RX_) (f.nt == 1 ? fp4_few_launch<X_, RX_, 1>(a, x, tail, f.waves, stream) : fp4_few_launch<X_, RX_, 2>(a, x, tail, f.waves, stream))
 #define QE_RX(X_) (a.M <= 2 ? QE_NT(X_, 2) : a.M <= 8 ? QE_NT(X_, 8) : a.M <= 16 ? QE_NT(X_, 16) : QE_NT(X_, 32))
     if (x_kind != X_FP4) return QE_RX(X_BF16);

@@ -12,51 +12,90 @@
 
 #define FP4_STAGE 128      // numbers of K
 
-// x [M, K] float32 -> planes [3][M][Kp] (low, middle, high) of bfloat16, zeros from K on; bfloat16 -> [M][Kp]
+// What the loads cannot take as it is, in one launch.  Blocks 0 .. x_blocks - 1: x [M, K] float32 -> planes [3][M][Kp] (low, middle, high) of
+// bfloat16, zeros from K on, or bfloat16 -> [M][Kp]; `whole`: K is a multiple of four and x lies at a whole four numbers.  The others:
+// scales [rows, blocks] -> [rows, words * 4], zeros behind.
+struct Fp4Copies {
+    const void* x;
+    uint16_t* planes;
+    int M, K, Kp;
+    unsigned x_blocks, per;             // blocks of a row of x
+    const unsigned char* scales;
+    uint32_t* scales_out;
+    unsigned all_words, words;          // of all rows, of a row
+    int blocks;
+    bool whole;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void fp4_planes_kernel(const T* __restrict__ x, uint16_t* __restrict__ planes, int M, int K, int Kp) {
-    const long plane = (long)M * Kp;
-    for (long row = blockIdx.y; row < M; row += gridDim.y) {
-        const int k = (blockIdx.x * 256 + threadIdx.x) * 4;
-        if (k >= Kp) return;
-        uint16_t hi[4], mid[4], lo[4];
+__global__ __launch_bounds__(256) void fp4_copies_kernel(Fp4Copies p) {
+    if (blockIdx.x >= p.x_blocks) {
+        const unsigned at = (blockIdx.x - p.x_blocks) * 256 + threadIdx.x, row = at / p.words;
+        if (at >= p.all_words) return;
+        const int b = (int)(at - row * p.words) * 4;
+        uint32_t v = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const bool have = k + e < K;
-            if constexpr (sizeof(T) == 4) cut_in_three(have ? x[row * K + k + e] : 0.f, hi[e], mid[e], lo[e]);
-            else hi[e] = have ? x[row * K + k + e].bits : 0;
-        }
-        uint16_t* to = planes + row * Kp + k;
-        if constexpr (sizeof(T) == 4) {
-            *(ushort4*)to = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
-            *(ushort4*)(to + plane) = make_ushort4(mid[0], mid[1], mid[2], mid[3]);
-            *(ushort4*)(to + 2 * plane) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-        } else {
-            *(ushort4*)to = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-        }
+        for (int e = 0; e < 4; ++e)
+            if (b + e < p.blocks) v |= (uint32_t)p.scales[(long)row * p.blocks + b + e] << (8 * e);
+        p.scales_out[at] = v;
+        return;
+    }
+    const unsigned row = blockIdx.x / p.per;
+    const int k = (int)((blockIdx.x - row * p.per) * 256 + threadIdx.x) * 4;
+    if (k >= p.Kp) return;
+    const T* x = (const T*)p.x + (long)row * p.K + k;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.whole) {
+        if (k < p.K) Vec4<T>::load(x, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (k + e < p.K) v[e] = Elem<T>::load(x + e);
+    }
+    uint16_t* to = p.planes + (long)row * p.Kp + k;
+    uint16_t hi[4], mid[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) cut_in_three(v[e], hi[e], mid[e], lo[e]);
+        else hi[e] = (uint16_t)(__float_as_uint(v[e]) >> 16);
+    }
+    if constexpr (sizeof(T) == 4) {
+        const long plane = (long)p.M * p.Kp;
+        *(ushort4*)to = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+        *(ushort4*)(to + plane) = make_ushort4(mid[0], mid[1], mid[2], mid[3]);
+        *(ushort4*)(to + 2 * plane) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+    } else {
+        *(ushort4*)to = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
     }
 }
 
-// scales [rows, blocks] -> [rows, words * 4], zeros behind
-__global__ __launch_bounds__(256) void fp4_scales_kernel(const unsigned char* __restrict__ scales, uint32_t* __restrict__ out, int rows,
-                                                         int blocks, unsigned words) {
-    const unsigned at = blockIdx.x * 256 + threadIdx.x, row = at / words;
-    if (row >= (unsigned)rows) return;
-    const int b = (int)(at - row * words) * 4;
-    uint32_t v = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (b + e < blocks) v |= (uint32_t)scales[(long)row * blocks + b + e] << (8 * e);
-    out[at] = v;
-}
+static int padded(int K) { return qe_cdiv(K, FP4_STAGE) * FP4_STAGE; }
 
 bool fp4_scales_whole(int K, const void* scales) { return K % FP4_SPAN == 0 && ((uintptr_t)scales & 15) == 0; }
 
 long fp4_scales_bytes(int rows, int K) { return (long)rows * qe_cdiv(K, FP4_SPAN) * (FP4_SPAN / 32); }
 
-void fp4_pad_scales(const unsigned char* scales, unsigned char* out, int rows, int blocks, int K, hipStream_t stream) {
-    const long words = fp4_scales_bytes(rows, K) / 4;      // (below 2^31 / 16: fp4_tiles_take, fp4_both_take)
-    fp4_scales_kernel<<<qe_cdiv(words, 256), 256, 0, stream>>>(scales, (uint32_t*)out, rows, blocks, (unsigned)(words / rows));
+long fp4_planes_bytes(int M, int K, int x_kind) { return (x_kind == X_F32 ? 6L : 2L) * M * padded(K); }
+
+Fp4Rows fp4_copies(const void* x, int M, int K, int x_kind, void* out, const unsigned char* scales, int rows, void* scales_out, hipStream_t stream) {
+    Fp4Copies p{};
+    p.x = x;
+    p.planes = (uint16_t*)out;
+    p.M = M;
+    p.K = K;
+    p.Kp = padded(K);
+    p.per = qe_cdiv(p.Kp, 1024);
+    p.x_blocks = out ? (unsigned)M * p.per : 0;
+    p.scales = scales;
+    p.scales_out = (uint32_t*)scales_out;
+    p.words = (unsigned)(fp4_scales_bytes(1, K) / 4);
+    p.all_words = scales_out ? (unsigned)rows * p.words : 0;      // (below 2^31 / 16: fp4_tiles_take)
+    p.blocks = qe_cdiv(K, 32);
+    p.whole = K % 4 == 0 && ((uintptr_t)x & (x_kind == X_F32 ? 15 : 7)) == 0;
+    const unsigned grid = p.x_blocks + qe_cdiv(p.all_words, 256);
+    if (x_kind == X_F32) fp4_copies_kernel<float><<<grid, 256, 0, stream>>>(p);
+    else fp4_copies_kernel<bf16_t><<<grid, 256, 0, stream>>>(p);
+    return {out, p.Kp * 2, x_kind == X_F32 ? 3 : 1};
 }
 
 struct Fp4Tiles {
@@ -333,18 +372,6 @@ static int fp4_tiles_launch(Fp4Tiles t, int splits, hipStream_t stream) {
     return 0;
 }
 
-static int padded(int K) { return qe_cdiv(K, FP4_STAGE) * FP4_STAGE; }
-
-long fp4_planes_bytes(int M, int K, int x_kind) { return (x_kind == X_F32 ? 6L : 2L) * M * padded(K); }
-
-Fp4Rows fp4_planes(const void* x, int M, int K, int x_kind, void* out, hipStream_t stream) {
-    const int Kp = padded(K);
-    const dim3 grid(qe_cdiv(Kp, 1024), M < 65535 ? M : 65535);
-    if (x_kind == X_F32) fp4_planes_kernel<float><<<grid, 256, 0, stream>>>((const float*)x, (uint16_t*)out, M, K, Kp);
-    else fp4_planes_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)x, (uint16_t*)out, M, K, Kp);
-    return {out, Kp * 2, x_kind == X_F32 ? 3 : 1};
-}
-
 // The kernel's 32-bit places reach all of the operands.
 bool fp4_tiles_take(int M, int N, int K, int x_kind) {
     return (long)N * padded(K) / 2 < (1L << 31) && (long)M * padded(K) * 2 * (x_kind == X_F32 ? 3 : 1) < (1L << 31);
@@ -413,10 +440,12 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     // the workspace: the cuts' products, then what is made of x, then of the scales
     float* parts = (float*)workspace;
     unsigned char* ws = (unsigned char*)workspace + (s.splits > 1 ? (4L * s.splits * a.M * a.N + 15) / 16 * 16 : 0);
+    const bool copy_x = x_kind == X_F32 || a.K % 8 || ((uintptr_t)a.x & 15), copy_scales = !fp4_scales_whole(a.K, a.scales);
+    unsigned char* const scales_at = ws + (copy_x ? fp4_planes_bytes(a.M, a.K, x_kind) : 0);
     Fp4Rows x{a.x, a.K * 2, 1};
-    if (x_kind == X_F32 || a.K % 8 || ((uintptr_t)a.x & 15)) {
-        x = fp4_planes(a.x, a.M, a.K, x_kind, ws, stream);
-        ws += fp4_planes_bytes(a.M, a.K, x_kind);
+    if (copy_x || copy_scales) {
+        const Fp4Rows copied = fp4_copies(a.x, a.M, a.K, x_kind, copy_x ? ws : nullptr, a.scales, a.N, copy_scales ? scales_at : nullptr, stream);
+        if (copy_x) x = copied;
     }
     t.planes = (const uint16_t*)x.data;
     t.num_planes = x.planes;
@@ -424,12 +453,8 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     t.k_in_row = x.row_bytes / 2;
     t.plane_bytes = t.row_bytes * (unsigned)a.M;
     t.x_bytes = t.plane_bytes * t.num_planes;
-    t.scales = a.scales;
+    t.scales = copy_scales ? scales_at : a.scales;
     t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
-    if (!fp4_scales_whole(a.K, a.scales)) {
-        fp4_pad_scales(a.scales, ws, a.N, a.blocks, a.K, stream);
-        t.scales = ws;
-    }
     if (s.splits > 1) t.a.out = parts;
     int rc;
 #define QE_GO(T_)                                                                            \

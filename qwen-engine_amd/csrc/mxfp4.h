@@ -185,7 +185,6 @@ __device__ __forceinline__ uintx4_t fp4_buffer(const void* p, unsigned bytes) {
 #define FP4_SPAN 512
 bool fp4_scales_whole(int K, const void* scales);
 long fp4_scales_bytes(int rows, int K);
-void fp4_pad_scales(const unsigned char* scales, unsigned char* out, int rows, int blocks, int K, hipStream_t stream);
 
 // partial products [splits][M][N] -> a.out, summed in their order, with the tail
 int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStream_t stream);
@@ -195,9 +194,10 @@ struct Fp4Rows {
     const void* data;
     int row_bytes, planes;
 };
-// gemm_mxfp4_tiles.hip: rows copied so, 32-bit ones in three planes of bfloat16 (low, middle, high), zeros from K to whole stages
+// gemm_mxfp4_tiles.hip: rows copied so (out null: they are not), 32-bit ones in three planes of bfloat16 (low, middle, high), zeros from K to whole
+// stages; and scales of so many rows in whole spans (scales_out null: they are not)
 long fp4_planes_bytes(int M, int K, int x_kind);
-Fp4Rows fp4_planes(const void* x, int M, int K, int x_kind, void* out, hipStream_t stream);
+Fp4Rows fp4_copies(const void* x, int M, int K, int x_kind, void* out, const unsigned char* scales, int rows, void* scales_out, hipStream_t stream);
 
 // gemm_mxfp4_rows.hip: few rows
 bool fp4_few_takes(int M, int N, int K, int x_kind, int tail);
