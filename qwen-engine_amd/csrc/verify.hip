@@ -13,8 +13,10 @@
 // Up to four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials), acceptance (a block a request, a wave a
 // draft), the spans' sums of what the token is drawn from (one row a request, and its draft's), the draw.
 #include "common.h"
+#include <cstdlib>
 
-#define VERIFY_SPAN 4096
+#define VERIFY_SPAN 4096        // what a block looks at; its quarters, a wave each, have sums of their own
+#define VERIFY_PIECE 1024
 
 struct VerifyArgs {
     const float* logits;        // [rows, V]
@@ -26,12 +28,12 @@ struct VerifyArgs {
     const float* draw;          // [R]
     int* tokens;                // [rows]
     int* accepted;              // [R]
-    int rows, V, R, spans;
+    int rows, V, R, spans, pieces;
     int four;                   // the rows lie at whole 16-byte pieces
 };
 
-struct VerifyPart {             // of a span of a row: the largest logit, the lowest column that has it, the sum of exp((z - top) / t)
-    double sum;
+struct VerifyPart {             // of a span of a row: the largest logit, the lowest column that has it, its pieces' sums of exp((z - top) / t)
+    double sums[4];
     float top;
     int at;
 };
@@ -95,24 +97,23 @@ __device__ __forceinline__ bool verify_rows(const VerifyArgs& a, int r, int& lo,
     return lo >= r && hi > lo && hi <= a.rows && hi - 1 - r <= a.rows - a.R;
 }
 
-// The column of number e of a thread's share of a span, THREADS threads to a block: four neighbours, four a round further on, and so on.
-template <int THREADS> __device__ __forceinline__ int verify_column(int e) { return e / 4 * (4 * THREADS) + threadIdx.x * 4 + e % 4; }
-
-// A thread's share of the span from c0 on of a row, as 16-byte pieces or one by one; beyond the row -infinity.
-template <int THREADS>
-__device__ __forceinline__ void verify_load(const float* row, int c0, int V, int four, float (&v)[VERIFY_SPAN / THREADS]) {
-    if (four && c0 + VERIFY_SPAN <= V) {
+// EACH numbers of a row: four neighbours from column c on, four 256 columns on, and so on (one: column c); as 16-byte pieces where `whole` says that
+// all of them are there and at such places, else one by one; beyond the row -infinity.
+template <int EACH> __device__ __forceinline__ int verify_column(int c, int e) { return c + e / 4 * 256 + e % 4; }
+template <int EACH>
+__device__ __forceinline__ void verify_load(const float* row, int c, int V, bool whole, float (&v)[EACH]) {
+    if (EACH % 4 == 0 && whole) {
 #pragma unroll
-        for (int e = 0; e < VERIFY_SPAN / THREADS; e += 4) {
-            const float4 q = *(const float4*)(row + c0 + verify_column<THREADS>(e));
+        for (int e = 0; e < EACH; e += 4) {
+            const float4 q = *(const float4*)(row + verify_column<EACH>(c, e));
             v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < VERIFY_SPAN / THREADS; ++e) {
-            const int c = c0 + verify_column<THREADS>(e);
-            v[e] = row[min(c, V - 1)];
-            if (c >= V) v[e] = -INFINITY;
+        for (int e = 0; e < EACH; ++e) {
+            const int at = verify_column<EACH>(c, e);
+            v[e] = row[min(at, V - 1)];
+            if (at >= V) v[e] = -INFINITY;
         }
     }
 }
@@ -148,18 +149,6 @@ __device__ __forceinline__ double verify_lane(double v, int lane) {
 
 __device__ __forceinline__ double verify_wave_sum(double v) { return verify_lane(verify_wave_scan(v), 63); }
 
-template <int THREADS>
-__device__ __forceinline__ double verify_block_sum(double v, double* shared) {
-    v = verify_wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) v += shared[w];
-    return v;
-}
-
 // The largest of the wave and the lowest column that has it, in every lane.
 __device__ __forceinline__ void verify_wave_top(float& top, int& at) {
     const float mine = top;
@@ -175,12 +164,12 @@ __device__ __forceinline__ void verify_wave_top(float& top, int& at) {
 __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyPart* parts) {
     __shared__ float tops[4];
     __shared__ int ats[4];
-    __shared__ double sums[4];
     const bool is_guess = (int)blockIdx.y >= a.rows;
     const int i = is_guess ? blockIdx.y - a.rows : blockIdx.y;
-    constexpr int EACH = VERIFY_SPAN / 256;
+    constexpr int EACH = VERIFY_PIECE / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.x * VERIFY_SPAN + wave * VERIFY_PIECE;
     float v[EACH];
-    verify_load<256>((is_guess ? a.guess : a.logits) + (long)i * a.V, blockIdx.x * VERIFY_SPAN, a.V, a.four, v);      // (on its way while the request is looked up)
+    verify_load<EACH>((is_guess ? a.guess : a.logits) + (long)i * a.V, c0 + lane * 4, a.V, a.four && c0 + VERIFY_PIECE <= a.V, v);      // (on its way while the request is looked up)
     // the request: the number of first[1 .. R] (less their index, for the drafts) that are not beyond i
     int low = 0, high = a.R;
     while (low < high) {
@@ -192,13 +181,12 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
     const bool greedy = verify_greedy(t);
     if (is_guess && greedy) return;
     const VerifyScale k(t);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float top = -INFINITY;
     int at = 0x7fffffff;
     if (greedy) {
 #pragma unroll
         for (int e = 0; e < EACH; ++e)
-            if (v[e] > top) { top = v[e]; at = blockIdx.x * VERIFY_SPAN + verify_column<256>(e); }      // (no NaN is larger than anything)
+            if (v[e] > top) { top = v[e]; at = verify_column<EACH>(c0 + lane * 4, e); }      // (no NaN is larger than anything)
         verify_wave_top(top, at);
     } else {                                       // (its column is not asked for)
 #pragma unroll
@@ -218,23 +206,27 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
 #pragma unroll
             for (int e = 0; e < EACH; ++e) sum += verify_finite_weight(v[e], top, k);
         }
-        sum = verify_block_sum<256>(sum, sums);
+        sum = verify_wave_sum(sum);
     }
-    if (threadIdx.x == 0) parts[(long)blockIdx.y * a.spans + blockIdx.x] = {sum, top, at};
+    VerifyPart& part = parts[(long)blockIdx.y * a.spans + blockIdx.x];
+    if (lane == 0) part.sums[wave] = sum;
+    if (threadIdx.x == 0) { part.top = top; part.at = at; }
 }
+
+__device__ __forceinline__ double verify_span_sum(const VerifyPart& p) { return (p.sums[0] + p.sums[1]) + (p.sums[2] + p.sums[3]); }
 
 // The whole row's largest logit, its column and sum, from its spans: by one wave, the same in all lanes.
 __device__ __forceinline__ void verify_join(const VerifyPart* parts, int spans, const VerifyScale& k, float& top, int& at, double& sum) {
     const int lane = threadIdx.x & 63;
-    VerifyPart mine = {0.0, -INFINITY, 0x7fffffff};
+    VerifyPart mine = {{0.0, 0.0, 0.0, 0.0}, -INFINITY, 0x7fffffff};
     if (lane < spans) mine = parts[lane];
     top = mine.top;
     at = mine.at;
     for (int s = lane + 64; s < spans; s += 64)
         if (parts[s].top > top) { top = parts[s].top; at = parts[s].at; }
     verify_wave_top(top, at);
-    sum = mine.sum * verify_weight(mine.top, top, k);
-    for (int s = lane + 64; s < spans; s += 64) sum += parts[s].sum * verify_weight(parts[s].top, top, k);
+    sum = verify_span_sum(mine) * verify_weight(mine.top, top, k);
+    for (int s = lane + 64; s < spans; s += 64) sum += verify_span_sum(parts[s]) * verify_weight(parts[s].top, top, k);
     sum = verify_wave_sum(sum);
 }
 
@@ -307,14 +299,13 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
     verify_accept(a, parts, choices, blockIdx.x, true);
 }
 
-// The weights in a draw of a thread's share of the span from c0 on, of the logits in the model's row and in the draft's (rest: with the draft's
-// distribution taken away).  The forms are told apart once, not at every number, so that the polynomials go side by side (1 request 0.9 us less).
-__device__ __forceinline__ void verify_draw_weights(const VerifyChoice& c, const float (&z)[VERIFY_SPAN / 1024], const float (&zq)[VERIFY_SPAN / 1024], int c0,
-                                                    bool rest, double (&w)[VERIFY_SPAN / 1024]) {
-    constexpr int EACH = VERIFY_SPAN / 1024;
+// The weights in a draw of EACH numbers from column c on, of their logits in the model's row and in the draft's (rest: with the draft's
+// distribution taken away).  The forms are told apart once, not at every number, so that the polynomials go side by side.
+template <int EACH>
+__device__ __forceinline__ void verify_draw_weights(const VerifyChoice& c, const float (&z)[EACH], const float (&zq)[EACH], int col, bool rest, double (&w)[EACH]) {
     const bool with_q = rest && c.q_each > 0.0;
     if (c.p_top == INFINITY || (with_q && c.q_top == INFINITY)) {
-#pragma unroll 1
+#pragma unroll
         for (int e = 0; e < EACH; ++e) {
             w[e] = verify_weight(z[e], c.p_top, c.t) * c.p_each;
             if (with_q) w[e] = __builtin_fmax(w[e] - verify_weight(zq[e], c.q_top, c.t) * c.q_each, 0.0);
@@ -329,113 +320,135 @@ __device__ __forceinline__ void verify_draw_weights(const VerifyChoice& c, const
     }
 #pragma unroll
     for (int e = 0; e < EACH; ++e)
-        if (rest && c0 + verify_column<1024>(e) == c.point) w[e] = 0.0;
+        if (rest && verify_column<EACH>(col, e) == c.point) w[e] = 0.0;
 }
 
-// A span's weights without the draft's: summed already.
-__device__ __forceinline__ double verify_plain_sum(const VerifyArgs& a, const VerifyPart* parts, const VerifyChoice& c, int span) {
-    const VerifyPart& p = parts[(long)c.row * a.spans + span];
-    return p.sum * verify_weight(p.top, c.p_top, c.t) * c.p_each;
+// A piece's weights without the draft's: summed already.
+__device__ __forceinline__ double verify_plain_sum(const VerifyArgs& a, const VerifyPart* parts, const VerifyChoice& c, int piece) {
+    const VerifyPart& p = parts[(long)c.row * a.spans + piece / 4];
+    return p.sums[piece % 4] * verify_weight(p.top, c.p_top, c.t) * c.p_each;
 }
 
-// The sum of the weights of a span.  ACCEPT: the block finds the choice for itself.
+// The sums of the weights of pieces, four numbers a thread, 256 threads a piece.  ACCEPT: the block finds the choice for itself, with its 16
+// waves, and has a whole span; else one piece.
 template <bool ACCEPT>
-__global__ __launch_bounds__(1024) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests) {
-    constexpr int EACH = VERIFY_SPAN / 1024;
-    __shared__ double shared[16];
-    const int r = blockIdx.y, span = blockIdx.x;
+__global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests) {
+    constexpr int EACH = VERIFY_PIECE / 256, HERE = ACCEPT ? 4 : 1;
+    __shared__ double shared[4 * HERE];
+    const int r = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), piece = blockIdx.x * HERE + wave / 4;
     VerifyChoice c;
-    if constexpr (ACCEPT) c = verify_accept(a, parts, choices, r, span == 0);
+    if constexpr (ACCEPT) c = verify_accept(a, parts, choices, r, blockIdx.x == 0);
     else c = choices[r];
     if (c.row < 0) return;
-    double sum = 0.0;
-    if (c.q_each == 0.0 && (c.point < 0 || c.point / VERIFY_SPAN != span)) {
-        if (threadIdx.x != 0) return;
-        sum = verify_plain_sum(a, parts, c, span);
-    } else {
+    const bool plain = c.q_each == 0.0 && (c.point < 0 || c.point / VERIFY_PIECE != piece);
+    if (!plain && piece < a.pieces) {
+        const int c0 = piece * VERIFY_PIECE, col = c0 + threadIdx.x % 256 * EACH;
+        const bool whole = a.four && c0 + VERIFY_PIECE <= a.V;
         float v[EACH], q[EACH];
-        verify_load<1024>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
+        verify_load<EACH>(a.logits + (long)c.row * a.V, col, a.V, whole, v);
 #pragma unroll
         for (int e = 0; e < EACH; ++e) q[e] = 0.f;
-        if (c.q_each > 0.0) verify_load<1024>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
-        double each[EACH];
-        verify_draw_weights(c, v, q, span * VERIFY_SPAN, true, each);
+        if (c.q_each > 0.0) verify_load<EACH>(a.guess + (long)c.guess_row * a.V, col, a.V, whole, q);
+        double each[EACH], sum = 0.0;
+        verify_draw_weights<EACH>(c, v, q, col, true, each);
 #pragma unroll
         for (int e = 0; e < EACH; ++e) sum += each[e];
-        sum = verify_block_sum<1024>(sum, shared);
+        sum = verify_wave_sum(sum);
+        if (threadIdx.x % 64 == 0) shared[wave] = sum;
     }
-    if (threadIdx.x == 0) rests[(long)r * a.spans + span] = sum;
+    __syncthreads();
+    if (threadIdx.x % 256 == 0 && piece < a.pieces)
+        rests[(long)r * a.pieces + piece] = plain ? verify_plain_sum(a, parts, c, piece) : (shared[wave] + shared[wave + 1]) + (shared[wave + 2] + shared[wave + 3]);
 }
 
-// The draw: a block a request.  Its span is the first whose sum reaches beyond the random number's share of the whole (every wave finds
-// it for itself, 64 spans at a time), then its token the first of the span: sums of four neighbours a thread, then a walk through
-// those.  Where a rounding lets a span's own sum fall short of the share, or the number is 1 or more, the token is the last one that
-// weighs anything.
-__global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
-    constexpr int EACH = VERIFY_SPAN / 1024;
-    __shared__ double shared[16];
-    __shared__ int founds[16], lasts[16];
+// The draw: a block a request.  Its piece is the first whose sum reaches beyond the random number's share of the whole (every wave finds
+// it for itself, 64 pieces at a time, the first 256 side by side), then its token the first of the piece, four numbers a thread (with 1024
+// threads four waves of a SIMD would do the search one after the other).  Where a rounding lets a piece's own sum fall short of the
+// share, or the number is 1 or more, the token is the last one that weighs anything.
+__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
+    constexpr int EACH = VERIFY_PIECE / 256;
+    __shared__ double shared[4];
+    __shared__ int founds[4], lasts[4];
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const double* rests = rests_all + (long)r * a.spans;
-    double v0 = lane < a.spans ? rests[lane] : 0.0;        // (nothing of them is used where nothing is drawn)
+    const double* rests = rests_all + (long)r * a.pieces;
+    double v0[4], scan0[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v0[i] = i * 64 + lane < a.pieces ? rests[i * 64 + lane] : 0.0;        // (nothing of them is used where nothing is drawn)
     const VerifyChoice c = choices[r];
     const float u = a.draw[r];
     // (all of the choice at once, with the sums, not part by part as it is wanted)
-    asm volatile("" : : "s"(c.row), "s"(c.guess_row), "s"(c.point), "s"(c.p_top), "s"(c.q_top), "s"(c.p_each), "s"(c.q_each), "s"(c.t.k), "s"(c.t.least), "s"(u), "v"(v0));
+    asm volatile("" : : "s"(c.row), "s"(c.guess_row), "s"(c.point), "s"(c.p_top), "s"(c.q_top), "s"(c.p_each), "s"(c.q_each), "s"(c.t.k), "s"(c.t.least), "s"(u), "v"(v0[0]));
     if (c.row < 0) return;
-    double scan0 = verify_wave_scan(v0), total = verify_lane(scan0, 63);
-    for (int s0 = 64; s0 < a.spans; s0 += 64) total += verify_wave_sum(s0 + lane < a.spans ? rests[s0 + lane] : 0.0);
+    double total = 0.0;
+    auto scan_all = [&](auto&& piece_sum) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            scan0[i] = verify_wave_scan(v0[i]);
+            total += verify_lane(scan0[i], 63);
+        }
+        for (int s0 = 256; s0 < a.pieces; s0 += 64) total += verify_wave_sum(piece_sum(s0 + lane));
+    };
+    auto rest_sum = [&](int s) { return s < a.pieces ? rests[s] : 0.0; };
+    auto plain_sum = [&](int s) { return s < a.pieces ? verify_plain_sum(a, parts, c, s) : 0.0; };
+    scan_all(rest_sum);
     // (nothing left: the draft's distribution is the model's, and only a rounding or a number beyond 1 refused the draft: p alone)
     const bool rest = total > 0.0;
-    auto span_sum = [&](int s) { return s >= a.spans ? 0.0 : rest ? rests[s] : verify_plain_sum(a, parts, c, s); };
     if (!rest) {
-        v0 = span_sum(lane);
-        scan0 = verify_wave_scan(v0);
         total = 0.0;
-        for (int s0 = 0; s0 < a.spans; s0 += 64) total += verify_wave_sum(span_sum(s0 + lane));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v0[i] = plain_sum(i * 64 + lane);
+        scan_all(plain_sum);
     }
     const double target = u > 0.f ? (double)u * total : 0.0;       // (NaN: 0)
-    int span = -1;
+    int piece = -1;
+    bool reached = false;
     double before = 0.0, run = 0.0;
-    for (int s0 = 0; s0 < a.spans; s0 += 64) {
-        const double v = s0 == 0 ? v0 : span_sum(s0 + lane), scan = s0 == 0 ? scan0 : verify_wave_scan(v);
+    auto look = [&](double v, double scan, int s0) {
         const unsigned long some = __ballot(v > 0.0), over = __ballot(v > 0.0 && run + scan > target);
         if (some) {
             const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
-            span = s0 + at;
+            piece = s0 + at;
             before = run + verify_lane(scan, at) - verify_lane(v, at);
         }
-        if (over) break;
         run += verify_lane(scan, 63);
+        reached = over != 0;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (!reached) look(v0[i], scan0[i], i * 64);
+    for (int s0 = 256; !reached && s0 < a.pieces; s0 += 64) {
+        const double v = rest ? rest_sum(s0 + lane) : plain_sum(s0 + lane);
+        look(v, verify_wave_scan(v), s0);
     }
-    if (span < 0) return;                      // (no weight anywhere)
-    const int c0 = span * VERIFY_SPAN + tid * EACH;        // (a thread's share is four neighbours)
-    double each[EACH], sum = 0.0;
+    if (piece < 0) return;                     // (no weight anywhere)
+    const int c0 = piece * VERIFY_PIECE, col = c0 + tid * EACH;
+    const bool whole = a.four && c0 + VERIFY_PIECE <= a.V;
     float v[EACH], q[EACH];
-    verify_load<1024>(a.logits + (long)c.row * a.V, span * VERIFY_SPAN, a.V, a.four, v);
+    verify_load<EACH>(a.logits + (long)c.row * a.V, col, a.V, whole, v);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) q[e] = 0.f;
-    if (rest && c.q_each > 0.0) verify_load<1024>(a.guess + (long)c.guess_row * a.V, span * VERIFY_SPAN, a.V, a.four, q);
+    if (rest && c.q_each > 0.0) verify_load<EACH>(a.guess + (long)c.guess_row * a.V, col, a.V, whole, q);
+    double each[EACH], sum = 0.0;
+    verify_draw_weights<EACH>(c, v, q, col, rest, each);
     int last = -1;
-    verify_draw_weights(c, v, q, span * VERIFY_SPAN, rest, each);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         sum += each[e];
-        if (each[e] > 0.0) last = c0 + e;
+        if (each[e] > 0.0) last = col + e;
     }
     const double scan = verify_wave_scan(sum);
     if (lane == 63) shared[wave] = scan;
     __syncthreads();
     run = before;
 #pragma unroll
-    for (int w = 0; w < 16; ++w)
+    for (int w = 0; w < 4; ++w)
         if (w < wave) run += shared[w];
     run += scan - sum;
     int found = -1;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         run += each[e];
-        if (found < 0 && each[e] > 0.0 && run > target) found = c0 + e;
+        if (found < 0 && each[e] > 0.0 && run > target) found = col + e;
     }
     // the wave's first that reaches beyond, and its last that weighs anything, then the block's (columns rise with the threads)
     const unsigned long over = __ballot(found >= 0), some = __ballot(last >= 0);
@@ -445,7 +458,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
     __syncthreads();
     if (tid != 0) return;
     int token = -1;
-    for (int w = 0; w < 16; ++w) {
+    for (int w = 0; w < 4; ++w) {
         if (founds[w] >= 0) { token = founds[w]; break; }
         if (lasts[w] >= 0) token = lasts[w];
     }
@@ -454,7 +467,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs a, const V
 
 extern "C" long qe_verify_drafts_workspace_bytes(int rows, int V, int R, int has_guess) {
     const long spans = qe_cdiv(V, VERIFY_SPAN), all = rows + (has_guess ? rows - R : 0);
-    return all * spans * (long)sizeof(VerifyPart) + (long)R * (long)sizeof(VerifyChoice) + (long)R * spans * 8;
+    return all * spans * (long)sizeof(VerifyPart) + (long)R * (long)sizeof(VerifyChoice) + (long)R * qe_cdiv(V, VERIFY_PIECE) * 8;
 }
 
 // logits float32 [rows, V], first int32 [R + 1], drafts int32 [rows - R], guess float32 [rows - R, V] or null, temperature and draw float32 [R],
@@ -465,7 +478,7 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
                                 void* workspace, long workspace_bytes, hipStream_t stream) {
     QE_REQUIRE(R >= 0 && V > 0 && V < (1 << 30) && rows >= R, "verify_drafts: bad sizes rows=%d V=%d R=%d", rows, V, R);
     if (R == 0) return 0;
-    const int spans = qe_cdiv(V, VERIFY_SPAN), all = rows + (guess ? rows - R : 0);
+    const int spans = qe_cdiv(V, VERIFY_SPAN), pieces = qe_cdiv(V, VERIFY_PIECE), all = rows + (guess ? rows - R : 0);
     QE_REQUIRE(all <= 65535, "verify_drafts: %d rows of logits are too many", all);
     QE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= qe_verify_drafts_workspace_bytes(rows, V, R, guess != nullptr),
                "verify_drafts: workspace too small");
@@ -473,17 +486,18 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     VerifyChoice* choices = (VerifyChoice*)(parts + (long)all * spans);
     double* rests = (double*)(choices + R);
     const int four = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)guess) & 15) == 0;
-    const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, four};
+    const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, pieces, four};
     verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts);
     // Few spans: every block accepts for itself, which saves a launch (spans of 1 request of 151936 15.1 us, in two launches 16.4; of 8, 304
     // spans, 27.2 and 28.1; of 16 40.4 and 36.3).
-    if ((long)spans * R <= 320) {
+    const char* e_ = getenv("QE_V");
+    if (e_ ? atoi(e_) : (long)spans * R <= 320) {
         verify_rest_kernel<true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
     } else {
         verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
-        verify_rest_kernel<false><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
+        verify_rest_kernel<false><<<dim3(pieces, R), 256, 0, stream>>>(a, parts, choices, rests);
     }
-    verify_draw_kernel<<<R, 1024, 0, stream>>>(a, parts, choices, rests);
+    verify_draw_kernel<<<R, 256, 0, stream>>>(a, parts, choices, rests);
     QE_LAUNCH_CHECK();
     return 0;
 }
