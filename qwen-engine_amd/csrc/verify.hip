@@ -13,7 +13,6 @@
 // Up to four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials), acceptance (a block a request, a wave a
 // draft), the spans' sums of what the token is drawn from (one row a request, and its draft's), the draw.
 #include "common.h"
-#include <cstdlib>
 
 #define VERIFY_SPAN 4096        // what a block looks at; its quarters, a wave each, have sums of their own
 #define VERIFY_PIECE 1024
@@ -215,11 +214,17 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
 
 __device__ __forceinline__ double verify_span_sum(const VerifyPart& p) { return (p.sums[0] + p.sums[1]) + (p.sums[2] + p.sums[3]); }
 
-// The whole row's largest logit, its column and sum, from its spans: by one wave, the same in all lanes.
-__device__ __forceinline__ void verify_join(const VerifyPart* parts, int spans, const VerifyScale& k, float& top, int& at, double& sum) {
+// The lane's span of a row's first 64.
+__device__ __forceinline__ VerifyPart verify_mine(const VerifyPart* parts, int spans) {
     const int lane = threadIdx.x & 63;
     VerifyPart mine = {{0.0, 0.0, 0.0, 0.0}, -INFINITY, 0x7fffffff};
     if (lane < spans) mine = parts[lane];
+    return mine;
+}
+
+// The whole row's largest logit, its column and sum, from its spans: by one wave, the same in all lanes.
+__device__ __forceinline__ void verify_join(const VerifyPart* parts, const VerifyPart& mine, int spans, const VerifyScale& k, float& top, int& at, double& sum) {
+    const int lane = threadIdx.x & 63;
     top = mine.top;
     at = mine.at;
     for (int s = lane + 64; s < spans; s += 64)
@@ -230,17 +235,16 @@ __device__ __forceinline__ void verify_join(const VerifyPart* parts, int spans, 
     sum = verify_wave_sum(sum);
 }
 
-// Which drafts of request r are accepted, and what its token is drawn from: by a block of 16 waves, a wave a draft, 16 at a time.  One of the
-// blocks that ask writes it down.
-__device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const VerifyPart* parts, VerifyChoice* choices, int r, bool write) {
+// Which drafts of request r are accepted, and what its token is drawn from: by a block of 16 waves, a wave a draft, 16 at a time.  accepted: how
+// many (-1: there are no such rows); token: the one behind them, of a request without temperature.
+__device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const VerifyPart* parts, int r, int& accepted, int& token) {
     __shared__ VerifyChoice tries[16];
     __shared__ int tokens[16], stops[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo, hi;
     if (!verify_rows(a, r, lo, hi)) {
         VerifyChoice none{};
-        none.row = -1;
-        if (write && threadIdx.x == 0) { a.accepted[r] = -1; choices[r] = none; }
+        none.row = accepted = token = -1;
         return none;
     }
     const float t = a.temperature[r];
@@ -251,7 +255,10 @@ __device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const
     for (;; j0 += 16) {
         const int j = j0 + wave;
         if (j <= n) {
+            const bool guessed = !greedy && j < n && a.guess;
             const int d = lo - r + j, x = j < n ? a.drafts[d] : -1;
+            const VerifyPart *parts_p = parts + (long)(lo + j) * a.spans, *parts_q = parts + (long)(a.rows + d) * a.spans;
+            const VerifyPart mine_p = verify_mine(parts_p, a.spans), mine_q = verify_mine(parts_q, guessed ? a.spans : 0);
             const bool inside = x >= 0 && x < a.V;
             const float zp = inside ? a.logits[(long)(lo + j) * a.V + x] : -INFINITY;
             const float zq = inside && a.guess ? a.guess[(long)d * a.V + x] : -INFINITY;
@@ -259,9 +266,9 @@ __device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const
             VerifyChoice c{};
             int at, unused;
             double p_sum, q_sum = 0.0;
-            verify_join(parts + (long)(lo + j) * a.spans, a.spans, k, c.p_top, at, p_sum);
-            if (!greedy && j < n && a.guess) verify_join(parts + (long)(a.rows + d) * a.spans, a.spans, k, c.q_top, unused, q_sum);
-            const int token = c.p_top > -INFINITY ? at : -1;
+            verify_join(parts_p, mine_p, a.spans, k, c.p_top, at, p_sum);
+            if (guessed) verify_join(parts_q, mine_q, a.spans, k, c.q_top, unused, q_sum);
+            const int largest = c.p_top > -INFINITY ? at : -1;
             c.t = k;
             c.row = greedy || !(p_sum > 0.0) ? -1 : lo + j;      // (no draw: the token is there, or there is none)
             c.p_each = p_sum > 0.0 ? 1.0 / p_sum : 0.0;
@@ -269,12 +276,12 @@ __device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const
             c.guess_row = d;
             c.point = j < n && !a.guess ? x : -1;
             bool take = false;
-            if (j < n && greedy) take = token >= 0 && x == token;
+            if (j < n && greedy) take = largest >= 0 && x == largest;
             else if (j < n) {
                 const double p = verify_weight(zp, c.p_top, k) * c.p_each, q = a.guess ? verify_weight(zq, c.q_top, k) * c.q_each : 1.0;
                 take = p > 0.0 && (double)u * q < p;
             }
-            if (lane == 0) { tries[wave] = c; tokens[wave] = token; stops[wave] = !take; }
+            if (lane == 0) { tries[wave] = c; tokens[wave] = largest; stops[wave] = !take; }
         } else if (lane == 0) {
             stops[wave] = 0;
         }
@@ -284,19 +291,27 @@ __device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const
         if (stop >= 0) break;                      // (row n is no draft: it stops)
         __syncthreads();
     }
-    if (write) {
-        const int accepted = j0 + stop;
-        for (int i = threadIdx.x; i <= n; i += 1024) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? tokens[stop] : -1;
-        if (threadIdx.x == 0) {
-            a.accepted[r] = accepted;
-            choices[r] = tries[stop];
-        }
-    }
+    accepted = j0 + stop;
+    token = tokens[stop];
     return tries[stop];
 }
 
+// Writes it down: of a request whose rows are there its tokens, -1 where the draw will put one and behind it.
+__device__ __forceinline__ void verify_write(const VerifyArgs& a, VerifyChoice* choices, int r, const VerifyChoice& c, int accepted, int token) {
+    if (threadIdx.x == 0) {
+        a.accepted[r] = accepted;
+        choices[r] = c;
+    }
+    if (accepted < 0) return;
+    const int lo = a.first[r], n = a.first[r + 1] - lo - 1;
+    const bool greedy = verify_greedy(a.temperature[r]);
+    for (int i = threadIdx.x; i <= n; i += 1024) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? token : -1;
+}
+
 __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices) {
-    verify_accept(a, parts, choices, blockIdx.x, true);
+    int accepted, token;
+    const VerifyChoice c = verify_accept(a, parts, blockIdx.x, accepted, token);
+    verify_write(a, choices, blockIdx.x, c, accepted, token);
 }
 
 // The weights in a draw of EACH numbers from column c on, of their logits in the model's row and in the draft's (rest: with the draft's
@@ -337,9 +352,13 @@ __global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(Verify
     __shared__ double shared[4 * HERE];
     const int r = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), piece = blockIdx.x * HERE + wave / 4;
     VerifyChoice c;
-    if constexpr (ACCEPT) c = verify_accept(a, parts, choices, r, blockIdx.x == 0);
+    int accepted = -1, token = -1;
+    if constexpr (ACCEPT) c = verify_accept(a, parts, r, accepted, token);
     else c = choices[r];
-    if (c.row < 0) return;
+    if (c.row < 0) {
+        if (ACCEPT && blockIdx.x == 0) verify_write(a, choices, r, c, accepted, token);
+        return;
+    }
     const bool plain = c.q_each == 0.0 && (c.point < 0 || c.point / VERIFY_PIECE != piece);
     if (!plain && piece < a.pieces) {
         const int c0 = piece * VERIFY_PIECE, col = c0 + threadIdx.x % 256 * EACH;
@@ -359,6 +378,7 @@ __global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(Verify
     __syncthreads();
     if (threadIdx.x % 256 == 0 && piece < a.pieces)
         rests[(long)r * a.pieces + piece] = plain ? verify_plain_sum(a, parts, c, piece) : (shared[wave] + shared[wave + 1]) + (shared[wave + 2] + shared[wave + 3]);
+    if (ACCEPT && blockIdx.x == 0) verify_write(a, choices, r, c, accepted, token);      // (last: the others have nothing to wait for then)
 }
 
 // The draw: a block a request.  Its piece is the first whose sum reaches beyond the random number's share of the whole (every wave finds
@@ -490,8 +510,7 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts);
     // Few spans: every block accepts for itself, which saves a launch (spans of 1 request of 151936 15.1 us, in two launches 16.4; of 8, 304
     // spans, 27.2 and 28.1; of 16 40.4 and 36.3).
-    const char* e_ = getenv("QE_V");
-    if (e_ ? atoi(e_) : (long)spans * R <= 320) {
+    if ((long)spans * R <= 320) {
         verify_rest_kernel<true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
     } else {
         verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
