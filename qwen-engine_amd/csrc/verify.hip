@@ -10,8 +10,9 @@
 // All weights and sums are 64-bit: a vocabulary of 150 000 has so many borders of running sums that 32-bit ones put the random number on
 // the other side of one in a few per cent of the draws.
 //
-// Up to four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials), acceptance (a block a request, a wave a
-// draft), the spans' sums of what the token is drawn from (one row a request, and its draft's), the draw.
+// Four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials: of 64 requests, 425 MB, 95 us), acceptance (a block a
+// request, a wave a draft, 7 us), the sums of pieces of 1024 of what the token is drawn from (one row a request, and its draft's, 15 us), the
+// draw (5 us); the last three in one where there are few spans.
 #include "common.h"
 
 #define VERIFY_SPAN 4096        // what a block looks at; its quarters, a wave each, have sums of their own
@@ -160,7 +161,7 @@ __device__ __forceinline__ void verify_wave_top(float& top, int& at) {
 }
 
 // One block a span of a row: blockIdx.y counts the rows of the logits, then those of the drafts' logits.
-__global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyPart* parts) {
+__global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyPart* parts, unsigned* done) {
     __shared__ float tops[4];
     __shared__ int ats[4];
     const bool is_guess = (int)blockIdx.y >= a.rows;
@@ -169,13 +170,18 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.x * VERIFY_SPAN + wave * VERIFY_PIECE;
     float v[EACH];
     verify_load<EACH>((is_guess ? a.guess : a.logits) + (long)i * a.V, c0 + lane * 4, a.V, a.four && c0 + VERIFY_PIECE <= a.V, v);      // (on its way while the request is looked up)
+    // (after the loads of what the host gives: behind a store they would not be scalar ones, 10 us for 64 requests)
+    auto clear = [&] {
+        if (blockIdx.x == 0 && blockIdx.y == 0)
+            for (int r = threadIdx.x; r < a.R; r += 256) done[r] = 0;
+    };
     // the request: the number of first[1 .. R] (less their index, for the drafts) that are not beyond i
     int low = 0, high = a.R;
     while (low < high) {
         const int mid = (low + high) / 2;
         if (a.first[mid + 1] - (is_guess ? mid + 1 : 0) <= i) low = mid + 1; else high = mid;
     }
-    if (low >= a.R) return;
+    if (low >= a.R) return clear();
     const float t = a.temperature[low];
     const bool greedy = verify_greedy(t);
     if (is_guess && greedy) return;
@@ -210,6 +216,7 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
     VerifyPart& part = parts[(long)blockIdx.y * a.spans + blockIdx.x];
     if (lane == 0) part.sums[wave] = sum;
     if (threadIdx.x == 0) { part.top = top; part.at = at; }
+    clear();
 }
 
 __device__ __forceinline__ double verify_span_sum(const VerifyPart& p) { return (p.sums[0] + p.sums[1]) + (p.sums[2] + p.sums[3]); }
@@ -296,7 +303,7 @@ __device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const
     return tries[stop];
 }
 
-// Writes it down: of a request whose rows are there its tokens, -1 where the draw will put one and behind it.
+// Writes it down: of a request whose rows are there its tokens, -1 behind them; the drawn one is left to the draw.
 __device__ __forceinline__ void verify_write(const VerifyArgs& a, VerifyChoice* choices, int r, const VerifyChoice& c, int accepted, int token) {
     if (threadIdx.x == 0) {
         a.accepted[r] = accepted;
@@ -305,7 +312,8 @@ __device__ __forceinline__ void verify_write(const VerifyArgs& a, VerifyChoice* 
     if (accepted < 0) return;
     const int lo = a.first[r], n = a.first[r + 1] - lo - 1;
     const bool greedy = verify_greedy(a.temperature[r]);
-    for (int i = threadIdx.x; i <= n; i += 1024) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? token : -1;
+    for (int i = threadIdx.x; i <= n; i += 1024)
+        if (lo + i != c.row) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? token : -1;
 }
 
 __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices) {
@@ -344,12 +352,147 @@ __device__ __forceinline__ double verify_plain_sum(const VerifyArgs& a, const Ve
     return p.sums[piece % 4] * verify_weight(p.top, c.p_top, c.t) * c.p_each;
 }
 
+// The draw, by the first four waves of a block.  Its piece is the first whose sum reaches beyond the random number's share of the whole (every
+// wave finds it for itself, 64 pieces at a time, the first 256 side by side), then its token the first of the piece, four numbers a
+// thread (with 16 waves four of a SIMD would do the search one after the other).  Where a rounding lets a piece's own sum fall short of
+// the share, or the number is 1 or more, the token is the last one that weighs anything.
+// The sums of the pieces go past the caches that a part of the units has for itself: other units read them in the same launch.
+__device__ __forceinline__ void verify_put(double* rests, int piece, double v) {
+    __hip_atomic_store((unsigned long*)rests + piece, __builtin_bit_cast(unsigned long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double verify_get(const double* rests, int piece) {
+    return __builtin_bit_cast(double, __hip_atomic_load((const unsigned long*)rests + piece, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+struct VerifyFirst {                // the lane's sums of the first 256 pieces
+    double v[4];
+};
+__device__ __forceinline__ VerifyFirst verify_first(const double* rests, int pieces) {
+    VerifyFirst f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = i * 64 + (threadIdx.x & 63);
+        f.v[i] = s < pieces ? verify_get(rests, s) : 0.0;
+    }
+    return f;
+}
+
+__device__ __forceinline__ void verify_draw(const VerifyArgs& a, const VerifyPart* parts, const VerifyChoice& c, const double* rests, VerifyFirst first, float u) {
+    constexpr int EACH = VERIFY_PIECE / 256;
+    __shared__ double shared[4];
+    __shared__ int founds[4], lasts[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int piece = -1;
+    double target = 0.0, run = 0.0, scan = 0.0, sum = 0.0, each[EACH];
+    if (wave < 4) {
+        double total = 0.0, scans[4];
+        auto scan_all = [&](auto&& piece_sum) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                scans[i] = verify_wave_scan(first.v[i]);
+                total += verify_lane(scans[i], 63);
+            }
+            for (int s0 = 256; s0 < a.pieces; s0 += 64) total += verify_wave_sum(piece_sum(s0 + lane));
+        };
+        auto rest_sum = [&](int s) { return s < a.pieces ? verify_get(rests, s) : 0.0; };
+        auto plain_sum = [&](int s) { return s < a.pieces ? verify_plain_sum(a, parts, c, s) : 0.0; };
+        scan_all(rest_sum);
+        // (nothing left: the draft's distribution is the model's, and only a rounding or a number beyond 1 refused the draft: p alone)
+        const bool rest = total > 0.0;
+        if (!rest) {
+            total = 0.0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) first.v[i] = plain_sum(i * 64 + lane);
+            scan_all(plain_sum);
+        }
+        target = u > 0.f ? (double)u * total : 0.0;            // (NaN: 0)
+        bool reached = false;
+        double before = 0.0;
+        auto look = [&](double v, double scan_v, int s0) {
+            const unsigned long some = __ballot(v > 0.0), over = __ballot(v > 0.0 && run + scan_v > target);
+            if (some) {
+                const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+                piece = s0 + at;
+                before = run + verify_lane(scan_v, at) - verify_lane(v, at);
+            }
+            run += verify_lane(scan_v, 63);
+            reached = over != 0;
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (!reached) look(first.v[i], scans[i], i * 64);
+        for (int s0 = 256; !reached && s0 < a.pieces; s0 += 64) {
+            const double v = rest ? rest_sum(s0 + lane) : plain_sum(s0 + lane);
+            look(v, verify_wave_scan(v), s0);
+        }
+        run = before;
+        if (piece >= 0) {
+            const int c0 = piece * VERIFY_PIECE, col = c0 + tid * EACH;
+            const bool whole = a.four && c0 + VERIFY_PIECE <= a.V;
+            float v[EACH], q[EACH];
+            verify_load<EACH>(a.logits + (long)c.row * a.V, col, a.V, whole, v);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) q[e] = 0.f;
+            if (rest && c.q_each > 0.0) verify_load<EACH>(a.guess + (long)c.guess_row * a.V, col, a.V, whole, q);
+            verify_draw_weights<EACH>(c, v, q, col, rest, each);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) sum += each[e];
+            scan = verify_wave_scan(sum);
+            if (lane == 63) shared[wave] = scan;
+        }
+    }
+    __syncthreads();
+    if (wave < 4) {
+        int found = -1, last = -1;
+        if (piece >= 0) {
+            const int col = piece * VERIFY_PIECE + tid * EACH;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                if (w < wave) run += shared[w];
+            run += scan - sum;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                run += each[e];
+                if (each[e] > 0.0) {
+                    last = col + e;
+                    if (found < 0 && run > target) found = col + e;
+                }
+            }
+        }
+        // the wave's first that reaches beyond, and its last that weighs anything, then the block's (columns rise with the threads)
+        const unsigned long over = __ballot(found >= 0), some = __ballot(last >= 0);
+        if (over) found = __builtin_amdgcn_readlane(found, __ffsll((unsigned long long)over) - 1);
+        if (some) last = __builtin_amdgcn_readlane(last, 63 - __clzll((long long)some));
+        if (lane == 0) { founds[wave] = over ? found : -1; lasts[wave] = some ? last : -1; }
+    }
+    __syncthreads();
+    if (tid != 0) return;
+    int token = -1;                            // (no weight anywhere: none)
+    for (int w = 0; w < 4; ++w) {
+        if (founds[w] >= 0) { token = founds[w]; break; }
+        if (lasts[w] >= 0) token = lasts[w];
+    }
+    a.tokens[c.row] = token;
+}
+
+__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
+    const int r = blockIdx.x;
+    const double* rests = rests_all + (long)r * a.pieces;
+    const VerifyFirst first = verify_first(rests, a.pieces);        // (nothing of them is used where nothing is drawn)
+    const VerifyChoice c = choices[r];
+    const float u = a.draw[r];
+    // (all of the choice at once, with the sums, not part by part as it is wanted)
+    asm volatile("" : : "s"(c.row), "s"(c.guess_row), "s"(c.point), "s"(c.p_top), "s"(c.q_top), "s"(c.p_each), "s"(c.q_each), "s"(c.t.k), "s"(c.t.least), "s"(u), "v"(first.v[0]));
+    if (c.row >= 0) verify_draw(a, parts, c, rests, first, u);
+}
+
 // The sums of the weights of pieces, four numbers a thread, 256 threads a piece.  ACCEPT: the block finds the choice for itself, with its 16
-// waves, and has a whole span; else one piece.
+// waves, and has a whole span; the request's last block to be done (`done` counts them; it waits for nothing) draws.  Else one piece.
 template <bool ACCEPT>
-__global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests) {
+__global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests, unsigned* done) {
     constexpr int EACH = VERIFY_PIECE / 256, HERE = ACCEPT ? 4 : 1;
     __shared__ double shared[4 * HERE];
+    __shared__ bool is_last;
     const int r = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), piece = blockIdx.x * HERE + wave / 4;
     VerifyChoice c;
     int accepted = -1, token = -1;
@@ -377,117 +520,23 @@ __global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(Verify
     }
     __syncthreads();
     if (threadIdx.x % 256 == 0 && piece < a.pieces)
-        rests[(long)r * a.pieces + piece] = plain ? verify_plain_sum(a, parts, c, piece) : (shared[wave] + shared[wave + 1]) + (shared[wave + 2] + shared[wave + 3]);
-    if (ACCEPT && blockIdx.x == 0) verify_write(a, choices, r, c, accepted, token);      // (last: the others have nothing to wait for then)
-}
-
-// The draw: a block a request.  Its piece is the first whose sum reaches beyond the random number's share of the whole (every wave finds
-// it for itself, 64 pieces at a time, the first 256 side by side), then its token the first of the piece, four numbers a thread (with 1024
-// threads four waves of a SIMD would do the search one after the other).  Where a rounding lets a piece's own sum fall short of the
-// share, or the number is 1 or more, the token is the last one that weighs anything.
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a, const VerifyPart* parts, const VerifyChoice* choices, const double* rests_all) {
-    constexpr int EACH = VERIFY_PIECE / 256;
-    __shared__ double shared[4];
-    __shared__ int founds[4], lasts[4];
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const double* rests = rests_all + (long)r * a.pieces;
-    double v0[4], scan0[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v0[i] = i * 64 + lane < a.pieces ? rests[i * 64 + lane] : 0.0;        // (nothing of them is used where nothing is drawn)
-    const VerifyChoice c = choices[r];
-    const float u = a.draw[r];
-    // (all of the choice at once, with the sums, not part by part as it is wanted)
-    asm volatile("" : : "s"(c.row), "s"(c.guess_row), "s"(c.point), "s"(c.p_top), "s"(c.q_top), "s"(c.p_each), "s"(c.q_each), "s"(c.t.k), "s"(c.t.least), "s"(u), "v"(v0[0]));
-    if (c.row < 0) return;
-    double total = 0.0;
-    auto scan_all = [&](auto&& piece_sum) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            scan0[i] = verify_wave_scan(v0[i]);
-            total += verify_lane(scan0[i], 63);
-        }
-        for (int s0 = 256; s0 < a.pieces; s0 += 64) total += verify_wave_sum(piece_sum(s0 + lane));
-    };
-    auto rest_sum = [&](int s) { return s < a.pieces ? rests[s] : 0.0; };
-    auto plain_sum = [&](int s) { return s < a.pieces ? verify_plain_sum(a, parts, c, s) : 0.0; };
-    scan_all(rest_sum);
-    // (nothing left: the draft's distribution is the model's, and only a rounding or a number beyond 1 refused the draft: p alone)
-    const bool rest = total > 0.0;
-    if (!rest) {
-        total = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v0[i] = plain_sum(i * 64 + lane);
-        scan_all(plain_sum);
+        verify_put(rests + (long)r * a.pieces, piece, plain ? verify_plain_sum(a, parts, c, piece) : (shared[wave] + shared[wave + 1]) + (shared[wave + 2] + shared[wave + 3]));
+    if constexpr (ACCEPT) {
+        // The block's sums have arrived before it is counted, and the others' are read after all blocks have been: the stores and loads go past
+        // the caches themselves, so that no fence has to write those back (with fences 25 us instead of 13.6).
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) is_last = __hip_atomic_fetch_add(done + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        if (blockIdx.x == 0) verify_write(a, choices, r, c, accepted, token);
+        __syncthreads();
+        if (!is_last) return;
+        verify_draw(a, parts, c, rests + (long)r * a.pieces, verify_first(rests + (long)r * a.pieces, a.pieces), a.draw[r]);
     }
-    const double target = u > 0.f ? (double)u * total : 0.0;       // (NaN: 0)
-    int piece = -1;
-    bool reached = false;
-    double before = 0.0, run = 0.0;
-    auto look = [&](double v, double scan, int s0) {
-        const unsigned long some = __ballot(v > 0.0), over = __ballot(v > 0.0 && run + scan > target);
-        if (some) {
-            const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
-            piece = s0 + at;
-            before = run + verify_lane(scan, at) - verify_lane(v, at);
-        }
-        run += verify_lane(scan, 63);
-        reached = over != 0;
-    };
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (!reached) look(v0[i], scan0[i], i * 64);
-    for (int s0 = 256; !reached && s0 < a.pieces; s0 += 64) {
-        const double v = rest ? rest_sum(s0 + lane) : plain_sum(s0 + lane);
-        look(v, verify_wave_scan(v), s0);
-    }
-    if (piece < 0) return;                     // (no weight anywhere)
-    const int c0 = piece * VERIFY_PIECE, col = c0 + tid * EACH;
-    const bool whole = a.four && c0 + VERIFY_PIECE <= a.V;
-    float v[EACH], q[EACH];
-    verify_load<EACH>(a.logits + (long)c.row * a.V, col, a.V, whole, v);
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) q[e] = 0.f;
-    if (rest && c.q_each > 0.0) verify_load<EACH>(a.guess + (long)c.guess_row * a.V, col, a.V, whole, q);
-    double each[EACH], sum = 0.0;
-    verify_draw_weights<EACH>(c, v, q, col, rest, each);
-    int last = -1;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        sum += each[e];
-        if (each[e] > 0.0) last = col + e;
-    }
-    const double scan = verify_wave_scan(sum);
-    if (lane == 63) shared[wave] = scan;
-    __syncthreads();
-    run = before;
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-        if (w < wave) run += shared[w];
-    run += scan - sum;
-    int found = -1;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        run += each[e];
-        if (found < 0 && each[e] > 0.0 && run > target) found = col + e;
-    }
-    // the wave's first that reaches beyond, and its last that weighs anything, then the block's (columns rise with the threads)
-    const unsigned long over = __ballot(found >= 0), some = __ballot(last >= 0);
-    if (over) found = __builtin_amdgcn_readlane(found, __ffsll((unsigned long long)over) - 1);
-    if (some) last = __builtin_amdgcn_readlane(last, 63 - __clzll((long long)some));
-    if (lane == 0) { founds[wave] = over ? found : -1; lasts[wave] = some ? last : -1; }
-    __syncthreads();
-    if (tid != 0) return;
-    int token = -1;
-    for (int w = 0; w < 4; ++w) {
-        if (founds[w] >= 0) { token = founds[w]; break; }
-        if (lasts[w] >= 0) token = lasts[w];
-    }
-    a.tokens[c.row] = token;
 }
 
 extern "C" long qe_verify_drafts_workspace_bytes(int rows, int V, int R, int has_guess) {
     const long spans = qe_cdiv(V, VERIFY_SPAN), all = rows + (has_guess ? rows - R : 0);
-    return all * spans * (long)sizeof(VerifyPart) + (long)R * (long)sizeof(VerifyChoice) + (long)R * qe_cdiv(V, VERIFY_PIECE) * 8;
+    return all * spans * (long)sizeof(VerifyPart) + (long)R * (long)sizeof(VerifyChoice) + (long)R * (qe_cdiv(V, VERIFY_PIECE) * 8L + 4);
 }
 
 // logits float32 [rows, V], first int32 [R + 1], drafts int32 [rows - R], guess float32 [rows - R, V] or null, temperature and draw float32 [R],
@@ -505,18 +554,19 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     VerifyPart* parts = (VerifyPart*)workspace;
     VerifyChoice* choices = (VerifyChoice*)(parts + (long)all * spans);
     double* rests = (double*)(choices + R);
+    unsigned* done = (unsigned*)(rests + (long)R * pieces);      // how many blocks of a request are done
     const int four = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)guess) & 15) == 0;
     const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, pieces, four};
-    verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts);
-    // Few spans: every block accepts for itself, which saves a launch (spans of 1 request of 151936 15.1 us, in two launches 16.4; of 8, 304
-    // spans, 27.2 and 28.1; of 16 40.4 and 36.3).
+    verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts, done);
+    // Few spans: every block accepts for itself and the last one draws, in one launch instead of three (1 request of 151936, 38 spans, 13.6 us, and
+    // 14.4; 8 requests, 304 spans, 25.4 and 25.9; 16 40.1 and 34.1; a program's call for 1 request 18.5 and 21.4).
     if ((long)spans * R <= 320) {
-        verify_rest_kernel<true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests);
+        verify_rest_kernel<true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests, done);
     } else {
         verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
-        verify_rest_kernel<false><<<dim3(pieces, R), 256, 0, stream>>>(a, parts, choices, rests);
+        verify_rest_kernel<false><<<dim3(pieces, R), 256, 0, stream>>>(a, parts, choices, rests, done);
+        verify_draw_kernel<<<R, 256, 0, stream>>>(a, parts, choices, rests);
     }
-    verify_draw_kernel<<<R, 256, 0, stream>>>(a, parts, choices, rests);
     QE_LAUNCH_CHECK();
     return 0;
 }
