@@ -2324,6 +2324,19 @@ def _on_current_device(t: torch.Tensor, what: str) -> None:
         raise KernelError(f"{what}: the operands are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _need_matrix(x: torch.Tensor, name: str) -> Tuple[int, int]:
+    """Rows and columns of a matrix in bfloat16 or float32.  (What passes is found out first, as in _need: a call for one row takes 8 us,
+    of which the checks are 2.)"""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.is_contiguous() and x.dtype in _DT and x.dim() == 2):
+        _need(x, name, _ACT, (None, None))
+    return x.shape
+
+
+def _need_vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, device: torch.device) -> None:
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.is_contiguous() and t.shape == (n,)):
+        _need(t, name, dtype, (n,), device)
+
+
 def _apart(written: torch.Tensor, read, what: str) -> None:
     """What is written lies beside what is read: other blocks still read it then."""
     a = written.data_ptr()
@@ -2331,6 +2344,9 @@ def _apart(written: torch.Tensor, read, what: str) -> None:
     for t in read:
         if t is not None and t.data_ptr() < b and a < t.data_ptr() + t.numel() * t.element_size():
             raise KernelError(f"{what}: the result lies over an operand")
+
+
+_U8 = torch.uint8
 
 
 class MxFp4(NamedTuple):
@@ -2347,12 +2363,11 @@ def _need_mxfp4(m: MxFp4, name: str, device=None) -> Tuple[int, int]:
     if not isinstance(m, MxFp4):
         raise KernelError(f"{name} is no 4-bit matrix")
     codes, scales, K = m
-    # (as in _need, what passes is found out first)
-    if isinstance(K, int) and K > 0 and isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and \
-            codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous():
-        at, T, blocks = codes.get_device(), scales.shape[0] if scales.dim() == 2 else -1, (K + 31) // 32
-        if at >= 0 and scales.get_device() == at and (device is None or device.index == at) and scales.shape == (T, blocks) and \
-                codes.shape == (T, blocks * 16) and codes.data_ptr() % 16 == 0:
+    if type(K) is int and K > 0 and isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype is _U8 and \
+            scales.dtype is _U8 and codes.is_contiguous() and scales.is_contiguous() and codes.dim() == 2:
+        at, (T, width), blocks = codes.get_device(), codes.shape, (K + 31) // 32
+        if width == blocks * 16 and at >= 0 and scales.get_device() == at and (device is None or device.index == at) and \
+                scales.shape == (T, blocks) and codes.data_ptr() % 16 == 0:
             return T, K
     K = int(K)
     if K <= 0:
@@ -2371,8 +2386,7 @@ def mxfp4_quantize(x: torch.Tensor) -> MxFp4:
     the largest code (2^-127 at least); a number goes to the nearest code, ties to the even one, what is beyond 6 to 6.  A block with
     an infinity or a NaN is all NaN."""
     lib = load_library()
-    _need(x, "x", _ACT, (None, None))
-    T, K = x.shape
+    T, K = _need_matrix(x, "x")
     if K == 0:
         raise KernelError("mxfp4_quantize: rows of no numbers")
     _on_current_device(x, "mxfp4_quantize")
@@ -2410,8 +2424,7 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
         data, scales, kind, dev = x.codes, x.scales, 2, x.codes.device
         out_dtype = out_dtype or torch.bfloat16
     else:
-        _need(x, "x", _ACT, (None, None))
-        M, K = x.shape
+        M, K = _need_matrix(x, "x")
         data, scales, kind, dev = x, None, int(x.dtype is torch.float32), x.device
         out_dtype = out_dtype or x.dtype
     N, columns = _need_mxfp4(w, "w", dev)
@@ -2440,10 +2453,14 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
     else:
         _need(out, "out", out_dtype, (M, wide), dev)
         _apart(out, (data, scales, w.codes, w.scales, bias), "gemm_mxfp4")
-    nbytes = lib.qe_gemm_mxfp4_workspace_bytes(data.data_ptr(), _ptr(scales), w.scales.data_ptr(), M, N, K, kind, tail)
-    ws = data.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
-    _check(lib.qe_gemm_mxfp4(data.data_ptr(), _ptr(scales), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), out.data_ptr(),
-                             M, N, K, kind, _DT[out_dtype], tail, _ptr(ws), nbytes, _stream()), "gemm_mxfp4")
+    at, ws_at, scales_at, nbytes = data.data_ptr(), None, None if scales is None else scales.data_ptr(), 0
+    if M > 16 or kind == 1 or K % 8 or at % 16:            # (else none is needed: a call that is not made, 0.7 us)
+        nbytes = lib.qe_gemm_mxfp4_workspace_bytes(at, scales_at, w.scales.data_ptr(), M, N, K, kind, tail)
+        if nbytes:
+            ws = data.new_empty((nbytes,), dtype=torch.uint8)
+            ws_at = ws.data_ptr()
+    _check(lib.qe_gemm_mxfp4(at, scales_at, w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                             M, N, K, kind, _DT[out_dtype], tail, ws_at, nbytes, _stream()), "gemm_mxfp4")
     return out
 
 
@@ -2475,27 +2492,27 @@ def verify_drafts(logits: torch.Tensor, first: torch.Tensor, drafts: torch.Tenso
     if V == 0:
         raise KernelError("verify_drafts: a vocabulary of no tokens")
     D = rows - R
-    _need(drafts, "drafts", torch.int32, (D,), dev)
+    _need_vector(drafts, "drafts", torch.int32, D, dev)
     if draft_logits is not None:
         _need(draft_logits, "draft_logits", torch.float32, (D, V), dev)
-    _need(temperature, "temperature", torch.float32, (R,), dev)
-    _need(accept_uniform, "accept_uniform", torch.float32, (D,), dev)
-    _need(draw_uniform, "draw_uniform", torch.float32, (R,), dev)
+    _need_vector(temperature, "temperature", torch.float32, R, dev)
+    _need_vector(accept_uniform, "accept_uniform", torch.float32, D, dev)
+    _need_vector(draw_uniform, "draw_uniform", torch.float32, R, dev)
     _on_current_device(logits, "verify_drafts")
     if tokens is None:
-        tokens = torch.empty((rows,), dtype=torch.int32, device=dev)
+        tokens = first.new_empty((rows,))
     else:
         _need(tokens, "tokens", torch.int32, (rows,), dev)
         _apart(tokens, (logits, first, drafts, draft_logits, temperature, accept_uniform, draw_uniform, accepted), "verify_drafts")
     if accepted is None:
-        accepted = torch.empty((R,), dtype=torch.int32, device=dev)
+        accepted = first.new_empty((R,))
     else:
         _need(accepted, "accepted", torch.int32, (R,), dev)
         _apart(accepted, (logits, first, drafts, draft_logits, temperature, accept_uniform, draw_uniform), "verify_drafts")
     if R == 0:
         return tokens, accepted
     nbytes = lib.qe_verify_drafts_workspace_bytes(rows, V, R, int(draft_logits is not None))
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    ws = first.new_empty((nbytes,), dtype=torch.uint8)
     _check(lib.qe_verify_drafts(logits.data_ptr(), first.data_ptr(), drafts.data_ptr(), _ptr(draft_logits), temperature.data_ptr(),
                                 accept_uniform.data_ptr(), draw_uniform.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
                                 rows, V, R, ws.data_ptr(), nbytes, _stream()), "verify_drafts")
