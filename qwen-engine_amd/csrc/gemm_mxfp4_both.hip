@@ -52,8 +52,9 @@ __global__ __launch_bounds__(256) void fp4_prepare_kernel(Fp4Prepare p) {
 struct Fp4Both {
     Fp4Args a;
     const unsigned char* x;     // codes, nothing behind K
-    const unsigned char *xs, *scales;   // of x and of the matrix, scale_bytes a row
-    int nk, scale_bytes, tiles_m, tiles_n;
+    const unsigned char *xs, *scales;   // of x and of the matrix, so many bytes from a row to the next
+    int x_scale_bytes, scale_bytes;
+    int nk, tiles_m, tiles_n;
     int per_split;                      // stages of a cut of K, whole spans: block (., y) sums those from y * per_split on
 };
 
@@ -96,8 +97,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void fp4_both_kernel(Fp4Bot
         const bool of_x = part < BM / 64;
         const int row = of_x ? (m0 + part * 64 + lane < a.M ? m0 + part * 64 + lane : -1)
                              : fp4_matrix_row<TAIL>(n0, (part - BM / 64) * 64 + lane, wide);
-        vs[i] = row >= 0 ? row * t.scale_bytes : FP4_OUT;
-        rsrc_s[i] = fp4_buffer(of_x ? t.xs : t.scales, (unsigned)((long)(of_x ? a.M : a.N) * t.scale_bytes));
+        const int scale_bytes = of_x ? t.x_scale_bytes : t.scale_bytes;
+        vs[i] = row >= 0 ? row * scale_bytes : FP4_OUT;
+        rsrc_s[i] = fp4_buffer(of_x ? t.xs : t.scales, (unsigned)((long)(of_x ? a.M : a.N) * scale_bytes));
     }
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
     const int first_stage = blockIdx.y * t.per_split, stages = min(t.nk - first_stage, t.per_split);
@@ -284,11 +286,11 @@ __global__ __launch_bounds__(256, 1) void fp4_both_large_kernel(Fp4Both t) {
             vb[g][i] = n >= 0 ? n * row_bytes + piece * 16 : FP4_OUT;
         }
     // scales of a span of two stages: 256 rows of x with its even stage, 256 of the matrix with its odd one, 64 a wave
-    vs[0] = m0 + wave * 64 + lane < a.M ? (m0 + wave * 64 + lane) * t.scale_bytes : FP4_OUT;
+    vs[0] = m0 + wave * 64 + lane < a.M ? (m0 + wave * 64 + lane) * t.x_scale_bytes : FP4_OUT;
     vs[1] = fp4_matrix_row<TAIL>(n0, wave * 64 + lane, wide);
     vs[1] = vs[1] >= 0 ? vs[1] * t.scale_bytes : FP4_OUT;
     const uintx4_t rsrc_a = fp4_buffer(t.x, (unsigned)((long)a.M * row_bytes)), rsrc_b = fp4_buffer(a.codes, (unsigned)((long)a.N * row_bytes));
-    const uintx4_t rsrc_x = fp4_buffer(t.xs, (unsigned)((long)a.M * t.scale_bytes)), rsrc_w = fp4_buffer(t.scales, (unsigned)((long)a.N * t.scale_bytes));
+    const uintx4_t rsrc_x = fp4_buffer(t.xs, (unsigned)((long)a.M * t.x_scale_bytes)), rsrc_w = fp4_buffer(t.scales, (unsigned)((long)a.N * t.scale_bytes));
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem + wave_s * 1024;
     const int off = piece < a.blocks - (nk - 1) * 8 ? 0 : FP4_OUT;      // (blocks of the last stage that lie beyond the row: out of range)
 #define REGION_AT(g_, par_) (((par_) * 4 + (g_)) * 16384)
@@ -473,16 +475,22 @@ static long fp4_both_parts(int M, int N, int K) {
     return splits > 1 ? (4L * splits * M * N + 15) / 16 * 16 : 0;
 }
 
+static int fp4_both_stage(int M, int N) { return fp4_both_large(M, N) ? 2 * FP4_STAGE : FP4_STAGE; }
+
 long fp4_both_workspace(int M, int N, int K, const void* xs, const void* scales) {
-    return fp4_both_parts(M, N, K) + (K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0) + (fp4_scales_whole(K, xs) ? 0 : fp4_scales_bytes(M, K)) +
-           (fp4_scales_whole(K, scales) ? 0 : fp4_scales_bytes(N, K));
+    const int stage = fp4_both_stage(M, N);
+    return fp4_both_parts(M, N, K) + (K % 32 ? (long)M * qe_cdiv(K, 32) * 16 : 0) + (fp4_scales_whole(K, xs, stage) ? 0 : fp4_scales_bytes(M, K)) +
+           (fp4_scales_whole(K, scales, stage) ? 0 : fp4_scales_bytes(N, K));
 }
 
 int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
     Fp4Both t{};
     t.a = a;
     t.nk = qe_cdiv(a.K, FP4_STAGE);
-    t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
+    const int stage = fp4_both_stage(a.M, a.N);
+    const bool x_whole = fp4_scales_whole(a.K, a.xs, stage), whole = fp4_scales_whole(a.K, a.scales, stage);
+    t.x_scale_bytes = fp4_scales_row(a.K, x_whole);
+    t.scale_bytes = fp4_scales_row(a.K, whole);
     float* parts = (float*)workspace;          // the workspace: the cuts' products, then what the loads do not take as it is
     unsigned char* ws = (unsigned char*)workspace + fp4_both_parts(a.M, a.N, a.K);
     int splits;
@@ -492,7 +500,7 @@ int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
     t.scales = a.scales;
     Fp4Prepare p{};
     p.blocks = a.blocks;
-    p.num_words = t.scale_bytes / 4;
+    p.num_words = fp4_scales_row(a.K, false) / 4;
     p.K = a.K;
     if (a.K % 32) {
         p.codes = (const uintx4_t*)a.x;
@@ -501,14 +509,14 @@ int fp4_both(const Fp4Args& a, int tail, void* workspace, hipStream_t stream) {
         t.x = ws;
         ws += (long)p.pieces * 16;
     }
-    if (!fp4_scales_whole(a.K, a.xs)) {
+    if (!x_whole) {
         p.xs = a.xs;
         p.xs_out = (uint32_t*)ws;
         p.x_words = (unsigned)(fp4_scales_bytes(a.M, a.K) / 4);
         t.xs = ws;
         ws += (long)p.x_words * 4;
     }
-    if (!fp4_scales_whole(a.K, a.scales)) {
+    if (!whole) {
         p.scales = a.scales;
         p.scales_out = (uint32_t*)ws;
         p.words = (unsigned)(fp4_scales_bytes(a.N, a.K) / 4);

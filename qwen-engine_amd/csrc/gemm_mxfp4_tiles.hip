@@ -71,10 +71,6 @@ __global__ __launch_bounds__(256) void fp4_copies_kernel(Fp4Copies p) {
 
 static int padded(int K) { return qe_cdiv(K, FP4_STAGE) * FP4_STAGE; }
 
-bool fp4_scales_whole(int K, const void* scales) { return K % FP4_SPAN == 0 && ((uintptr_t)scales & 15) == 0; }
-
-long fp4_scales_bytes(int rows, int K) { return (long)rows * qe_cdiv(K, FP4_SPAN) * (FP4_SPAN / 32); }
-
 long fp4_planes_bytes(int M, int K, int x_kind) { return (x_kind == X_F32 ? 6L : 2L) * M * padded(K); }
 
 Fp4Rows fp4_copies(const void* x, int M, int K, int x_kind, void* out, const unsigned char* scales, int rows, void* scales_out, hipStream_t stream) {
@@ -103,7 +99,7 @@ struct Fp4Tiles {
     const uint16_t* planes;     // rows of x, row_bytes apart, plane after plane
     unsigned row_bytes, plane_bytes, x_bytes;      // (x_bytes: of all planes)
     const unsigned char* scales;
-    int scale_bytes;            // of a row
+    int scale_bytes;            // from a row to the next
     int num_planes, nk, k_in_row;                  // (numbers of K that a row holds: K, or whole stages where it is a plane's)
     int tiles_m, tiles_n;
     int per_split;              // stages of a cut: block (., y) sums the stages from y * per_split on
@@ -428,7 +424,7 @@ long fp4_tiles_workspace(int M, int N, int K, int x_kind, const void* x, const v
     const Fp4Shape s = fp4_tiles_shape(M, N, K, x_kind);
     long bytes = s.splits > 1 ? (4L * s.splits * M * N + 15) / 16 * 16 : 0;
     if (x_kind == X_F32 || K % 8 || !aligned) bytes += fp4_planes_bytes(M, K, x_kind);
-    return bytes + (fp4_scales_whole(K, scales) ? 0 : fp4_scales_bytes(N, K));
+    return bytes + (fp4_scales_whole(K, scales, s.sk) ? 0 : fp4_scales_bytes(N, K));
 }
 
 int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
@@ -440,7 +436,7 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     // the workspace: the cuts' products, then what is made of x, then of the scales
     float* parts = (float*)workspace;
     unsigned char* ws = (unsigned char*)workspace + (s.splits > 1 ? (4L * s.splits * a.M * a.N + 15) / 16 * 16 : 0);
-    const bool copy_x = x_kind == X_F32 || a.K % 8 || ((uintptr_t)a.x & 15), copy_scales = !fp4_scales_whole(a.K, a.scales);
+    const bool copy_x = x_kind == X_F32 || a.K % 8 || ((uintptr_t)a.x & 15), copy_scales = !fp4_scales_whole(a.K, a.scales, s.sk);
     unsigned char* const scales_at = ws + (copy_x ? fp4_planes_bytes(a.M, a.K, x_kind) : 0);
     Fp4Rows x{a.x, a.K * 2, 1};
     if (copy_x || copy_scales) {
@@ -454,7 +450,7 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
     t.plane_bytes = t.row_bytes * (unsigned)a.M;
     t.x_bytes = t.plane_bytes * t.num_planes;
     t.scales = copy_scales ? scales_at : a.scales;
-    t.scale_bytes = qe_cdiv(a.K, FP4_SPAN) * (FP4_SPAN / 32);
+    t.scale_bytes = fp4_scales_row(a.K, !copy_scales);
     if (s.splits > 1) t.a.out = parts;
     int rc;
 #define QE_GO(T_)                                                                            \

@@ -297,6 +297,32 @@ def test_tiles_of_every_height(ops, kind, M, N, K):
     assert ((got - act).nan_to_num().abs() <= bound).all()
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M,N,K", [(70, 301, 128), (70, 301, 640), (300, 517, 384), (300, 1030, 1152), (3100, 4200, 768), (3100, 4200, 128)])
+@pytest.mark.parametrize("at", [0, 1, 4])
+def test_scales_of_rows_that_end_inside_a_span(ops, kind, M, N, K, at):
+    """Scales travel 16 at a time, from any whole word on: rows of 4, 12, 20 or more scales, from the given byte of an allocation on, between
+    others that are NaN; every sum exact (halves of at most 48 K)."""
+    codes, scales, v = whole_matrix(N, K, K)
+    scales[1::7] = 255
+    v = torch.where((scales == 255).any(1, keepdim=True), torch.full_like(v, math.nan), v).to(DEV)
+
+    def placed(s):
+        room = torch.full((s.numel() + 64,), 255, dtype=torch.uint8, device=DEV)
+        room[at:at + s.numel()] = s.to(DEV).view(-1)
+        return room[at:at + s.numel()].view(s.shape)
+    w = ops.MxFp4(codes.to(DEV), placed(scales), K)
+    if kind == "fp4":
+        xc, xs, xv = whole_matrix(M, K, 7)
+        x = ops.MxFp4(xc.to(DEV), placed(xs), K)
+    else:
+        xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+        x = xv.to(getattr(torch, kind)).to(DEV)
+    want = xv.to(DEV) @ v.T
+    got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32).double()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
 def test_rows_at_odd_elements(ops):
     """x, bias and out at no whole 16-byte piece; the numbers before and behind out stay."""
     M, N, K = 19, 40, 96
