@@ -1,13 +1,17 @@
 // Products of many rows of 16-bit or 32-bit numbers with a 4-bit matrix (see mxfp4.h): out[M, N] = x[M, K] . V[N, K]^T.
 //
 // A block of four waves computes BM rows by BN columns.  K is walked in stages of 128 or 64 through a ring in shared memory: of 128, 256 bytes of a
-// row of x, 64 of codes and 4 of scales (a word each there) of a row of the matrix, brought by loads that write to shared memory directly.  A
+// row of x and 64 of codes of a row of the matrix, and for 512 of K 16 of its scales, brought by loads that write to shared memory directly.  A
 // wave multiplies its part in tiles of 32 x 32 with v_mfma_f32_32x32x16_bf16: lane (r, h) = (lane % 32, lane / 32) takes, of row r,
 // block 2 b + h of the stage, so that a 16-byte piece of codes with one scale gives four matrix instructions' operands, eight numbers
 // each, by four conversions each.  The conversions for the next k step stand between the matrix instructions of this one.
 //
 // Rows of 32-bit numbers come as three planes of bfloat16 (cut_in_three) that are walked one after the other, the smallest
 // first, against the same matrix; they are made by a launch of their own, which also fills K up to whole stages.
+//
+// 2048 rows against 24576 x 4096 take 319 us (1.29 PFLOP/s): the matrix units are 65 % busy at the clock that the power leaves.  64 rows against that take 23.4 us:
+// they are 34 % busy, the one wave of a SIMD issues half of its time (conversions, fragments, loads and their places, one after
+// the other) and waits for 30 %; a ring of six stages instead of three changes nothing.
 #include "mxfp4.h"
 
 #define FP4_STAGE 128      // numbers of K
