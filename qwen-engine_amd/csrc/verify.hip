@@ -326,6 +326,7 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const
 // distribution taken away).  The forms are told apart once, not at every number, so that the polynomials go side by side.
 template <int EACH>
 __device__ __forceinline__ void verify_draw_weights(const VerifyChoice& c, const float (&z)[EACH], const float (&zq)[EACH], int col, bool rest, double (&w)[EACH]) {
+#pragma clang fp contract(off)                 // (both products are rounded: where p and q are alike nothing is left, not the difference of a product and its rounding)
     const bool with_q = rest && c.q_each > 0.0;
     if (c.p_top == INFINITY || (with_q && c.q_top == INFINITY)) {
 #pragma unroll

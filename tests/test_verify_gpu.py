@@ -132,6 +132,25 @@ def test_many_requests(ops):
     check(ops, case(counts, 300, 3))
 
 
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("V,counts", [(262145, [1, 0, 2]), (300001, [2, 0, 1]), (1100003, [1]), (1100003, [0, 2, 1])])
+def test_very_wide_vocabularies(ops, V, counts, lookup):
+    """More pieces and spans than a wave looks at in one go, in one launch and in several; the tokens lie all over the vocabulary."""
+    c = case(counts, V, V % 1000, spread=0.5, lookup=lookup, greedy_every=100)
+    tokens = set()
+    for u in (0.0, 0.2, 0.45, 0.7, 0.9, 0.999):
+        c["draw"] = torch.full((len(counts),), u)
+        want = check(ops, c)
+        tokens |= {t * 8 // V for t in want[0] if t >= 0}
+    assert len(tokens) >= 5
+    if not lookup:                                                 # (the draft's distribution is the model's, and a number beyond 1 refuses the drafts: p alone)
+        drafted = torch.cat([torch.arange(n + 1) < n for n in counts])
+        c["guess"], c["accept"] = c["logits"][drafted].clone(), torch.full_like(c["accept"], 1.5)
+        for u in (0.1, 0.6, 0.97):
+            c["draw"] = torch.full((len(counts),), u)
+            check(ops, c)
+
+
 def test_flat_distributions(ops):
     """Nearly equal weights: as many borders of running sums as tokens."""
     check(ops, case([2, 1, 0, 3, 2, 2, 2, 1], 151936, 8, spread=1e-3, greedy_every=100))
