@@ -69,9 +69,7 @@ __device__ __forceinline__ double verify_term(double a, double b, double c) {
 // n stands in the sum's low bits), f in [-1/2, 1/2], and 2^f by a polynomial of degree 10 through the Chebyshev points of that
 // interval (off by 3.2e-16 of it at the most).  What is NaN on the way (a NaN logit; -infinity less itself) becomes 0 at the maximum, as what
 // is below 2^-1080 does.
-__device__ __forceinline__ double verify_finite_weight(float z, float top, const VerifyScale& t) {
-    const double d = __builtin_fmax((double)z - (double)top, t.least);
-    const double y = __builtin_fma(d, t.k, 0x1.8p52), f = __builtin_fma(d, t.k, -(y - 0x1.8p52));
+__device__ __forceinline__ double verify_power(double f) {          // 2^f
     double v = verify_term(f, 0x1.e6063f9b91935p-28, 0x1.b675bd687d9b8p-24);
     v = verify_term(v, f, 0x1.62bfd477051e0p-20);
     v = verify_term(v, f, 0x1.ffcb540541227p-17);
@@ -81,9 +79,53 @@ __device__ __forceinline__ double verify_finite_weight(float z, float top, const
     v = verify_term(v, f, 0x1.c6b08d703ce45p-5);
     v = verify_term(v, f, 0x1.ebfbdff82c598p-3);
     v = verify_term(v, f, 0x1.62e42fefa3a19p-1);
-    v = __builtin_fma(v, f, 1.0);
-    return __builtin_amdgcn_ldexp(v, (int)__builtin_bit_cast(unsigned long, y));
+    return __builtin_fma(v, f, 1.0);
 }
+__device__ __forceinline__ double verify_finite_weight(float z, float top, const VerifyScale& t) {
+    const double d = __builtin_fmax((double)z - (double)top, t.least);
+    const double y = __builtin_fma(d, t.k, 0x1.8p52), f = __builtin_fma(d, t.k, -(y - 0x1.8p52));
+    return __builtin_amdgcn_ldexp(verify_power(f), (int)__builtin_bit_cast(unsigned long, y));
+}
+
+// The same for a sum over many logits of a row, with fewer operations (64 requests 120 us, so 115: what counts there is how many 64-bit operations a
+// logit takes, next to its bytes): 2^(z k) = 2^m 2^(j / 32) 2^f, where 32 m + j is 32 z k rounded (1.5 2^47 added) and |f| <= 1/64, so
+// that a polynomial of degree 5 does (off by 1.5e-16 at the most); 2^(j / 32) comes from a table in shared memory, in 32 pairs of banks of its
+// own, which holds the high words less j 2^15: 32 m + j, shifted by 15 and added, makes 2^m 2^(j / 32) of them.  The row's own number of the
+// kind, 2^(top k), counts for the sum as a whole: its rounded exponent is taken off with the constant that rounds 32 z k, the rest
+// multiplied at the end.  What is far below the top (or no number) counts as 2^-1000 of it, which the logit's 32-bit maximum with `floor` sees
+// to.  Not for a top that is infinite, beyond 2^25 / k or less than 1000 / k away from the end of what 32 bits hold.
+__device__ const unsigned long verify_table[32] = {
+    0x3ff0000000000000ul, 0x3fefd9b0d3158574ul, 0x3fefb5586cf9890ful, 0x3fef9301d0125b51ul, 0x3fef72b83c7d517bul, 0x3fef54873168b9aaul, 0x3fef387a6e756238ul, 0x3fef1e9df51fdee1ul,
+    0x3fef06fe0a31b715ul, 0x3feef1a7373aa9cbul, 0x3feedea64c123422ul, 0x3feece086061892dul, 0x3feebfdad5362a27ul, 0x3feeb42b569d4f82ul, 0x3feeab07dd485429ul, 0x3feea47eb03a5585ul,
+    0x3feea09e667f3bcdul, 0x3fee9f75e8ec5f74ul, 0x3feea11473eb0187ul, 0x3feea589994cce13ul, 0x3feeace5422aa0dbul, 0x3feeb737b0cdc5e5ul, 0x3feec49182a3f090ul, 0x3feed503b23e255dul,
+    0x3feee89f995ad3adul, 0x3feeff76f2fb5e47ul, 0x3fef199bdd85529cul, 0x3fef3720dcef9069ul, 0x3fef5818dcfba487ul, 0x3fef7c97337b9b5ful, 0x3fefa4afa2a490daul, 0x3fefd0765b6e4540ul};
+
+struct VerifySum {
+    double k, round;            // round: 1.5 2^47 less the top's exponent
+    float floor;
+    bool fits;
+    __device__ __forceinline__ VerifySum(const VerifyScale& t, float top) {
+        k = t.k;
+        const double at = (double)top * k;
+        round = 0x1.8p47 - __builtin_rint(at);
+        floor = (float)((double)top - 1000.0 / k);
+        fits = __builtin_fabs(at) < 0x1p25 && floor > -INFINITY;
+    }
+    // sum and the weight of z; table: in shared memory
+    __device__ __forceinline__ double add(double sum, float z, const unsigned long* table) const {
+        typedef __attribute__((ext_vector_type(2))) uint32_t words;
+        const double d = (double)fmaxf(z, floor), y = __builtin_fma(d, k, round), f = __builtin_fma(d, k, -(y - round));
+        const uint32_t at = __builtin_bit_cast(words, y)[0];
+        words scale = __builtin_bit_cast(words, table[at & 31]);
+        scale[1] += at << 15;
+        double v = verify_term(f, 0x1.5d884e708e6aap-10, 0x1.3b2b1bee88b09p-7);
+        v = verify_term(v, f, 0x1.c6b08d70400d0p-5);
+        v = verify_term(v, f, 0x1.ebfbdff8131c3p-3);
+        v = verify_term(v, f, 0x1.62e42fefa39efp-1);
+        return __builtin_fma(__builtin_fma(v, f, 1.0), __builtin_bit_cast(double, scale), sum);
+    }
+    __device__ __forceinline__ double rest(float top) const { return verify_power(-__builtin_fma((double)top, k, -(0x1.8p47 - round))); }
+};
 
 // The same for any row: infinite logits share everything.
 __device__ __forceinline__ double verify_weight(float z, float top, const VerifyScale& t) {
@@ -164,6 +206,7 @@ __device__ __forceinline__ void verify_wave_top(float& top, int& at) {
 __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyPart* parts, unsigned* done) {
     __shared__ float tops[4];
     __shared__ int ats[4];
+    __shared__ unsigned long table[32];
     const bool is_guess = (int)blockIdx.y >= a.rows;
     const int i = is_guess ? blockIdx.y - a.rows : blockIdx.y;
     constexpr int EACH = VERIFY_PIECE / 64;
@@ -198,20 +241,24 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
         for (int e = 0; e < EACH; ++e) top = fmaxf(top, v[e]);
         top = wave_max(top);
     }
+    if (threadIdx.x < 32) table[threadIdx.x] = verify_table[threadIdx.x];
     if (lane == 0) { tops[wave] = top; ats[wave] = at; }
     __syncthreads();
     for (int w = 0; w < 4; ++w)
         if (tops[w] > top || (tops[w] == top && ats[w] < at)) { top = tops[w]; at = ats[w]; }
     double sum = 0.0;
     if (!greedy) {
-        if (top == INFINITY) {
+        const VerifySum all(k, top);
+        if (all.fits) {
 #pragma unroll
-            for (int e = 0; e < EACH; ++e) sum += v[e] == top ? 1.0 : 0.0;
+            for (int e = 0; e < EACH; ++e) sum = all.add(sum, v[e], table);
+            sum = verify_wave_sum(sum) * all.rest(top);
+            if (sum < 0x1p-900) sum = 0.0;         // (nothing there but what counts as 2^-1000)
         } else {
 #pragma unroll
-            for (int e = 0; e < EACH; ++e) sum += verify_finite_weight(v[e], top, k);
+            for (int e = 0; e < EACH; ++e) sum += verify_weight(v[e], top, k);
+            sum = verify_wave_sum(sum);
         }
-        sum = verify_wave_sum(sum);
     }
     VerifyPart& part = parts[(long)blockIdx.y * a.spans + blockIdx.x];
     if (lane == 0) part.sums[wave] = sum;
