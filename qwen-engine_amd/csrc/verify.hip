@@ -93,7 +93,7 @@ __device__ __forceinline__ double verify_finite_weight(float z, float top, const
 // own, which holds the high words less j 2^15: 32 m + j, shifted by 15 and added, makes 2^m 2^(j / 32) of them.  The row's own number of the
 // kind, 2^(top k), counts for the sum as a whole: its rounded exponent is taken off with the constant that rounds 32 z k, the rest
 // multiplied at the end.  What is far below the top (or no number) counts as 2^-1000 of it, which the logit's 32-bit maximum with `floor` sees
-// to.  Not for a top that is infinite, beyond 2^25 / k or less than 1000 / k away from the end of what 32 bits hold.
+// to.  Not for a top that is infinite or beyond 2^25 / k, nor where 32 bits hold no number some 1000 / k below it.
 __device__ const unsigned long verify_table[32] = {
     0x3ff0000000000000ul, 0x3fefd9b0d3158574ul, 0x3fefb5586cf9890ful, 0x3fef9301d0125b51ul, 0x3fef72b83c7d517bul, 0x3fef54873168b9aaul, 0x3fef387a6e756238ul, 0x3fef1e9df51fdee1ul,
     0x3fef06fe0a31b715ul, 0x3feef1a7373aa9cbul, 0x3feedea64c123422ul, 0x3feece086061892dul, 0x3feebfdad5362a27ul, 0x3feeb42b569d4f82ul, 0x3feeab07dd485429ul, 0x3feea47eb03a5585ul,
@@ -104,12 +104,13 @@ struct VerifySum {
     double k, round;            // round: 1.5 2^47 less the top's exponent
     float floor;
     bool fits;
-    __device__ __forceinline__ VerifySum(const VerifyScale& t, float top) {
-        k = t.k;
+    __device__ __forceinline__ VerifySum(double k_, float t, float top) {
+        k = k_;
         const double at = (double)top * k;
         round = 0x1.8p47 - __builtin_rint(at);
-        floor = (float)((double)top - 1000.0 / k);
-        fits = __builtin_fabs(at) < 0x1p25 && floor > -INFINITY;
+        floor = top - 693.147181f * t;             // (1000 ln 2)
+        const double far = ((double)floor - (double)top) * k;
+        fits = __builtin_fabs(at) < 0x1p25 && far > -1015.0 && far < -950.0;
     }
     // sum and the weight of z; table: in shared memory
     __device__ __forceinline__ double add(double sum, float z, const unsigned long* table) const {
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
         if (tops[w] > top || (tops[w] == top && ats[w] < at)) { top = tops[w]; at = ats[w]; }
     double sum = 0.0;
     if (!greedy) {
-        const VerifySum all(k, top);
+        const VerifySum all(k.k, t, top);
         if (all.fits) {
 #pragma unroll
             for (int e = 0; e < EACH; ++e) sum = all.add(sum, v[e], table);

@@ -151,6 +151,23 @@ def test_very_wide_vocabularies(ops, V, counts, lookup):
             check(ops, c)
 
 
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("offset", [0.0, -300.0, 5e4, 2e9])
+def test_temperatures_of_all_sizes(ops, offset, lookup):
+    """From the smallest that 32 bits hold, where the largest logit has everything, to the largest, where all that is not masked is alike."""
+    temperatures = [1e-45, 1e-38, 1e-20, 1e-8, 1e-5, 1e-3, 0.05, 1.0, 30.0, 1e4, 1e9, 1e30, 1e37, 3e38]
+    counts = [2] * len(temperatures)
+    c = case(counts, 5003, 17, spread=3.0, lookup=lookup, greedy_every=1000)
+    c["logits"] += offset
+    masked = torch.rand(c["logits"].shape, generator=torch.Generator().manual_seed(4)) < 0.3
+    masked[torch.cat([torch.arange(3) < 2 for _ in counts]).nonzero()[:, 0], c["drafts"].long()] = False
+    c["logits"][masked] = -math.inf
+    c["temperature"] = torch.tensor(temperatures)
+    for seed in range(3):
+        c["draw"] = torch.rand(len(counts), generator=torch.Generator().manual_seed(seed))
+        check(ops, c)
+
+
 def test_flat_distributions(ops):
     """Nearly equal weights: as many borders of running sums as tokens."""
     check(ops, case([2, 1, 0, 3, 2, 2, 2, 1], 151936, 8, spread=1e-3, greedy_every=100))
