@@ -6,8 +6,9 @@
 // block 2 b + h of the stage, so that a 16-byte piece of codes with one scale gives four matrix instructions' operands, eight numbers
 // each, by four conversions each.  The conversions for the next k step stand between the matrix instructions of this one.
 //
-// Rows of 32-bit numbers come as three planes of bfloat16 (cut_in_three) that are walked one after the other, the smallest
-// first, against the same matrix; they are made by a launch of their own, which also fills K up to whole stages.
+// Rows of 32-bit numbers come as three planes of bfloat16 (cut_in_three), made by a launch of their own, which also fills K up to whole
+// stages.  They are walked one after the other, the smallest first, against the same matrix; or a tile has 32 rows of all three, so that the
+// codes are loaded and converted once (130 rows of 2568 numbers against 5120 24 us, walked three times 30).
 //
 // 2048 rows against 24576 x 4096 take 319 us (1.29 PFLOP/s): the matrix units are 65 % busy at the clock that the power leaves.  64 rows against that take 23.4 us:
 // they are 34 % busy, the one wave of a SIMD issues half of its time (conversions, fragments, loads and their places, one after
@@ -153,8 +154,9 @@ int fp4_join(const Fp4Args& a, const float* parts, int splits, int tail, hipStre
     return 0;
 }
 
-// BM x BN: the tile; WR x WC: the waves; SK: numbers of K of a stage, 128 or 64 (whole lines of x either way); RING: stages in shared memory
-template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>
+// BM x BN: the tile; WR x WC: the waves; SK: numbers of K of a stage, 128 or 64 (whole lines of x either way); RING: stages in shared memory;
+// PLANES: 3: the tile's rows are those of x in each of the three planes, whose sums are added at the end, the smallest first
+template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING, int PLANES>
 __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) {
     constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, MI = WM / 32, NJ = WN / 32, QS = SK / 16, BL = SK / 32;
     constexpr int LDA = BM * SK / (512 * NW), LDB = BN * SK / (2048 * NW), LD = LDA + LDB;      // a wave's loads of a stage: x, codes
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 
     int tile_m, tile_n;
     if (!fp4_tile_of(blockIdx.x, t.tiles_m, t.tiles_n, tile_m, tile_n)) return;
-    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int m0 = tile_m * (BM / PLANES), n0 = tile_n * BN;
     const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
     const int wide = TAIL == TAIL_SILU ? a.N / 2 : a.N;
 
@@ -183,8 +185,8 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
     const int a_piece = SK == 128 ? (lane & 15) ^ (a_row & 15) : (lane & 7) ^ ((a_row >> 1) & 7);
 #pragma unroll
     for (int i = 0; i < LDA; ++i) {
-        const int row = i * NW * AR + a_row;
-        va[i] = m0 + row < a.M ? row * (int)t.row_bytes + a_piece * 16 : FP4_OUT;
+        const int row = i * NW * AR + a_row, plane = row / (BM / PLANES), of_plane = row % (BM / PLANES);
+        va[i] = m0 + of_plane < a.M ? plane * (int)t.plane_bytes + of_plane * (int)t.row_bytes + a_piece * 16 : FP4_OUT;
     }
     const int line = lane >> 3, idx = (lane & 7) ^ ((line >> 1) & (SK == 128 ? 3 : 1)), b_piece = idx & (BL - 1);      // (a load is eight lines)
 #pragma unroll
@@ -356,19 +358,27 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void fp4_tiles_kernel(Fp4Tiles t) 
 #undef READ_CODES
 #undef EXPAND
     static_assert(4 * fp4_strip_bytes<NJ>() <= S_AT, "the waves' strips must fit the ring");
-    fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn, smem + wave * fp4_strip_bytes<NJ>());
+    if constexpr (PLANES == 3) {
+        static_assert(MI == 3 && WR == 1, "a plane is a wave's 32 rows");
+        floatx16_t sum[1][NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sum[0][j] = acc[0][j] + acc[1][j] + acc[2][j];
+        fp4_store_tiles<TAIL, 1, NJ>(a, sum, m0, n0 + wn, smem + wave * fp4_strip_bytes<NJ>());
+    } else {
+        fp4_store_tiles<TAIL, MI, NJ>(a, acc, m0 + wm, n0 + wn, smem + wave * fp4_strip_bytes<NJ>());
+    }
 }
 
-template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING>
+template <int TAIL, int BM, int BN, int WR, int WC, int SK, int RING, int PLANES = 1>
 static int fp4_tiles_launch(Fp4Tiles t, int splits, hipStream_t stream) {
     constexpr int SHARED = RING * (BM * SK * 2 + BN * SK / 2) + (RING + 1) * BN * 16;
     static_assert(SHARED <= 160 * 1024, "the ring must fit a compute unit");
-    t.tiles_m = qe_cdiv(t.a.M, BM);
+    t.tiles_m = qe_cdiv(t.a.M, BM / PLANES);
     t.tiles_n = qe_cdiv(t.a.N, BN);
     const long blocks = ((long)t.tiles_m * t.tiles_n + 7) / 8 * 8;
     QE_REQUIRE(blocks <= 2147483647L, "gemm_mxfp4: too many tiles");
-    QE_RAISE_SHARED((fp4_tiles_kernel<TAIL, BM, BN, WR, WC, SK, RING>), SHARED);
-    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, SK, RING><<<dim3((unsigned)blocks, (unsigned)splits), 256, SHARED, stream>>>(t);
+    QE_RAISE_SHARED((fp4_tiles_kernel<TAIL, BM, BN, WR, WC, SK, RING, PLANES>), SHARED);
+    fp4_tiles_kernel<TAIL, BM, BN, WR, WC, SK, RING, PLANES><<<dim3((unsigned)blocks, (unsigned)splits), 256, SHARED, stream>>>(t);
     return 0;
 }
 
@@ -377,7 +387,7 @@ bool fp4_tiles_take(int M, int N, int K, int x_kind) {
     return (long)N * padded(K) / 2 < (1L << 31) && (long)M * padded(K) * 2 * (x_kind == X_F32 ? 3 : 1) < (1L << 31);
 }
 
-// The rows of a tile, the numbers of K of its stages, and in how many cuts of K the tiles fill the chip.
+// The rows of x of a tile (32: of three planes), the numbers of K of its stages, and in how many cuts of K the tiles fill the chip.
 struct Fp4Shape {
     int bm, sk, per_split, splits;
 };
@@ -388,7 +398,7 @@ struct Fp4TileCost {
     int bm;
     double round, stage;
 };
-static const Fp4TileCost fp4_tile_costs[] = {{64, 3.4, 1.04}, {96, 4.1, 0.68}, {128, 4.6, 0.80}, {160, 6.0, 0.93}, {256, 12.8, 2.27}};
+static const Fp4TileCost fp4_tile_costs[] = {{32, 4.1, 0.68}, {64, 3.4, 1.04}, {96, 4.1, 0.68}, {128, 4.6, 0.80}, {160, 6.0, 0.93}, {256, 12.8, 2.27}};
 
 // The tiles that are done first by these times: what counts is how many rounds the units make and how many of a tile's rows are idle (65 rows
 // against 24576 x 4096 by 96 rows 27.5 us, by 64 36.4; 160 rows by 160 37.4, by 64 51.8; 256 rows by 64 58.8, by 160 71; 700 against
@@ -400,10 +410,11 @@ static Fp4Shape fp4_tiles_shape(int M, int N, int K, int x_kind) {
     Fp4Shape best{};
     double least = 0.0;
     for (const Fp4TileCost& c : fp4_tile_costs) {
+        if (c.bm == 32 && x_kind != X_F32) continue;
         Fp4Shape s;
         s.bm = c.bm;
         s.sk = c.bm == 256 ? 64 : 128;
-        const int planes = x_kind == X_F32 ? 3 : 1, stages = qe_cdiv(K, s.sk) * planes;
+        const int planes = x_kind == X_F32 && c.bm != 32 ? 3 : 1, stages = qe_cdiv(K, s.sk) * planes;
         const long tiles = (long)qe_cdiv(M, s.bm) * qe_cdiv(N, s.bm == 256 ? 256 : 128);
         long splits = s.bm == 256 ? 1 : 256 / tiles;
         if (splits > stages / 8) splits = stages / 8;
@@ -448,11 +459,11 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
         if (copy_x) x = copied;
     }
     t.planes = (const uint16_t*)x.data;
-    t.num_planes = x.planes;
+    t.num_planes = s.bm == 32 ? 1 : x.planes;          // (that are walked)
     t.row_bytes = (unsigned)x.row_bytes;
     t.k_in_row = x.row_bytes / 2;
     t.plane_bytes = t.row_bytes * (unsigned)a.M;
-    t.x_bytes = t.plane_bytes * t.num_planes;
+    t.x_bytes = t.plane_bytes * x.planes;
     t.scales = copy_scales ? scales_at : a.scales;
     t.scale_bytes = fp4_scales_row(a.K, !copy_scales);
     if (s.splits > 1) t.a.out = parts;
@@ -462,11 +473,13 @@ int fp4_tiles(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream
          : s.bm == 160 ? fp4_tiles_launch<T_, 160, 128, 1, 4, 128, 3>(t, s.splits, stream)    \
          : s.bm == 128 ? fp4_tiles_launch<T_, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)    \
          : s.bm == 96  ? fp4_tiles_launch<T_, 96, 128, 1, 4, 128, 3>(t, s.splits, stream)     \
+         : s.bm == 32  ? fp4_tiles_launch<T_, 96, 128, 1, 4, 128, 3, 3>(t, s.splits, stream)  \
                        : fp4_tiles_launch<T_, 64, 128, 1, 4, 128, 3>(t, s.splits, stream)
     if (s.splits > 1)
         rc = s.bm == 160   ? fp4_tiles_launch<TAIL_PARTIAL, 160, 128, 1, 4, 128, 3>(t, s.splits, stream)
              : s.bm == 128 ? fp4_tiles_launch<TAIL_PARTIAL, 128, 128, 2, 2, 128, 3>(t, s.splits, stream)
              : s.bm == 96  ? fp4_tiles_launch<TAIL_PARTIAL, 96, 128, 1, 4, 128, 3>(t, s.splits, stream)
+             : s.bm == 32  ? fp4_tiles_launch<TAIL_PARTIAL, 96, 128, 1, 4, 128, 3, 3>(t, s.splits, stream)
                            : fp4_tiles_launch<TAIL_PARTIAL, 64, 128, 1, 4, 128, 3>(t, s.splits, stream);
     else if (tail == TAIL_STORE) QE_GO(TAIL_STORE);
     else if (tail == TAIL_ADD) QE_GO(TAIL_ADD);
