@@ -270,9 +270,10 @@ def test_large_tiles_and_what_lies_behind_a_row(ops, kind, K):
 
 @pytest.mark.parametrize("kind", ["bfloat16", "float32"])
 @pytest.mark.parametrize("M,N,K", [(200, 8230, 712), (300, 8230, 712), (470, 8230, 712), (500, 4200, 1312), (1000, 4200, 330), (70, 20100, 200),
-                                   (330, 1000, 12000), (600, 1000, 12000), (600, 1000, 4160), (3100, 302, 12000), (270, 1002, 4168)])
+                                   (330, 1000, 12000), (600, 1000, 12000), (600, 1000, 4160), (3100, 302, 12000), (270, 1002, 4168),
+                                   (20, 302, 4160), (40, 20100, 200), (3100, 302, 1312), (20, 4200, 4160)])
 def test_tiles_of_every_height(ops, kind, M, N, K):
-    """Rows and columns that tiles of 64, 96, 128, 160 and 256 rows are taken for, with K in one piece and in cuts; every seventh column
+    """Rows and columns that tiles of 32, 64, 96, 128, 160 and 256 rows are taken for, with K in one piece and in cuts; every seventh column
     and every fifth row is NaN, every other sum exact (halves of at most 48 K < 2^21), the activation within its own arithmetic."""
     codes, scales, v = whole_matrix(N, K, K)
     scales[1::7] = 255
