@@ -1,5 +1,6 @@
 // Products of few rows (up to 32, of 32 bits 16, in 4 bits 64) with a 4-bit matrix (see mxfp4.h): bound by the matrix's bytes on their way from memory.
-// Rows of bfloat16 lie at whole 16-byte pieces; those of 32-bit numbers come as three planes, one behind the other, and K is walked three times.
+// Rows of bfloat16 lie at whole 16-byte pieces.  Up to four rows of 32-bit numbers are cut into three planes of bfloat16 where they are multiplied;
+// of more the planes come from memory, one behind the other, and K is walked three times.
 //
 // A block takes NT tiles of 16 columns, its waves chunks of 256 of K in turn, each wave by itself: it asks for a chunk of the codes (128
 // bytes of a row, a line) and of x straight to its own piece of shared memory, and multiplies it when it has come.  The scales of
@@ -13,10 +14,18 @@
 // other rows, and a load of 64 places of 64 lines takes four times the cycles of one of eight lines.
 #include "mxfp4.h"
 
+// A wave's piece of shared memory: a chunk's loads of x (LX, 1 KB each: two rows of bfloat16, a row of 32-bit numbers, eight in 4 bits), of codes (2
+// a tile), and the planes that are made of 32-bit rows.
+template <int X, int RX, int NT> struct Fp4Slot {
+    static constexpr int LX = X == X_BF16 ? RX / 2 : X == X_F32 ? RX : (RX + 7) / 8;
+    static constexpr int PLANES_AT = (LX + 2 * NT) * 1024, BYTES = PLANES_AT + (X == X_F32 ? 3 * RX * 512 : 0);
+};
+
 template <int X, int RX, int NT>
 __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int tail, int scale_bytes) {
-    constexpr int MT = (RX + 15) / 16, LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8;        // tiles of 16 rows; a chunk's loads of x (and 2 NT of codes)
-    constexpr int SLOT = (LX + 2 * NT) * 1024;
+    constexpr int MT = (RX + 15) / 16, LX = Fp4Slot<X, RX, NT>::LX, SLOT = Fp4Slot<X, RX, NT>::BYTES;        // (MT: tiles of 16 rows)
+    constexpr int CHUNK = X == X_BF16 ? 512 : X == X_F32 ? 1024 : 128, NP = X == X_F32 ? 3 : 1;             // bytes of a row of x in a chunk; planes that are multiplied
+    static_assert(X != X_F32 || RX <= 8, "the planes of a tile");
     static_assert(NT * MT * 1024 <= SLOT, "a wave's sums go where its slot was");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];                // scales (x's, the matrix's), then a slot a wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15, g = lane >> 4;
@@ -44,12 +53,12 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
     }
 
     // the loads of a chunk: per lane the bytes within the rows of x and of a tile's columns
-    const int x_row = X == X_BF16 ? lane >> 5 : lane >> 3;
+    const int x_row = X == X_BF16 ? lane >> 5 : X == X_F32 ? 0 : lane >> 3;
     int vx[LX], px[LX], vc[2];
 #pragma unroll
     for (int i = 0; i < LX; ++i) {
-        const int row = (X == X_BF16 ? i * 2 : i * 8) + x_row;
-        px[i] = X == X_BF16 ? (lane & 31) ^ (row & 7) : (lane & 7) ^ (row & 7);
+        const int row = (X == X_BF16 ? i * 2 : X == X_F32 ? i : i * 8) + x_row;
+        px[i] = X == X_BF16 ? (lane & 31) ^ (row & 7) : X == X_F32 ? lane : (lane & 7) ^ (row & 7);
         vx[i] = row < RX && row < a.M ? row * x.row_bytes + px[i] * 16 : FP4_OUT;
     }
     const int pc = (lane & 7) ^ (lane >> 3);               // (a load is eight rows)
@@ -60,15 +69,15 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
     uintx4_t rsrc_w[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) rsrc_w[p] = fp4_buffer(a.codes + ((long)(silu && p ? wide : 0) + n0) * row_bytes, (unsigned)(cols * row_bytes));
-    const int left = a.blocks - (per - 1) * 8, x_left = x.row_bytes - (per - 1) * (X == X_BF16 ? 512 : 128);      // blocks of the last chunk, bytes of its x
-    const unsigned char* const slot = smem + scale_bytes + wave * SLOT;
+    const int left = a.blocks - (per - 1) * 8, x_left = x.row_bytes - (per - 1) * CHUNK;      // blocks of the last chunk, bytes of its x
+    unsigned char* const slot = smem + scale_bytes + wave * SLOT;
     const unsigned slot_to = lds0 + scale_bytes + wave * SLOT;
 #define ASK(c_)                                                                                                      \
     {                                                                                                                \
         const int plane_ = (c_) / per, k_ = (c_) - plane_ * per, ends_ = k_ == per - 1 ? -1 : 0;                     \
         _Pragma("unroll") for (int i = 0; i < LX; ++i) {                                                             \
             const int not_ = (px[i] * 16 < x_left ? 0 : FP4_OUT) & ends_;                                            \
-            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, plane_ * plane_bytes + k_ * (X == X_BF16 ? 512 : 128), "4", ""); \
+            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, plane_ * plane_bytes + k_ * CHUNK, "4", "");                    \
         }                                                                                                            \
         const int not_ = (pc < left ? 0 : FP4_OUT) & ends_;                                                          \
         _Pragma("unroll") for (int t = 0; t < NT; ++t)                                                               \
@@ -79,31 +88,87 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
                 else QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], k_ * 128, "4", "");       \
             }                                                                                                        \
     }
-    floatx4_t acc[NT][MT];
+    floatx4_t acc[NT][MT], small[NT];                      // (small: of the low and middle planes, added at the end)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+        small[t] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[t][i] = {0.f, 0.f, 0.f, 0.f};
+    }
     if (wave < chunks) ASK(wave)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");           // (the scales are there for all waves, too)
 
     for (int c = wave; c < chunks; c += waves) {
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-        uintx4_t xv[2][MT][X == X_BF16 ? 4 : 1], cv[NT][2];
+        uintx4_t xv[NP][2][MT][X == X_FP4 ? 1 : 4], cv[NT][2];
         int ws[NT][2], xs[2][MT];
+        unsigned char* const planes = slot + Fp4Slot<X, RX, NT>::PLANES_AT;
+        if constexpr (X == X_F32) {
+            // four numbers a lane of every row, none from K on, as three planes of rows as bfloat16 ones would lie
+            const int left_k = a.K - (c % per * 256 + lane * 4);
+            uintx4_t v[RX];
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < RX; ++i) v[i] = *(const uintx4_t*)(slot + i * 1024 + lane * 16);
+            if (c % per == per - 1) {
+#pragma unroll
+                for (int i = 0; i < RX; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e >= left_k) v[i][e] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < RX; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = max(most, v[i][e] & 0x7fffffffu);
+            const bool all_finite = __ballot(most >= 0x7f800000u) == 0;
+#pragma unroll
+            for (int i = 0; i < RX; ++i) {
+                uint32_t h[3][4];                          // (the upper halves count)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[2][e] = v[i][e];
+                    const float r = __uint_as_float(v[i][e]) - __uint_as_float(v[i][e] & 0xffff0000u);
+                    h[1][e] = __float_as_uint(r);
+                    h[0][e] = __float_as_uint(r - __uint_as_float(h[1][e] & 0xffff0000u));
+                }
+                if (!all_finite) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint16_t hi, mid, lo;
+                        cut_in_three(__uint_as_float(v[i][e]), hi, mid, lo);
+                        h[2][e] = (uint32_t)hi << 16;
+                        h[1][e] = (uint32_t)mid << 16;
+                        h[0][e] = (uint32_t)lo << 16;
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    typedef __attribute__((ext_vector_type(2))) uint32_t words;
+                    const words two = {__builtin_amdgcn_perm(h[p][1], h[p][0], 0x07060302u), __builtin_amdgcn_perm(h[p][3], h[p][2], 0x07060302u)};
+                    *(words*)(planes + p * RX * 512 + i * 512 + (((lane >> 1) ^ (i & 7)) * 16) + (lane & 1) * 8) = two;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int b = s * 4 + g, block = min(c % per * 8 + b, a.blocks - 1);      // (beyond the last block codes and x are zero)
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const int xr = (i * 16 + r) & (RX - 1);    // (a row of the tile that x does not have: another one's, and not stored)
-                if constexpr (X == X_BF16) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) xv[s][i][j] = *(const uintx4_t*)(slot + xr * 512 + (((b * 4 + j) ^ (xr & 7)) * 16));
-                } else {
-                    xv[s][i][0] = *(const uintx4_t*)(slot + xr * 128 + ((b ^ (xr & 7)) * 16));
+                if constexpr (X == X_FP4) {
+                    xv[0][s][i][0] = *(const uintx4_t*)(slot + xr * 128 + ((b ^ (xr & 7)) * 16));
                     xs[s][i] = smem[min(xr, a.M - 1) * a.blocks + block];
-                    if (a.K % 32 && c == chunks - 1 && a.K - block * 32 < 32) xv[s][i][0] = first_codes(xv[s][i][0], a.K - block * 32);
+                    if (a.K % 32 && c == chunks - 1 && a.K - block * 32 < 32) xv[0][s][i][0] = first_codes(xv[0][s][i][0], a.K - block * 32);
+                } else {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            xv[p][s][i][j] = *(const uintx4_t*)((X == X_F32 ? planes + p * RX * 512 : slot) + xr * 512 + (((b * 4 + j) ^ (xr & 7)) * 16));
                 }
             }
 #pragma unroll
@@ -121,19 +186,22 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                if constexpr (X == X_BF16) {
+                if constexpr (X != X_FP4) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const bf16x8_t w = fp4_to_bf16(cv[t][s][j], __uint_as_float((uint32_t)ws[t][s] << 23));
 #pragma unroll
+                        for (int p = 0; p < NP - 1; ++p)
+                            small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, xv[p][s][0][j]), w, small[t], 0, 0, 0);
+#pragma unroll
                         for (int i = 0; i < MT; ++i)
-                            acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, xv[s][i][j]), w, acc[t][i], 0, 0, 0);
+                            acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, xv[NP - 1][s][i][j]), w, acc[t][i], 0, 0, 0);
                     }
                 } else {
                     const intx8_t wb = {(int)cv[t][s][0], (int)cv[t][s][1], (int)cv[t][s][2], (int)cv[t][s][3], 0, 0, 0, 0};
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        const uintx4_t& q = xv[s][i][0];
+                        const uintx4_t& q = xv[0][s][i][0];
                         const intx8_t xa = {(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
                         acc[t][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][i], 4, 4, 0, xs[s][i], 0, ws[t][s]);
                     }
@@ -141,6 +209,10 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
             }
     }
 #undef ASK
+    if constexpr (X == X_F32) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][0] += small[t];
+    }
     float* sums = (float*)(smem + scale_bytes);            // of wave w from byte w SLOT on: [NT][MT * 16][16]
     constexpr int APART = SLOT / 4, TILE = MT * 256;
 #pragma unroll
@@ -166,7 +238,7 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
 
 template <int X, int RX, int NT>
 static int fp4_few_launch(const Fp4Args& a, const Fp4Rows& x, int tail, int waves, hipStream_t stream) {
-    constexpr int LX = X == X_BF16 ? RX / 2 : (RX + 7) / 8, SLOT = (LX + 2 * NT) * 1024;
+    constexpr int SLOT = Fp4Slot<X, RX, NT>::BYTES;
     const int scale_bytes = ((X == X_FP4 ? (a.M * a.blocks + 15) / 16 * 16 : 0) + NT * 16 * a.blocks + 15) / 16 * 16;
     const int wide = tail == TAIL_SILU ? a.N / 2 : a.N, cols = tail == TAIL_SILU ? NT * 8 : NT * 16;
     QE_RAISE_SHARED((fp4_few_kernel<X, RX, NT>), 160 * 1024);
@@ -174,14 +246,20 @@ static int fp4_few_launch(const Fp4Args& a, const Fp4Rows& x, int tail, int wave
     return 0;
 }
 
+// Rows of 32-bit numbers that a block cuts into planes by itself, a chunk at a time, with the codes read and converted once for the three (1 row
+// against 24576 x 4096 15.4 us, 3 20.5, by a launch of their own 27.7; against 4096 x 4096 6.0, 7.1 and 10.3).  Of more rows every block has too
+// much to cut (8 33.5 and 26.6, 9.7 and 10.7).
+#define FP4_CUT 4
+
 // Tiles of columns and waves of a block; waves 0: not taken (the scales leave no room in shared memory).
 struct Fp4Few {
     int nt, waves;
 };
 
 static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
-    const int blocks = qe_cdiv(K, 32), chunks = qe_cdiv(blocks, 8) * (x_kind == X_F32 ? 3 : 1);
-    const int rx = M <= 2 ? 2 : M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    const bool cut = x_kind == X_F32 && M <= FP4_CUT;
+    const int blocks = qe_cdiv(K, 32), chunks = qe_cdiv(blocks, 8) * (x_kind == X_F32 && !cut ? 3 : 1);
+    const int rx = M <= 2 ? 2 : cut && M <= 4 ? 4 : M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
     Fp4Few f{};
     // Two tiles where four blocks a unit are left then: every block reads all of x (16 rows against 24576 x 4096 13.2 us, with one tile 14.7; against
     // 4096 x 4096, 128 blocks with two, 6.7 and 5.6; with four tiles 14.9 and more).
@@ -192,7 +270,7 @@ static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
     // two 16.6, three 21.4; 32 against 4096 x 4096 with eight 8.2, four 9.2).
     const int grid = qe_cdiv(tail == TAIL_SILU ? N / 2 : N, tail == TAIL_SILU ? 16 : f.nt * 16);
     const int room = 160 * 1024 - ((x_kind == X_FP4 ? M * blocks : 0) + f.nt * 16 * blocks + 32);
-    const int fit = room / (((x_kind == X_FP4 ? (rx + 7) / 8 : rx / 2) + 2 * f.nt) * 1024);
+    const int fit = room / ((x_kind == X_FP4 ? (rx + 7) / 8 * 1024 : cut ? rx * 2560 : rx * 512) + 2 * f.nt * 1024);
     f.waves = f.nt == 1 || grid <= 256 ? (chunks < 8 ? chunks : 8) : chunks < 8 || rx > 16 ? 2 : 4;
     if (f.waves > fit) f.waves = fit;
     return f;
@@ -207,14 +285,18 @@ bool fp4_few_takes(int M, int N, int K, int x_kind, int tail) {
     return M <= (x_kind == X_FP4 ? 64 : x_kind == X_F32 ? 16 : 32) && K < (1 << 20) && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
 }
 
-long fp4_few_workspace(const void* x, int M, int K, int x_kind) { return as_it_is(x, K, x_kind) ? 0 : fp4_planes_bytes(M, K, x_kind); }
+long fp4_few_workspace(const void* x, int M, int K, int x_kind) {
+    return as_it_is(x, K, x_kind) || (x_kind == X_F32 && M <= FP4_CUT) ? 0 : fp4_planes_bytes(M, K, x_kind);
+}
 
 int fp4_few(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t stream) {
     const Fp4Few f = fp4_few_shape(a.M, a.N, a.K, x_kind, tail);
-    Fp4Rows x{a.x, x_kind == X_FP4 ? a.blocks * 16 : a.K * 2, 1};
-    if (!as_it_is(a.x, a.K, x_kind)) x = fp4_copies(a.x, a.M, a.K, x_kind, workspace, nullptr, 0, nullptr, stream);
+    const bool cut = x_kind == X_F32 && a.M <= FP4_CUT;
+    Fp4Rows x{a.x, x_kind == X_FP4 ? a.blocks * 16 : cut ? a.K * 4 : a.K * 2, 1};
+    if (!cut && !as_it_is(a.x, a.K, x_kind)) x = fp4_copies(a.x, a.M, a.K, x_kind, workspace, nullptr, 0, nullptr, stream);
 #define QE_NT(X_, RX_) (f.nt == 1 ? fp4_few_launch<X_, RX_, 1>(a, x, tail, f.waves, stream) : fp4_few_launch<X_, RX_, 2>(a, x, tail, f.waves, stream))
 #define QE_RX(X_) (a.M <= 2 ? QE_NT(X_, 2) : a.M <= 8 ? QE_NT(X_, 8) : a.M <= 16 ? QE_NT(X_, 16) : QE_NT(X_, 32))
+    if (cut) return a.M <= 2 ? QE_NT(X_F32, 2) : QE_NT(X_F32, 4);
     if (x_kind != X_FP4) return QE_RX(X_BF16);
     return a.M > 32 ? QE_NT(X_FP4, 64) : QE_RX(X_FP4);
 #undef QE_RX

@@ -213,6 +213,29 @@ def test_float32_rows_lose_nothing(ops):
     assert ((got - x.double() @ v.T).abs() <= sums_bound(9, x.double().abs() @ v.abs().T)).all()
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8])
+@pytest.mark.parametrize("K", [1, 3, 255, 257, 1023, 2570, 4096])
+def test_few_float32_rows(ops, M, K):
+    """Rows of any length from any number of an allocation on, NaN on both sides of them and infinities inside: nothing of a neighbour's joins,
+    the lowest bits count, and a row's infinity stays its own."""
+    N = 130
+    w_raw = torch.randn(N, K, generator=gen(K)).abs() + 0.5                # (no zeros: infinity stays infinity)
+    w = ops.mxfp4_quantize(w_raw.to(DEV))
+    v = values_of(*codes_of(w_raw), K)
+    x = torch.randn(M, K, generator=gen(M)) * torch.exp2(torch.randint(-30, 31, (M, K), generator=gen(M + 1)).float())
+    for before in (0, 1, 2, 3):
+        room = torch.full((M * K + 16,), math.nan, device=DEV)
+        room[before:before + M * K] = x.to(DEV).view(-1)
+        got = ops.gemm_mxfp4(room[before:before + M * K].view(M, K), w).cpu().double()
+        assert ((got - x.double() @ v.T).abs() <= sums_bound(3 * K, x.double().abs() @ v.abs().T)).all()
+    x[M // 2, K // 2] = math.inf
+    got = ops.gemm_mxfp4(x.to(DEV), w).cpu()
+    assert (got[M // 2] == math.inf).all()
+    others = [m for m in range(M) if m != M // 2]
+    want = x[others].double() @ v.T
+    assert ((got[others].double() - want).abs() <= sums_bound(3 * K, x[others].double().abs() @ v.abs().T)).all()
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
 def test_nan_and_infinities(ops, kind):
     """A NaN block of the matrix spoils its own output column and no other; a row with a NaN or an infinity its own row."""
