@@ -150,7 +150,7 @@ static int fp4_rows(const Fp4Args& a, int tail, hipStream_t stream) {
 enum { BY_FEW, BY_TILES, BY_ROWS };
 static int fp4_way(int M, int N, int K, int x_kind, int tail) {
     if (fp4_few_takes(M, N, K, x_kind, tail)) return BY_FEW;
-    return M > 16 && (x_kind == X_FP4 ? fp4_both_take(M, N, K) : fp4_tiles_take(M, N, K, x_kind)) ? BY_TILES : BY_ROWS;
+    return M > (x_kind == X_F32 ? 8 : 16) && (x_kind == X_FP4 ? fp4_both_take(M, N, K) : fp4_tiles_take(M, N, K, x_kind)) ? BY_TILES : BY_ROWS;
 }
 
 // Bytes of workspace that qe_gemm_mxfp4 needs for these operands.

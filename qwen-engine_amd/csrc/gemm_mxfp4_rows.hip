@@ -1,6 +1,6 @@
-// Products of few rows (up to 32, of 32 bits 16, in 4 bits 64) with a 4-bit matrix (see mxfp4.h): bound by the matrix's bytes on their way from memory.
+// Products of few rows (up to 32, of 32 bits 8 or 16, in 4 bits 64) with a 4-bit matrix (see mxfp4.h): bound by the matrix's bytes on their way from memory.
 // Rows of bfloat16 lie at whole 16-byte pieces.  Up to four rows of 32-bit numbers are cut into three planes of bfloat16 where they are multiplied;
-// of more the planes come from memory, one behind the other, and K is walked three times.
+// of more the planes come from memory.  Either way the codes are read and converted once for the three.
 //
 // A block takes NT tiles of 16 columns, its waves chunks of 256 of K in turn, each wave by itself: it asks for a chunk of the codes (128
 // bytes of a row, a line) and of x straight to its own piece of shared memory, and multiplies it when it has come.  The scales of
@@ -14,25 +14,27 @@
 // other rows, and a load of 64 places of 64 lines takes four times the cycles of one of eight lines.
 #include "mxfp4.h"
 
+enum { X_PLANES = 3 };             // 32-bit rows as planes
+
 // A wave's piece of shared memory: a chunk's loads of x (LX, 1 KB each: two rows of bfloat16, a row of 32-bit numbers, eight in 4 bits), of codes (2
 // a tile), and the planes that are made of 32-bit rows.
 template <int X, int RX, int NT> struct Fp4Slot {
-    static constexpr int LX = X == X_BF16 ? RX / 2 : X == X_F32 ? RX : (RX + 7) / 8;
+    static constexpr int LX = X == X_BF16 ? RX / 2 : X == X_PLANES ? 3 * RX / 2 : X == X_F32 ? RX : (RX + 7) / 8;
     static constexpr int PLANES_AT = (LX + 2 * NT) * 1024, BYTES = PLANES_AT + (X == X_F32 ? 3 * RX * 512 : 0);
 };
 
 template <int X, int RX, int NT>
 __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int tail, int scale_bytes) {
     constexpr int MT = (RX + 15) / 16, LX = Fp4Slot<X, RX, NT>::LX, SLOT = Fp4Slot<X, RX, NT>::BYTES;        // (MT: tiles of 16 rows)
-    constexpr int CHUNK = X == X_BF16 ? 512 : X == X_F32 ? 1024 : 128, NP = X == X_F32 ? 3 : 1;             // bytes of a row of x in a chunk; planes that are multiplied
-    static_assert(X != X_F32 || RX <= 8, "the planes of a tile");
+    constexpr int CHUNK = X == X_FP4 ? 128 : X == X_F32 ? 1024 : 512, NP = X == X_F32 || X == X_PLANES ? 3 : 1;      // bytes of a row of x in a chunk; planes that are multiplied
+    static_assert(NP == 1 || RX <= 16, "the planes of a tile");
     static_assert(NT * MT * 1024 <= SLOT, "a wave's sums go where its slot was");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];                // scales (x's, the matrix's), then a slot a wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15, g = lane >> 4;
     const bool silu = tail == TAIL_SILU;
     const int wide = silu ? a.N / 2 : a.N, halves = silu ? 2 : 1, tiles = NT / halves;  // tiles of columns that are stored
     const int n0 = blockIdx.x * tiles * 16, cols = min(tiles * 16, wide - n0);
-    const int row_bytes = a.blocks * 16, per = (a.blocks + 7) / 8, chunks = per * x.planes;       // chunks of a row, of all its planes
+    const int row_bytes = a.blocks * 16, chunks = (a.blocks + 7) / 8;
     const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
 
     // The scales: of x (in 4 bits), of the columns (silu: of the gates, of the ups).  Where a part is whole pieces of 16 bytes it is copied by
@@ -53,39 +55,38 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
     }
 
     // the loads of a chunk: per lane the bytes within the rows of x and of a tile's columns
-    const int x_row = X == X_BF16 ? lane >> 5 : X == X_F32 ? 0 : lane >> 3;
+    const int x_row = X == X_FP4 ? lane >> 3 : X == X_F32 ? 0 : lane >> 5, plane_bytes = a.M * x.row_bytes;
     int vx[LX], px[LX], vc[2];
 #pragma unroll
     for (int i = 0; i < LX; ++i) {
-        const int row = (X == X_BF16 ? i * 2 : X == X_F32 ? i : i * 8) + x_row;
-        px[i] = X == X_BF16 ? (lane & 31) ^ (row & 7) : X == X_F32 ? lane : (lane & 7) ^ (row & 7);
-        vx[i] = row < RX && row < a.M ? row * x.row_bytes + px[i] * 16 : FP4_OUT;
+        const int row = (X == X_BF16 ? i * 2 : X == X_PLANES ? i % (RX / 2) * 2 : X == X_F32 ? i : i * 8) + x_row, plane = X == X_PLANES ? i / (RX / 2) : 0;
+        px[i] = X == X_FP4 ? (lane & 7) ^ (row & 7) : X == X_F32 ? lane : (lane & 31) ^ (row & 7);
+        vx[i] = row < RX && row < a.M ? plane * plane_bytes + row * x.row_bytes + px[i] * 16 : FP4_OUT;
     }
     const int pc = (lane & 7) ^ (lane >> 3);               // (a load is eight rows)
 #pragma unroll
     for (int i = 0; i < 2; ++i) vc[i] = (i * 8 + (lane >> 3)) * row_bytes + pc * 16;
-    const int plane_bytes = a.M * x.row_bytes;
     const uintx4_t rsrc_x = fp4_buffer(x.data, (unsigned)(plane_bytes * x.planes));
     uintx4_t rsrc_w[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) rsrc_w[p] = fp4_buffer(a.codes + ((long)(silu && p ? wide : 0) + n0) * row_bytes, (unsigned)(cols * row_bytes));
-    const int left = a.blocks - (per - 1) * 8, x_left = x.row_bytes - (per - 1) * CHUNK;      // blocks of the last chunk, bytes of its x
+    const int left = a.blocks - (chunks - 1) * 8, x_left = x.row_bytes - (chunks - 1) * CHUNK;      // blocks of the last chunk, bytes of its x
     unsigned char* const slot = smem + scale_bytes + wave * SLOT;
     const unsigned slot_to = lds0 + scale_bytes + wave * SLOT;
 #define ASK(c_)                                                                                                      \
     {                                                                                                                \
-        const int plane_ = (c_) / per, k_ = (c_) - plane_ * per, ends_ = k_ == per - 1 ? -1 : 0;                     \
+        const int ends_ = (c_) == chunks - 1 ? -1 : 0;                                                               \
         _Pragma("unroll") for (int i = 0; i < LX; ++i) {                                                             \
             const int not_ = (px[i] * 16 < x_left ? 0 : FP4_OUT) & ends_;                                            \
-            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, plane_ * plane_bytes + k_ * CHUNK, "4", "");                    \
+            QE_LOAD_TO_SHARED(slot_to + i * 1024, vx[i] | not_, rsrc_x, (c_) * CHUNK, "4", "");                      \
         }                                                                                                            \
         const int not_ = (pc < left ? 0 : FP4_OUT) & ends_;                                                          \
         _Pragma("unroll") for (int t = 0; t < NT; ++t)                                                               \
             _Pragma("unroll") for (int i = 0; i < 2; ++i) {                                                          \
                 const int in_ = silu ? t % (NT > 1 ? NT / 2 : 1) : t;        /* the tile within its half */          \
                 const int v_ = (vc[i] + in_ * 16 * row_bytes) | not_;                                                \
-                if (silu && t >= NT / 2) { QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[1], k_ * 128, "4", ""); } \
-                else QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], k_ * 128, "4", "");       \
+                if (silu && t >= NT / 2) { QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[1], (c_) * 128, "4", ""); } \
+                else QE_LOAD_TO_SHARED(slot_to + (LX + t * 2 + i) * 1024, v_, rsrc_w[0], (c_) * 128, "4", "");     \
             }                                                                                                        \
     }
     floatx4_t acc[NT][MT], small[NT];                      // (small: of the low and middle planes, added at the end)
@@ -105,12 +106,12 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
         unsigned char* const planes = slot + Fp4Slot<X, RX, NT>::PLANES_AT;
         if constexpr (X == X_F32) {
             // four numbers a lane of every row, none from K on, as three planes of rows as bfloat16 ones would lie
-            const int left_k = a.K - (c % per * 256 + lane * 4);
+            const int left_k = a.K - (c * 256 + lane * 4);
             uintx4_t v[RX];
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < RX; ++i) v[i] = *(const uintx4_t*)(slot + i * 1024 + lane * 16);
-            if (c % per == per - 1) {
+            if (c == chunks - 1) {
 #pragma unroll
                 for (int i = 0; i < RX; ++i)
 #pragma unroll
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int b = s * 4 + g, block = min(c % per * 8 + b, a.blocks - 1);      // (beyond the last block codes and x are zero)
+            const int b = s * 4 + g, block = min(c * 8 + b, a.blocks - 1);      // (beyond the last block codes and x are zero)
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const int xr = (i * 16 + r) & (RX - 1);    // (a row of the tile that x does not have: another one's, and not stored)
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
                     for (int p = 0; p < NP; ++p)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            xv[p][s][i][j] = *(const uintx4_t*)((X == X_F32 ? planes + p * RX * 512 : slot) + xr * 512 + (((b * 4 + j) ^ (xr & 7)) * 16));
+                            xv[p][s][i][j] = *(const uintx4_t*)((X == X_F32 ? planes : slot) + p * RX * 512 + xr * 512 + (((b * 4 + j) ^ (xr & 7)) * 16));
                 }
             }
 #pragma unroll
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
             }
     }
 #undef ASK
-    if constexpr (X == X_F32) {
+    if constexpr (NP == 3) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][0] += small[t];
     }
@@ -258,7 +259,7 @@ struct Fp4Few {
 
 static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
     const bool cut = x_kind == X_F32 && M <= FP4_CUT;
-    const int blocks = qe_cdiv(K, 32), chunks = qe_cdiv(blocks, 8) * (x_kind == X_F32 && !cut ? 3 : 1);
+    const int blocks = qe_cdiv(K, 32), chunks = qe_cdiv(blocks, 8);
     const int rx = M <= 2 ? 2 : cut && M <= 4 ? 4 : M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
     Fp4Few f{};
     // Two tiles where four blocks a unit are left then: every block reads all of x (16 rows against 24576 x 4096 13.2 us, with one tile 14.7; against
@@ -270,7 +271,7 @@ static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
     // two 16.6, three 21.4; 32 against 4096 x 4096 with eight 8.2, four 9.2).
     const int grid = qe_cdiv(tail == TAIL_SILU ? N / 2 : N, tail == TAIL_SILU ? 16 : f.nt * 16);
     const int room = 160 * 1024 - ((x_kind == X_FP4 ? M * blocks : 0) + f.nt * 16 * blocks + 32);
-    const int fit = room / ((x_kind == X_FP4 ? (rx + 7) / 8 * 1024 : cut ? rx * 2560 : rx * 512) + 2 * f.nt * 1024);
+    const int fit = room / ((x_kind == X_FP4 ? (rx + 7) / 8 * 1024 : cut ? rx * 2560 : x_kind == X_F32 ? rx * 1536 : rx * 512) + 2 * f.nt * 1024);
     f.waves = f.nt == 1 || grid <= 256 ? (chunks < 8 ? chunks : 8) : chunks < 8 || rx > 16 ? 2 : 4;
     if (f.waves > fit) f.waves = fit;
     return f;
@@ -279,10 +280,10 @@ static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
 // Rows that the loads take as they are: of bfloat16, at whole 16-byte pieces.
 static bool as_it_is(const void* x, int K, int x_kind) { return x_kind == X_FP4 || (x_kind == X_BF16 && K % 8 == 0 && ((uintptr_t)x & 15) == 0); }
 
-// (Of 32 bits, whose planes are walked one after the other, 16 rows: 8 against 24576 x 4096 26.6 us, by tiles 27.6, against 4096 x 4096 10.7 and 14.6;
-// 16 30.9, 28.6 and 13.1, 15.8; 24 41.5, 28.8 and 17.3, 16.3.)
+// (Of 32 bits 8 rows, or 16 against narrow matrices: 8 against 24576 x 4096 23.7 us, by tiles 27.6, against 4096 x 4096 10.1 and 14.6; 16 34.2, 28.6 and
+// 12.6, 15.8, against 151936 x 1024 59 and 44; 24, when K was walked three times, 41.5, 28.8 and 17.3, 16.3.)
 bool fp4_few_takes(int M, int N, int K, int x_kind, int tail) {
-    return M <= (x_kind == X_FP4 ? 64 : x_kind == X_F32 ? 16 : 32) && K < (1 << 20) && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
+    return M <= (x_kind == X_FP4 ? 64 : x_kind == X_BF16 ? 32 : N < 16384 ? 16 : 8) && K < (1 << 20) && fp4_few_shape(M, N, K, x_kind, tail).waves > 0;
 }
 
 long fp4_few_workspace(const void* x, int M, int K, int x_kind) {
@@ -297,7 +298,8 @@ int fp4_few(const Fp4Args& a, int x_kind, int tail, void* workspace, hipStream_t
 #define QE_NT(X_, RX_) (f.nt == 1 ? fp4_few_launch<X_, RX_, 1>(a, x, tail, f.waves, stream) : fp4_few_launch<X_, RX_, 2>(a, x, tail, f.waves, stream))
 #define QE_RX(X_) (a.M <= 2 ? QE_NT(X_, 2) : a.M <= 8 ? QE_NT(X_, 8) : a.M <= 16 ? QE_NT(X_, 16) : QE_NT(X_, 32))
     if (cut) return a.M <= 2 ? QE_NT(X_F32, 2) : QE_NT(X_F32, 4);
-    if (x_kind != X_FP4) return QE_RX(X_BF16);
+    if (x_kind == X_F32) return a.M <= 8 ? QE_NT(X_PLANES, 8) : QE_NT(X_PLANES, 16);
+    if (x_kind == X_BF16) return QE_RX(X_BF16);
     return a.M > 32 ? QE_NT(X_FP4, 64) : QE_RX(X_FP4);
 #undef QE_RX
 #undef QE_NT

@@ -213,12 +213,11 @@ def test_float32_rows_lose_nothing(ops):
     assert ((got - x.double() @ v.T).abs() <= sums_bound(9, x.double().abs() @ v.abs().T)).all()
 
 
-@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8])
-@pytest.mark.parametrize("K", [1, 3, 255, 257, 1023, 2570, 4096])
-def test_few_float32_rows(ops, M, K):
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("N,K", [(130, 1), (130, 3), (130, 255), (130, 257), (16390, 257), (130, 1023), (16390, 2570), (130, 4096)])
+def test_few_float32_rows(ops, M, N, K):
     """Rows of any length from any number of an allocation on, NaN on both sides of them and infinities inside: nothing of a neighbour's joins,
     the lowest bits count, and a row's infinity stays its own."""
-    N = 130
     w_raw = torch.randn(N, K, generator=gen(K)).abs() + 0.5                # (no zeros: infinity stays infinity)
     w = ops.mxfp4_quantize(w_raw.to(DEV))
     v = values_of(*codes_of(w_raw), K)
