@@ -2454,7 +2454,7 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
         _need(out, "out", out_dtype, (M, wide), dev)
         _apart(out, (data, scales, w.codes, w.scales, bias), "gemm_mxfp4")
     at, ws_at, scales_at, nbytes = data.data_ptr(), None, None if scales is None else scales.data_ptr(), 0
-    if M > 4 if kind == 1 else M > 16 or K % 8 or at % 16:         # (else none is needed: a call that is not made, 0.7 us)
+    if M > 4 if kind == 1 else M > 16 or kind == 0 and (K % 2 or at % 4):         # (else none is needed: a call that is not made, 0.7 us)
         nbytes = lib.qe_gemm_mxfp4_workspace_bytes(at, scales_at, w.scales.data_ptr(), M, N, K, kind, tail)
         if nbytes:
             ws = data.new_empty((nbytes,), dtype=torch.uint8)

@@ -235,6 +235,27 @@ def test_few_float32_rows(ops, M, N, K):
     assert ((got[others].double() - want).abs() <= sums_bound(3 * K, x[others].double().abs() @ v.abs().T)).all()
 
 
+@pytest.mark.parametrize("M", [1, 2, 7, 16, 17, 32])
+@pytest.mark.parametrize("N,K", [(130, 2), (130, 6), (130, 31), (130, 254), (130, 258), (16390, 260), (130, 1022), (16390, 2566), (130, 4100)])
+def test_few_bfloat16_rows(ops, M, N, K):
+    """Rows whose last 16 bytes go on in the next row, from any number of an allocation on, NaN on both sides of them; a row of NaN stays alone."""
+    w_raw = torch.randn(N, K, generator=gen(K))
+    w = ops.mxfp4_quantize(w_raw.to(DEV))
+    w.codes[:, (K + 1) // 2:] = 0x77                               # (behind the columns: sixes)
+    v = values_of(*codes_of(w_raw), K).to(DEV)
+    x = torch.randn(M, K, generator=gen(M)).to(torch.bfloat16)
+    if M > 2:
+        x[1::3] = math.nan
+    want = x.to(DEV).double() @ v.T
+    bound = sums_bound(K, x.to(DEV).double().abs() @ v.abs().T)
+    for before in (0, 1, 2, 4, 7):
+        room = torch.full((M * K + 16,), math.nan, dtype=torch.bfloat16, device=DEV)
+        room[before:before + M * K] = x.to(DEV).view(-1)
+        got = ops.gemm_mxfp4(room[before:before + M * K].view(M, K), w, out_dtype=torch.float32).double()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert ((got - want).nan_to_num().abs() <= bound.nan_to_num()).all()
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
 def test_nan_and_infinities(ops, kind):
     """A NaN block of the matrix spoils its own output column and no other; a row with a NaN or an infinity its own row."""
