@@ -203,7 +203,8 @@ __device__ __forceinline__ void verify_wave_top(float& top, int& at) {
     at = __builtin_amdgcn_readlane(at, 63);
 }
 
-// One block a span of a row: blockIdx.y counts the rows of the logits, then those of the drafts' logits.
+// One block a span of a row: blockIdx.y counts the rows of the logits, then those of the drafts' logits.  done[R]: whether first[] fails to rise
+// somewhere, which misleads the search for a row's request; verify_accept sees to that.
 __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyPart* parts, unsigned* done) {
     __shared__ float tops[4];
     __shared__ int ats[4];
@@ -216,14 +217,21 @@ __global__ __launch_bounds__(256) void verify_spans_kernel(VerifyArgs a, VerifyP
     verify_load<EACH>((is_guess ? a.guess : a.logits) + (long)i * a.V, c0 + lane * 4, a.V, a.four && c0 + VERIFY_PIECE <= a.V, v);      // (on its way while the request is looked up)
     // (after the loads of what the host gives: behind a store they would not be scalar ones, 10 us for 64 requests)
     auto clear = [&] {
-        if (blockIdx.x == 0 && blockIdx.y == 0)
+        if (blockIdx.x == 0 && blockIdx.y == 0) {
             for (int r = threadIdx.x; r < a.R; r += 256) done[r] = 0;
+            if (wave == 0) {
+                bool falls = false;
+                for (int r = lane; r < a.R; r += 64) falls |= a.first[r + 1] <= a.first[r];
+                const unsigned any = __ballot(falls) != 0;
+                if (lane == 0) done[a.R] = any;
+            }
+        }
     };
     // the request: the number of first[1 .. R] (less their index, for the drafts) that are not beyond i
     int low = 0, high = a.R;
     while (low < high) {
         const int mid = (low + high) / 2;
-        if (a.first[mid + 1] - (is_guess ? mid + 1 : 0) <= i) low = mid + 1; else high = mid;
+        if ((int)((unsigned)a.first[mid + 1] - (is_guess ? mid + 1 : 0)) <= i) low = mid + 1; else high = mid;
     }
     if (low >= a.R) return clear();
     const float t = a.temperature[low];
@@ -290,19 +298,55 @@ __device__ __forceinline__ void verify_join(const VerifyPart* parts, const Verif
     sum = verify_wave_sum(sum);
 }
 
+// The parts of request r's rows once more, where first[] falls: those that are there may be another temperature's, or none at all.  By a block of 16
+// waves, a wave a span.  (In the launch that accepts in every block, a request's blocks all write the same.)
+__device__ __forceinline__ void verify_redo(const VerifyArgs& a, VerifyPart* parts, int r, int lo, int n) {
+    const int lane = threadIdx.x & 63;
+    const float t = a.temperature[r];
+    const bool greedy = verify_greedy(t);
+    const VerifyScale k(t);
+    const int rows = n + 1 + (a.guess && !greedy ? n : 0);
+    for (int i = threadIdx.x >> 6; i < rows * a.spans; i += 16) {
+        const int row = i / a.spans, c0 = i % a.spans * VERIFY_SPAN;
+        const bool is_guess = row > n;
+        const int at_row = is_guess ? lo - r + row - (n + 1) : lo + row;
+        const float* z = (is_guess ? a.guess : a.logits) + (long)at_row * a.V;
+        VerifyPart part = {{0.0, 0.0, 0.0, 0.0}, -INFINITY, 0x7fffffff};
+        for (int c = c0 + lane; c < min(c0 + VERIFY_SPAN, a.V); c += 64)
+            if (z[c] > part.top) { part.top = z[c]; part.at = c; }
+        verify_wave_top(part.top, part.at);
+        for (int q = 0; q < 4 && !greedy; ++q) {
+            double sum = 0.0;
+            const int from = c0 + q * VERIFY_PIECE;
+            for (int c = from + lane; c < min(from + VERIFY_PIECE, a.V); c += 64) sum += verify_weight(z[c], part.top, k);
+            part.sums[q] = verify_wave_sum(sum);
+        }
+        if (lane == 0) parts[(long)((is_guess ? a.rows : 0) + at_row) * a.spans + i % a.spans] = part;
+    }
+    __syncthreads();
+}
+
 // Which drafts of request r are accepted, and what its token is drawn from: by a block of 16 waves, a wave a draft, 16 at a time.  accepted: how
-// many (-1: there are no such rows); token: the one behind them, of a request without temperature.
-__device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, const VerifyPart* parts, int r, int& accepted, int& token) {
+// many (-1: there are no such rows, or they or its drafts are not behind those of all requests before); token: the one behind them, of a request
+// without temperature.  falls: whether first[] does so somewhere.
+__device__ __forceinline__ VerifyChoice verify_accept(const VerifyArgs& a, VerifyPart* parts, unsigned falls, int r, int& accepted, int& token) {
     __shared__ VerifyChoice tries[16];
     __shared__ int tokens[16], stops[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo, hi;
-    if (!verify_rows(a, r, lo, hi)) {
+    bool there = verify_rows(a, r, lo, hi);
+    const float t = a.temperature[r];
+    if (falls) {                                   // (first[k] - k: where request k's drafts begin; where none is beyond lo - r no first[k] is beyond lo)
+        bool behind = true;
+        for (int k = threadIdx.x; k < r; k += 1024) behind &= (long)a.first[k] - k <= (long)lo - r;
+        there = __syncthreads_and(behind) && there;
+        if (there) verify_redo(a, parts, r, lo, hi - lo - 1);
+    }
+    if (!there) {
         VerifyChoice none{};
         none.row = accepted = token = -1;
         return none;
     }
-    const float t = a.temperature[r];
     const bool greedy = verify_greedy(t);
     const VerifyScale k(t);
     const int n = hi - lo - 1;
@@ -364,9 +408,9 @@ __device__ __forceinline__ void verify_write(const VerifyArgs& a, VerifyChoice* 
         if (lo + i != c.row) a.tokens[lo + i] = i < accepted ? a.drafts[lo - r + i] : greedy && i == accepted ? token : -1;
 }
 
-__global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices) {
+__global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a, VerifyPart* parts, VerifyChoice* choices, const unsigned* done) {
     int accepted, token;
-    const VerifyChoice c = verify_accept(a, parts, blockIdx.x, accepted, token);
+    const VerifyChoice c = verify_accept(a, parts, done[a.R], blockIdx.x, accepted, token);
     verify_write(a, choices, blockIdx.x, c, accepted, token);
 }
 
@@ -538,14 +582,14 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a, const Ve
 // The sums of the weights of pieces, four numbers a thread, 256 threads a piece.  ACCEPT: the block finds the choice for itself, with its 16
 // waves, and has a whole span; the request's last block to be done (`done` counts them; it waits for nothing) draws.  Else one piece.
 template <bool ACCEPT>
-__global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(VerifyArgs a, const VerifyPart* parts, VerifyChoice* choices, double* rests, unsigned* done) {
+__global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(VerifyArgs a, VerifyPart* parts, VerifyChoice* choices, double* rests, unsigned* done) {
     constexpr int EACH = VERIFY_PIECE / 256, HERE = ACCEPT ? 4 : 1;
     __shared__ double shared[4 * HERE];
     __shared__ bool is_last;
     const int r = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), piece = blockIdx.x * HERE + wave / 4;
     VerifyChoice c;
     int accepted = -1, token = -1;
-    if constexpr (ACCEPT) c = verify_accept(a, parts, r, accepted, token);
+    if constexpr (ACCEPT) c = verify_accept(a, parts, done[a.R], r, accepted, token);
     else c = choices[r];
     if (c.row < 0) {
         if (ACCEPT && blockIdx.x == 0) verify_write(a, choices, r, c, accepted, token);
@@ -585,12 +629,12 @@ __global__ __launch_bounds__(ACCEPT ? 1024 : 256) void verify_rest_kernel(Verify
 
 extern "C" long qe_verify_drafts_workspace_bytes(int rows, int V, int R, int has_guess) {
     const long spans = qe_cdiv(V, VERIFY_SPAN), all = rows + (has_guess ? rows - R : 0);
-    return all * spans * (long)sizeof(VerifyPart) + (long)R * (long)sizeof(VerifyChoice) + (long)R * (qe_cdiv(V, VERIFY_PIECE) * 8L + 4);
+    return all * spans * (long)sizeof(VerifyPart) + (long)R * (long)sizeof(VerifyChoice) + (long)R * (qe_cdiv(V, VERIFY_PIECE) * 8L + 4) + 4;
 }
 
 // logits float32 [rows, V], first int32 [R + 1], drafts int32 [rows - R], guess float32 [rows - R, V] or null, temperature and draw float32 [R],
 // accept float32 [rows - R] -> tokens int32 [rows] (accepted drafts, the token drawn, -1), accepted int32 [R] (-1: first[] names no
-// rows that there are; nothing of the request is written then).
+// rows that there are, or none behind those of all requests before; nothing of the request is written then).
 extern "C" int qe_verify_drafts(const float* logits, const int* first, const int* drafts, const float* guess, const float* temperature,
                                 const float* accept, const float* draw, int* tokens, int* accepted, int rows, int V, int R,
                                 void* workspace, long workspace_bytes, hipStream_t stream) {
@@ -603,7 +647,7 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     VerifyPart* parts = (VerifyPart*)workspace;
     VerifyChoice* choices = (VerifyChoice*)(parts + (long)all * spans);
     double* rests = (double*)(choices + R);
-    unsigned* done = (unsigned*)(rests + (long)R * pieces);      // how many blocks of a request are done
+    unsigned* done = (unsigned*)(rests + (long)R * pieces);      // how many blocks of a request are done, then whether first[] falls
     const int four = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)guess) & 15) == 0;
     const VerifyArgs a{logits, guess, first, drafts, temperature, accept, draw, tokens, accepted, rows, V, R, spans, pieces, four};
     verify_spans_kernel<<<dim3(spans, all), 256, 0, stream>>>(a, parts, done);
@@ -612,7 +656,7 @@ extern "C" int qe_verify_drafts(const float* logits, const int* first, const int
     if ((long)spans * R <= 320) {
         verify_rest_kernel<true><<<dim3(spans, R), 1024, 0, stream>>>(a, parts, choices, rests, done);
     } else {
-        verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices);
+        verify_accept_kernel<<<R, 1024, 0, stream>>>(a, parts, choices, done);
         verify_rest_kernel<false><<<dim3(pieces, R), 256, 0, stream>>>(a, parts, choices, rests, done);
         verify_draw_kernel<<<R, 256, 0, stream>>>(a, parts, choices, rests);
     }

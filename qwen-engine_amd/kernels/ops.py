@@ -2480,7 +2480,8 @@ def verify_drafts(logits: torch.Tensor, first: torch.Tensor, drafts: torch.Tenso
 
     tokens holds, at the request's rows, the accepted drafts, the token, and -1 behind; rows of no request are not written.
     Logits of -infinity and NaN weigh nothing; a row where nothing weighs gives the token -1.  A draft outside the vocabulary is
-    not accepted.  accepted[r] is -1 where first[] names rows that there are not."""
+    not accepted.  accepted[r] is -1, and nothing of the request written, where first[] names rows that there are not, or where it
+    does not rise: rows or drafts that are not behind those of all requests before."""
     lib = load_library()
     _need(logits, "logits", torch.float32, (None, None))
     rows, V = logits.shape

@@ -265,6 +265,45 @@ def test_rows_of_no_request_and_bad_rows(ops):
             assert got == [-1, -1, -1] and (tokens == 99).all()
 
 
+@pytest.mark.parametrize("R,V", [(6, 600), (6, 200003), (400, 300), (1300, 40)])
+@pytest.mark.parametrize("lookup", [False, True])
+def test_first_rows_that_fall(ops, R, V, lookup):
+    """first[] that falls or stands still somewhere: a request whose rows, or whose drafts' rows, are not behind all earlier ones' is marked
+    and nothing of it written; every other one gets the tokens that its own rows and temperature give, in one launch and in several."""
+    g = np.random.default_rng(R + V)
+    counts = [int(v) for v in g.integers(0, 4, R)]
+    c = case(counts, V, R, lookup=lookup, greedy_every=2)
+    n = lambda v: None if v is None else v.numpy()
+    z, d, q, t, a, u = (n(c[k]) for k in ("logits", "drafts", "guess", "temperature", "accept", "draw"))
+    rows, starts = len(z), first_of(counts).tolist()
+    lists = [[0, 3, 2] + starts[3:], starts[:3] + [starts[2]] + starts[4:], starts[:-1] + [starts[-3]]]
+    for _ in range(4):
+        bad = list(starts)
+        for k in g.integers(0, R + 1, max(1, R // 100)):
+            bad[k] = int(g.integers(-2, rows + 3))
+        lists.append(bad)
+    marked = served = 0
+    for first in lists:
+        tokens = torch.full((rows,), 99, dtype=torch.int32, device=DEV)
+        up = lambda v: None if v is None else v.to(DEV)
+        tokens, accepted = ops.verify_drafts(up(c["logits"]), torch.tensor(first, dtype=torch.int32, device=DEV), up(c["drafts"]), up(c["guess"]),
+                                             up(c["temperature"]), up(c["accept"]), up(c["draw"]), tokens=tokens)
+        want, kept = [99] * rows, []
+        for r, (lo, hi) in enumerate(zip(first, first[1:])):
+            if not (hi > lo >= r and hi <= rows and hi - 1 - r <= rows - R and all(first[k] - k <= lo - r for k in range(r))):
+                kept.append(-1)
+                continue
+            m = hi - lo - 1
+            here = slice(lo - r, lo - r + m)
+            got = plain(z[lo:hi], [m], d[here], None if q is None else q[here], t[r:r + 1], a[here], u[r:r + 1])
+            want[lo:hi] = got[0]
+            kept += got[1]
+        marked, served = marked + kept.count(-1), served + len(kept) - kept.count(-1)
+        assert accepted.tolist() == kept, first[:8]
+        assert tokens.tolist() == want, first[:8]
+    assert marked and served
+
+
 def test_no_requests(ops):
     e = lambda *s, dtype=torch.float32: torch.empty(*s, dtype=dtype, device=DEV)
     tokens, accepted = ops.verify_drafts(e(0, 50), torch.zeros(1, dtype=torch.int32, device=DEV), e(0, dtype=torch.int32), None, e(0), e(0), e(0))
