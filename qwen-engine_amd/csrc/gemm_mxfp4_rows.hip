@@ -181,15 +181,17 @@ __global__ __launch_bounds__(512) void fp4_few_kernel(Fp4Args a, Fp4Rows x, int 
             }
         }
         if (X == X_BF16 && a.K % 8 && c == chunks - 1) {       // (the row's last piece goes on in the next row)
+            int words_left = (a.K - c * 256 + 1) / 2 - g * 16;     // (kept from the compiler: else all comparisons go in front of the loop and their results to spilled registers)
+            asm volatile("" : "+v"(words_left));
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int j = 0; j < (X == X_FP4 ? 1 : 4); ++j)
 #pragma unroll
-                    for (int j = 0; j < (X == X_FP4 ? 1 : 4); ++j)
+                    for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (c * 256 + ((s * 4 + g) * 4 + j) * 8 + e * 2 >= a.K) xv[0][s][i][j][e] = 0;
+                        for (int i = 0; i < MT; ++i)
+                            if (s * 64 + j * 4 + e >= words_left) xv[0][s][i][j][e] = 0;
         }
         // (the slot is read: the next chunk may come)
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");

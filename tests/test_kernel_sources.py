@@ -73,3 +73,29 @@ def test_loads_to_shared_memory_wait_for_their_scalar_operands(tmp_path):
                     waited += s
             before = before[-7:] + [(states, wrote)]
     assert loads and not early, early[:4]
+
+
+def _registers(tmp_path):
+    """What the built library says of its kernels: name -> spilled scalar registers, spilled vector registers, bytes of scratch memory."""
+    from qwen_engine_amd.kernels import build
+    tools = [shutil.which(t) or f"/opt/rocm/llvm/bin/{t}" for t in ("llvm-objdump", "llvm-readelf")]
+    if not all(Path(t).exists() for t in tools):
+        pytest.skip("no llvm-objdump or no llvm-readelf")
+    lib = tmp_path / "lib.so"
+    shutil.copy(build.library_path(), lib)
+    subprocess.run([tools[0], "--offloading", lib.name], cwd=tmp_path, check=True, capture_output=True)
+    out = {}
+    for part in sorted(tmp_path.glob("*gfx950")):
+        text = subprocess.run([tools[1], "--notes", part.name], cwd=tmp_path, check=True, capture_output=True, text=True).stdout
+        for kernel in re.split(r"\n  - ", text)[1:]:
+            name = re.search(r"^ *\.name: +'?(_Z\w+)", kernel, re.M)
+            number = {k: int(v) for k, v in re.findall(r"\.(sgpr_spill_count|vgpr_spill_count|private_segment_fixed_size): +(\d+)", kernel)}
+            if name:
+                out[name.group(1)] = (number["sgpr_spill_count"], number["vgpr_spill_count"], number["private_segment_fixed_size"])
+    return out
+
+
+def test_kernels_of_few_rows_keep_their_scalars_in_registers(tmp_path):
+    """A scalar register that is spilled comes back lane by lane in every chunk of K."""
+    kernels = {k: v for k, v in _registers(tmp_path).items() if "fp4_few_kernel" in k}
+    assert len(kernels) >= 20 and all(v == (0, 0, 0) for v in kernels.values()), kernels
