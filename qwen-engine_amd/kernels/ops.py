@@ -2352,7 +2352,8 @@ _U8 = torch.uint8
 class MxFp4(NamedTuple):
     """A matrix [T, K] in microscaled 4-bit floating point: blocks of 32 numbers along K, each with a scale 2^(s - 127) (a byte
     s; 255: the block is NaN) and 32 codes of 4 bits (sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6),
-    two a byte, the first in its low half.  Numbers behind K in the last block do not count."""
+    two a byte, the first in its low half.  Numbers behind K in the last block do not count.  Scales of 253 and 254, which
+    mxfp4_quantize does not give, hold numbers beyond float32 (4 and 6 under 253, 2 and more under 254)."""
     codes: torch.Tensor      # uint8 [T, ceil(K / 32) * 16]
     scales: torch.Tensor     # uint8 [T, ceil(K / 32)]
     columns: int             # K
@@ -2398,7 +2399,8 @@ def mxfp4_quantize(x: torch.Tensor) -> MxFp4:
 
 
 def mxfp4_values(m: MxFp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The numbers that a 4-bit matrix stands for, [T, K] in bfloat16 or float32 (both hold them exactly)."""
+    """The numbers that a 4-bit matrix stands for, [T, K] in bfloat16 or float32 (both hold them exactly; what is beyond float32 becomes
+    infinite)."""
     lib = load_library()
     T, K = _need_mxfp4(m, "the matrix")
     if dtype not in _DT:
@@ -2413,7 +2415,8 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
                epilogue: int = EPI_STORE) -> torch.Tensor:
     """x [M, K] . w [N, K]^T (+ bias [N], 32-bit) -> [M, N] in out_dtype (default: x's; bfloat16 for a 4-bit x), w in 4 bits, x in
-    bfloat16, float32 or 4 bits.  Products are exact and summed in 32-bit.
+    bfloat16, float32 or 4 bits.  Products are exact and summed in 32-bit.  (Scales of 253 and 254: a number of w beyond float32 makes
+    its column infinite or NaN beside rows in bfloat16 or float32; beside rows in 4 bits it counts as what it is.)
 
     epilogue EPI_RESIDUAL: the product is added into ``out``, the 32-bit stream [M, N].
     epilogue EPI_SILU_MUL: w is [2 N, K] (gate rows, then up rows); the result is silu(x . gate^T) * (x . up^T), [M, N]; a bias

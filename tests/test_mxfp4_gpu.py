@@ -278,6 +278,48 @@ def test_nan_and_infinities(ops, kind):
 
 
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M,N,K", [(1, 130, 256), (7, 130, 250), (16, 16390, 330), (20, 48, 640), (40, 300, 256), (200, 8230, 712), (300, 8230, 712),
+                                   (470, 8230, 712), (130, 302, 4160), (3100, 4200, 256), (3, 20, 400001)])
+def test_scales_at_the_ends(ops, kind, M, N, K):
+    """The smallest scales (also where sums lie below the least normal number: there a sum of n terms is off by at most n + 8 times 2^-149 more),
+    the largest that quantisation gives, 252, and the two beyond it, under which the larger codes are beyond float32: beside rows in 16 or 32
+    bits a column that has such a one is infinite or NaN and no other is touched, beside rows in 4 bits every sum is right."""
+    blocks = (K + 31) // 32
+
+    def matrix(rows, scales, seed, some=None):
+        code = torch.randint(0, 16, (rows, blocks, 32), generator=gen(seed))
+        if some is not None:                                   # (every other row has no code of 2 or more)
+            code = torch.where((torch.arange(rows) % 2 == some).view(-1, 1, 1), code & 11, code)
+        scale = torch.tensor(scales)[torch.arange(rows) // 2 % len(scales)].view(-1, 1).expand(rows, blocks).contiguous()
+        v = values_of(code, scale, K).to(DEV)
+        return ops.MxFp4(packed(code).to(DEV), scale.to(torch.uint8).to(DEV), K), v
+
+    def rows(power):
+        x = (torch.randn(M, K, generator=gen(8)) * 2.0 ** power).to(torch.float32 if kind == "float32" else torch.bfloat16).to(DEV)
+        return x, x.double()
+
+    def check(x, xv, w, v, infinite=None):
+        want, off = xv @ v.T, sums_bound(3 * K, xv.abs() @ v.abs().T) + (3 * K + 8) * 2.0 ** -149
+        assert float((want.abs() + off).max()) < torch.finfo(torch.float32).max or infinite is not None
+        got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32).double()
+        if infinite is not None:
+            assert not got[:, infinite].isfinite().any()
+            got, want, off = got[:, ~infinite], want[:, ~infinite], off[:, ~infinite]
+        assert ((got - want).abs() <= off).all()
+
+    if kind == "fp4":
+        for x_scales, w_scales in (([252, 253, 254], [100, 101]), ([0, 1], [252, 253, 254]), ([0, 1, 2], [127]), ([0, 1], [0, 1]), ([127], [0, 1, 2])):
+            check(*matrix(M, x_scales, 7), *matrix(N, w_scales, 5))
+        return
+    for power, scales in ((20, [0, 1]), (0, [0, 1]), (-10, [0, 1]), (-30, [251, 252])):
+        check(*rows(power), *matrix(N, scales, 5))
+    w, v = matrix(N, [127, 253, 252, 254], 5, some=0)
+    beyond = (v.abs() > torch.finfo(torch.float32).max).any(1)
+    assert beyond.any() and not beyond.all()
+    check(*rows(-30), w, v, beyond)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
 @pytest.mark.parametrize("K", [40, 64, 96, 160, 200, 700, 1312])
 def test_large_tiles_and_what_lies_behind_a_row(ops, kind, K):
     """Enough rows and columns for the largest tiles; K ends inside a stage, and the row behind is NaN: every other column is exact."""
