@@ -2418,10 +2418,12 @@ def gemm_mxfp4(x: Union[torch.Tensor, MxFp4], w: MxFp4, bias: Optional[torch.Ten
     bfloat16, float32 or 4 bits.  Products are exact and summed in 32-bit.  (Scales of 253 and 254: a number of w beyond float32 makes
     its column infinite or NaN beside rows in bfloat16 or float32; beside rows in 4 bits it counts as what it is.)
 
-    epilogue EPI_RESIDUAL: the product is added into ``out``, the 32-bit stream [M, N].
+    epilogue EPI_RESIDUAL: the product is added into ``out``, the 32-bit stream [M, N] (no other out_dtype is taken).
     epilogue EPI_SILU_MUL: w is [2 N, K] (gate rows, then up rows); the result is silu(x . gate^T) * (x . up^T), [M, N]; a bias
     (in w's order of rows, [2 N]) joins before the activation."""
     lib = load_library()
+    if epilogue == EPI_RESIDUAL and out_dtype is not None and out_dtype is not torch.float32:
+        raise KernelError(f"gemm_mxfp4: a result in {out_dtype}: the stream to add into is 32-bit")
     if isinstance(x, MxFp4):
         M, K = _need_mxfp4(x, "x")
         data, scales, kind, dev = x.codes, x.scales, 2, x.codes.device

@@ -120,6 +120,16 @@ def test_gemm(fake):
         refused(lambda: ops.gemm_mxfp4(t(2, 40), w, epilogue=e), "epilogue")
 
 
+def test_type_of_the_stream(fake):
+    """A product that is added into the 32-bit stream has no other type, whatever the type of its rows is."""
+    t = fake
+    for x in (t(2, 40), t(2, 40, dtype=B), mat(t, 2, 40)):
+        refused(lambda: ops.gemm_mxfp4(x, mat(t, 6, 40), out_dtype=B, out=t(2, 6), epilogue=ops.EPI_RESIDUAL), "stream")
+        for same in (None, F):
+            with pytest.raises(Launched):
+                ops.gemm_mxfp4(x, mat(t, 6, 40), out_dtype=same, out=t(2, 6), epilogue=ops.EPI_RESIDUAL)
+
+
 def test_results_over_operands(fake, monkeypatch):
     t = fake
     x, w = t(2, 64), mat(t, 64, 64)
