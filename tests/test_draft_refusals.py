@@ -120,14 +120,15 @@ def test_gemm(fake):
         refused(lambda: ops.gemm_mxfp4(t(2, 40), w, epilogue=e), "epilogue")
 
 
-def test_type_of_the_stream(fake):
+def test_type_of_the_stream(fake, monkeypatch):
     """A product that is added into the 32-bit stream has no other type, whatever the type of its rows is."""
     t = fake
-    for x in (t(2, 40), t(2, 40, dtype=B), mat(t, 2, 40)):
-        refused(lambda: ops.gemm_mxfp4(x, mat(t, 6, 40), out_dtype=B, out=t(2, 6), epilogue=ops.EPI_RESIDUAL), "stream")
+    place(monkeypatch, n18=4096)
+    for x in (t(3, 40), t(3, 40, dtype=B)):
+        refused(lambda: ops.gemm_mxfp4(x, mat(t, 6, 40), out_dtype=B, out=t(3, 6), epilogue=ops.EPI_RESIDUAL), "stream")
         for same in (None, F):
             with pytest.raises(Launched):
-                ops.gemm_mxfp4(x, mat(t, 6, 40), out_dtype=same, out=t(2, 6), epilogue=ops.EPI_RESIDUAL)
+                ops.gemm_mxfp4(x, mat(t, 6, 40), out_dtype=same, out=t(3, 6), epilogue=ops.EPI_RESIDUAL)
 
 
 def test_results_over_operands(fake, monkeypatch):
