@@ -140,9 +140,17 @@ static int fp4_rows(const Fp4Args& a, int tail, hipStream_t stream) {
     const int steps = qe_cdiv(a.blocks, 4);
     int waves = steps >= 48 ? 16 : steps >= 12 ? 8 : steps >= 4 ? 4 : 2;
     if (tail == TAIL_SILU && waves > 8) waves = 8;
-    const dim3 grid(qe_cdiv(wide, 16), qe_cdiv(a.M, 16));
-    if (tail == TAIL_SILU) fp4_rows_kernel<X, 2><<<grid, 64 * waves, waves * 2048, stream>>>(a, tail);
-    else fp4_rows_kernel<X, 1><<<grid, 64 * waves, waves * 1024, stream>>>(a, tail);
+    // (as many rows a launch as a grid's second axis holds)
+    for (long m = 0; m < a.M; m += 65535 * 16) {
+        Fp4Args s = a;
+        s.M = (int)(a.M - m < 65535 * 16 ? a.M - m : 65535 * 16);
+        s.x = (const unsigned char*)a.x + m * (X == X_FP4 ? a.blocks * 16L : a.K * (X == X_BF16 ? 2L : 4L));
+        if (X == X_FP4) s.xs = a.xs + m * a.blocks;
+        s.out = (unsigned char*)a.out + m * wide * (a.out_f32 ? 4L : 2L);
+        const dim3 grid(qe_cdiv(wide, 16), qe_cdiv(s.M, 16));
+        if (tail == TAIL_SILU) fp4_rows_kernel<X, 2><<<grid, 64 * waves, waves * 2048, stream>>>(s, tail);
+        else fp4_rows_kernel<X, 1><<<grid, 64 * waves, waves * 1024, stream>>>(s, tail);
+    }
     return 0;
 }
 
@@ -175,7 +183,7 @@ extern "C" int qe_gemm_mxfp4(const void* x, const void* x_scales, const void* co
     QE_REQUIRE(tail != TAIL_SILU || N % 2 == 0, "gemm_mxfp4: gate|up of an odd number of rows");
     QE_REQUIRE(((uintptr_t)codes & 15) == 0, "gemm_mxfp4: the codes do not begin at a whole 16-byte piece");
     QE_REQUIRE(x_kind != X_FP4 || ((uintptr_t)x & 15) == 0, "gemm_mxfp4: the codes of x do not begin at a whole 16-byte piece");
-    QE_REQUIRE(M <= 65535 * 16, "gemm_mxfp4: %d rows are too many", M);
+    QE_REQUIRE(M <= (1 << 30), "gemm_mxfp4: %d rows are too many", M);
     if (M == 0) return 0;
     const Fp4Args a{x, (const unsigned char*)x_scales, (const unsigned char*)codes, (const unsigned char*)scales, bias, out, M, N, K,
                     qe_cdiv(K, 32), out_dtype == QE_F32};

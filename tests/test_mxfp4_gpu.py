@@ -492,6 +492,39 @@ def test_matrices_beyond_32_bits(ops):
     assert torch.equal(ops.mxfp4_values(w, torch.bfloat16)[-3:], last)
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("K", [64, 1100, 4128])
+def test_more_than_a_million_rows(ops, kind, K):
+    """More rows than a grid's second axis holds tiles of 16, by tiles and, where the rows are more than 2^31 bytes, 16 at a time; every sum
+    exact (halves of at most 48 K < 2^18), the row behind the last one as it was."""
+    M, N = 65535 * 16 + 21, 6
+    codes, scales, v = whole_matrix(N, K, 3)
+    w, v = ops.MxFp4(codes.to(DEV), scales.to(DEV), K), v.to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    if kind == "fp4":
+        blocks = (K + 31) // 32
+        x = ops.MxFp4(torch.randint(0, 256, (M, blocks * 16), dtype=torch.uint8, device=DEV, generator=g),
+                      torch.randint(127, 129, (M, blocks), device=DEV, generator=g).to(torch.uint8), K)
+        part = lambda a, b: ops.mxfp4_values(ops.MxFp4(x.codes[a:b], x.scales[a:b], K), torch.float32)
+    else:
+        x = torch.randint(-4, 5, (M, K), dtype=torch.int8, device=DEV, generator=g).to(getattr(torch, kind))
+        part = lambda a, b: x[a:b]
+    hold = torch.full((M + 1, N), 7.0, device=DEV)
+    bias = torch.arange(N, device=DEV, dtype=torch.float32)
+    ops.gemm_mxfp4(x, w, bias, out_dtype=torch.float32, out=hold[:M])
+    half = ops.gemm_mxfp4(x, w, out_dtype=torch.bfloat16, epilogue=ops.EPI_SILU_MUL)
+    assert (hold[M] == 7).all()
+    for a in range(0, M, 1 << 17):
+        b = min(M, a + (1 << 17))
+        want = part(a, b).double() @ v.T
+        assert torch.equal(hold[a:b].double(), want + bias.double()), a
+        gate, up = want[:, :N // 2], want[:, N // 2:]
+        act = gate * torch.sigmoid(gate) * up
+        # (the activation's own arithmetic and gates below -88.73, as in the large tiles' test, and a rounding to bfloat16)
+        bound = (8 + gate.abs()) * 2.0 ** -23 * act.abs() + 2.0 ** -121 * up.abs()
+        assert ((half[a:b].double() - act).abs() <= bound + 2.0 ** -8 * (act.abs() + bound)).all(), a
+
+
 def test_quantize_beyond_32_bits(ops):
     T, K = 66000, 32768                                        # more than 2^31 numbers
     rows = torch.randn(7, K, generator=gen(3)).to(torch.bfloat16).to(DEV)
