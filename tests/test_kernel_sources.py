@@ -99,3 +99,9 @@ def test_kernels_of_few_rows_keep_their_scalars_in_registers(tmp_path):
     """A scalar register that is spilled comes back lane by lane in every chunk of K."""
     kernels = {k: v for k, v in _registers(tmp_path).items() if "fp4_few_kernel" in k}
     assert len(kernels) >= 20 and all(v == (0, 0, 0) for v in kernels.values()), kernels
+
+
+def test_kernels_of_drafting_keep_out_of_scratch_memory(tmp_path):
+    """The kernels of the 4-bit matrices and of the verification of drafts hold what they work on in registers."""
+    kernels = {k: v for k, v in _registers(tmp_path).items() if re.search(r"fp4|verify_", k)}
+    assert len(kernels) >= 60 and all(v[1:] == (0, 0) for v in kernels.values()), {k: v for k, v in kernels.items() if v[1:] != (0, 0)}
