@@ -355,17 +355,17 @@ __global__ __launch_bounds__(256, 1) void fp4_both_large_kernel(Fp4Both t) {
     // (a k step is four of the quarter's 16 matrix instructions: beside each of the first eight a piece is read, beside every fourth a load goes out)
 #define QUAD_STEP(ks_, ha_, hb_, rg_, rst_, rpar_, lg_, lst_, lpar_)                                                      \
     {                                                                                                                     \
-        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4)                                                           \
+        if constexpr ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4)                                                           \
         MULTIPLY(ha_, hb_, 0, 0, ks_)                                                                                     \
         __builtin_amdgcn_sched_barrier(0);                                                                                \
-        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 1)                                                       \
+        if constexpr ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 1)                                                       \
         MULTIPLY(ha_, hb_, 0, 1, ks_)                                                                                     \
         LOAD_REGION(lg_, lst_, lpar_, ks_)                                                                                \
         __builtin_amdgcn_sched_barrier(0);                                                                                \
-        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 2)                                                       \
+        if constexpr ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 2)                                                       \
         MULTIPLY(ha_, hb_, 1, 0, ks_)                                                                                     \
         __builtin_amdgcn_sched_barrier(0);                                                                                \
-        if ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 3)                                                       \
+        if constexpr ((ks_) < 2) READ_REGION(rg_, rpar_, rst_, (ks_) * 4 + 3)                                                       \
         MULTIPLY(ha_, hb_, 1, 1, ks_)                                                                                     \
         __builtin_amdgcn_sched_barrier(0);                                                                                \
     }

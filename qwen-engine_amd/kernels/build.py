@@ -118,6 +118,9 @@ def build(verbose: bool = True, jobs: Optional[int] = None) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise BuildError(f"hipcc failed on {src.name}:\n{_filter(r.stdout + r.stderr)}")
+        said = _filter(r.stdout + r.stderr)
+        if said:
+            _log(f"hipcc on {src.name}:\n{said}", verbose)
         return obj
 
     objs = []

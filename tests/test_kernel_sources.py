@@ -1,7 +1,9 @@
 """What the kernels' asm has to say to the compiler, read from the sources, and to keep itself, read from the built library."""
+import os
 import re
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 import pytest
@@ -105,3 +107,21 @@ def test_kernels_of_drafting_keep_out_of_scratch_memory(tmp_path):
     """The kernels of the 4-bit matrices and of the verification of drafts hold what they work on in registers."""
     kernels = {k: v for k, v in _registers(tmp_path).items() if re.search(r"fp4|verify_", k)}
     assert len(kernels) >= 60 and all(v[1:] == (0, 0) for v in kernels.values()), {k: v for k, v in kernels.items() if v[1:] != (0, 0)}
+
+
+def test_sources_compile_without_a_warning():
+    """One that is wrong would not be seen among others.  (Said anyhow: that the host does not know the feature which is taken off, and that
+    nothing is linked.)"""
+    from qwen_engine_amd.kernels import build
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not Path(hipcc).exists():
+        pytest.skip("no hipcc")
+
+    def said(path):
+        r = subprocess.run([hipcc, *build.HIPCC_FLAGS, "-I", str(CSRC), "-fsyntax-only", str(path)], capture_output=True, text=True)
+        return [f"{path.name}: {line}" for line in (r.stdout + r.stderr).splitlines()
+                if re.search("warning|error", line) and not re.search("packed-fp32-ops|--hip-link", line)]
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        lines = [line for part in pool.map(said, build.sources()) for line in part]
+    assert not lines, lines[:4]
