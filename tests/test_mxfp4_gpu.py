@@ -213,6 +213,28 @@ def test_float32_rows_lose_nothing(ops):
     assert ((got - x.double() @ v.T).abs() <= sums_bound(9, x.double().abs() @ v.abs().T)).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(17, 130, 2600), (20, 302, 4160), (40, 20100, 200), (90, 302, 6000), (70, 20100, 200), (200, 8230, 712),
+                                   (330, 1000, 12000), (500, 4200, 1312), (300, 8230, 712), (512, 8192, 4096), (3100, 302, 1312), (470, 8230, 712),
+                                   (600, 1000, 12000), (1000, 4200, 330), (3100, 302, 12000), (3100, 4200, 768), (600, 1000, 4160)])
+def test_float32_rows_lose_nothing_in_tiles(ops, M, N, K):
+    """The same where the planes are walked one after the other by tiles of 64, 96, 128, 160 and 256 rows, in one piece and in cuts that begin and end
+    inside a plane (and by the tiles of 32 rows of all three): three numbers a row, all over K, the last ones of K among them.  (Nine terms that are
+    not zero; the others are added without a rounding.)"""
+    m = torch.arange(M)
+    x = torch.zeros(M, K)
+    for i, at in enumerate((m * 131 % K, K - 1 - m % 40, torch.randint(0, K, (M,), generator=gen(6)))):
+        x[m, at] = torch.randn(M, generator=gen(100 + i)) * torch.exp2((m % 20 * 6 - 60).float())
+    w_raw = torch.randn(N, K, generator=gen(21))
+    w = ops.mxfp4_quantize(w_raw.to(DEV))
+    x, v = x.to(DEV), ops.mxfp4_values(w, torch.float32).double()
+    off = sums_bound(9, x.double().abs() @ v.abs().T)
+    assert ((ops.gemm_mxfp4(x, w).double() - x.double() @ v.T).abs() <= off).all()
+    # (the test would see it: without the last eight bits, and without the eight before, many sums are off by more)
+    for bits in (0xff, 0xff00):
+        less = (x.view(torch.int32) & ~bits).view(torch.float32)
+        assert (((less.double() - x.double()) @ v.T).abs() > off).any()
+
+
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9, 16])
 @pytest.mark.parametrize("N,K", [(130, 1), (130, 3), (130, 255), (130, 257), (16390, 257), (130, 1023), (16390, 2570), (130, 4096)])
 def test_few_float32_rows(ops, M, N, K):
