@@ -304,6 +304,169 @@ def test_first_rows_that_fall(ops, R, V, lookup):
     assert marked and served
 
 
+def full(c):
+    """The requests of a case over and over, with numbers of their own, until there are so many that acceptance, sums and draw are launches of
+    their own (more than 320 spans of 4096 logits)."""
+    times = 321 // (len(c["counts"]) * -(-c["logits"].shape[1] // 4096)) + 1
+    g = torch.Generator().manual_seed(77)
+    d = {k: v * times if k == "counts" else v if v is None else v.repeat(times, *[1] * (v.dim() - 1)) for k, v in c.items()}
+    for k in ("accept", "draw"):
+        d[k][len(c[k]):] = torch.rand(len(d[k]) - len(c[k]), generator=g)
+    return d
+
+
+@pytest.mark.parametrize("lookup", [False, True])
+def test_masks_in_a_full_batch(ops, lookup):
+    """The masks, NaN and infinities of test_masks, and rows where nothing weighs, in the launches of a full batch."""
+    c = case([2, 2, 2, 2, 2, 2, 2, 2, 1, 0], 5000, 6, greedy_every=100, lookup=lookup)
+    z, q = c["logits"], c["guess"]
+    z[0, 1000:] = -math.inf
+    z[3] = -math.inf
+    z[6, 10:4990] = math.nan
+    z[9, [17, 4099]] = math.inf
+    z[12] = -math.inf
+    z[12, 4500] = -3.0
+    if q is not None:
+        q[8] = -math.inf
+        q[10] = math.nan
+        q[12, 5:] = -math.inf
+    z[24:26] = -3e38
+    c["temperature"][9] = 1e-30
+    z[26] = math.nan
+    z[26, 3] = 2.0
+    check(ops, full(c))
+    for t in (0.0, -1.0):
+        c["temperature"][:] = t
+        check(ops, full(c))
+    c["temperature"][:] = math.inf
+    z[9] = 0.0
+    check(ops, full(c))
+
+
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("offset", [0.0, -300.0, 5e4, 2e9])
+def test_temperatures_of_all_sizes_in_a_full_batch(ops, offset, lookup):
+    temperatures = [1e-45, 1e-38, 1e-20, 1e-8, 1e-5, 1e-3, 0.05, 1.0, 30.0, 1e4, 1e9, 1e30, 1e37, 3e38]
+    counts = [2] * len(temperatures)
+    c = case(counts, 5003, 17, spread=3.0, lookup=lookup, greedy_every=1000)
+    c["logits"] += offset
+    masked = torch.rand(c["logits"].shape, generator=torch.Generator().manual_seed(4)) < 0.3
+    masked[torch.cat([torch.arange(3) < 2 for _ in counts]).nonzero()[:, 0], c["drafts"].long()] = False
+    c["logits"][masked] = -math.inf
+    c["temperature"] = torch.tensor(temperatures)
+    check(ops, full(c))
+
+
+def test_flat_distributions_in_a_full_batch(ops):
+    check(ops, case([2, 1, 0, 3, 2, 2, 2, 1, 1], 151936, 8, spread=1e-3, greedy_every=100))
+
+
+def test_ties_and_drafts_outside_in_a_full_batch(ops):
+    c = case([2, 2, 2, 1], 4200, 9, greedy_every=1)
+    z = c["logits"]
+    z[0, [40, 4150]] = 50.0
+    z[3, [4150, 4199]] = 50.0
+    c["drafts"][0], c["drafts"][2] = 40, 4199
+    check(ops, full(c))
+    for bad in (-1, 4200, 2 ** 31 - 1, -2 ** 31):
+        for t in (0.0, 0.8):
+            for guess in (c["guess"], None):
+                d = dict(c, drafts=c["drafts"].clone(), temperature=torch.full((4,), t), guess=guess)
+                d["drafts"][1::2] = bad
+                check(ops, full(d))
+
+
+def test_numbers_at_the_ends_in_a_full_batch(ops):
+    c = full(case([3, 1, 0, 2], 4500, 10, greedy_every=100))
+    c["logits"][:, 0] = -math.inf
+    c["logits"][:, -1] = -math.inf
+    for u in (0.0, 1 - 2.0 ** -24):
+        for a in (0.0, 1 - 2.0 ** -24):
+            c["draw"].fill_(u)
+            c["accept"].fill_(a)
+            check(ops, c)
+    c["accept"].fill_(math.nan)
+    first = first_of(c["counts"])[:-1].long().to(DEV)
+    for u in (1.0, 5.0, -1.0, math.nan, math.inf):
+        c["draw"].fill_(u)
+        tokens, accepted = go(ops, c)
+        assert (accepted == 0).all() and ((tokens[first] > 0) & (tokens[first] < 4499)).all()
+
+
+@pytest.mark.parametrize("batch", [False, True])
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_many_drafts(ops, temperature, lookup, batch):
+    """More drafts than a block has waves: the first that is refused among the first 16, the last of them, the first behind them, later, and none."""
+    counts = [15, 16, 17, 40, 40, 40, 40, 40, 33, 32, 1]
+    refused = [15, 15, 16, 14, 15, 16, 31, 32, 33, 7, 0]           # (as many as there are drafts: none)
+    c = case(counts, 700, 60, lookup=lookup, greedy_every=1000)
+    c["temperature"].fill_(temperature)
+    row = d = 0
+    for n, r in zip(counts, refused):
+        c["drafts"][d:d + n] = c["logits"][row:row + n].argmax(1)
+        c["accept"][d:d + n] = 0.0
+        if r < n:
+            c["accept"][d + r:d + n] = 1e30
+            c["drafts"][d + r] = (c["drafts"][d + r] + 1) % 700
+        row, d = row + n + 1, d + n
+    if batch:                                                      # (behind one another as they are: the numbers decide)
+        c = {k: v * 30 if k == "counts" else v if v is None else v.repeat(30, *[1] * (v.dim() - 1)) for k, v in c.items()}
+        refused = refused * 30
+    assert check(ops, c)[1] == refused
+
+
+def test_rows_of_no_request_in_a_full_batch(ops):
+    c = full(case([2, 1, 3], 600, 11))
+    rows, D = len(c["logits"]), len(c["drafts"])
+    want = plain(*(v.numpy() if isinstance(v, torch.Tensor) else v for v in (c["logits"], c["counts"], c["drafts"], c["guess"],
+                                                                             c["temperature"], c["accept"], c["draw"])))
+    pad = dict(c, logits=torch.cat([c["logits"], torch.zeros(4, 600)]), drafts=torch.cat([c["drafts"], torch.full((4,), 77, dtype=torch.int32)]),
+               guess=torch.cat([c["guess"], torch.zeros(4, 600)]), accept=torch.cat([c["accept"], torch.zeros(4)]))
+    tokens = torch.full((rows + 4,), 99, dtype=torch.int32, device=DEV)
+    tokens, accepted = go(ops, pad, tokens=tokens)
+    assert tokens.tolist() == want[0] + [99] * 4 and accepted.tolist() == want[1] and D
+
+
+def test_recorded_and_two_streams_in_a_full_batch(ops):
+    """Recorded twice and replayed on other numbers, with eager work between; then overlapping calls on two streams."""
+    cs = [full(case([2, 0, 4, 1], 9001, 20 + i)) for i in range(3)]
+    names = ("logits", "drafts", "guess", "temperature", "accept", "draw")
+    held = [{k: c[k].to(DEV) for k in names} for c in cs]
+    first = first_of(cs[0]["counts"]).to(DEV)
+
+    def run(s):
+        return ops.verify_drafts(s["logits"], first, s["drafts"], s["guess"], s["temperature"], s["accept"], s["draw"])
+
+    want = [run(h) for h in held]
+    assert want[0][1].tolist() == check(ops, cs[0])[1]
+    static = {k: v.clone() for k, v in held[0].items()}
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(static)
+        graphs.append((graph, out))
+    for _ in range(2):
+        for h, w in zip(held, want):
+            for k in names:
+                static[k].copy_(h[k])
+            for graph, out in graphs:
+                graph.replay()
+            run(held[1])
+            torch.cuda.synchronize()
+            for graph, out in graphs:
+                assert torch.equal(out[0], w[0]) and torch.equal(out[1], w[1])
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(held[i]))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(t, w[0]) and torch.equal(a, w[1]) for t, a in g)
+
+
 def test_no_requests(ops):
     e = lambda *s, dtype=torch.float32: torch.empty(*s, dtype=dtype, device=DEV)
     tokens, accepted = ops.verify_drafts(e(0, 50), torch.zeros(1, dtype=torch.int32, device=DEV), e(0, dtype=torch.int32), None, e(0), e(0), e(0))
