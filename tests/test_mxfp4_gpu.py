@@ -476,6 +476,44 @@ def test_very_wide_rows(ops, kind, K):
     assert ((got - act).abs() <= (8 + want[:, :half].abs()) * 2.0 ** -23 * act.abs() + 2.0 ** -121 * want[:, half:].abs()).all()
 
 
+# The widest rows whose scales still leave a wave of the few rows' kernel its place in shared memory: with one tile of columns, and with two.
+@pytest.mark.parametrize("kind,M,one,two", [("bfloat16", 2, 321472, 158688), ("bfloat16", 8, 315328, 155616), ("bfloat16", 16, 307136, 151520),
+                                            ("bfloat16", 32, 290752, 143328), ("float32", 2, 313280, 154592), ("float32", 4, 303040, 149472),
+                                            ("float32", 8, 298944, 147424), ("float32", 16, 274368, 135136), ("fp4", 2, 285728, 149344),
+                                            ("fp4", 8, 214304, 126944), ("fp4", 16, 159712, 105088), ("fp4", 32, 105088, 77792),
+                                            ("fp4", 64, 61408, 50496)])
+def test_rows_at_the_limit_of_shared_memory(ops, kind, M, one, two):
+    """Rows just within these widths, where one to three waves are left, and just beyond, where other kernels take over; junk behind the columns.
+    One number in twenty is not zero, so that all sums stay below 2^21 (32 bits of them are exact from there on down to eighths)."""
+    N = 20
+    widest = one + 1
+    codes, scales, v = whole_matrix(N, widest, 5)
+    some = torch.rand(M, widest, generator=gen(6)) < 0.05
+    if kind == "fp4":
+        code, scale = torch.where(some, 5, 0).long(), torch.full((M, (widest + 31) // 32), 127)      # (threes)
+    else:
+        xv_all = torch.where(some, torch.randint(-4, 5, (M, widest), generator=gen(9)), 0).double()
+    for K in (two - 30000, two - 9001, two - 2047, two, two + 1, one - 30000, one - 9001, one - 2047, one, one + 1):
+        blocks = (K + 31) // 32
+        w = ops.MxFp4(codes[:, :blocks * 16].contiguous().to(DEV), scales[:, :blocks].contiguous().to(DEV), K)
+        if kind == "fp4":
+            c = torch.full((M, blocks * 32), 7, dtype=torch.int64)
+            c[:, :K] = code[:, :K]
+            c = c.view(M, -1, 32)
+            x, xv = ops.MxFp4(packed(c).to(DEV), scale[:, :blocks].to(torch.uint8).to(DEV), K), values_of(c, scale[:, :blocks], K)
+        else:
+            xv = xv_all[:, :K]
+            x = xv.to(getattr(torch, kind)).to(DEV)
+        want = xv @ v[:, :K].T
+        assert float((xv.abs() @ v[:, :K].abs().T).max()) < 2.0 ** 21
+        assert torch.equal(ops.gemm_mxfp4(x, w, out_dtype=torch.float32).cpu().double(), want), K
+        gate, up = want[:, :N // 2], want[:, N // 2:]
+        act = gate * torch.sigmoid(gate) * up
+        got = ops.gemm_mxfp4(x, w, out_dtype=torch.float32, epilogue=ops.EPI_SILU_MUL).cpu().double()
+        # (the activation's own arithmetic, and gates below -88.73, as in the very wide rows' test)
+        assert ((got - act).abs() <= (8 + gate.abs()) * 2.0 ** -23 * act.abs() + 2.0 ** -121 * up.abs()).all(), K
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
 @pytest.mark.parametrize("M", [1, 9, 30, 50, 90])
 def test_rows_of_a_larger_matrix(ops, kind, M):
