@@ -10,9 +10,9 @@
 // All weights and sums are 64-bit: a vocabulary of 150 000 has so many borders of running sums that 32-bit ones put the random number on
 // the other side of one in a few per cent of the draws.
 //
-// Four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials: of 64 requests, 425 MB, 95 us), acceptance (a block a
-// request, a wave a draft, 7 us), the sums of pieces of 1024 of what the token is drawn from (one row a request, and its draft's, 15 us), the
-// draw (5 us); the last three in one where there are few spans.
+// Four launches: spans of 4096 logits (all rows, bound by their bytes and exponentials: of 64 requests, 425 MB, 85 to 97 us), acceptance (a block a
+// request, a wave a draft, 6 to 7.5 us), the sums of pieces of 1024 of what the token is drawn from (one row a request, and its draft's, 16 to
+// 19 us), the draw (5 to 6 us); the last three in one where there are few spans.
 #include "common.h"
 
 #define VERIFY_SPAN 4096        // what a block looks at; its quarters, a wave each, have sums of their own
@@ -88,9 +88,10 @@ __device__ __forceinline__ double verify_finite_weight(float z, float top, const
 }
 
 // The same for a sum over many logits of a row, with fewer operations (64 requests 120 us, so 115: what counts there is how many 64-bit operations a
-// logit takes, next to its bytes): 2^(z k) = 2^m 2^(j / 32) 2^f, where 32 m + j is 32 z k rounded (1.5 2^47 added) and |f| <= 1/64, so
+// logit takes, next to its bytes).  The method is the exponential by a table of 32 and a short polynomial of P. T. P. Tang (Table-driven implementation
+// of the exponential function in IEEE floating-point arithmetic, ACM Transactions on Mathematical Software 15, 1989), in powers of two: 2^(z k) = 2^m 2^(j / 32) 2^f, where 32 m + j is 32 z k rounded (1.5 2^47 added) and |f| <= 1/64, so
 // that a polynomial of degree 5 does (off by 1.5e-16 at the most); 2^(j / 32) comes from a table in shared memory, in 32 pairs of banks of its
-// own, which holds the high words less j 2^15: 32 m + j, shifted by 15 and added, makes 2^m 2^(j / 32) of them.  The row's own number of the
+// own, the nearest 64-bit numbers with their high words less j 2^15: 32 m + j, shifted by 15 and added, makes 2^m 2^(j / 32) of them.  The row's own number of the
 // kind, 2^(top k), counts for the sum as a whole: its rounded exponent is taken off with the constant that rounds 32 z k, the rest
 // multiplied at the end.  What is far below the top (or no number) counts as 2^-1000 of it, which the logit's 32-bit maximum with `floor` sees
 // to.  Not for a top that is infinite or beyond 2^25 / k, nor where 32 bits hold no number some 1000 / k below it.
