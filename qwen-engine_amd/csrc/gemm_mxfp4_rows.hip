@@ -290,8 +290,8 @@ static Fp4Few fp4_few_shape(int M, int N, int K, int x_kind, int tail) {
     return f;
 }
 
-// Rows that the loads take as they are: of bfloat16, at whole words (5 rows of 2566 numbers against 5120 5.5 us; of 2567, through
-// a copy, 7.8).
+// Rows that the loads take as they are: of bfloat16, at whole words (5 rows of 2566 numbers against 5120 4.9 us; of 2567, through
+// a copy, 7.4).
 static bool as_it_is(const void* x, int K, int x_kind) { return x_kind == X_FP4 || (x_kind == X_BF16 && K % 2 == 0 && ((uintptr_t)x & 3) == 0); }
 
 // (Of 32 bits 8 rows, or 16 against narrow matrices: 8 against 24576 x 4096 23.7 us, by tiles 27.6, against 4096 x 4096 10.1 and 14.6; 16 34.2, 28.6 and

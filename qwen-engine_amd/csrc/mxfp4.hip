@@ -9,7 +9,8 @@
 // depend on how this is computed.
 //
 // Bound by memory: a lane takes eight numbers, four lanes a block; the largest is found by two exchanges among the four.  24576 rows of 4096
-// bfloat16 numbers, 201 MB, take 50 us to codes (5.1 TB/s) and 36 us back; 77 rows of 2570 a launch's 3 us each way.
+// bfloat16 numbers, 201 MB, take 43 to 50 us to codes (5.1 to 5.9 TB/s) and 36 to 42 us back; 77 rows of 2570 a launch's 3 us each way.  Rows that are not
+// whole blocks go number by number: 24576 of 4098 119 us to codes and 134 back in bfloat16, 170 and 252 in float32 (2.7 to 1.8 TB/s).
 #include "common.h"
 
 // The scale's byte of a block whose largest magnitude has these bits (sign cleared).

@@ -2483,6 +2483,8 @@ def verify_drafts(logits: torch.Tensor, first: torch.Tensor, drafts: torch.Tenso
     ``sample`` draws.  temperature <= 0: drafts are accepted as long as they are the largest logit (lowest index on ties), and
     the token is that.  Weights and sums are 64-bit.
 
+    Rows of logits and of draft_logits together: 65535 at the most.
+
     tokens holds, at the request's rows, the accepted drafts, the token, and -1 behind; rows of no request are not written.
     Logits of -infinity and NaN weigh nothing; a row where nothing weighs gives the token -1.  A draft outside the vocabulary is
     not accepted.  accepted[r] is -1, and nothing of the request written, where first[] names rows that there are not, or where it

@@ -199,6 +199,23 @@ def test_silu_and_bias(ops, kind, M, N, K, out_dtype):
     assert ((got - want).abs() <= off + half * (want.abs() + off)).all()
 
 
+@pytest.mark.parametrize("M", [1, 16, 70, 300])
+def test_gate_and_up_rows_in_turn(ops, M):
+    """A matrix whose gate and up rows alternate in blocks of 32, as a loaded model's: the plain store and silu_mul over such columns give what
+    the epilogue gives of gate rows followed by up rows.  (Both are within the sums' and the activation's arithmetic, as in test_silu_and_bias.)"""
+    I, K = 352, 512
+    gate, up = (torch.randn(I, K, generator=gen(i)) * 0.2 for i in (61, 62))
+    x = torch.randn(M, K, generator=gen(63)).to(DEV)
+    w, turn = (ops.mxfp4_quantize(t.to(DEV)) for t in (torch.cat([gate, up]), ops.interleave_gate_up(gate, up)))
+    v = ops.mxfp4_values(w, torch.float32).double()
+    y, off = x.double() @ v.T, sums_bound(3 * K, x.double().abs() @ v.abs().T)
+    g, u, og, ou = y[:, :I], y[:, I:], off[:, :I], off[:, I:]
+    want = g * torch.sigmoid(g) * u
+    off = 1.1 * og * (u.abs() + ou) + (g * torch.sigmoid(g)).abs() * ou + (5 + g.abs()) * 2.0 ** -23 * want.abs()
+    for got in (ops.silu_mul(ops.gemm_mxfp4(x, turn), interleaved=True), ops.gemm_mxfp4(x, w, epilogue=ops.EPI_SILU_MUL)):
+        assert ((got.double() - want).abs() <= off).all()
+
+
 def test_float32_rows_lose_nothing(ops):
     """Three numbers a row, of all magnitudes: a product that leaves out any of the 24 bits is off by more than the bound."""
     M, N, K = 20, 48, 640
