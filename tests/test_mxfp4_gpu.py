@@ -602,6 +602,52 @@ def test_more_than_a_million_rows(ops, kind, K):
         assert ((half[a:b].double() - act).abs() <= bound + 2.0 ** -8 * (act.abs() + bound)).all(), a
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+def test_results_beyond_32_bits(ops, kind):
+    """More than 2^31 numbers of a result, by tiles, stored and added into a stream: exact sums (halves of at most 48 K), in bfloat16 rounded once."""
+    M, N, K = 66003, 33002, 64
+    codes, scales, v = whole_matrix(N, K, 3)
+    w, v = ops.MxFp4(codes.to(DEV), scales.to(DEV), K), v.to(DEV)
+    if kind == "fp4":
+        xc, xs, xv = whole_matrix(M, K, 7)
+        x = ops.MxFp4(xc.to(DEV), xs.to(DEV), K)
+    else:
+        xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+        x = xv.to(getattr(torch, kind)).to(DEV)
+    xv = xv.to(DEV)
+    got = ops.gemm_mxfp4(x, w, out_dtype=torch.bfloat16)
+    stream = torch.ones(M, N, device=DEV)
+    ops.gemm_mxfp4(x, w, out=stream, epilogue=ops.EPI_RESIDUAL)
+    for a in (0, 32000, 64000, 65071, M - 100):
+        want = xv[a:a + 100] @ v.T
+        assert torch.equal(got[a:a + 100], want.float().to(torch.bfloat16)), a
+        assert torch.equal(stream[a:a + 100].double(), want + 1), a
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "fp4"])
+@pytest.mark.parametrize("M", [1, 5, 12, 40, 200])
+@pytest.mark.parametrize("K", [1, 33, 500])
+def test_narrowest_gate_and_up(ops, kind, M, K):
+    """One to three gate columns with their ups, beside numbers that stay: the activation within its own arithmetic (exact sums)."""
+    for I in (1, 2, 3):
+        codes, scales, v = whole_matrix(2 * I, K, I)
+        w = ops.MxFp4(codes.to(DEV), scales.to(DEV), K)
+        if kind == "fp4":
+            xc, xs, xv = whole_matrix(M, K, 7)
+            x = ops.MxFp4(xc.to(DEV), xs.to(DEV), K)
+        else:
+            xv = torch.randint(-4, 5, (M, K), generator=gen(9)).double()
+            x = xv.to(getattr(torch, kind)).to(DEV)
+        want = xv @ v.T
+        gate, up = want[:, :I], want[:, I:]
+        act = gate * torch.sigmoid(gate) * up
+        hold = torch.full((M * I + 2,), 7.0, device=DEV)
+        ops.gemm_mxfp4(x, w, out_dtype=torch.float32, out=hold[1:-1].view(M, I), epilogue=ops.EPI_SILU_MUL)
+        got = hold[1:-1].view(M, I).cpu().double()
+        assert ((got - act).abs() <= (8 + gate.abs()) * 2.0 ** -23 * act.abs() + 2.0 ** -121 * up.abs()).all()
+        assert hold[0] == 7 and hold[-1] == 7
+
+
 def test_quantize_beyond_32_bits(ops):
     T, K = 66000, 32768                                        # more than 2^31 numbers
     rows = torch.randn(7, K, generator=gen(3)).to(torch.bfloat16).to(DEV)
